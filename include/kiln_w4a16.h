@@ -283,6 +283,79 @@ kiln_marlin_status_t kiln_w4a16_gemm_adapter_sides(
     int swiglu, int n_adapters, const int *ranks, const float *scales);
 
 /*
+ * A bank of low-rank adapters of one projection, one rank for all (an adapter of a lower rank has zero rows in lora_a, zero
+ * columns in lora_b).  All three in device memory, lora_a and lora_b on 16 bytes.  rank a multiple of 8, 8 ... 64; count 1 ... 4096.
+ */
+typedef struct {
+    const void *lora_a;   /* bf16 [count, rank, k] */
+    const void *lora_b;   /* bf16 [count, n, rank] */
+    const float *scales;  /* f32  [count] */
+    int count, rank;
+} kiln_w4a16_adapter_bank;
+
+/*
+ * C[i] = A[i] * dequant(B, s) + scales[a] * (A[i] * lora_a[a]^T) * lora_b[a]^T with a = adapter_of[i]: rows of many requests, each
+ * with an adapter of its own, beside one shared projection (the reference's formula for one adapter of all rows:
+ * crates/kiln-model/src/lora_loader.rs:213-232).  Any m, rows of an adapter anywhere among the others.
+ *   adapter_of  int32 [m], device memory; a value outside [0, count) is no adapter: the row is the plain GEMM's
+ *   workspace   as for the plain GEMM of the same sizes (kiln_w4a16_workspace_bytes)
+ *   scratch     kiln_w4a16_gemm_bank_scratch_bytes, on 16 bytes; never decreases with m; holds nothing between calls
+ * The low-rank term is summed in f32 (the projection kept to 2^-17 of itself) and added to the plain GEMM's result in bf16, which
+ * is rounded once more: as the reference adds a delta to its bf16 base.
+ */
+size_t kiln_w4a16_gemm_bank_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank);
+kiln_marlin_status_t kiln_w4a16_gemm_bank(
+    const void *A, const void *B, void *C, const void *s, int prob_m, int prob_n, int prob_k,
+    void *workspace, int groupsize, int dev, void *stream,
+    const kiln_w4a16_adapter_bank *bank, const int *adapter_of, void *scratch);
+
+/*
+ * The gradients of kiln_w4a16_gemm_bank, the packed weight frozen (the reference trains adapters over a frozen base; it has no
+ * packed counterpart):  with a = adapter_of[i], dC bf16 [m, n] the gradient of C,
+ *   dA[i]       = dC[i] * dequant(B, s)^T + scales[a] * (dC[i] * lora_b[a]) * lora_a[a]           bf16 [m, k]
+ *   d_lora_a[a] = scales[a] * sum over the rows of a of (dC[i] * lora_b[a])^T * A[i]              bf16 [count, rank, k]
+ *   d_lora_b[a] = scales[a] * sum over the rows of a of dC[i]^T * (A[i] * lora_a[a]^T)            bf16 [count, n, rank]
+ * every result written (an adapter without rows: zeros) and rounded once from f32 sums whose order does not vary.  A weight enters
+ * the product with dC rounded to bf16.  bank == NULL: dA alone, of the plain GEMM (A, adapter_of and the d_ pointers unused).
+ * No workspace; scratch: kiln_w4a16_gemm_bank_backward_scratch_bytes (count = rank = 0 without a bank), on 16 bytes, holds nothing
+ * between calls.
+ */
+size_t kiln_w4a16_gemm_bank_backward_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank);
+kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(
+    const void *dC, const void *A, const void *B, const void *s, int prob_m, int prob_n, int prob_k,
+    int groupsize, int dev, void *stream, const kiln_w4a16_adapter_bank *bank, const int *adapter_of,
+    void *dA, void *d_lora_a, void *d_lora_b, void *scratch);
+
+/*
+ * y[i] = sum_j weights[i, j] * down_e( silu(gate_e(x[i])) * up_e(x[i]) ), e = expert_of[i, j]: the experts of a mixture-of-experts MLP
+ * for a few tokens, kiln_w4a16_mlp with its rows' own choice of packs.  No counterpart in the reference, whose model family is dense.
+ *   x                    bf16 [m, hidden]; any m (runs of 64 rows: each reads the packs of its own experts)
+ *   expert_of, weights   int32 and f32 [m, top_k], device memory; an id outside [0, experts) adds nothing (an expert held elsewhere);
+ *                        an expert named twice by a row counts twice; top_k 1 ... 16
+ *   b_gate_up, s_gate_up [experts] packs of 2 * n_out columns, one after the other, each as for kiln_w4a16_mlp
+ *   b_down, s_down       [experts] packs [n_out, n_down]
+ *   y                    bf16 [m, n_down], rounded once; a row without experts is zero
+ *   scratch              kiln_w4a16_moe_scratch_bytes, on 16 bytes, holds nothing between calls
+ * silu(gate) * up is rounded to bf16 between the two products, as in kiln_w4a16_mlp.  hidden % 128 == 0, n_out % 128 == 0,
+ * n_down % 256 == 0, experts 1 ... 1024.
+ */
+size_t kiln_w4a16_moe_scratch_bytes(int prob_m, int top_k, int n_out, int n_down);
+kiln_marlin_status_t kiln_w4a16_moe(
+    const void *x, const int *expert_of, const float *weights, const void *b_gate_up, const void *s_gate_up,
+    const void *b_down, const void *s_down, void *y, int prob_m, int top_k, int experts, int hidden, int n_out, int n_down,
+    int groupsize, int dev, void *stream, void *scratch);
+
+/*
+ * The router's choice for kiln_w4a16_moe: of each row of logits [m, experts] (dtype 0 f32, 1 bf16, 2 f16) the top_k largest, ties to the
+ * lowest index, in falling order, and their share of the row's softmax (f32), divided by the shares' sum if `renormalise`.
+ * An expert at -inf is never chosen: places left over hold id -1 and weight 0.  A row with a NaN chooses as if that logit were -inf, and its
+ * weights are NaN, as a row's with +inf.  experts 1 ... 1024, top_k 1 ... 16 and <= experts.
+ */
+kiln_marlin_status_t kiln_moe_route(
+    const void *logits, int dtype, int prob_m, int experts, int top_k, int renormalise,
+    int *expert_of, float *weights, int dev, void *stream);
+
+/*
  * out[k, n] (f32, row-major) = (code - 8) * f32(scale), read from the tile
  * layout on the device.  The device-side statement of lib.rs:425; used to
  * prove the repack bit-exact.  No counterpart entry point in the reference.

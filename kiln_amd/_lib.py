@@ -30,6 +30,10 @@ EXPORTS = (
     "kiln_w4a16_takes_rank",
     "kiln_w4a16_takes_adapter_sides",
     "kiln_w4a16_gemm_adapter_sides",
+    "kiln_w4a16_gemm_bank_scratch_bytes",
+    "kiln_w4a16_gemm_bank",
+    "kiln_w4a16_gemm_bank_backward_scratch_bytes",
+    "kiln_w4a16_gemm_bank_backward",
     "kiln_w4a16_quantize_and_pack_device",
     "kiln_w4a16_quantize_and_pack_many_device",
     "kiln_w4a16_interleave_gate_up_device",
@@ -93,6 +97,12 @@ TUNING_EXPORTS = (
     "kiln_w4a16_debug_mid", "kiln_w4a16_debug_gmp", "kiln_w4a16_debug_flagged", "kiln_w4a16_debug_lora_fold",
     "kiln_w4a16_debug_rowsum_fold", "kiln_w4a16_debug_mid_waves", "kiln_w4a16_debug_meeting",
 )
+
+class AdapterBank(ctypes.Structure):
+    """kiln_w4a16_adapter_bank"""
+    _fields_ = [("lora_a", ctypes.c_void_p), ("lora_b", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("count", ctypes.c_int), ("rank", ctypes.c_int)]
+
 
 _libs: dict[bool, ctypes.CDLL] = {}
 _active_tuning = False
@@ -214,6 +224,15 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_takes_adapter_sides.argtypes = [i, i, i, vp, i, i, i, i]
     L.kiln_w4a16_gemm_adapter_sides.restype = i
     L.kiln_w4a16_gemm_adapter_sides.argtypes = [vp, vp, vp, vp, i, i, i, vp, i, i, vp, vp, i, i, i, c.POINTER(c.c_int), c.POINTER(c.c_float)]
+    bank = c.POINTER(AdapterBank)
+    L.kiln_w4a16_gemm_bank_scratch_bytes.restype = c.c_size_t
+    L.kiln_w4a16_gemm_bank_scratch_bytes.argtypes = [i, i, i, i, i]
+    L.kiln_w4a16_gemm_bank.restype = i
+    L.kiln_w4a16_gemm_bank.argtypes = [vp, vp, vp, vp, i, i, i, vp, i, i, vp, bank, vp, vp]
+    L.kiln_w4a16_gemm_bank_backward_scratch_bytes.restype = c.c_size_t
+    L.kiln_w4a16_gemm_bank_backward_scratch_bytes.argtypes = [i, i, i, i, i]
+    L.kiln_w4a16_gemm_bank_backward.restype = i
+    L.kiln_w4a16_gemm_bank_backward.argtypes = [vp, vp, vp, vp, i, i, i, i, i, vp, bank, vp, vp, vp, vp, vp]
     L.kiln_w4a16_stack_adapters.restype = i
     L.kiln_w4a16_stack_adapters.argtypes = [c.POINTER(vp), c.POINTER(vp), c.POINTER(i), c.POINTER(i), c.POINTER(i), i, i, i, i, i,
                                             vp, vp, vp]

@@ -1,0 +1,38 @@
+// What the calls on a bank of adapters share: the order of their rows, and the product of the rows with their own adapters' matrices.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "kiln_w4a16.h"
+
+namespace kiln {
+
+constexpr int kBankMaxRank = 64;
+constexpr int kBankRowTile = 16;
+constexpr int kBankOrderedFrom = 65;   // calls of fewer rows take them as they stand
+constexpr int kBankMaxSlices = 32;     // of the contraction of a projection
+
+inline size_t bank_up256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+// The rows of a call by position: position p is row order[p] (p itself without `order`), rows of one adapter together.
+// first[a] .. first[a + 1] are adapter a's positions, those of rows without an adapter come last.
+struct BankRows {
+    const int *of;      // [rows] adapter of a row; outside [0, count): none
+    const int *order;   // [rows], or null
+    const int *first;   // [count + 2], or null
+    int rows, count;
+};
+
+bool bank_ok(const kiln_w4a16_adapter_bank &bank);
+size_t bank_order_bytes(int rows, int count);
+// launches the ordering (calls of kBankOrderedFrom rows and more, or `always`); `at`: bank_order_bytes of scratch
+BankRows bank_order(const int *of, int rows, int count, bool always, void *at, hipStream_t stream);
+
+// slices of K that a projection of `rows` rows is cut into
+int bank_slices(int rows, int K);
+size_t bank_projected_rows(int rows, int K);
+// t[slice][position][rank] = the slice's share of src[row, K] * mat[adapter of row][rank, K]^T, f32; positions without an adapter are not written
+void bank_project(const void *src, const void *mat, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream);
+
+}  // namespace kiln

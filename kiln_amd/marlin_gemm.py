@@ -541,3 +541,126 @@ def marlin_w4a16_gemm_swiglu_lora(a: torch.Tensor, b_packed: torch.Tensor, scale
         raise MarlinGemmError(f"kiln_w4a16_gemm_swiglu_lora failed with status {status}: "
                               f"{_lib.status_string(status)} (m={m}, n_out={n_out}, k={k}, r_total={r_total})")
     return out
+
+
+def _check_bank(device, k: int, n: int, m: int, bank_a, bank_b, bank_scales, adapter_of):
+    """The bank of `marlin_w4a16_gemm_bank`: shapes, types, devices.  Returns (count, rank)."""
+    if bank_a.dim() != 3 or bank_b.dim() != 3 or bank_scales.dim() != 1 or adapter_of.dim() != 1:
+        _bail("a bank is bank_a [count, rank, k], bank_b [count, n, rank], bank_scales [count], adapter_of [m]")
+    count, rank = bank_a.shape[:2]
+    if tuple(bank_a.shape) != (count, rank, k) or tuple(bank_b.shape) != (count, n, rank) or tuple(bank_scales.shape) != (count,):
+        _bail(f"bank shapes {tuple(bank_a.shape)} / {tuple(bank_b.shape)} / {tuple(bank_scales.shape)} do not match "
+              f"[count, rank, k={k}] / [count, n={n}, rank] / [count]")
+    if not 1 <= count <= 4096:
+        _bail(f"a bank holds 1 to 4096 adapters (got {count})")
+    if rank % 8 != 0 or not 8 <= rank <= 64:
+        _bail(f"a bank's rank is a multiple of 8 up to 64 (got {rank})")
+    if tuple(adapter_of.shape) != (m,):
+        _bail(f"adapter_of must be [m={m}] (got {tuple(adapter_of.shape)})")
+    if bank_a.dtype != torch.bfloat16 or bank_b.dtype != torch.bfloat16:
+        _bail("bank_a and bank_b must be bf16")
+    if bank_scales.dtype != torch.float32 or adapter_of.dtype != torch.int32:
+        _bail("bank_scales must be f32 and adapter_of i32")
+    for t in (bank_a, bank_b, bank_scales, adapter_of):
+        if t.device != device:
+            _bail(f"the bank and adapter_of must be on {device} (got {t.device})")
+    return count, rank
+
+
+def _check_out(name: str, out, shape, device):
+    """A caller's result tensor, or a new one."""
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous():
+        _bail(f"{name} must be a contiguous bf16 {tuple(shape)} tensor on {device}")
+    return out
+
+
+def marlin_w4a16_gemm_bank(a: torch.Tensor, b_packed: torch.Tensor, scales: torch.Tensor, groupsize: int,
+                           bank_a: torch.Tensor, bank_b: torch.Tensor, bank_scales: torch.Tensor, adapter_of: torch.Tensor,
+                           *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`y[i] = a[i] @ dequant(b_packed) + s_j * (a[i] @ A_j^T) @ B_j^T` with `j = adapter_of[i]`: rows of many requests, each with
+    an adapter of its own, beside one shared projection (one adapter of all rows: crates/kiln-model/src/lora_loader.rs:213-232).
+
+    `bank_a` bf16 `[count, rank, k]`, `bank_b` bf16 `[count, n, rank]`, `bank_scales` f32 `[count]`, `adapter_of` i32 `[m]`; rank a
+    multiple of 8 up to 64 (zero rows of A and columns of B for adapters of a lower rank: `lora.make_bank`).  A row whose
+    `adapter_of` is outside `[0, count)` has no adapter and is `marlin_w4a16_gemm`'s row.
+    """
+    m, k, n = _check_gemm_args(a, b_packed, scales, groupsize)
+    count, rank = _check_bank(a.device, k, n, m, bank_a, bank_b, bank_scales, adapter_of)
+    out = _check_out("out", out, (m, n), a.device)
+    if m == 0:
+        return out
+    lib = _lib.load()
+    a, b_packed, scales = a.contiguous(), b_packed.contiguous(), scales.contiguous()
+    bank_a, bank_b, bank_scales, adapter_of = (t.contiguous() for t in (bank_a, bank_b, bank_scales, adapter_of))
+    bank = _lib.AdapterBank(bank_a.data_ptr(), bank_b.data_ptr(), bank_scales.data_ptr(), count, rank)
+    with torch.cuda.device(a.device):
+        stream = torch.cuda.current_stream(a.device).cuda_stream
+        ws = _workspace(a.device, stream, lib.kiln_w4a16_workspace_bytes(m, n, k))
+        scratch = torch.empty(lib.kiln_w4a16_gemm_bank_scratch_bytes(m, n, k, count, rank), dtype=torch.uint8, device=a.device)
+        status = lib.kiln_w4a16_gemm_bank(a.data_ptr(), b_packed.data_ptr(), out.data_ptr(), scales.data_ptr(), m, n, k, ws.data_ptr(),
+                                          groupsize, a.device.index or 0, stream, ctypes.byref(bank), adapter_of.data_ptr(),
+                                          scratch.data_ptr())
+    if status != 0:
+        raise MarlinGemmError(f"kiln_w4a16_gemm_bank failed with status {status}: {_lib.status_string(status)} "
+                              f"(m={m}, n={n}, k={k}, count={count}, rank={rank})")
+    return out
+
+
+def marlin_w4a16_gemm_bank_backward(dy: torch.Tensor, a: torch.Tensor, b_packed: torch.Tensor, scales: torch.Tensor, groupsize: int,
+                                    bank_a: torch.Tensor, bank_b: torch.Tensor, bank_scales: torch.Tensor,
+                                    adapter_of: torch.Tensor):
+    """The gradients of `marlin_w4a16_gemm_bank(a, ...)` from `dy` bf16 `[m, n]`, the packed weight frozen: `(da, d_bank_a, d_bank_b)`,
+    bf16, of the shapes of `a`, `bank_a` and `bank_b`.  With `j = adapter_of[i]`:
+    `da[i] = dy[i] @ W^T + s_j (dy[i] @ B_j) @ A_j`, `d_bank_a[j] = s_j sum (dy[i] @ B_j)^T a[i]`,
+    `d_bank_b[j] = s_j sum dy[i]^T (a[i] @ A_j^T)`, the sums over the rows of j; zeros for an adapter without rows."""
+    m, k, n = _check_gemm_args(a, b_packed, scales, groupsize)
+    count, rank = _check_bank(a.device, k, n, m, bank_a, bank_b, bank_scales, adapter_of)
+    _check_gradient(dy, m, n, a.device)
+    lib = _lib.load()
+    a, b_packed, scales, dy = a.contiguous(), b_packed.contiguous(), scales.contiguous(), dy.contiguous()
+    bank_a, bank_b, bank_scales, adapter_of = (t.contiguous() for t in (bank_a, bank_b, bank_scales, adapter_of))
+    da, d_bank_a, d_bank_b = torch.empty_like(a), torch.empty_like(bank_a), torch.empty_like(bank_b)
+    bank = _lib.AdapterBank(bank_a.data_ptr(), bank_b.data_ptr(), bank_scales.data_ptr(), count, rank)
+    with torch.cuda.device(a.device):
+        scratch = torch.empty(lib.kiln_w4a16_gemm_bank_backward_scratch_bytes(m, n, k, count, rank), dtype=torch.uint8, device=a.device)
+        status = lib.kiln_w4a16_gemm_bank_backward(
+            dy.data_ptr(), a.data_ptr(), b_packed.data_ptr(), scales.data_ptr(), m, n, k, groupsize, a.device.index or 0,
+            torch.cuda.current_stream(a.device).cuda_stream, ctypes.byref(bank), adapter_of.data_ptr(), da.data_ptr(),
+            d_bank_a.data_ptr(), d_bank_b.data_ptr(), scratch.data_ptr())
+    if status != 0:
+        raise MarlinGemmError(f"kiln_w4a16_gemm_bank_backward failed with status {status}: {_lib.status_string(status)} "
+                              f"(m={m}, n={n}, k={k}, count={count}, rank={rank})")
+    return da, d_bank_a, d_bank_b
+
+
+def _check_gradient(dy, m: int, n: int, device) -> None:
+    if dy.dim() != 2 or tuple(dy.shape) != (m, n) or dy.dtype != torch.bfloat16 or dy.device != device:
+        _bail(f"dy must be bf16 [{m}, {n}] on {device} (got {dy.dtype} {tuple(dy.shape)} on {dy.device})")
+
+
+def marlin_w4a16_gemm_backward(dy: torch.Tensor, b_packed: torch.Tensor, scales: torch.Tensor, groupsize: int) -> torch.Tensor:
+    """`dy @ dequant(b_packed)^T`: `[m, n]` bf16 -> `[m, k]` bf16, the gradient of `marlin_w4a16_gemm`'s rows (the packed weight is frozen):
+    what a trainer of adapters on some projections needs of those without."""
+    if not dy.is_cuda:
+        _bail("dy must be on CUDA")
+    if dy.dim() != 2 or b_packed.dim() != 2:
+        _bail("dy, b_packed and scales must be 2-D")
+    k = b_packed.shape[0] * 16
+    _, k, n = _check_gemm_args(dy.new_empty((0, k)), b_packed, scales, groupsize)
+    m = dy.shape[0]
+    _check_gradient(dy, m, n, dy.device)
+    lib = _lib.load()
+    dy, b_packed, scales = dy.contiguous(), b_packed.contiguous(), scales.contiguous()
+    da = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device)
+    if m == 0:
+        return da
+    with torch.cuda.device(dy.device):
+        scratch = torch.empty(lib.kiln_w4a16_gemm_bank_backward_scratch_bytes(m, n, k, 0, 0), dtype=torch.uint8, device=dy.device)
+        status = lib.kiln_w4a16_gemm_bank_backward(
+            dy.data_ptr(), None, b_packed.data_ptr(), scales.data_ptr(), m, n, k, groupsize, dy.device.index or 0,
+            torch.cuda.current_stream(dy.device).cuda_stream, None, None, da.data_ptr(), None, None, scratch.data_ptr())
+    if status != 0:
+        raise MarlinGemmError(f"kiln_w4a16_gemm_bank_backward failed with status {status}: {_lib.status_string(status)} (m={m}, n={n}, k={k})")
+    return da
