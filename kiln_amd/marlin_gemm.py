@@ -664,3 +664,88 @@ def marlin_w4a16_gemm_backward(dy: torch.Tensor, b_packed: torch.Tensor, scales:
     if status != 0:
         raise MarlinGemmError(f"kiln_w4a16_gemm_bank_backward failed with status {status}: {_lib.status_string(status)} (m={m}, n={n}, k={k})")
     return da
+
+
+_ROUTE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def moe_route(logits: torch.Tensor, top_k: int, renormalise: bool = True):
+    """The router's choice for `marlin_w4a16_moe`: of each row of `logits` `[m, experts]` (f32, bf16 or f16) the `top_k` largest, ties to
+    the lowest index, and their share of the row's softmax, divided by the shares' sum if `renormalise`: `(expert_of i32 [m, top_k],
+    weights f32 [m, top_k])` in falling order.  An expert at -inf is never chosen: places left over hold id -1 and weight 0.  The weights
+    of a row with a NaN or +inf are NaN."""
+    if not logits.is_cuda:
+        _bail("logits must be on CUDA")
+    if logits.dim() != 2 or logits.dtype not in _ROUTE_TYPES:
+        _bail(f"logits must be [m, experts], f32, bf16 or f16 (got {logits.dtype} {tuple(logits.shape)})")
+    m, experts = logits.shape
+    if not 1 <= experts <= 1024:
+        _bail(f"a router has 1 to 1024 experts (got {experts})")
+    if not 1 <= top_k <= min(16, experts):
+        _bail(f"top_k must be 1 to 16 and at most experts={experts} (got {top_k})")
+    logits = logits.contiguous()
+    expert_of = torch.empty((m, top_k), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((m, top_k), dtype=torch.float32, device=logits.device)
+    with torch.cuda.device(logits.device):
+        status = _lib.load().kiln_moe_route(logits.data_ptr(), _ROUTE_TYPES[logits.dtype], m, experts, top_k, int(bool(renormalise)),
+                                            expert_of.data_ptr(), weights.data_ptr(), logits.device.index or 0,
+                                            torch.cuda.current_stream(logits.device).cuda_stream)
+    if status != 0:
+        raise MarlinGemmError(f"kiln_moe_route failed with status {status}: {_lib.status_string(status)} (m={m}, experts={experts}, top_k={top_k})")
+    return expert_of, weights
+
+
+def marlin_w4a16_moe(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Tensor, b_gate_up: torch.Tensor, s_gate_up: torch.Tensor,
+                     b_down: torch.Tensor, s_down: torch.Tensor, groupsize: int, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`y[i] = sum_j weights[i, j] * down_e(silu(gate_e(x[i])) * up_e(x[i]))`, `e = expert_of[i, j]`: the experts of a mixture-of-experts
+    MLP for a few tokens, `marlin_w4a16_mlp` with its rows' own choice of packs.
+
+    `x` bf16 `[m, hidden]`, `expert_of` i32 and `weights` f32 `[m, top_k]` (`moe_route`; an id outside `[0, experts)` adds nothing), the
+    packs of `marlin_w4a16_mlp` with the experts in front: `b_gate_up` `[experts, hidden/16, 4 n_out]`, `s_gate_up` `[experts, hidden/g,
+    2 n_out]`, `b_down` `[experts, n_out/16, 2 n_down]`, `s_down` `[experts, n_out/g, n_down]` (`moe.pack_experts`)."""
+    if not x.is_cuda:
+        _bail("x must be on CUDA")
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        _bail(f"x must be bf16 [m, hidden] (got {x.dtype} {tuple(x.shape)})")
+    m, hidden = x.shape
+    if expert_of.dim() != 2 or expert_of.shape[0] != m or tuple(weights.shape) != tuple(expert_of.shape):
+        _bail(f"expert_of and weights must be [m={m}, top_k] (got {tuple(expert_of.shape)} and {tuple(weights.shape)})")
+    top_k = expert_of.shape[1]
+    if not 1 <= top_k <= 16:
+        _bail(f"top_k must be 1 to 16 (got {top_k})")
+    if expert_of.dtype != torch.int32 or weights.dtype != torch.float32:
+        _bail("expert_of must be i32 and weights f32")
+    if not (groupsize == -1 or groupsize == 128):
+        _bail(f"groupsize must be -1 or 128 (got {groupsize})")
+    if any(t.dim() != 3 for t in (b_gate_up, s_gate_up, b_down, s_down)):
+        _bail("the experts' packs are 3-D, experts first")
+    experts, n_out, n_down = b_gate_up.shape[0], s_gate_up.shape[2] // 2, s_down.shape[2]
+    if hidden == 0 or n_out == 0 or n_down == 0 or hidden % 128 or n_out % 128 or n_down % 256:
+        _bail(f"hidden={hidden} and n_out={n_out} must be multiples of 128, n_down={n_down} of 256")
+    if not 1 <= experts <= 1024:
+        _bail(f"a layer has 1 to 1024 experts (got {experts})")
+    g_in, g_out = (1, 1) if groupsize == -1 else (hidden // 128, n_out // 128)
+    for name, t, shape, dtype in (("b_gate_up", b_gate_up, (experts, hidden // 16, 4 * n_out), torch.int32),
+                                  ("s_gate_up", s_gate_up, (experts, g_in, 2 * n_out), torch.float16),
+                                  ("b_down", b_down, (experts, n_out // 16, 2 * n_down), torch.int32),
+                                  ("s_down", s_down, (experts, g_out, n_down), torch.float16)):
+        if tuple(t.shape) != shape or t.dtype != dtype:
+            _bail(f"{name} must be {dtype} {shape} (got {t.dtype} {tuple(t.shape)})")
+    for t in (expert_of, weights, b_gate_up, s_gate_up, b_down, s_down):
+        if t.device != x.device:
+            _bail(f"every operand must be on {x.device} (got {t.device})")
+    out = _check_out("out", out, (m, n_down), x.device)
+    if m == 0:
+        return out
+    lib = _lib.load()
+    x, expert_of, weights = x.contiguous(), expert_of.contiguous(), weights.contiguous()
+    b_gate_up, s_gate_up, b_down, s_down = (t.contiguous() for t in (b_gate_up, s_gate_up, b_down, s_down))
+    with torch.cuda.device(x.device):
+        scratch = torch.empty(lib.kiln_w4a16_moe_scratch_bytes(m, top_k, n_out, n_down), dtype=torch.uint8, device=x.device)
+        status = lib.kiln_w4a16_moe(x.data_ptr(), expert_of.data_ptr(), weights.data_ptr(), b_gate_up.data_ptr(), s_gate_up.data_ptr(),
+                                    b_down.data_ptr(), s_down.data_ptr(), out.data_ptr(), m, top_k, experts, hidden, n_out, n_down, groupsize,
+                                    x.device.index or 0, torch.cuda.current_stream(x.device).cuda_stream, scratch.data_ptr())
+    if status != 0:
+        raise MarlinGemmError(f"kiln_w4a16_moe failed with status {status}: {_lib.status_string(status)} "
+                              f"(m={m}, top_k={top_k}, experts={experts}, hidden={hidden}, n_out={n_out}, n_down={n_down})")
+    return out
