@@ -351,7 +351,7 @@ kiln_marlin_status_t kiln_w4a16_moe(
  * An expert at -inf is never chosen: places left over hold id -1 and weight 0.  A row with a NaN chooses as if that logit were -inf, and its
  * weights are NaN, as a row's with +inf.  experts 1 ... 1024, top_k 1 ... 16 and <= experts.
  */
-kiln_marlin_status_t kiln_moe_route(
+kiln_marlin_status_t kiln_w4a16_moe_route(
     const void *logits, int dtype, int prob_m, int experts, int top_k, int renormalise,
     int *expert_of, float *weights, int dev, void *stream);
 

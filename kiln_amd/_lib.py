@@ -36,7 +36,7 @@ EXPORTS = (
     "kiln_w4a16_gemm_bank_backward",
     "kiln_w4a16_moe_scratch_bytes",
     "kiln_w4a16_moe",
-    "kiln_moe_route",
+    "kiln_w4a16_moe_route",
     "kiln_w4a16_quantize_and_pack_device",
     "kiln_w4a16_quantize_and_pack_many_device",
     "kiln_w4a16_interleave_gate_up_device",
@@ -240,8 +240,8 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_moe_scratch_bytes.argtypes = [i, i, i, i]
     L.kiln_w4a16_moe.restype = i
     L.kiln_w4a16_moe.argtypes = [vp] * 8 + [i] * 8 + [vp, vp]
-    L.kiln_moe_route.restype = i
-    L.kiln_moe_route.argtypes = [vp, i, i, i, i, i, vp, vp, i, vp]
+    L.kiln_w4a16_moe_route.restype = i
+    L.kiln_w4a16_moe_route.argtypes = [vp, i, i, i, i, i, vp, vp, i, vp]
     L.kiln_w4a16_stack_adapters.restype = i
     L.kiln_w4a16_stack_adapters.argtypes = [c.POINTER(vp), c.POINTER(vp), c.POINTER(i), c.POINTER(i), c.POINTER(i), i, i, i, i, i,
                                             vp, vp, vp]

@@ -42,6 +42,13 @@ struct Library {
     decltype(&kiln_w4a16_takes_rank) takes_rank = nullptr;
     decltype(&kiln_w4a16_gemm_adapter_sides) gemm_sides = nullptr;
     decltype(&kiln_w4a16_repack_gptq_device) repack = nullptr;
+    decltype(&kiln_w4a16_gemm_bank) bank = nullptr;
+    decltype(&kiln_w4a16_gemm_bank_scratch_bytes) bank_scratch_bytes = nullptr;
+    decltype(&kiln_w4a16_gemm_bank_backward) bank_backward = nullptr;
+    decltype(&kiln_w4a16_gemm_bank_backward_scratch_bytes) bank_backward_scratch_bytes = nullptr;
+    decltype(&kiln_w4a16_moe) moe = nullptr;
+    decltype(&kiln_w4a16_moe_scratch_bytes) moe_scratch_bytes = nullptr;
+    decltype(&kiln_w4a16_moe_route) moe_route = nullptr;
 };
 Library g_lib;  // written by bind() under the interpreter lock, like everything below
 
@@ -672,6 +679,148 @@ PyObject *py_repack(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+at::Tensor empty_of(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+
+// The bank of args[0 ... 3] (bank_a, bank_b, bank_scales, adapter_of): everything marlin_gemm._check_bank asks for, and contiguity.
+struct Bank {
+    const at::Tensor *a = nullptr, *b = nullptr, *scales = nullptr, *of = nullptr;
+    kiln_w4a16_adapter_bank c{};
+};
+bool bank_of(PyObject *const *args, const Problem &p, Bank *l) {
+    l->a = tensor_of(args[0]);
+    l->b = tensor_of(args[1]);
+    l->scales = tensor_of(args[2]);
+    l->of = tensor_of(args[3]);
+    if (!l->a || !l->b || !l->scales || !l->of || !plain(*l->a, at::kBFloat16, 3, p.device) || !plain(*l->b, at::kBFloat16, 3, p.device) ||
+        !plain(*l->scales, at::kFloat, 1, p.device) || !plain(*l->of, at::kInt, 1, p.device))
+        return false;
+    const int64_t count = l->a->size(0), rank = l->a->size(1);
+    if (count < 1 || count > 4096 || rank < 8 || rank > 64 || rank % 8 != 0 || l->a->size(2) != p.k || l->b->size(0) != count ||
+        l->b->size(1) != p.n || l->b->size(2) != rank || l->scales->size(0) != count || l->of->size(0) != p.m)
+        return false;
+    l->c = {l->a->data_ptr(), l->b->data_ptr(), static_cast<const float *>(l->scales->data_ptr()), (int)count, (int)rank};
+    return true;
+}
+
+// gemm_bank(x, b_packed, scales, groupsize, bank_a, bank_b, bank_scales, adapter_of, out)
+PyObject *py_gemm_bank(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Problem p;
+    Bank l;
+    if (nargs != 9 || !problem_of(args, 2, &p) || !bank_of(args + 4, p, &l)) Py_RETURN_NONE;
+    Launch at_(p.device);
+    if (!at_.find_workspace(p.device, g_lib.workspace_bytes(p.m, p.n, p.k))) Py_RETURN_NONE;
+    at::Tensor out;
+    if (!output_of(args[8], *p.x, p.n, p.device, &out)) Py_RETURN_NONE;
+    const at::Tensor scratch = empty_of({(int64_t)g_lib.bank_scratch_bytes(p.m, p.n, p.k, l.c.count, l.c.rank)}, at::kByte, p.device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.bank(p.x->data_ptr(), p.b->data_ptr(), out.data_ptr(), p.s->data_ptr(), p.m, p.n, p.k, at_.workspace.data_ptr(), p.groupsize,
+                    p.device.index(), at_.stream, &l.c, static_cast<const int *>(l.of->data_ptr()), scratch.data_ptr());
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// gemm_bank_backward(dy, x, b_packed, scales, groupsize, bank_a, bank_b, bank_scales, adapter_of) -> (dx, d_bank_a, d_bank_b)
+PyObject *py_gemm_bank_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Problem p;
+    Bank l;
+    if (nargs != 9 || !problem_of(args + 1, 2, &p) || !bank_of(args + 5, p, &l)) Py_RETURN_NONE;
+    const at::Tensor *dy = tensor_of(args[0]);
+    if (!dy || !plain(*dy, at::kBFloat16, 2, p.device) || dy->size(0) != p.m || dy->size(1) != p.n) Py_RETURN_NONE;
+    Launch at_(p.device);
+    at::Tensor out[3] = {empty_bf16({p.m, p.k}, p.device), empty_bf16(l.a->sizes(), p.device), empty_bf16(l.b->sizes(), p.device)};
+    const at::Tensor scratch = empty_of({(int64_t)g_lib.bank_backward_scratch_bytes(p.m, p.n, p.k, l.c.count, l.c.rank)}, at::kByte, p.device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.bank_backward(dy->data_ptr(), p.x->data_ptr(), p.b->data_ptr(), p.s->data_ptr(), p.m, p.n, p.k, p.groupsize, p.device.index(),
+                             at_.stream, &l.c, static_cast<const int *>(l.of->data_ptr()), out[0].data_ptr(), out[1].data_ptr(),
+                             out[2].data_ptr(), scratch.data_ptr());
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    PyObject *parts[3], *all = nullptr;
+    for (int i = 0; i < 3; ++i) parts[i] = THPVariable_Wrap(std::move(out[i]));
+    if (parts[0] && parts[1] && parts[2]) all = PyTuple_Pack(3, parts[0], parts[1], parts[2]);
+    for (PyObject *part : parts) Py_XDECREF(part);
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// moe(x, expert_of, weights, b_gate_up, s_gate_up, b_down, s_down, groupsize, out)
+PyObject *py_moe(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int g;
+    if (nargs != 9 || !g_lib.moe || !groupsize_of(args[7], &g)) Py_RETURN_NONE;
+    const at::Tensor *t[7];
+    for (int i = 0; i < 7; ++i)
+        if (!(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &x = *t[0];
+    if (!x.is_cuda()) Py_RETURN_NONE;
+    const c10::Device device = x.device();
+    if (!plain(x, at::kBFloat16, 2, device) || !plain(*t[1], at::kInt, 2, device) || !plain(*t[2], at::kFloat, 2, device) ||
+        !plain(*t[3], at::kInt, 3, device) || !plain(*t[4], at::kHalf, 3, device) || !plain(*t[5], at::kInt, 3, device) ||
+        !plain(*t[6], at::kHalf, 3, device))
+        Py_RETURN_NONE;
+    const int64_t m = x.size(0), hidden = x.size(1), top = t[1]->size(1), experts = t[3]->size(0), n_out = t[4]->size(2) / 2, n_down = t[6]->size(2);
+    const int64_t g_in = g == -1 ? 1 : hidden / 128, g_out = g == -1 ? 1 : n_out / 128;
+    if (m < 1 || m > INT32_MAX || hidden < 128 || hidden > INT32_MAX || n_out < 128 || n_out > INT32_MAX / 2 || n_down < 256 || n_down > INT32_MAX ||
+        hidden % 128 || n_out % 128 || n_down % 256 || top < 1 || top > 16 || experts < 1 || experts > 1024 || t[1]->size(0) != m ||
+        t[2]->sizes() != t[1]->sizes() || t[3]->sizes() != at::IntArrayRef({experts, hidden / 16, 4 * n_out}) ||
+        t[4]->sizes() != at::IntArrayRef({experts, g_in, 2 * n_out}) || t[5]->sizes() != at::IntArrayRef({experts, n_out / 16, 2 * n_down}) ||
+        t[6]->sizes() != at::IntArrayRef({experts, g_out, n_down}))
+        Py_RETURN_NONE;
+    Launch at_(device);
+    at::Tensor out;
+    if (!output_of(args[8], x, n_down, device, &out)) Py_RETURN_NONE;
+    const at::Tensor scratch = empty_of({(int64_t)g_lib.moe_scratch_bytes((int)m, (int)top, (int)n_out, (int)n_down)}, at::kByte, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe(x.data_ptr(), static_cast<const int *>(t[1]->data_ptr()), static_cast<const float *>(t[2]->data_ptr()), t[3]->data_ptr(),
+                   t[4]->data_ptr(), t[5]->data_ptr(), t[6]->data_ptr(), out.data_ptr(), (int)m, (int)top, (int)experts, (int)hidden, (int)n_out,
+                   (int)n_down, g, device.index(), at_.stream, scratch.data_ptr());
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_route(logits, top_k, renormalise) -> (expert_of, weights)
+PyObject *py_moe_route(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *l = nargs == 3 && g_lib.moe_route ? tensor_of(args[0]) : nullptr;
+    if (!l || !l->is_cuda() || !PyLong_CheckExact(args[1]) || !PyBool_Check(args[2])) Py_RETURN_NONE;
+    const at::ScalarType type = l->scalar_type();
+    const int dtype = type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : type == at::kHalf ? 2 : -1;
+    const long top = PyLong_AsLong(args[1]);
+    if (top == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const c10::Device device = l->device();
+    if (dtype < 0 || !plain(*l, type, 2, device)) Py_RETURN_NONE;
+    const int64_t m = l->size(0), experts = l->size(1);
+    if (m < 1 || m > INT32_MAX || experts < 1 || experts > 1024 || top < 1 || top > 16 || top > experts) Py_RETURN_NONE;
+    Launch at_(device);
+    at::Tensor of = empty_of({m, top}, at::kInt, device), weights = empty_of({m, top}, at::kFloat, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe_route(l->data_ptr(), dtype, (int)m, (int)experts, (int)top, args[2] == Py_True, static_cast<int *>(of.data_ptr()),
+                         static_cast<float *>(weights.data_ptr()), device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    PyObject *a = THPVariable_Wrap(std::move(of)), *b = THPVariable_Wrap(std::move(weights));
+    PyObject *pair = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
 // set_workspaces(marlin_gemm's dictionary of them)
 PyObject *py_set_workspaces(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (nargs != 1 || !PyDict_CheckExact(args[0])) {
@@ -686,12 +835,12 @@ PyObject *py_set_workspaces(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 
 // bind(addresses of the library's functions, in the order of Library)
 PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    if (nargs != 13) {
-        PyErr_SetString(PyExc_TypeError, "bind takes thirteen function addresses");
+    if (nargs != 20) {
+        PyErr_SetString(PyExc_TypeError, "bind takes twenty function addresses");
         return nullptr;
     }
-    void *p[13];
-    for (int i = 0; i < 13; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+    void *p[20];
+    for (int i = 0; i < 20; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
     g_lib.gemm = reinterpret_cast<decltype(g_lib.gemm)>(p[0]);
     g_lib.gemm_lora = reinterpret_cast<decltype(g_lib.gemm_lora)>(p[1]);
@@ -706,6 +855,13 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     g_lib.gemm_sides = reinterpret_cast<decltype(g_lib.gemm_sides)>(p[10]);
     g_lib.repack = reinterpret_cast<decltype(g_lib.repack)>(p[11]);
     g_lib.takes_rank = reinterpret_cast<decltype(g_lib.takes_rank)>(p[12]);
+    g_lib.bank = reinterpret_cast<decltype(g_lib.bank)>(p[13]);
+    g_lib.bank_scratch_bytes = reinterpret_cast<decltype(g_lib.bank_scratch_bytes)>(p[14]);
+    g_lib.bank_backward = reinterpret_cast<decltype(g_lib.bank_backward)>(p[15]);
+    g_lib.bank_backward_scratch_bytes = reinterpret_cast<decltype(g_lib.bank_backward_scratch_bytes)>(p[16]);
+    g_lib.moe = reinterpret_cast<decltype(g_lib.moe)>(p[17]);
+    g_lib.moe_scratch_bytes = reinterpret_cast<decltype(g_lib.moe_scratch_bytes)>(p[18]);
+    g_lib.moe_route = reinterpret_cast<decltype(g_lib.moe_route)>(p[19]);
     Py_RETURN_NONE;
 }
 
@@ -724,7 +880,9 @@ PyObject *py_set_adapter_types(PyObject *, PyObject *const *args, Py_ssize_t nar
 
 #define FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST("linear", py_linear), FAST("linear_lora", py_linear_lora), FAST("linear_sides", py_linear_sides),
-                           FAST("mlp", py_mlp), FAST("quantize", py_quantize), FAST("repack", py_repack), FAST("set_workspaces", py_set_workspaces), FAST("bind", py_bind),
+                           FAST("mlp", py_mlp), FAST("quantize", py_quantize), FAST("repack", py_repack),
+                           FAST("gemm_bank", py_gemm_bank), FAST("gemm_bank_backward", py_gemm_bank_backward), FAST("moe", py_moe),
+                           FAST("moe_route", py_moe_route), FAST("set_workspaces", py_set_workspaces), FAST("bind", py_bind),
                            FAST("set_adapter_types", py_set_adapter_types), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

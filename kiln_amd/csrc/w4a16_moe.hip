@@ -327,7 +327,7 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
 
-kiln_marlin_status_t kiln_moe_route(const void *logits, int dtype, int prob_m, int experts, int top_k, int renormalise, int *expert_of,
+kiln_marlin_status_t kiln_w4a16_moe_route(const void *logits, int dtype, int prob_m, int experts, int top_k, int renormalise, int *expert_of,
                                     float *weights, int dev, void *stream) {
     (void)dev;
     if (prob_m < 0) return KILN_W4A16_ERR_PROB_SHAPE;

@@ -586,6 +586,9 @@ def marlin_w4a16_gemm_bank(a: torch.Tensor, b_packed: torch.Tensor, scales: torc
     multiple of 8 up to 64 (zero rows of A and columns of B for adapters of a lower rank: `lora.make_bank`).  A row whose
     `adapter_of` is outside `[0, count)` has no adapter and is `marlin_w4a16_gemm`'s row.
     """
+    y = _calls.gemm_bank(a, b_packed, scales, groupsize, bank_a, bank_b, bank_scales, adapter_of, out)
+    if y is not None:
+        return y
     m, k, n = _check_gemm_args(a, b_packed, scales, groupsize)
     count, rank = _check_bank(a.device, k, n, m, bank_a, bank_b, bank_scales, adapter_of)
     out = _check_out("out", out, (m, n), a.device)
@@ -615,6 +618,9 @@ def marlin_w4a16_gemm_bank_backward(dy: torch.Tensor, a: torch.Tensor, b_packed:
     bf16, of the shapes of `a`, `bank_a` and `bank_b`.  With `j = adapter_of[i]`:
     `da[i] = dy[i] @ W^T + s_j (dy[i] @ B_j) @ A_j`, `d_bank_a[j] = s_j sum (dy[i] @ B_j)^T a[i]`,
     `d_bank_b[j] = s_j sum dy[i]^T (a[i] @ A_j^T)`, the sums over the rows of j; zeros for an adapter without rows."""
+    made = _calls.gemm_bank_backward(dy, a, b_packed, scales, groupsize, bank_a, bank_b, bank_scales, adapter_of)
+    if made is not None:
+        return made
     m, k, n = _check_gemm_args(a, b_packed, scales, groupsize)
     count, rank = _check_bank(a.device, k, n, m, bank_a, bank_b, bank_scales, adapter_of)
     _check_gradient(dy, m, n, a.device)
@@ -674,6 +680,9 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalise: bool = True):
     the lowest index, and their share of the row's softmax, divided by the shares' sum if `renormalise`: `(expert_of i32 [m, top_k],
     weights f32 [m, top_k])` in falling order.  An expert at -inf is never chosen: places left over hold id -1 and weight 0.  The weights
     of a row with a NaN or +inf are NaN."""
+    made = _calls.moe_route(logits, top_k, renormalise)
+    if made is not None:
+        return made
     if not logits.is_cuda:
         _bail("logits must be on CUDA")
     if logits.dim() != 2 or logits.dtype not in _ROUTE_TYPES:
@@ -687,11 +696,11 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalise: bool = True):
     expert_of = torch.empty((m, top_k), dtype=torch.int32, device=logits.device)
     weights = torch.empty((m, top_k), dtype=torch.float32, device=logits.device)
     with torch.cuda.device(logits.device):
-        status = _lib.load().kiln_moe_route(logits.data_ptr(), _ROUTE_TYPES[logits.dtype], m, experts, top_k, int(bool(renormalise)),
+        status = _lib.load().kiln_w4a16_moe_route(logits.data_ptr(), _ROUTE_TYPES[logits.dtype], m, experts, top_k, int(bool(renormalise)),
                                             expert_of.data_ptr(), weights.data_ptr(), logits.device.index or 0,
                                             torch.cuda.current_stream(logits.device).cuda_stream)
     if status != 0:
-        raise MarlinGemmError(f"kiln_moe_route failed with status {status}: {_lib.status_string(status)} (m={m}, experts={experts}, top_k={top_k})")
+        raise MarlinGemmError(f"kiln_w4a16_moe_route failed with status {status}: {_lib.status_string(status)} (m={m}, experts={experts}, top_k={top_k})")
     return expert_of, weights
 
 
@@ -703,6 +712,9 @@ def marlin_w4a16_moe(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Te
     `x` bf16 `[m, hidden]`, `expert_of` i32 and `weights` f32 `[m, top_k]` (`moe_route`; an id outside `[0, experts)` adds nothing), the
     packs of `marlin_w4a16_mlp` with the experts in front: `b_gate_up` `[experts, hidden/16, 4 n_out]`, `s_gate_up` `[experts, hidden/g,
     2 n_out]`, `b_down` `[experts, n_out/16, 2 n_down]`, `s_down` `[experts, n_out/g, n_down]` (`moe.pack_experts`)."""
+    y = _calls.moe(x, expert_of, weights, b_gate_up, s_gate_up, b_down, s_down, groupsize, out)
+    if y is not None:
+        return y
     if not x.is_cuda:
         _bail("x must be on CUDA")
     if x.dim() != 2 or x.dtype != torch.bfloat16:
