@@ -10,7 +10,7 @@ namespace kiln {
 
 constexpr int kBankMaxRank = 64;
 constexpr int kBankRowTile = 16;
-constexpr int kBankOrderedFrom = 65;   // calls of fewer rows take them as they stand
+constexpr int kBankOrderedFrom = 257;  // calls of fewer rows take them as they stand
 constexpr int kBankMaxSlices = 32;     // of the contraction of a projection
 
 inline size_t bank_up256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }

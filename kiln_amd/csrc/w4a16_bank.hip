@@ -2,9 +2,9 @@
 // y[i] = x[i] W + s_a (x[i] A_a^T) B_a^T, a = adapter_of[i].
 //
 // Three steps: T = x A^T (w4a16_bank project, f32), the plain GEMM, and y += s T B^T in place.  Rows are handled in tiles of 16
-// positions; a tile multiplies with each adapter that is present among its rows, once, and rows of other adapters are left out of
-// the product, so any order of the rows is right and one in which an adapter's rows are together reads its matrices least often:
-// from 65 rows on a launch in front puts them so.  The reference serves one adapter set per process
+// positions or 64; a tile multiplies with each adapter that is present among its rows, once, and rows of other adapters are left out
+// of the product, so any order of the rows is right and one in which an adapter's rows are together reads its matrices least often:
+// from 257 rows on a launch in front puts them so.  The reference serves one adapter set per process
 // (crates/kiln-model/src/lora_loader.rs:213-232); this is its formula with the adapter a row's own.
 #include "bank.h"
 #include "device_common.h"
@@ -12,48 +12,57 @@
 namespace kiln {
 namespace {
 
-// order[] and first[]: a wavefront per adapter (and one for the rows without) counts the rows of lower adapters and places its own,
-// 64 rows per ballot; no block waits for another and rows keep their order inside an adapter.
-constexpr int kOrderUnroll = 8;
-__global__ __launch_bounds__(256) void bank_order_kernel(const int *__restrict__ of, int *__restrict__ order, int *__restrict__ first, int rows,
-                                                         int count) {
-    const int lane = threadIdx.x & 63;
-    const int a = blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-    if (a > count) return;
-    int less = 0;
-    for (int r0 = 0; r0 < rows; r0 += 64 * kOrderUnroll) {
-        int v[kOrderUnroll];
+// order[] and first[]: a block per adapter (and one for the rows without) counts the rows of lower adapters and places its own, 64 rows
+// per ballot, its sixteen wavefronts a sixteenth of the rows each: no block waits for another and rows keep their order inside an
+// adapter.  Up to 8192 rows a wavefront's part is in registers and read once.  2048 rows, 8 adapters: a wavefront for each took 14 us.
+constexpr int kOrderWaves = 16, kOrderUnroll = 8;
+__global__ __launch_bounds__(kOrderWaves * 64) void bank_order_kernel(const int *__restrict__ of, int *__restrict__ order, int *__restrict__ first,
+                                                                      int rows, int count) {
+    __shared__ int less_of[kOrderWaves], mine_of[kOrderWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = blockIdx.x;
+    const int each = (rows + kOrderWaves * 64 - 1) / (kOrderWaves * 64) * 64;
+    const int begin = wave * each, end = min(rows, begin + each);
+    int key[kOrderUnroll];
+    auto read = [&](int r0) {
 #pragma unroll
         for (int u = 0; u < kOrderUnroll; ++u) {
             const int r = r0 + 64 * u + lane;
-            v[u] = r < rows ? of[r] : -1;
+            key[u] = r < end ? of[r] : -1;
         }
 #pragma unroll
         for (int u = 0; u < kOrderUnroll; ++u) {
-            const bool in = r0 + 64 * u + lane < rows;
-            const int key = (unsigned)v[u] < (unsigned)count ? v[u] : count;
-            less += __popcll(__ballot(in && key < a));
+            if ((unsigned)key[u] >= (unsigned)count) key[u] = count;
+            if (r0 + 64 * u + lane >= end) key[u] = INT32_MAX;
+        }
+    };
+    int less = 0, mine = 0;
+    for (int r0 = begin; r0 < end; r0 += 64 * kOrderUnroll) {
+        read(r0);
+#pragma unroll
+        for (int u = 0; u < kOrderUnroll; ++u) {
+            less += __popcll(__ballot(key[u] < a));
+            mine += __popcll(__ballot(key[u] == a));
         }
     }
     if (lane == 0) {
-        first[a] = less;
+        less_of[wave] = less;
+        mine_of[wave] = mine;
+    }
+    __syncthreads();
+    int at = 0;
+    for (int w = 0; w < kOrderWaves; ++w) at += less_of[w];
+    if (threadIdx.x == 0) {
+        first[a] = at;
         if (a == count) first[count + 1] = rows;
     }
-    for (int r0 = 0; r0 < rows; r0 += 64 * kOrderUnroll) {
-        int v[kOrderUnroll];
+    for (int w = 0; w < wave; ++w) at += mine_of[w];
+    for (int r0 = begin; r0 < end; r0 += 64 * kOrderUnroll) {
+        if (each > 64 * kOrderUnroll) read(r0);
 #pragma unroll
         for (int u = 0; u < kOrderUnroll; ++u) {
-            const int r = r0 + 64 * u + lane;
-            v[u] = r < rows ? of[r] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < kOrderUnroll; ++u) {
-            const int r = r0 + 64 * u + lane;
-            const int key = (unsigned)v[u] < (unsigned)count ? v[u] : count;
-            const bool mine = r < rows && key == a;
-            const unsigned long long all = __ballot(mine);
-            if (mine) order[less + __popcll(all & ((1ull << lane) - 1))] = r;
-            less += __popcll(all);
+            const unsigned long long all = __ballot(key[u] == a);
+            if (key[u] == a) order[at + __popcll(all & ((1ull << lane) - 1))] = r0 + 64 * u + lane;
+            at += __popcll(all);
         }
     }
 }
@@ -62,138 +71,311 @@ __device__ __forceinline__ bf16x8 load_bf16x8(const uint16_t *p) {
     return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(p));
 }
 
-// The row and the adapter (-1: none) of position p0 + (lane & 15).
-__device__ __forceinline__ void row_of_lane(const BankRows &r, int p, int &row, int &a) {
+// The row and the adapter (-1: none) of position p.
+__device__ __forceinline__ void row_at(const BankRows &r, int p, int &row, int &a) {
     row = p < r.rows ? (r.order ? r.order[p] : p) : -1;
     a = row >= 0 ? r.of[row] : -1;
     if ((unsigned)a >= (unsigned)r.count) a = -1;
 }
 
-// U steps of a projection's contraction, all their loads in front of their products.
-constexpr int kProjectAhead = 4;
-template <int JT, int U>
-__device__ __forceinline__ void project_steps(const uint16_t *__restrict__ x, const uint16_t *__restrict__ m, int K, int rank, int c,
-                                              f32x4 (&acc)[JT]) {
-    bf16x8 xv[U], b[U][JT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        xv[u] = load_bf16x8(x + 128 * u);
-#pragma unroll
-        for (int j = 0; j < JT; ++j) b[u][j] = 16 * j + c < rank ? load_bf16x8(m + (size_t)16 * j * K + 128 * u) : bf16x8_zero();
-    }
+// U pieces of a projection's contraction, 64 long each and 256 apart, all their loads in front of their products.  A lane's part of a
+// piece is 16 values side by side, the first eight for one product and the rest for the next (which values meet in a product does not
+// matter), so that four lanes read a row's 128 bytes together.
+template <int JT, int RT, int W, int U>
+__device__ __forceinline__ void project_pieces(const uint16_t *const (&x)[RT], const uint16_t *const (&m)[JT], int at, f32x4 (&acc)[RT][JT]) {
+    bf16x8 xv[U][RT][2], b[U][JT][2];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < JT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[u], b[u][j], acc[j], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) xv[u][i][h] = load_bf16x8(x[i] + at + 64 * W * u + 8 * h);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) b[u][j][h] = load_bf16x8(m[j] + at + 64 * W * u + 8 * h);
+        }
+    __builtin_amdgcn_sched_barrier(0);  // left alone, the compiler has eight loads in flight at a time
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < JT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[u][i][h], b[u][j][h], acc[i][j], 0, 0, 0);
 }
 
-// A block: 16 positions, one slice of K, and of the adapters present among them those whose turn (in the order they are met) is
-// blockIdx.z modulo gridDim.z.  Its four wavefronts take every fourth 32 of K and meet in LDS.
-template <int JT>
-__global__ __launch_bounds__(256) void bank_project_kernel(const uint16_t *__restrict__ src, const uint16_t *__restrict__ mat, BankRows rows,
+// T: a block takes 16 RT positions, one slice of K, and of the adapters present among them those whose turn (in the order they are met)
+// is blockIdx.z modulo gridDim.z.  Its W wavefronts take every W-th 64 of K and meet in LDS.  Blocks go through the slices first, so
+// that with eight of them a die's blocks share one, whose part of the adapters' matrices its L2 then holds.
+template <int JT, int RT, int W>
+__global__ __launch_bounds__(W * 64) void bank_project_kernel(const uint16_t *__restrict__ src, const uint16_t *__restrict__ mat, BankRows rows,
                                                            float *__restrict__ t, int K, int steps, int rank) {
-    __shared__ float part[4][16][JT * 16 + 4];
+    constexpr int P = 16 * RT, kAhead = JT + RT <= 4 ? 4 : 2;
+    __shared__ float part[W][P][JT * 16 + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int p0 = blockIdx.x * kBankRowTile;
+    const int p0 = blockIdx.y * P;
     int row, a;
-    row_of_lane(rows, p0 + c, row, a);
-    const int k0 = blockIdx.y * steps * 128 + 32 * wave + 8 * q;
-    const int n_steps = min(steps, K / 128 - (int)blockIdx.y * steps);
-    const uint16_t *x = src + (size_t)max(row, 0) * K + k0;
-    unsigned left = (unsigned)__ballot(a >= 0) & 0xFFFFu;
+    row_at(rows, p0 + (lane & (P - 1)), row, a);
+    constexpr unsigned long long kAll = P == 64 ? ~0ull : (1ull << P) - 1;
+    unsigned long long left = __ballot(a >= 0) & kAll;
+    const int k0 = blockIdx.x * steps * 128, k1 = min(K, k0 + steps * 128), own = k0 + 64 * wave;
+    const int pieces = own < k1 ? (k1 - own + 64 * W - 1) / (64 * W) : 0;
+    const uint16_t *x[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) x[i] = src + (size_t)max(__shfl(row, 16 * i + c), 0) * K + own + 16 * q;
     for (unsigned turn = 0; left; ++turn) {
-        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
-        const unsigned mine = (unsigned)__ballot(a == cur) & 0xFFFFu;
+        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+        const unsigned long long mine = __ballot(a == cur) & kAll;
         left &= ~mine;
         if (turn % gridDim.z != blockIdx.z) continue;
-        const uint16_t *m = mat + ((size_t)cur * rank + c) * K + k0;
-        f32x4 acc[JT];
+        const uint16_t *m[JT];  // rows past the rank: the last one again, their sums are dropped
 #pragma unroll
-        for (int j = 0; j < JT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < JT; ++j) m[j] = mat + ((size_t)cur * rank + min(16 * j + c, rank - 1)) * K + own + 16 * q;
+        f32x4 acc[RT][JT] = {};
         int s = 0;
-        for (; s + kProjectAhead <= n_steps; s += kProjectAhead) project_steps<JT, kProjectAhead>(x + 128 * s, m + 128 * s, K, rank, c, acc);
-        for (; s < n_steps; ++s) project_steps<JT, 1>(x + 128 * s, m + 128 * s, K, rank, c, acc);
+        for (; s + kAhead <= pieces; s += kAhead) project_pieces<JT, RT, W, kAhead>(x, m, 64 * W * s, acc);
+        if (kAhead > 2 && s + 2 <= pieces) {
+            project_pieces<JT, RT, W, 2>(x, m, 64 * W * s, acc);
+            s += 2;
+        }
+        if (s < pieces) project_pieces<JT, RT, W, 1>(x, m, 64 * W * s, acc);
 #pragma unroll
-        for (int j = 0; j < JT; ++j)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][4 * q + i][16 * j + c] = acc[j][i];
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][16 * r + 4 * q + i][16 * j + c] = acc[r][j][i];
         __syncthreads();
-        float *out = t + ((size_t)blockIdx.y * rows.rows + p0) * rank;
-        for (int e = tid; e < 16 * rank; e += 256) {
+        float *out = t + ((size_t)blockIdx.x * rows.rows + p0) * rank;
+        for (int e = tid; e < P * rank; e += 64 * W) {
             const int r = e / rank, j = e - r * rank;
-            if (mine >> r & 1) out[e] = (part[0][r][j] + part[1][r][j]) + (part[2][r][j] + part[3][r][j]);
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v += part[w][r][j];
+            if (mine >> r & 1) out[e] = v;
         }
         __syncthreads();
     }
 }
 
-// y[row] += s_a T[row] B_a^T on 16 positions x 256 columns, 64 to a wavefront, as B_a (its rows the columns of y) times T^T: a lane
-// then holds four consecutive columns of one row.  T goes in as two bf16 parts whose sum is within 2^-17 of it, side by side on the
-// contraction, which has room: 32 for a rank of 16.
+// y[row] += s_a T[row] B_a^T, formed as B_a (its rows the columns of y) times T^T, so that a lane holds consecutive columns of one row:
+// two products of 16 columns, whose rows of B_a are dealt out such that their results are eight columns side by side.  T goes in as two
+// bf16 parts whose sum is within 2^-17 of it, one product each with the same rows of B.  S: the contraction's steps of 32.
+// A product's result is taken by the rows of its adapter alone (a lane has one row): what another adapter holds that is no number
+// stays with its own rows.
+__device__ __forceinline__ int column_of(int tile, int c) { return 32 * (tile >> 1) + 8 * (c >> 2) + 4 * (tile & 1) + (c & 3); }
+
+template <int S>
+struct ExpandRow {  // this lane's part of its row's T
+    bf16x8 hi[S], lo[S];
+    __device__ __forceinline__ void set(const float *t, float scale, bool live, int q, int rank) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int at = 32 * s + 8 * q;
+            hi[s] = lo[s] = bf16x8_zero();
+            if (live && at < rank)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float f = t[at + i] * scale;
+                    hi[s][i] = (__bf16)f;
+                    lo[s][i] = (__bf16)(f - (float)hi[s][i]);
+                }
+        }
+    }
+};
+// 16 TILES columns from n0 on, of adapter `mat`'s rows of B (past the rank: the last eight again, times zeros)
+template <int S, int TILES>
+__device__ __forceinline__ void expand_rows(const uint16_t *__restrict__ mat, int c, int q, int rank, bf16x8 (&b)[TILES][S]) {
+#pragma unroll
+    for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+        for (int s = 0; s < S; ++s) b[tile][s] = load_bf16x8(mat + (size_t)column_of(tile, c) * rank + min(32 * s + 8 * q, rank - 8));
+}
+template <int S, int TILES>
+__device__ __forceinline__ void expand_product(const bf16x8 (&b)[TILES][S], const ExpandRow<S> &t, bool own, f32x4 (&acc)[TILES]) {
+#pragma unroll
+    for (int tile = 0; tile < TILES; ++tile) {
+        f32x4 v = acc[tile];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[tile][s], t.hi[s], v, 0, 0, 0);
+            v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[tile][s], t.lo[s], v, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[tile][i] = own ? v[i] : acc[tile][i];
+    }
+}
+// eight columns of y to the accumulators of two tiles, and back
+__device__ __forceinline__ void take_columns(u32x4 v, f32x4 &even, f32x4 &odd) {
+    even = f32x4{__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xFFFF0000u), __builtin_bit_cast(float, v.y << 16),
+                 __builtin_bit_cast(float, v.y & 0xFFFF0000u)};
+    odd = f32x4{__builtin_bit_cast(float, v.z << 16), __builtin_bit_cast(float, v.z & 0xFFFF0000u), __builtin_bit_cast(float, v.w << 16),
+                __builtin_bit_cast(float, v.w & 0xFFFF0000u)};
+}
+__device__ __forceinline__ u32x4 give_columns(const f32x4 &even, const f32x4 &odd) {
+    auto pair = [](float lo, float hi) { return f32_to_bf16_bits(lo) | (uint32_t)f32_to_bf16_bits(hi) << 16; };
+    return u32x4{pair(even[0], even[1]), pair(even[2], even[3]), pair(odd[0], odd[1]), pair(odd[2], odd[3])};
+}
+// T's slices summed, [positions][rank] of this block's from p0 on
+template <int P>
+__device__ __forceinline__ void sum_projected(const float *__restrict__ t, const BankRows &rows, int p0, int rank, int slices, int tid,
+                                              float (&ts)[P][kBankMaxRank + 4]) {
+    const size_t stride = (size_t)rows.rows * rank;
+    for (int e = tid; e < P * rank; e += 256) {
+        const int r = e / rank;
+        const float *from = t + (size_t)p0 * rank + e;
+        float v = 0.f;
+        if (p0 + r < rows.rows) {
+            int s = 0;
+            for (; s + 4 <= slices; s += 4) {
+                const float v0 = from[s * stride], v1 = from[(s + 1) * stride], v2 = from[(s + 2) * stride], v3 = from[(s + 3) * stride];
+                v += (v0 + v1) + (v2 + v3);
+            }
+            for (; s < slices; ++s) v += from[s * stride];
+        }
+        ts[r][e - r * rank] = v;
+    }
+    __syncthreads();
+}
+
+// Rows as they stand: 16 of them x 64 columns to a block, the adapters met dealt out to its four wavefronts, each of which takes the
+// rows of its own: nothing to add up, and with an adapter per row (a decode step) the loads of four adapters' rows of B go out together.
+// Bound by those loads' latency.  16 rows of 16 adapters, 18432 columns, rank 16: 27 us with the adapters one after the other.
 template <int S>
 __global__ __launch_bounds__(256) void bank_expand_kernel(uint16_t *__restrict__ y, const uint16_t *__restrict__ mat, const float *__restrict__ t,
                                                           const float *__restrict__ scales, BankRows rows, int N, int rank, int slices) {
+    constexpr int kTogether = S == 1 ? 4 : 2;
     __shared__ float ts[16][kBankMaxRank + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int p0 = blockIdx.y * kBankRowTile;
+    const int p0 = blockIdx.y * kBankRowTile, n0 = blockIdx.x * 64;
     int row, a;
-    row_of_lane(rows, p0 + c, row, a);
+    row_at(rows, p0 + c, row, a);
     unsigned left = (unsigned)__ballot(a >= 0) & 0xFFFFu;
     if (!left) return;
-    for (int e = tid; e < 16 * rank; e += 256) {
-        const int r = e / rank, j = e - r * rank;
-        float v = 0.f;
-        if (p0 + r < rows.rows)
-            for (int s = 0; s < slices; ++s) v += t[((size_t)s * rows.rows + p0 + r) * rank + j];
-        ts[r][j] = v;
-    }
-    __syncthreads();
-    const int n0 = blockIdx.x * 256 + wave * 64, octets = rank >> 3;
-    const bool live = a >= 0;
-    const float scale = live ? scales[a] : 0.f;
-    uint16_t *dst = y + (size_t)max(row, 0) * N + n0 + 4 * q;
-    f32x4 acc[4];
-#pragma unroll
-    for (int tile = 0; tile < 4; ++tile) {
-        const u32x2 v = live ? *reinterpret_cast<const u32x2 *>(dst + 16 * tile) : u32x2{0u, 0u};
-        acc[tile] = f32x4{__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xFFFF0000u),
-                          __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xFFFF0000u)};
-    }
-    while (left) {
+    int mine[4] = {0, 0, 0, 0}, count = 0;  // the adapters of this wavefront
+    bool live = false;
+    for (int turn = 0; left; ++turn) {
         const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
         left &= ~((unsigned)__ballot(a == cur) & 0xFFFFu);
-        const uint16_t *m = mat + ((size_t)cur * N + n0 + c) * rank;
+        if ((turn & 3) != wave) continue;
+        if (count == 0) mine[0] = cur;
+        else if (count == 1) mine[1] = cur;
+        else if (count == 2) mine[2] = cur;
+        else mine[3] = cur;
+        ++count;
+        live |= a == cur;
+    }
+    const float scale = live ? scales[a] : 0.f;
+    uint16_t *dst = y + (size_t)max(row, 0) * N + n0 + 8 * q;
+    u32x4 was[2];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int o = 4 * s + q;
-            const bool lower = o >= octets, used = o < 2 * octets;
-            const int at = 8 * (used ? (lower ? o - octets : o) : 0);
-            bf16x8 tv = bf16x8_zero();
-            if (used && a == cur)
+    for (int i = 0; i < 2; ++i) was[i] = *reinterpret_cast<const u32x4 *>(dst + 32 * i);
+    f32x4 acc[4];
+    ExpandRow<S> tv;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = ts[c][at + i] * scale;
-                    const __bf16 hi = (__bf16)v;
-                    tv[i] = lower ? (__bf16)(v - (float)hi) : hi;
-                }
+    for (int first = 0; first < 4; first += kTogether) {
+        bf16x8 b[kTogether][4][S];
 #pragma unroll
-            for (int tile = 0; tile < 4; ++tile) {
-                const bf16x8 b = used ? load_bf16x8(m + (size_t)16 * tile * rank + at) : bf16x8_zero();
-                acc[tile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, tv, acc[tile], 0, 0, 0);
-            }
+        for (int g = 0; g < kTogether; ++g) {
+            if (first + g >= count) break;
+            expand_rows<S, 4>(mat + ((size_t)mine[first + g] * N + n0) * rank, c, q, rank, b[g]);
+        }
+        if (first == 0) {
+            sum_projected<16>(t, rows, p0, rank, slices, tid, ts);
+            tv.set(ts[c], scale, live, q, rank);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) take_columns(was[i], acc[2 * i], acc[2 * i + 1]);
+        }
+#pragma unroll
+        for (int g = 0; g < kTogether; ++g) {
+            if (first + g >= count) break;
+            expand_product<S, 4>(b[g], tv, a == mine[first + g], acc);
         }
     }
-    if (!live) return;
+    if (live)
 #pragma unroll
-    for (int tile = 0; tile < 4; ++tile) {
-        u32x2 v;
-        v.x = f32_to_bf16_bits(acc[tile][0]) | (uint32_t)f32_to_bf16_bits(acc[tile][1]) << 16;
-        v.y = f32_to_bf16_bits(acc[tile][2]) | (uint32_t)f32_to_bf16_bits(acc[tile][3]) << 16;
-        *reinterpret_cast<u32x2 *>(dst + 16 * tile) = v;
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(dst + 32 * i) = give_columns(acc[2 * i], acc[2 * i + 1]);
+}
+
+// Rows in the order of their adapters: 64 positions x `columns` columns to a block, 64 at a time to each wavefront, so that a wavefront's
+// rows of B serve four tiles of rows; T is read and split once, y of the next columns on its way meanwhile.  Bound by y, read and written:
+// 2048 rows of 18432 columns, rank 32, 45 us behind the GEMM that wrote them, 3.4 TB/s (with 16 positions to a wavefront, 128 columns at a time, the same).
+template <int S>
+__global__ __launch_bounds__(256) void bank_expand_ordered_kernel(uint16_t *__restrict__ y, const uint16_t *__restrict__ mat,
+                                                                  const float *__restrict__ t, const float *__restrict__ scales, BankRows rows,
+                                                                  int N, int rank, int slices, int columns) {
+    __shared__ float ts[64][kBankMaxRank + 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+    const int p0 = blockIdx.y * 64;
+    int row, a;
+    row_at(rows, p0 + lane, row, a);
+    const unsigned long long present = __ballot(a >= 0);
+    if (!present) return;
+    const float scale = a >= 0 ? scales[a] : 0.f;
+    const int end = min(N, (int)(blockIdx.x + 1) * columns);
+    int n0 = blockIdx.x * columns + 64 * wave;
+    int a_of[4];
+    uint16_t *dst[4];
+    u32x4 was[4][2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        a_of[r] = __shfl(a, 16 * r + c);
+        dst[r] = y + (size_t)max(__shfl(row, 16 * r + c), 0) * N + 8 * q;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) was[r][i] = *reinterpret_cast<const u32x4 *>(dst[r] + min(n0, end - 64) + 32 * i);
+    }
+    sum_projected<64>(t, rows, p0, rank, slices, tid, ts);
+    ExpandRow<S> tv[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) tv[r].set(ts[16 * r + c], __shfl(scale, 16 * r + c), a_of[r] >= 0, q, rank);
+    for (; n0 < end; n0 += 256) {
+        f32x4 acc[4][4];
+        bool taken = false;
+        for (unsigned long long left = present; left;) {
+            const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+            const unsigned long long mine = __ballot(a == cur);
+            left &= ~mine;
+            bf16x8 b[4][S];
+            expand_rows<S, 4>(mat + ((size_t)cur * N + n0) * rank, c, q, rank, b);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!taken)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        take_columns(was[r][i], acc[r][2 * i], acc[r][2 * i + 1]);
+                        was[r][i] = *reinterpret_cast<const u32x4 *>(dst[r] + min(n0 + 256, end - 64) + 32 * i);
+                    }
+            taken = true;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (mine >> (16 * r) & 0xFFFFu) expand_product<S, 4>(b, tv[r], a_of[r] == cur, acc[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (a_of[r] >= 0)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(dst[r] + n0 + 32 * i) = give_columns(acc[r][2 * i], acc[r][2 * i + 1]);
     }
 }
 
-int tiles_of(int rows) { return (rows + kBankRowTile - 1) / kBankRowTile; }
+int tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
+
+// Rows in order and a long contraction: 32 positions to a block, which the adapters' matrices are read for once, and eight slices (2048
+// rows of K 18432 and rank 32: 33 us, 37 with 64 positions).  A short one has too few such blocks: 16 positions, eight wavefronts and
+// slices of 1536 at most (K 2560, by itself: 6.9 us with 32 positions and five slices, 6.2).
+constexpr int kLongContraction = 8192;
+bool long_ordered(int rows, int K) { return rows >= kBankOrderedFrom && K >= kLongContraction; }
+
+template <int JT, int RT, int W>
+void launch_project(const uint16_t *s, const uint16_t *m, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream) {
+    const int groups = K / 128, steps = (groups + slices - 1) / slices, tiles = tiles_of(r.rows, 16 * RT);
+    // the adapters that a tile may hold side by side: as many as it has rows, but where they are together few tiles have more than one
+    int turns = r.order ? 1 + r.count / tiles : 16;
+    if (turns > 16) turns = 16;
+    if (turns > r.count) turns = r.count;
+    bank_project_kernel<JT, RT, W><<<dim3(slices, tiles, turns), W * 64, 0, stream>>>(s, m, r, t, K, steps, rank);
+}
 
 }  // namespace
 
@@ -208,38 +390,66 @@ BankRows bank_order(const int *of, int rows, int count, bool always, void *at, h
     if (rows < kBankOrderedFrom && !always) return r;
     int *order = reinterpret_cast<int *>(at);
     int *first = reinterpret_cast<int *>(reinterpret_cast<char *>(at) + bank_up256((size_t)rows * 4));
-    bank_order_kernel<<<(count + 4) / 4, 256, 0, stream>>>(of, order, first, rows, count);
+    bank_order_kernel<<<count + 1, kOrderWaves * 64, 0, stream>>>(of, order, first, rows, count);
     r.order = order;
     r.first = first;
     return r;
 }
 
-// slices * rows <= this, and it does not fall with `rows`
-size_t bank_projected_rows(int rows, int K) {
-    const size_t tiles = tiles_of(rows), most = K / 128 < kBankMaxSlices ? K / 128 : kBankMaxSlices;
-    return kBankRowTile * (tiles * most < tiles + 511 ? tiles * most : tiles + 511);
-}
-
+// Slices are 512 of K at least: two pieces to a wavefront, whose loads are in flight together; shorter ones leave whoever sums them more
+// to read (16 rows of K 2560: 20 slices instead of 5 cost the next launch 20 KB a block).
 int bank_slices(int rows, int K) {
-    const int groups = K / 128, want = (511 + tiles_of(rows)) / tiles_of(rows);
-    int slices = want < kBankMaxSlices ? want : kBankMaxSlices;
-    if (slices > groups) slices = groups;
+    const int groups = K / 128;
+    int slices;
+    if (rows < kBankOrderedFrom) slices = (groups + 3) / 4 < kBankMaxSlices ? (groups + 3) / 4 : kBankMaxSlices;
+    else slices = long_ordered(rows, K) ? 8 : (groups + 11) / 12;
     const int steps = (groups + slices - 1) / slices;
     return (groups + steps - 1) / steps;
 }
 
+// slices * rows <= this, and it does not fall with `rows`
+size_t bank_projected_rows(int rows, int K) {
+    const size_t below = (size_t)(rows < kBankOrderedFrom ? rows : kBankOrderedFrom) * bank_slices(1, K);
+    const size_t here = (size_t)rows * bank_slices(rows, K);
+    return here > below ? here : below;
+}
+
 void bank_project(const void *src, const void *mat, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream) {
-    const int groups = K / 128, steps = (groups + slices - 1) / slices;
-    const int turns = r.count < (r.order ? 4 : 16) ? r.count : (r.order ? 4 : 16);
-    const dim3 grid(tiles_of(r.rows), slices, turns);
     const uint16_t *s = (const uint16_t *)src, *m = (const uint16_t *)mat;
-    switch ((rank + 15) / 16) {
-        case 1: bank_project_kernel<1><<<grid, 256, 0, stream>>>(s, m, r, t, K, steps, rank); break;
-        case 2: bank_project_kernel<2><<<grid, 256, 0, stream>>>(s, m, r, t, K, steps, rank); break;
-        case 3: bank_project_kernel<3><<<grid, 256, 0, stream>>>(s, m, r, t, K, steps, rank); break;
-        default: bank_project_kernel<4><<<grid, 256, 0, stream>>>(s, m, r, t, K, steps, rank); break;
+    const int jt = (rank + 15) / 16;
+    if (!r.order || r.rows < kBankOrderedFrom) {
+        if (jt == 1) launch_project<1, 1, 4>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 2) launch_project<2, 1, 4>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 3) launch_project<3, 1, 4>(s, m, r, t, K, rank, slices, stream);
+        else launch_project<4, 1, 4>(s, m, r, t, K, rank, slices, stream);
+    } else if (long_ordered(r.rows, K)) {
+        if (jt == 1) launch_project<1, 2, 4>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 2) launch_project<2, 2, 4>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 3) launch_project<3, 2, 4>(s, m, r, t, K, rank, slices, stream);
+        else launch_project<4, 2, 4>(s, m, r, t, K, rank, slices, stream);
+    } else {
+        if (jt == 1) launch_project<1, 1, 8>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 2) launch_project<2, 1, 8>(s, m, r, t, K, rank, slices, stream);
+        else if (jt == 3) launch_project<3, 1, 8>(s, m, r, t, K, rank, slices, stream);
+        else launch_project<4, 1, 8>(s, m, r, t, K, rank, slices, stream);
     }
 }
+
+namespace {
+
+template <int S>
+void launch_expand(uint16_t *y, const uint16_t *m, const float *t, const float *scales, const BankRows &r, int N, int rank, int slices, hipStream_t stream) {
+    if (!r.order) {
+        bank_expand_kernel<S><<<dim3(N / 64, tiles_of(r.rows, 16)), 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices);
+        return;
+    }
+    const int tiles = tiles_of(r.rows, 64);
+    int columns = 1024;  // (2048 rows of 18432 columns: 256 60 us, 512 49, 1024 45, 2048 50)
+    while (columns > 256 && tiles * ((N + columns - 1) / columns) < 512) columns /= 2;
+    bank_expand_ordered_kernel<S><<<dim3((N + columns - 1) / columns, tiles), 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices, columns);
+}
+
+}  // namespace
 
 }  // namespace kiln
 
@@ -273,15 +483,10 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
     const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
     bank_project(A, bank->lora_a, rows, t, prob_k, rank, slices, hs);
-    const dim3 grid(prob_n / 256, tiles_of(prob_m));
     uint16_t *y = (uint16_t *)C;
     const uint16_t *m = (const uint16_t *)bank->lora_b;
-    switch ((2 * (rank / 8) + 3) / 4) {
-        case 1: bank_expand_kernel<1><<<grid, 256, 0, hs>>>(y, m, t, bank->scales, rows, prob_n, rank, slices); break;
-        case 2: bank_expand_kernel<2><<<grid, 256, 0, hs>>>(y, m, t, bank->scales, rows, prob_n, rank, slices); break;
-        case 3: bank_expand_kernel<3><<<grid, 256, 0, hs>>>(y, m, t, bank->scales, rows, prob_n, rank, slices); break;
-        default: bank_expand_kernel<4><<<grid, 256, 0, hs>>>(y, m, t, bank->scales, rows, prob_n, rank, slices); break;
-    }
+    if (rank <= 32) launch_expand<1>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);
+    else launch_expand<2>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
 
