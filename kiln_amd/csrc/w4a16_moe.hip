@@ -1,9 +1,9 @@
 // The experts of a mixture-of-experts MLP for a few tokens, and the router's choice of them.
 //
-// Two launches over the packs of the experts that have rows, which is what the call has to read (a token of 8 experts of 64 reads an
-// eighth of the layer): gate, up and silu(gate) * up of every (token, expert) pair, then the down projection with the sum over a token's
-// experts.  A block works out by itself which experts are present and which pairs are theirs: the ids of a run, 64 tokens at most, are a
-// few KB, and a launch in front that sorts them costs more than reading them in every block.
+// Bound by the packs of the experts that have rows, read once (a token of 8 experts of 64 reads an eighth of the layer).  Three launches:
+// gate, up and silu(gate) * up of every (token, expert) pair, the down projection of every pair, and the sum over a token's pairs.  A
+// block works out by itself which experts are present and which pairs are theirs: the ids of a run, 64 tokens at most, are a few KB,
+// and a launch in front that sorts them costs more than reading them in every block.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,41 +25,44 @@ struct MoeArgs {
     const u32x4 *b_in, *b_out;  // packs, one expert after the other
     const uint16_t *s_in, *s_out;
     uint16_t *h;                // bf16 [pairs, n_out]
+    float *down;                // f32 [pairs, n_down]
     uint16_t *y;                // bf16 [tokens, n_down]
     int tokens, top, experts, hidden, n_out, n_down, per_column;
 };
 
-// The pairs of a run in LDS: ids (-1: none; also for a pair whose expert its token names earlier: that pair's weight goes to the earlier
-// one) and which experts are present.
+// Which experts are present among a run's pairs, and which pairs are theirs.  A wavefront looks at the pairs of as many whole tokens as
+// fit its lanes at a time, ids in registers (FEW: all of them fit) or LDS.
 struct MoePairs {
-    int id[kMoeMaxPairs];
-    float weight[kMoeMaxPairs];
+    int id[kMoeMaxPairs];  // -1: none
     unsigned present[kMoeMaxExperts / 32];
 };
 
+__device__ __forceinline__ int id_of(const MoeArgs &p, int pair, int pairs) {
+    const int e = pair < pairs ? p.expert_of[pair] : -1;
+    return (unsigned)e < (unsigned)p.experts ? e : -1;
+}
+// the expert in place `slot` in the order in which they are met (-1: there are fewer)
+__device__ __forceinline__ int expert_in_lanes(int id, int slot) {
+    for (unsigned long long left = __ballot(id >= 0); left; --slot) {
+        const int e = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        if (slot == 0) return e;
+        left &= ~__ballot(id == e);
+    }
+    return -1;
+}
 __device__ __forceinline__ void read_pairs(const MoeArgs &p, MoePairs &lds, int tid, int threads) {
     for (int i = tid; i < kMoeMaxExperts / 32; i += threads) lds.present[i] = 0u;
     __syncthreads();
     const int pairs = p.tokens * p.top;
     for (int i = tid; i < pairs; i += threads) {
-        int e = p.expert_of[i];
-        float w = p.weights[i];
-        const int first = i - i % p.top;
-        if ((unsigned)e >= (unsigned)p.experts) e = -1;
-        for (int j = first; j < first + p.top; ++j)
-            if (j != i && e >= 0 && p.expert_of[j] == e) {
-                if (j < i) e = -1;
-                else w += p.weights[j];
-            }
+        const int e = id_of(p, i, pairs);
         lds.id[i] = e;
-        lds.weight[i] = w;
         if (e >= 0) atomicOr(&lds.present[e >> 5], 1u << (e & 31));
     }
     __syncthreads();
 }
-
-// How many experts are present, and the one in place `slot` among them (-1: there are fewer).  Every lane gets both.
-__device__ __forceinline__ int expert_in_slot(const MoePairs &lds, int slot, int lane, int *count) {
+// ... and out of LDS, in the order of their ids
+__device__ __forceinline__ int expert_in_lds(const MoePairs &lds, int slot, int lane) {
     const unsigned word = lane < kMoeMaxExperts / 32 ? lds.present[lane] : 0u;
     int upto = __popc(word);
 #pragma unroll
@@ -67,143 +70,189 @@ __device__ __forceinline__ int expert_in_slot(const MoePairs &lds, int slot, int
         const int below = __shfl_up(upto, d);
         if (lane >= d) upto += below;
     }
-    *count = __builtin_amdgcn_readlane(upto, 31);
-    if (slot >= *count) return -1;
+    if (slot >= __builtin_amdgcn_readlane(upto, 31)) return -1;
     const int at = __builtin_ctzll(__ballot(lane < 32 && upto > slot));
     unsigned w = __builtin_amdgcn_readlane(word, at);
     for (int skip = slot - (__builtin_amdgcn_readlane(upto, at) - __popc(w)); skip > 0; --skip) w &= w - 1;
     return at * 32 + __builtin_ctz(w);
 }
-
-// The pairs of expert e in their order, into a list of this wavefront's own (64: a token is there at most once).  Returns their count.
-__device__ __forceinline__ int pairs_of(const MoePairs &lds, int pairs, int e, int lane, int *list) {
+// The pairs of expert e in their order, into a list of this wavefront's own; of a token that names e more than once the first, so 64 at
+// most.  Returns their count.
+__device__ __forceinline__ int pairs_of(const MoeArgs &p, const MoePairs *lds, int id_in_lane, int e, int lane, int *list) {
+    const int pairs = p.tokens * p.top, step = 64 / p.top * p.top;
+    const int before = lane - lane % p.top;                                        // the first of this lane's token
+    const unsigned long long earlier = ((1ull << lane) - 1) & ~((1ull << before) - 1);  // ... and those between it and this lane
     int count = 0;
-    for (int p0 = 0; p0 < pairs; p0 += 64) {
-        const bool mine = p0 + lane < pairs && lds.id[p0 + lane] == e;
-        const unsigned long long all = __ballot(mine);
-        if (mine) list[count + __popcll(all & ((1ull << lane) - 1))] = p0 + lane;
-        count += __popcll(all);
+    for (int p0 = 0; p0 < pairs; p0 += step) {
+        const int pair = p0 + lane, id = lds ? (lane < step && pair < pairs ? lds->id[pair] : -1) : id_in_lane;
+        const bool mine = id == e && (__ballot(id == e) & earlier) == 0;
+        const unsigned long long firsts = __ballot(mine);
+        if (mine) list[count + __popcll(firsts & ((1ull << lane) - 1))] = pair;
+        count += __popcll(firsts);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     return count;
 }
 
-// 16 rows times the chunks of column tiles nt ... nt + CT - 1, groups g0, g0 + stride, ... < G: the f32 sums, scales applied.
-// row: this lane's row of the left operand, 8 * (lane / 16) values in.  The sum of a row over a group, which the zero-point and the
-// bias of the expanded codes are taken off with, comes out of a product with ones.
-template <int CT>
-__device__ __forceinline__ void expert_product(const uint16_t *__restrict__ row, const u32x4 *__restrict__ b, const uint16_t *__restrict__ s, int G,
-                                               int nt, int g0, int stride, bool per_column, int lane, const DequantConsts &dc, f32x4 (&total)[CT]) {
-    const int c = lane & 15;
-    const bf16x8 ones = bf16x8_splat_one();
-    for (int g = g0; g < G; g += stride) {
-        u32x4 w[CT];
-        float scale[CT];
-        bf16x8 x[4];
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-            w[i] = b[((size_t)(nt + i) * G + g) * 64 + lane];
-            scale[i] = f16_bits_to_f32(s[scale_index(per_column ? 0 : g, (nt + i) * kTileN + c, per_column ? 1 : G)]);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = *reinterpret_cast<const bf16x8 *>(row + g * kGroupK + 32 * t);
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t], ones, sum, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], codes_to_bf16x8(w[i].x, dc), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], codes_to_bf16x8(w[i].y, dc), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[2], codes_to_bf16x8(w[i].z, dc), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[3], codes_to_bf16x8(w[i].w, dc), acc, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) total[i][e] += scale[i] * (acc[e] - kCodeBias * sum[e]);
-        }
-    }
-}
-
-// h[pair] = silu(gate) * up: a block takes kInTiles column tiles (8 gate and 8 up columns each) of the expert in slot blockIdx.y, its
-// wavefronts every fourth group; they meet in LDS.
-constexpr int kInTiles = 2;
-__global__ __launch_bounds__(256) void moe_in_kernel(MoeArgs p) {
+// Up to 16 rows of one expert times S column tiles of its pack.  The groups of K are dealt out to W wavefronts, GW to each, whose part of
+// the rows stays in registers while the columns go by: per tile nothing is read but its chunks (GW KB a wavefront, the next tile's asked
+// for before the present one is multiplied) and their scales.  The rows' sums over the groups, which the zero-point and the bias of the
+// expanded codes are taken off with, come out of products with ones, once, and go in as what the products start from.  K beyond W GW
+// groups: in passes, the sums kept.  The wavefronts meet in LDS at the end.
+// With the rows read again for every tile or two (64 tokens, 8 of 64 experts, 2560 -> 1024 -> 2560) the two launches took 54 and 51 us: the
+// wavefronts waited for rows, 4 KB of them to a KB of codes.
+template <bool IN, bool FEW, int W, int GW, int S>
+__global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
     __shared__ MoePairs pairs;
-    __shared__ int lists[4][kMoeRun];
-    __shared__ float part[4][16][kInTiles * 16 + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
+    __shared__ int lists[W][kMoeRun];
+    constexpr int kPitch = S * 16 + 4;
+    __shared__ float part[W][16][kPitch];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
     const DequantConsts dc = dequant_consts();
-    read_pairs(p, pairs, tid, 256);
-    int present;
-    const int e = expert_in_slot(pairs, blockIdx.y, lane, &present);
+    int e, id = -1;
+    if constexpr (FEW) {
+        id = id_of(p, lane, p.tokens * p.top);
+        e = expert_in_lanes(id, blockIdx.y);
+    } else {
+        read_pairs(p, pairs, tid, W * 64);
+        e = expert_in_lds(pairs, blockIdx.y, lane);
+    }
     if (e < 0) return;
     int *list = lists[wave];
-    const int count = pairs_of(pairs, p.tokens * p.top, e, lane, list);
-    const int G = p.hidden / kGroupK, nt = blockIdx.x * kInTiles, N = 2 * p.n_out;
-    const u32x4 *b = p.b_in + (size_t)e * (N / kTileN) * G * 64;
-    const uint16_t *s = p.s_in + (size_t)e * N * (p.per_column ? 1 : G);
+    const int count = pairs_of(p, FEW ? nullptr : &pairs, id, e, lane, list);
+    const int K = IN ? p.hidden : p.n_out, N = IN ? 2 * p.n_out : p.n_down, G = K / kGroupK, Gs = p.per_column ? 1 : G;
+    const int nt0 = blockIdx.x * S;
+    const u32x4 *b = (IN ? p.b_in : p.b_out) + ((size_t)e * (N / kTileN) + nt0) * G * 64 + lane;
+    const uint16_t *s = (IN ? p.s_in : p.s_out) + ((size_t)e * (N / kTileN) + nt0) * Gs * kTileN + c;
+    const bf16x8 ones = bf16x8_splat_one();
     for (int r0 = 0; r0 < count; r0 += 16) {
-        const uint16_t *row = p.x + (size_t)(list[min(r0 + c, count - 1)] / p.top) * p.hidden + 8 * q;
-        f32x4 total[kInTiles] = {};
-        expert_product<kInTiles>(row, b, s, G, nt, wave, 4, p.per_column, lane, dc, total);
+        const int pair = list[min(r0 + c, count - 1)];
+        const uint16_t *row = (IN ? p.x + (size_t)(pair / p.top) * K : p.h + (size_t)pair * K) + 8 * q;
+        f32x4 total[S];
 #pragma unroll
-        for (int i = 0; i < kInTiles; ++i)
+        for (int i = 0; i < S; ++i) total[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int first = wave * GW; first < G; first += W * GW) {
+            // groups past the last: the last again, with a scale of zero
+            auto group = [&](int u) { return min(first + u, G - 1); };
+            u32x4 w[2][GW];
+            uint16_t scale[2][GW];
+            auto fetch = [&](int tile) {
+#pragma unroll
+                for (int u = 0; u < GW; ++u) {
+                    w[tile & 1][u] = b[(size_t)(tile * G + group(u)) * 64];
+                    scale[tile & 1][u] = s[(size_t)(tile * Gs + (p.per_column ? 0 : group(u))) * kTileN];
+                }
+            };
+            fetch(0);
+            bf16x8 x[GW][4];
+            f32x4 start[GW];
+#pragma unroll
+            for (int u = 0; u < GW; ++u)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) x[u][t] = *reinterpret_cast<const bf16x8 *>(row + group(u) * kGroupK + 32 * t);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < GW; ++u) {
+                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][t], ones, sum, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) start[u][i] = -kCodeBias * sum[i];
+            }
+#pragma unroll
+            for (int tile = 0; tile < S; ++tile) {
+                if (tile + 1 < S) fetch(tile + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < GW; ++u) {
+                    const u32x4 &v = w[tile & 1][u];
+                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][0], codes_to_bf16x8(v.x, dc), start[u], 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][1], codes_to_bf16x8(v.y, dc), acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][2], codes_to_bf16x8(v.z, dc), acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][3], codes_to_bf16x8(v.w, dc), acc, 0, 0, 0);
+                    const float sc = first + u < G ? f16_bits_to_f32(scale[tile & 1][u]) : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) total[tile][i] += sc * acc[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) part[wave][4 * q + r][16 * i + c] = total[i][r];
         __syncthreads();
-        const int r = tid >> 4, col = (tid & 15) + (tid & 8);  // 8 gate columns of the first tile, 8 of the second
-        if (r0 + r < count) {
-            const float gate = (part[0][r][col] + part[1][r][col]) + (part[2][r][col] + part[3][r][col]);
-            const float up = (part[0][r][col + 8] + part[1][r][col + 8]) + (part[2][r][col + 8] + part[3][r][col + 8]);
-            p.h[(size_t)list[r0 + r] * p.n_out + nt * 8 + (tid & 15)] = f32_to_bf16_bits(gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up);
+        auto sum_of = [&](int r, int col) {
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) v += part[i][r][col];
+            return v;
+        };
+        const int rows = min(16, count - r0);
+        if constexpr (IN) {  // 8 gate columns of a tile, then the 8 matching up columns
+            for (int i = tid; i < rows * S * 8; i += W * 64) {
+                const int r = i / (S * 8), j = i % (S * 8), col = 16 * (j >> 3) + (j & 7);
+                const float gate = sum_of(r, col), up = sum_of(r, col + 8);
+                p.h[(size_t)list[r0 + r] * p.n_out + nt0 * 8 + j] = f32_to_bf16_bits(gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up);
+            }
+        } else {
+            for (int i = tid; i < rows * S * 16; i += W * 64) {
+                const int r = i / (S * 16), col = i % (S * 16);
+                p.down[(size_t)list[r0 + r] * N + nt0 * 16 + col] = sum_of(r, col);
+            }
         }
         __syncthreads();
     }
 }
 
-// y[token] = sum over its experts: a block takes one column tile for all tokens; its wavefronts share out the present experts (and, where
-// those are fewer than wavefronts, parts of their groups), each with an f32 sum per token and column in LDS, added up at the end in the
-// wavefronts' order.
-constexpr int kOutWaves = 8;
-__global__ __launch_bounds__(kOutWaves * 64) void moe_out_kernel(MoeArgs p) {
-    __shared__ MoePairs pairs;
-    __shared__ int lists[kOutWaves][kMoeRun];
-    __shared__ float sums[kOutWaves][kMoeRun][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const DequantConsts dc = dequant_consts();
-    for (int i = lane; i < p.tokens * 16; i += 64) sums[wave][i >> 4][i & 15] = 0.f;
-    read_pairs(p, pairs, tid, kOutWaves * 64);
-    int present;
-    expert_in_slot(pairs, 0, lane, &present);
-    const int G = p.n_out / kGroupK, nt = blockIdx.x, N = p.n_down;
-    if (present) {
-        const int parts = min(G, (kOutWaves + present - 1) / present);
-        int *list = lists[wave];
-        for (int unit = wave; unit < present * parts; unit += kOutWaves) {
-            int again;
-            const int slot = unit / parts, e = expert_in_slot(pairs, slot, lane, &again);
-            const int count = pairs_of(pairs, p.tokens * p.top, e, lane, list);
-            const u32x4 *b = p.b_out + (size_t)e * (N / kTileN) * G * 64;
-            const uint16_t *s = p.s_out + (size_t)e * N * (p.per_column ? 1 : G);
-            for (int r0 = 0; r0 < count; r0 += 16) {
-                const uint16_t *row = p.h + (size_t)list[min(r0 + c, count - 1)] * p.n_out + 8 * q;
-                f32x4 total[1] = {};
-                expert_product<1>(row, b, s, G, nt, unit - slot * parts, parts, p.per_column, lane, dc, total);
+// y[token] = sum of its pairs' rows times their weights, in the pairs' order, rounded once; four columns to a thread.  Bound by its
+// start and two loads' latency: the rows of eight pairs are asked for together.
+__global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs p) {
+    const int lane = threadIdx.x & 63, col = (blockIdx.x * 256 + threadIdx.x) * 4, token = blockIdx.y;
+    const int e = lane < p.top ? p.expert_of[(size_t)token * p.top + lane] : -1;
+    const float weight = lane < p.top ? p.weights[(size_t)token * p.top + lane] : 0.f;
+    const unsigned long long here = __ballot((unsigned)e < (unsigned)p.experts);
+    const float *down = p.down + (size_t)token * p.top * p.n_down + min(col, p.n_down - 4);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < p.top; j0 += 8) {
+        f32x4 d[8];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = r0 + 4 * q + r;
-                    if (at < count) sums[wave][list[at] / p.top][c] += pairs.weight[list[at]] * total[0][r];
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int u = 0; u < 8; ++u) {  // where an expert is named twice its row is with the first
+            const int at = __builtin_ctzll(__ballot(e == __builtin_amdgcn_readlane(e, j0 + u)));
+            if (here >> (j0 + u) & 1) d[u] = *reinterpret_cast<const f32x4 *>(down + (size_t)at * p.n_down);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j0 + u));
+            if (here >> (j0 + u) & 1)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += w * d[u][i];
         }
     }
-    __syncthreads();
-    for (int i = tid; i < p.tokens * 16; i += kOutWaves * 64) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kOutWaves; ++w) v += sums[w][i >> 4][i & 15];
-        p.y[(size_t)(i >> 4) * N + nt * 16 + (i & 15)] = f32_to_bf16_bits(v);
-    }
+    if (col >= p.n_down) return;
+    u32x2 o;
+    o.x = f32_to_bf16_bits(v[0]) | (uint32_t)f32_to_bf16_bits(v[1]) << 16;
+    o.y = f32_to_bf16_bits(v[2]) | (uint32_t)f32_to_bf16_bits(v[3]) << 16;
+    *reinterpret_cast<u32x2 *>(p.y + (size_t)token * p.n_down + col) = o;
+}
+
+// Column tiles to a block: many where the blocks are enough all the same (their rows and lists are read once each), two where the experts
+// present are few.  Wavefronts and groups by K: five groups to a wavefront at most.
+template <bool IN, bool FEW, int W, int GW>
+void launch_expert(const MoeArgs &a, int slots, hipStream_t stream) {
+    constexpr int kMany = W == 4 ? 8 : 4;
+    const int tiles = (IN ? 2 * a.n_out : a.n_down) / kTileN;
+    if (slots * (tiles / kMany) >= 512) moe_expert_kernel<IN, FEW, W, GW, kMany><<<dim3(tiles / kMany, slots), W * 64, 0, stream>>>(a);
+    else moe_expert_kernel<IN, FEW, W, GW, 2><<<dim3(tiles / 2, slots), W * 64, 0, stream>>>(a);
+}
+template <bool IN, bool FEW>
+void launch_experts(const MoeArgs &a, int slots, hipStream_t stream) {
+    const int G = (IN ? a.hidden : a.n_out) / kGroupK;
+    if (G <= 8) launch_expert<IN, FEW, 4, 2>(a, slots, stream);
+    else if (G <= 12) launch_expert<IN, FEW, 4, 3>(a, slots, stream);
+    else if (G <= 16) launch_expert<IN, FEW, 4, 4>(a, slots, stream);
+    else if (G <= 20) launch_expert<IN, FEW, 4, 5>(a, slots, stream);
+    else if (G <= 32) launch_expert<IN, FEW, 8, 4>(a, slots, stream);
+    else launch_expert<IN, FEW, 8, 5>(a, slots, stream);
 }
 
 // ---- the router's choice -------------------------------------------------------------------------------------------
@@ -296,10 +345,13 @@ using namespace kiln;
 
 extern "C" {
 
+static size_t moe_h_bytes(int m, int top_k, int n_out) {
+    return ((size_t)(m < kMoeRun ? m : kMoeRun) * top_k * n_out * 2 + 255) & ~(size_t)255;
+}
+
 size_t kiln_w4a16_moe_scratch_bytes(int prob_m, int top_k, int n_out, int n_down) {
-    (void)n_down;
-    if (prob_m < 1 || top_k < 1 || n_out < 1) return 256;
-    return (size_t)(prob_m < kMoeRun ? prob_m : kMoeRun) * top_k * n_out * 2;
+    if (prob_m < 1 || top_k < 1 || n_out < 1 || n_down < 1) return 256;
+    return moe_h_bytes(prob_m, top_k, n_out) + (size_t)(prob_m < kMoeRun ? prob_m : kMoeRun) * top_k * n_down * 4;
 }
 
 kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const float *weights, const void *b_gate_up, const void *s_gate_up,
@@ -317,12 +369,19 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     for (int m0 = 0; m0 < prob_m; m0 += kMoeRun) {
         const int m = prob_m - m0 < kMoeRun ? prob_m - m0 : kMoeRun;
-        MoeArgs a{(const uint16_t *)x + (size_t)m0 * hidden, expert_of + (size_t)m0 * top_k, weights + (size_t)m0 * top_k,
-                  (const u32x4 *)b_gate_up, (const u32x4 *)b_down, (const uint16_t *)s_gate_up, (const uint16_t *)s_down,
-                  (uint16_t *)scratch, (uint16_t *)y + (size_t)m0 * n_down, m, top_k, experts, hidden, n_out, n_down, groupsize == -1};
+        const MoeArgs a{(const uint16_t *)x + (size_t)m0 * hidden, expert_of + (size_t)m0 * top_k, weights + (size_t)m0 * top_k,
+                        (const u32x4 *)b_gate_up, (const u32x4 *)b_down, (const uint16_t *)s_gate_up, (const uint16_t *)s_down,
+                        (uint16_t *)scratch, reinterpret_cast<float *>(static_cast<char *>(scratch) + moe_h_bytes(prob_m, top_k, n_out)),
+                        (uint16_t *)y + (size_t)m0 * n_down, m, top_k, experts, hidden, n_out, n_down, groupsize == -1};
         const int slots = m * top_k < experts ? m * top_k : experts;
-        moe_in_kernel<<<dim3(2 * n_out / (16 * kInTiles), slots), 256, 0, hs>>>(a);
-        moe_out_kernel<<<n_down / 16, kOutWaves * 64, 0, hs>>>(a);
+        if (m <= 64 / top_k) {  // whole tokens in a wavefront's lanes
+            launch_experts<true, true>(a, slots, hs);
+            launch_experts<false, true>(a, slots, hs);
+        } else {
+            launch_experts<true, false>(a, slots, hs);
+            launch_experts<false, false>(a, slots, hs);
+        }
+        moe_sum_kernel<<<dim3((n_down / 4 + 255) / 256, m), 256, 0, hs>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
