@@ -222,9 +222,12 @@ __global__ __launch_bounds__(256) void sum_dx_kernel(const f32x4 *__restrict__ p
 }
 
 // ---- dA and dB -------------------------------------------------------------------------------------------------
-// out = s_a sum over the rows of adapter a of f[position][rank]^T src[row][columns], f = U with src = x (dA) or T with src = dy (dB).  The f32
-// matrix instruction takes one value per lane of either operand, four rows at a time: a lane's eight columns of a row are its operands of
-// eight products, so nothing is turned, and T and U stay f32.  A block takes 128 columns, its four wavefronts every fourth four rows.
+// out = s_a sum over the rows of adapter a of f[position][rank]^T src[row][columns], f = U with src = x (dA) or T with src = dy (dB).
+// Bound by src, read once: a block takes 128 columns, its W wavefronts every W-th 32 rows.  The contraction runs over the rows, of which
+// an operand of the matrix instruction wants eight to a lane: a lane reads eight columns of each of its eight rows and pairs the rows'
+// values column by column (v_perm), so that nothing goes through LDS; its eight columns are eight products.  T and U go in as two bf16
+// parts, within 2^-17 of their f32 values.  (With the f32 matrix instruction, which needs no pairing, the products took as long as the reads:
+// 2048 rows, 20992 columns, rank 32: 62 us.)
 struct GradArgs {
     const uint16_t *x, *dy;
     const float *t, *u, *scales;
@@ -233,33 +236,9 @@ struct GradArgs {
     int K, N, rank;
 };
 
-template <int JT, int U>
-__device__ __forceinline__ void grad_steps(const uint16_t *__restrict__ src, const float *__restrict__ f, const BankRows &rows, int p, int end, int stride,
-                                           int len, int rank, int c, f32x4 (&acc)[8][JT]) {
-    u32x4 v[U];
-    float w[U][JT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int at = p + u * stride;
-        const bool in = at < end;
-        v[u] = in ? *reinterpret_cast<const u32x4 *>(src + (size_t)rows.order[at] * len) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int j = 0; j < JT; ++j) w[u][j] = in && 16 * j + c < rank ? f[(size_t)at * rank + 16 * j + c] : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t pair = v[u][e >> 1];
-            const float b = __builtin_bit_cast(float, e & 1 ? pair & 0xFFFF0000u : pair << 16);
-#pragma unroll
-            for (int j = 0; j < JT; ++j) acc[e][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][j], b, acc[e][j], 0, 0, 0);
-        }
-}
-
 constexpr int kGradPitch = 128 + 4;
-template <int JT>
-__global__ __launch_bounds__(256) void bank_grad_kernel(GradArgs p) {
+template <int JT, int W>
+__global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     __shared__ float sum[JT * 16 * kGradPitch];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
     const int a = blockIdx.y;
@@ -268,13 +247,56 @@ __global__ __launch_bounds__(256) void bank_grad_kernel(GradArgs p) {
     const uint16_t *src = (is_b ? p.dy : p.x) + c0 + 8 * c;
     const float *f = is_b ? p.t : p.u;
     const int begin = p.rows.first[a], end = p.rows.first[a + 1];
+    int col[JT];  // past the rank: the last again, dropped at the end
+#pragma unroll
+    for (int j = 0; j < JT; ++j) col[j] = min(16 * j + c, p.rank - 1);
     f32x4 acc[8][JT];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
         for (int j = 0; j < JT; ++j) acc[e][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int at = begin + 4 * wave; at < end; at += 64) grad_steps<JT, 4>(src, f, p.rows, at + q, end, 16, len, p.rank, c, acc);
-    for (int w = 0; w < 4; ++w) {  // the wavefronts' sums one after the other: the same order always
+    int row[8];
+    auto rows_at = [&](int at) {  // positions past the last: the last again, times zeros
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[i] = p.rows.order[min(at + 8 * q + i, end - 1)];
+    };
+    int at = begin + 32 * wave;
+    if (at < end) rows_at(at);
+    for (; at < end; at += 32 * W) {
+        u32x4 v[8];
+        float w[JT][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const u32x4 *>(src + (size_t)row[i] * len);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < JT; ++j) w[j][i] = f[(size_t)min(at + 8 * q + i, end - 1) * p.rank + col[j]];
+        rows_at(at + 32 * W);
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 hi[JT], lo[JT];
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = at + 8 * q + i < end ? w[j][i] : 0.f;
+                hi[j][i] = (__bf16)x;
+                lo[j][i] = (__bf16)(x - (float)hi[j][i]);
+            }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            u32x4 pairs;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                pairs[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+            const bf16x8 b = __builtin_bit_cast(bf16x8, pairs);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+                acc[e][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi[j], b, acc[e][j], 0, 0, 0);
+                acc[e][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo[j], b, acc[e][j], 0, 0, 0);
+            }
+        }
+    }
+    for (int w = 0; w < W; ++w) {  // the wavefronts' sums one after the other: the same order always
         if (wave == w)
 #pragma unroll
             for (int j = 0; j < JT; ++j)
@@ -288,7 +310,7 @@ __global__ __launch_bounds__(256) void bank_grad_kernel(GradArgs p) {
     }
     const float scale = p.scales[a];
     uint16_t *out = is_b ? p.db + ((size_t)a * p.N + c0) * p.rank : p.da + (size_t)a * p.rank * p.K + c0;
-    for (int e = tid; e < p.rank * 16; e += 256) {  // eight results each
+    for (int e = tid; e < p.rank * 16; e += W * 64) {  // eight results each
         const int r = is_b ? e % (p.rank / 8) : e >> 4, col = is_b ? e / (p.rank / 8) : e & 15;
         u32x4 o;
 #pragma unroll
@@ -299,6 +321,13 @@ __global__ __launch_bounds__(256) void bank_grad_kernel(GradArgs p) {
         }
         *reinterpret_cast<u32x4 *>(is_b ? out + (size_t)col * p.rank + 8 * r : out + (size_t)r * p.K + 8 * col) = o;
     }
+}
+
+template <int JT>
+void launch_grad(const GradArgs &g, hipStream_t stream) {
+    const dim3 grid(g.N / 128 + g.K / 128, g.rows.count);
+    if (grid.x * grid.y >= 512) bank_grad_kernel<JT, 4><<<grid, 256, 0, stream>>>(g);
+    else bank_grad_kernel<JT, 8><<<grid, 512, 0, stream>>>(g);
 }
 
 // ---- the plan ----------------------------------------------------------------------------------------------------
@@ -393,12 +422,11 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
                 sum_slices_kernel<<<dim3((unsigned)(((size_t)m * rank + 255) / 256), 2), 256, 0, hs>>>(t, w.t_slices, u, w.u_slices, (size_t)m * rank);
         }
         GradArgs g{(const uint16_t *)A, (const uint16_t *)dC, t, u, bank->scales, (uint16_t *)d_lora_a, (uint16_t *)d_lora_b, dx.rows, k, n, rank};
-        const dim3 grid(n / 128 + k / 128, count);
         switch ((rank + 15) / 16) {
-            case 1: bank_grad_kernel<1><<<grid, 256, 0, hs>>>(g); break;
-            case 2: bank_grad_kernel<2><<<grid, 256, 0, hs>>>(g); break;
-            case 3: bank_grad_kernel<3><<<grid, 256, 0, hs>>>(g); break;
-            default: bank_grad_kernel<4><<<grid, 256, 0, hs>>>(g); break;
+            case 1: launch_grad<1>(g, hs); break;
+            case 2: launch_grad<2>(g, hs); break;
+            case 3: launch_grad<3>(g, hs); break;
+            default: launch_grad<4>(g, hs); break;
         }
         dx.at = a_t;
         dx.u = u;
