@@ -45,16 +45,27 @@ __global__ __launch_bounds__(512) void dequant_rows_kernel(const u32x4 *__restri
 }
 
 // ---- the adapters' matrices turned -------------------------------------------------------------------------------
-// z = 0: at[a][k][rank] of a[a][rank][k]; z = 1: bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block
+// z = 0: at[a][k][rank] of a[a][rank][k]; z = 1: bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows
+// of several adapters at once, zeros for those of others, so it holds finite values alone; where A holds others, odd[a][k / 64] is set and
+// bank_grad_kernel adds their products for the rows of that adapter.
 __global__ __launch_bounds__(256) void turn_bank_kernel(const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, uint16_t *__restrict__ at,
-                                                        uint16_t *__restrict__ bt, int K, int N, int rank) {
+                                                        uint16_t *__restrict__ bt, uint8_t *__restrict__ odd, int K, int N, int rank) {
     __shared__ uint16_t tile[64][kBankMaxRank + 2];
     const int tid = threadIdx.x, which = blockIdx.z, len = which ? N : K, l0 = blockIdx.x * 64;
     if (l0 >= len) return;
     const size_t base = (size_t)blockIdx.y * rank * len;
     if (which == 0) {
-        for (int e = tid; e < rank * 64; e += 256) tile[e & 63][e >> 6] = a[base + (size_t)(e >> 6) * len + l0 + (e & 63)];
-        __syncthreads();
+        bool any = false;
+        for (int e = tid; e < rank * 64; e += 256) {
+            uint16_t v = a[base + (size_t)(e >> 6) * len + l0 + (e & 63)];
+            if ((v & 0x7F80u) == 0x7F80u) {
+                any = true;
+                v = 0;
+            }
+            tile[e & 63][e >> 6] = v;
+        }
+        any = __syncthreads_or(any);
+        if (tid == 0) odd[(size_t)blockIdx.y * (K / 64) + blockIdx.x] = any;
         for (int e = tid; e < 64 * rank; e += 256) at[base + (size_t)l0 * rank + e] = tile[e / rank][e % rank];
     } else {
         for (int e = tid; e < 64 * rank; e += 256) tile[e / rank][e % rank] = b[base + (size_t)l0 * rank + e];
@@ -75,64 +86,55 @@ __global__ __launch_bounds__(256) void sum_slices_kernel(float *__restrict__ t, 
 }
 
 // ---- dx --------------------------------------------------------------------------------------------------------
-// dx[row][k] = sum_n dy[row][n] W[k][n] (+ s U A), both operands with the contraction contiguous.  A block of four wavefronts takes
-// 64 TM rows x 64 TN of k, 64 of the contraction at a time: both tiles go straight to LDS, one in flight while the other is
-// multiplied.  A row of a tile is eight 16-byte units, unit u at place u ^ (row & 7), so that the eight lanes that LDS serves
-// together find their units in different banks.
+// dx[row][k] = sum_n dy[row][n] W[k][n] (+ s U A), both operands with the contraction contiguous.  A block of WM x WN wavefronts takes
+// 32 TM WM rows x 32 TN WN of k, 32 of the contraction at a time: both tiles go straight to LDS, kStages - 1 of them in flight while one is
+// multiplied.  A row of a tile is four 16-byte units, unit u at place u ^ (row / 2 & 3), so that the eight lanes that LDS serves together
+// find their units in different banks.
+constexpr int kStages = 4;
 struct DxArgs {
     const uint16_t *dy, *wt, *at;   // [rows, N], [K, N], [count, K, rank]
     const float *u, *scales;        // [rows by position, rank], or null without a bank
     uint16_t *dx;
     float *partial;                 // [slices, rows, K], or null with one slice
     BankRows rows;
-    int K, N, rank, steps;          // steps of 64 of the contraction to a slice
+    int K, N, rank, steps;          // steps of 32 of the contraction to a slice
+    int m_tiles, k_tiles;
 };
 
-__device__ __forceinline__ unsigned unit_at(int row, int unit) { return (unsigned)(row * 8 + (unit ^ (row & 7))) * 16; }
+__device__ __forceinline__ unsigned unit_at(int row, int unit) { return (unsigned)(row * 4 + (unit ^ (row >> 1 & 3))) * 16; }
 
-template <int TM, int TN>
-__device__ __forceinline__ void dx_product(const char *lds, int wm, int wn, int lane, f32x16 (&acc)[TN][TM]) {
-    constexpr int BM = 64 * TM;
-    const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-        bf16x8 x[TM], w[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) x[i] = *reinterpret_cast<const bf16x8 *>(lds + unit_at(32 * (TM * wm + i) + r, 2 * kk + h));
-#pragma unroll
-        for (int j = 0; j < TN; ++j) w[j] = *reinterpret_cast<const bf16x8 *>(lds + BM * 128 + unit_at(32 * (TN * wn + j) + r, 2 * kk + h));
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
-    }
-}
-
-template <int TM, int TN>
-__global__ __launch_bounds__(256) void bank_dx_kernel(DxArgs p) {
-    constexpr int BM = 64 * TM, BN = 64 * TN, kStage = (BM + BN) * 128;
+template <int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(WM * WN * 64) void bank_dx_kernel(DxArgs p) {
+    constexpr int W = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, kStage = (BM + BN) * 64;
+    constexpr int LM = BM / 16 / W, LN = BN / 16 / W;  // 16-row loads of either tile to a wavefront
+    static_assert(BM % (16 * W) == 0 && BN % (16 * W) == 0, "");
     extern __shared__ __align__(16) char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave & 1, wn = wave >> 1;
-    const int k0 = blockIdx.x * BN, p0 = blockIdx.y * BM;
-    const int first = blockIdx.z * p.steps, last = min(p.N / 64, first + p.steps);
-    // this lane's part of a stage: rows 8 (i + TM.. * wave) + lane / 8 of either tile
-    const uint16_t *xs[2 * TM], *ws[2 * TN];
-    const int unit = (lane & 7) ^ (lane >> 3);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+    // Blocks go to the eight dies in turn: a die's blocks are those side by side in (slice, k, m), m first, which share most of what
+    // they read.
+    const int total = gridDim.x, die = blockIdx.x % 8, each = total / 8, more = total % 8;
+    const int id = die * each + min(die, more) + blockIdx.x / 8;
+    const int m_tile = id % p.m_tiles, k_tile = id / p.m_tiles % p.k_tiles, slice = id / (p.m_tiles * p.k_tiles);
+    const int k0 = k_tile * BN, p0 = m_tile * BM;
+    const int first = slice * p.steps, last = min(p.N / 32, first + p.steps);
+    const uint16_t *xs[LM], *ws[LN];
+    const int unit = (lane & 3) ^ (lane >> 3 & 3);
 #pragma unroll
-    for (int i = 0; i < 2 * TM; ++i) {
-        const int at = min(p0 + 8 * (2 * TM * wave + i) + (lane >> 3), p.rows.rows - 1);
+    for (int i = 0; i < LM; ++i) {
+        const int at = min(p0 + 16 * (LM * wave + i) + (lane >> 2), p.rows.rows - 1);
         xs[i] = p.dy + (size_t)(p.rows.order ? p.rows.order[at] : at) * p.N + 8 * unit;
     }
 #pragma unroll
-    for (int i = 0; i < 2 * TN; ++i) ws[i] = p.wt + (size_t)min(k0 + 8 * (2 * TN * wave + i) + (lane >> 3), p.K - 1) * p.N + 8 * unit;
+    for (int i = 0; i < LN; ++i) ws[i] = p.wt + (size_t)min(k0 + 16 * (LN * wave + i) + (lane >> 2), p.K - 1) * p.N + 8 * unit;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr_t)lds);
-    auto fetch = [&](int step, int buffer) {
-        const unsigned at = lds0 + buffer * kStage + wave * (TM * 2048);
+    auto fetch = [&](int step) {  // past the slice's end: its last step again, so that the count of loads in flight stays what it is
+        const int buffer = (step - first) % kStages;
+        const size_t from = (size_t)min(step, last - 1) * 32;
+        const unsigned at = lds0 + buffer * kStage + wave * (LM * 1024), bt = lds0 + buffer * kStage + BM * 64 + wave * (LN * 1024);
 #pragma unroll
-        for (int i = 0; i < 2 * TM; ++i) load_to_lds_b128(xs[i] + (size_t)step * 64, at + i * 1024);
-        const unsigned bt = lds0 + buffer * kStage + BM * 128 + wave * (TN * 2048);
+        for (int i = 0; i < LM; ++i) load_to_lds_b128(xs[i] + from, at + i * 1024);
 #pragma unroll
-        for (int i = 0; i < 2 * TN; ++i) load_to_lds_b128(ws[i] + (size_t)step * 64, bt + i * 1024);
+        for (int i = 0; i < LN; ++i) load_to_lds_b128(ws[i] + from, bt + i * 1024);
     };
     f32x16 acc[TN][TM];
 #pragma unroll
@@ -141,71 +143,87 @@ __global__ __launch_bounds__(256) void bank_dx_kernel(DxArgs p) {
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
-    fetch(first, 0);
+    const int r = lane & 31, h = lane >> 5;
+    auto product = [&](const char *stage) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            bf16x8 x[TM], w[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) x[i] = *reinterpret_cast<const bf16x8 *>(stage + unit_at(32 * (TM * wm + i) + r, 2 * kk + h));
+#pragma unroll
+            for (int j = 0; j < TN; ++j) w[j] = *reinterpret_cast<const bf16x8 *>(stage + BM * 64 + unit_at(32 * (TN * wn + j) + r, 2 * kk + h));
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) fetch(first + s);
     for (int step = first; step < last; ++step) {
-        const int buffer = (step - first) & 1;
-        wait_vector_loads<0>();
-        __syncthreads();
-        if (step + 1 < last) fetch(step + 1, buffer ^ 1);
-        dx_product<TM, TN>(lds + buffer * kStage, wm, wn, lane, acc);
+        wait_vector_loads<(kStages - 2) * (LM + LN)>();
+        __builtin_amdgcn_s_barrier();
+        fetch(step + kStages - 1);
+        product(lds + (step - first) % kStages * kStage);
+        wait_lds_reads();
     }
-    if (p.u && blockIdx.z == 0) {
-        // U A: the runs of rows of one adapter among the block's positions, each as one step (rank <= 32: both parts of U side by
-        // side on the 64 of the contraction) or two (U's bf16 value, then what that leaves)
+    wait_vector_loads<0>();
+    if (p.u && slice == 0) {
+        // U A: the runs of rows of one adapter among the block's positions, 32 of the rank at a time, U's bf16 value and then what that
+        // leaves, zeros for the rows of others (and `at` holds finite values alone: turn_bank_kernel).
         const int end = min(p0 + BM, p.rows.first[p.rows.count]);
-        const int sides = p.rank <= 32 ? 1 : 2, half = p.rank <= 32 ? 32 : 64;
         for (int q0 = p0; q0 < end;) {
             const int a = p.rows.of[p.rows.order[q0]], q1 = min(p.rows.first[a + 1], end);
             const float scale = p.scales[a];
-            for (int side = 0; side < sides; ++side) {
-                __syncthreads();
-                for (int e = tid; e < BM * 8; e += 256) {
-                    const int row = e >> 3, unit = e & 7, col = (8 * unit) % half;
-                    const bool lower = sides == 1 ? unit >= 4 : side == 1;
-                    bf16x8 v = bf16x8_zero();
-                    if (p0 + row >= q0 && p0 + row < q1 && col < p.rank) {
-                        const float *u = p.u + (size_t)(p0 + row) * p.rank + col;
+            for (int c0 = 0; c0 < p.rank; c0 += 32)
+                for (int side = 0; side < 2; ++side) {
+                    __syncthreads();
+                    for (int e = tid; e < BM * 4; e += W * 64) {
+                        const int row = e >> 2, unit = e & 3, col = c0 + 8 * unit;
+                        bf16x8 v = bf16x8_zero();
+                        if (p0 + row >= q0 && p0 + row < q1 && col < p.rank) {
+                            const float *u = p.u + (size_t)(p0 + row) * p.rank + col;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float f = u[i] * scale;
-                            const __bf16 hi = (__bf16)f;
-                            v[i] = lower ? (__bf16)(f - (float)hi) : hi;
+                            for (int i = 0; i < 8; ++i) {
+                                const float f = u[i] * scale;
+                                const __bf16 hi = (__bf16)f;
+                                v[i] = side ? (__bf16)(f - (float)hi) : hi;
+                            }
                         }
+                        *reinterpret_cast<bf16x8 *>(lds + unit_at(row, unit)) = v;
                     }
-                    *reinterpret_cast<bf16x8 *>(lds + unit_at(row, unit)) = v;
+                    if (side == 0)
+                        for (int e = tid; e < BN * 4; e += W * 64) {
+                            const int row = e >> 2, unit = e & 3, col = c0 + 8 * unit;
+                            u32x4 v = {0u, 0u, 0u, 0u};
+                            if (k0 + row < p.K && col < p.rank) v = *reinterpret_cast<const u32x4 *>(p.at + ((size_t)a * p.K + k0 + row) * p.rank + col);
+                            *reinterpret_cast<u32x4 *>(lds + BM * 64 + unit_at(row, unit)) = v;
+                        }
+                    __syncthreads();
+                    product(lds);
                 }
-                for (int e = tid; e < BN * 8; e += 256) {
-                    const int row = e >> 3, unit = e & 7, col = (8 * unit) % half;
-                    u32x4 v = {0u, 0u, 0u, 0u};
-                    if (k0 + row < p.K && col < p.rank) v = *reinterpret_cast<const u32x4 *>(p.at + ((size_t)a * p.K + k0 + row) * p.rank + col);
-                    *reinterpret_cast<u32x4 *>(lds + BM * 128 + unit_at(row, unit)) = v;
-                }
-                __syncthreads();
-                dx_product<TM, TN>(lds, wm, wn, lane, acc);
-            }
             q0 = q1;
         }
     }
     // a lane holds column lane & 31 (a row of dx) and four consecutive k at 8 g + 4 (lane >> 5)
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int at = p0 + 32 * (TM * wm + i) + (lane & 31);
+        const int at = p0 + 32 * (TM * wm + i) + r;
         if (at >= p.rows.rows) continue;
         const int row = p.rows.order ? p.rows.order[at] : at;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int k = k0 + 32 * (TN * wn + j) + 8 * g + 4 * (lane >> 5);
+                const int k = k0 + 32 * (TN * wn + j) + 8 * g + 4 * h;
                 if (k >= p.K) continue;
-                const f32x16 &v = acc[j][i];
+                f32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
                 if (p.partial) {
-                    *reinterpret_cast<f32x4 *>(p.partial + ((size_t)blockIdx.z * p.rows.rows + row) * p.K + k) =
-                        f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                    *reinterpret_cast<f32x4 *>(p.partial + ((size_t)slice * p.rows.rows + row) * p.K + k) = v;
                 } else {
                     u32x2 o;
-                    o.x = f32_to_bf16_bits(v[4 * g]) | (uint32_t)f32_to_bf16_bits(v[4 * g + 1]) << 16;
-                    o.y = f32_to_bf16_bits(v[4 * g + 2]) | (uint32_t)f32_to_bf16_bits(v[4 * g + 3]) << 16;
+                    o.x = f32_to_bf16_bits(v[0]) | (uint32_t)f32_to_bf16_bits(v[1]) << 16;
+                    o.y = f32_to_bf16_bits(v[2]) | (uint32_t)f32_to_bf16_bits(v[3]) << 16;
                     *reinterpret_cast<u32x2 *>(p.dx + (size_t)row * p.K + k) = o;
                 }
             }
@@ -234,6 +252,9 @@ struct GradArgs {
     uint16_t *da, *db;
     BankRows rows;
     int K, N, rank;
+    const uint16_t *a;   // the adapters' A as they lie, [count, rank, K]
+    const uint8_t *odd;  // [count, K / 64]: where A holds values that are no finite numbers,
+    uint16_t *dx;        // whose products are still to be added here
 };
 
 constexpr int kGradPitch = 128 + 4;
@@ -321,6 +342,19 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
         }
         *reinterpret_cast<u32x4 *>(is_b ? out + (size_t)col * p.rank + 8 * r : out + (size_t)r * p.K + 8 * col) = o;
     }
+    if (is_b) return;
+    const uint8_t *odd = p.odd + (size_t)a * (p.K / 64) + c0 / 64;
+    if (!(odd[0] | odd[1])) return;
+    for (int i = tid; i < (end - begin) * 128; i += W * 64) {
+        const int at = begin + i / 128, k = c0 + i % 128;
+        uint16_t *dx = p.dx + (size_t)p.rows.order[at] * p.K + k;
+        float v = __builtin_bit_cast(float, (uint32_t)*dx << 16);
+        for (int r = 0; r < p.rank; ++r) {
+            const uint16_t bits = p.a[((size_t)a * p.rank + r) * p.K + k];
+            if ((bits & 0x7F80u) == 0x7F80u) v += p.u[(size_t)at * p.rank + r] * scale * __builtin_bit_cast(float, (uint32_t)bits << 16);
+        }
+        *dx = f32_to_bf16_bits(v);
+    }
 }
 
 template <int JT>
@@ -331,18 +365,49 @@ void launch_grad(const GradArgs &g, hipStream_t stream) {
 }
 
 // ---- the plan ----------------------------------------------------------------------------------------------------
-constexpr int kMaxDxSlices = 8;
-int dx_slices(int m, int n, int k) {
-    const int tiles = ((m + 127) / 128) * (k / 128), steps = n / 64;
-    int slices = 1;
-    while (slices < kMaxDxSlices && tiles * slices < 384 && steps / (slices + 1) >= 4) ++slices;
-    const int each = (steps + slices - 1) / slices;
-    return (steps + each - 1) / each;
+// The block of the product for dx and the slices of its contraction.  A block of 256 x 256 is the fastest by its area (2048 rows of n 18432, k
+// 2560, three slices: 189 us, 1.02 PFLOP/s; 128 x 256 216, 128 x 128 237), a smaller one where those would leave compute units without
+// work (777 rows, 2560 -> 9216: 128 x 256 49 us, 128 x 128 55, 256 x 256 79).  Times by a model: so many rounds of blocks, each its steps
+// at what one takes, measured, and with slices what writing, reading and adding them takes.
+struct DxPlan {
+    int kind;    // 0: 128 x 128, two blocks to a compute unit; 1: 128 x 256; 2: 256 x 256
+    int slices;
+};
+constexpr int kMaxDxSlices = 8, kComputeUnits = 256;
+constexpr int kDxTileM[3] = {128, 128, 256}, kDxTileK[3] = {128, 256, 256};
+DxPlan dx_plan(int m, int n, int k) {
+    DxPlan best{0, 1};
+    float least = 0.f;
+    for (int kind = 0; kind < 3; ++kind)
+        for (int slices = 1; slices <= kMaxDxSlices; ++slices) {
+            const int steps = n / 32, each = (steps + slices - 1) / slices;
+            if (slices > 1 && (each < 8 || (steps + each - 1) / each != slices)) continue;
+            const int64_t tiles = (int64_t)((m + kDxTileM[kind] - 1) / kDxTileM[kind]) * ((k + kDxTileK[kind] - 1) / kDxTileK[kind]) * slices;
+            const float rounds = kind ? (float)((tiles + kComputeUnits - 1) / kComputeUnits)
+                                      : tiles <= kComputeUnits ? 0.54f : (float)((tiles + 2 * kComputeUnits - 1) / (2 * kComputeUnits));
+            const float step_us = kind == 2 ? 0.85f : kind == 1 ? 0.52f : 0.54f;
+            const float t = rounds * (each + 6) * step_us + (slices > 1 ? 3.f + 2e-6f * slices * (float)m * (float)k : 0.f);
+            if ((kind == 0 && slices == 1) || t < least) {
+                least = t;
+                best = DxPlan{kind, slices};
+            }
+        }
+    return best;
+}
+
+template <int WM, int WN, int TM, int TN>
+void launch_dx(DxArgs p, int slices, hipStream_t stream) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
+    p.m_tiles = (p.rows.rows + BM - 1) / BM;
+    p.k_tiles = (p.K + BN - 1) / BN;
+    p.steps = (p.N / 32 + slices - 1) / slices;
+    bank_dx_kernel<WM, WN, TM, TN><<<p.m_tiles * p.k_tiles * slices, WM * WN * 64, kStages * (BM + BN) * 64, stream>>>(p);
 }
 
 struct BackwardScratch {
-    size_t wt, at, bt, order, t, u, partial, total;
-    int t_slices, u_slices, dx_slices;
+    size_t wt, at, bt, odd, order, t, u, partial, total;
+    int t_slices, u_slices;
+    DxPlan dx;
 };
 BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
     BackwardScratch s{};
@@ -356,19 +421,18 @@ BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
     if (count > 0) {
         s.at = take((size_t)count * rank * k * 2);
         s.bt = take((size_t)count * rank * n * 2);
+        s.odd = take((size_t)count * (k / 64));
         s.order = take(bank_order_bytes(m, count));
         s.t_slices = bank_slices(m, k);
         s.u_slices = bank_slices(m, n);
         s.t = take((size_t)s.t_slices * m * rank * 4);
         s.u = take((size_t)s.u_slices * m * rank * 4);
     }
-    s.dx_slices = dx_slices(m, n, k);
-    s.partial = take(s.dx_slices > 1 ? (size_t)s.dx_slices * m * k * 4 : 0);
+    s.dx = dx_plan(m, n, k);
+    s.partial = take(s.dx.slices > 1 ? (size_t)s.dx.slices * m * k * 4 : 0);
     s.total = at;
     return s;
 }
-
-constexpr int kTileM = 2, kTileK = 2;
 
 }  // namespace
 }  // namespace kiln
@@ -378,8 +442,8 @@ using namespace kiln;
 extern "C" {
 
 size_t kiln_w4a16_gemm_bank_backward_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank) {
-    if (prob_m < 1 || prob_n < 256 || prob_k < 128 || count < 0 || rank < 0) return 256;
-    return backward_scratch(prob_m, prob_n, prob_k, count, rank).total;
+    if (prob_n < 256 || prob_k < 128 || count < 0 || rank < 0) return 256;
+    return backward_scratch(prob_m < 1 ? 1 : prob_m, prob_n, prob_k, count, rank).total;
 }
 
 kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A, const void *B, const void *s, int prob_m, int prob_n, int prob_k,
@@ -405,42 +469,50 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     dx.dy = (const uint16_t *)dC;
     dx.wt = wt;
     dx.dx = (uint16_t *)dA;
-    dx.partial = w.dx_slices > 1 ? reinterpret_cast<float *>(at + w.partial) : nullptr;
+    dx.partial = w.dx.slices > 1 ? reinterpret_cast<float *>(at + w.partial) : nullptr;
     dx.rows = BankRows{nullptr, nullptr, nullptr, m, 0};
     dx.K = k;
     dx.N = n;
-    dx.steps = (n / 64 + w.dx_slices - 1) / w.dx_slices;
+    GradArgs grad{};
+    if (m > 0)
+        dequant_rows_kernel<<<dim3(n / 128, k / 128), 512, 0, hs>>>((const u32x4 *)B, (const uint16_t *)s, wt, k, n, groupsize == -1 ? 1 : k / 128);
     if (bank) {
         uint16_t *a_t = reinterpret_cast<uint16_t *>(at + w.at), *b_t = reinterpret_cast<uint16_t *>(at + w.bt);
+        uint8_t *odd = reinterpret_cast<uint8_t *>(at + w.odd);
         float *t = reinterpret_cast<float *>(at + w.t), *u = reinterpret_cast<float *>(at + w.u);
+        const uint16_t *lora_a = (const uint16_t *)bank->lora_a;
         dx.rows = bank_order(adapter_of, m, count, true, at + w.order, hs);
         if (m > 0) {
-            turn_bank_kernel<<<dim3((k > n ? k : n) / 64, count, 2), 256, 0, hs>>>((const uint16_t *)bank->lora_a, (const uint16_t *)bank->lora_b, a_t, b_t, k, n, rank);
-            bank_project(A, bank->lora_a, dx.rows, t, k, rank, w.t_slices, hs);
+            turn_bank_kernel<<<dim3((k > n ? k : n) / 64, count, 2), 256, 0, hs>>>(lora_a, (const uint16_t *)bank->lora_b, a_t, b_t, odd, k, n, rank);
+            bank_project(A, lora_a, dx.rows, t, k, rank, w.t_slices, hs);
             bank_project(dC, b_t, dx.rows, u, n, rank, w.u_slices, hs);
             if (w.t_slices > 1 || w.u_slices > 1)
                 sum_slices_kernel<<<dim3((unsigned)(((size_t)m * rank + 255) / 256), 2), 256, 0, hs>>>(t, w.t_slices, u, w.u_slices, (size_t)m * rank);
         }
-        GradArgs g{(const uint16_t *)A, (const uint16_t *)dC, t, u, bank->scales, (uint16_t *)d_lora_a, (uint16_t *)d_lora_b, dx.rows, k, n, rank};
-        switch ((rank + 15) / 16) {
-            case 1: launch_grad<1>(g, hs); break;
-            case 2: launch_grad<2>(g, hs); break;
-            case 3: launch_grad<3>(g, hs); break;
-            default: launch_grad<4>(g, hs); break;
-        }
+        grad = GradArgs{(const uint16_t *)A, (const uint16_t *)dC, t, u, bank->scales, (uint16_t *)d_lora_a, (uint16_t *)d_lora_b,
+                        dx.rows, k, n, rank, lora_a, odd, (uint16_t *)dA};
         dx.at = a_t;
         dx.u = u;
         dx.scales = bank->scales;
         dx.rank = rank;
     }
     if (m > 0) {
-        dequant_rows_kernel<<<dim3(n / 128, k / 128), 512, 0, hs>>>((const u32x4 *)B, (const uint16_t *)s, wt, k, n, groupsize == -1 ? 1 : k / 128);
-        constexpr int BM = 64 * kTileM, BN = 64 * kTileK;
-        constexpr int lds = 2 * (BM + BN) * 128;
-        bank_dx_kernel<kTileM, kTileK><<<dim3(k / BN, (m + BM - 1) / BM, w.dx_slices), 256, lds, hs>>>(dx);
+        switch (w.dx.kind) {
+            case 0: launch_dx<2, 2, 2, 2>(dx, w.dx.slices, hs); break;
+            case 1: launch_dx<2, 4, 2, 2>(dx, w.dx.slices, hs); break;
+            default: launch_dx<2, 2, 4, 4>(dx, w.dx.slices, hs); break;
+        }
         if (dx.partial) {
             const size_t units = (size_t)m * k / 4;
-            sum_dx_kernel<<<(unsigned)((units + 255) / 256), 256, 0, hs>>>((const f32x4 *)dx.partial, (u32x2 *)dA, w.dx_slices, units);
+            sum_dx_kernel<<<(unsigned)((units + 255) / 256), 256, 0, hs>>>((const f32x4 *)dx.partial, (u32x2 *)dA, w.dx.slices, units);
+        }
+    }
+    if (bank) {  // behind dx, to which it adds where an adapter holds what is no finite number
+        switch ((rank + 15) / 16) {
+            case 1: launch_grad<1>(grad, hs); break;
+            case 2: launch_grad<2>(grad, hs); break;
+            case 3: launch_grad<3>(grad, hs); break;
+            default: launch_grad<4>(grad, hs); break;
         }
     }
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;

@@ -105,3 +105,136 @@ def test_forward(m, k, n, g, count, rank, pattern):
 def test_backward(m, k, n, g, count, rank, pattern):
     p = problem(m, k, n, g, count, rank, pattern, seed=1)
     check_backward(p, *backward(p))
+
+
+def bits(ts):
+    return [t.view(torch.int16).clone() for t in (ts if isinstance(ts, tuple) else (ts,))]
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_an_adapter_that_holds_no_numbers_stays_with_its_own_rows(m):
+    """Infinities and NaN in one adapter, and in one row of the activations, reach the rows and gradients that the formula says and no other."""
+    p = problem(m, 256, 512, 128, 5, 24, "any", seed=2)
+    p["of"][0], p["of"][1] = 2, 3                 # both there
+    bad = {**p, "a_": p["a_"].clone(), "b_": p["b_"].clone()}
+    bad["a_"][2, 3, 17], bad["a_"][2, 5, 200], bad["b_"][2, 400, 1] = float("inf"), float("nan"), float("-inf")
+    mine = p["of"] == 2
+    y, z = forward(p), forward(bad)
+    assert torch.equal(y[~mine].view(torch.int16), z[~mine].view(torch.int16))
+    assert not bool(torch.isfinite(z[mine]).any())                        # T of such a row is NaN, and goes to every column
+    (da, d_a, d_b), (ea, e_a, e_b) = backward(p), backward(bad)
+    assert torch.equal(da[~mine].view(torch.int16), ea[~mine].view(torch.int16))
+    others = [0, 1, 3, 4]
+    assert torch.equal(d_a[others].view(torch.int16), e_a[others].view(torch.int16))
+    assert torch.equal(d_b[others].view(torch.int16), e_b[others].view(torch.int16))
+    # B's infinity makes U's column 1 of these rows infinite: with A finite there dx is infinite wherever A[1] is not zero, NaN elsewhere
+    only_a = {**p, "a_": bad["a_"]}
+    fa = backward(only_a)[0]
+    odd = torch.zeros(256, dtype=torch.bool, device="cuda")
+    odd[17] = odd[200] = True
+    assert not bool(torch.isfinite(fa[mine][:, odd]).any()) and bool(torch.isfinite(fa[mine][:, ~odd]).all())
+    assert bool(torch.isnan(fa[mine][:, 200]).all())
+    assert torch.equal(fa[mine][:, ~odd].view(torch.int16), da[mine][:, ~odd].view(torch.int16))
+    x = p["x"].clone()
+    x[1, 7] = float("nan")                        # a row of adapter 3
+    z = forward({**p, "x": x})
+    keep = torch.arange(m, device="cuda") != 1
+    assert torch.equal(y[keep].view(torch.int16), z[keep].view(torch.int16)) and bool(torch.isnan(z[1]).all())
+
+
+@pytest.mark.parametrize("m", [7, 130, 400])
+def test_same_bits_again_on_views_other_streams_and_into_a_given_tensor(m):
+    p = problem(m, 384, 512, 128, 6, 16, "any", seed=3)
+    y, g = bits(forward(p)), bits(backward(p))
+    wide = {**p, "x": torch.cat([p["x"], p["x"]], 1)[:, :384], "dy": torch.cat([p["dy"], p["dy"]], 1)[:, 512:],
+            "of": torch.stack([p["of"], p["of"]], 1)[:, 0], "a_": p["a_"].transpose(1, 2).contiguous().transpose(1, 2)}
+    assert not any(wide[k].is_contiguous() for k in ("x", "dy", "a_")) and (m == 1 or not wide["of"].is_contiguous())
+    out = torch.full((m, 512), float("nan"), dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        again = bits(forward(p, out=out)), bits(backward(p))
+    stream.synchronize()
+    for got in ((bits(forward(wide)), bits(backward(wide))), again, (bits(out), bits(backward(p)))):
+        assert all(torch.equal(a, b) for a, b in zip(got[0] + got[1], y + g))
+
+
+@pytest.mark.parametrize("m", [5, 300])
+def test_replayed_from_a_graph(m):
+    """Captured calls replayed with other contents in the same tensors, eager calls and synchronisations between the replays."""
+    parts = [problem(m, 256, 512, 128, 4, 8, "any", seed=s) for s in (4, 5, 6)]
+    live = {k: v.clone() if torch.is_tensor(v) else v for k, v in parts[0].items()}
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        forward(live), backward(live)                 # the stream's workspace
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            made = (forward(live), *backward(live))
+        for p in parts + parts:
+            for k, v in p.items():
+                if torch.is_tensor(v):
+                    live[k].copy_(v)
+            graph.replay()
+            stream.synchronize()
+            got = bits(made)
+            want = bits((forward(p), *backward(p)))
+            stream.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_rows_and_the_plain_gradient():
+    p = problem(0, 256, 512, 128, 3, 8, "one", seed=7)
+    assert forward(p).shape == (0, 512)
+    da, d_a, d_b = backward(p)
+    assert da.shape == (0, 256) and not bool(d_a.any()) and not bool(d_b.any())
+    assert marlin_gemm.marlin_w4a16_gemm_backward(p["dy"], p["b"], p["s"], 128).shape == (0, 256)
+    for m in (1, 50, 700):
+        p = problem(m, 640, 512, -1, 3, 8, "none", seed=8)
+        assert torch.equal(marlin_gemm.marlin_w4a16_gemm_backward(p["dy"], p["b"], p["s"], -1).view(torch.int16), backward(p)[0].view(torch.int16))
+
+
+def test_gradients_against_differences():
+    """d(sum y * dy) along a direction of x, A and B, by the forward in steps either way, against the gradients."""
+    p = problem(24, 256, 256, 128, 3, 8, "any", seed=9)
+    da, d_a, d_b = (t.double() for t in backward(p))
+    w = marlin_gemm.dequant_f32(p["b"], p["s"], 128).double()
+
+    def loss(x, a, b):
+        y = x @ w
+        for j in range(3):
+            mine = p["of"] == j
+            y[mine] += p["sc"][j].double() * ((x[mine] @ a[j].t()) @ b[j].t())
+        return (y * p["dy"].double()).sum()
+
+    at = [p[k].double() for k in ("x", "a_", "b_")]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for i, grad in enumerate((da, d_a, d_b)):
+        d = torch.randn(at[i].shape, dtype=torch.float64, device="cuda", generator=gen)
+        step = [[t + sign * 1e-3 * d if j == i else t for j, t in enumerate(at)] for sign in (1, -1)]
+        slope = (loss(*step[0]) - loss(*step[1])) / 2e-3                   # exact: the loss is linear in each of them
+        bound = 4 * U * (grad * d).abs().sum() + 64 * U * grad.abs().max()
+        assert abs((grad * d).sum() - slope) <= bound
+
+
+def test_rows_behind_and_around_the_result_stay_as_they_were():
+    p = problem(37, 256, 512, 128, 4, 16, "any", seed=10)
+    room = torch.full((37 + 2, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    y = forward(p, out=room[1:38])
+    assert y.data_ptr() == room[1:38].data_ptr() and bool((room[0] == 7).all()) and bool((room[38] == 7).all())
+    assert torch.equal(bits(y)[0], bits(forward(p))[0])
+
+
+def test_refusals():
+    p = problem(6, 256, 512, 128, 3, 16, "any")
+    for change, text in ((dict(a_=p["a_"][:, :, :128]), "bank shapes"), (dict(b_=p["b_"][:2]), "bank shapes"), (dict(sc=p["sc"][:2]), "bank shapes"),
+                         (dict(of=p["of"][:5]), "adapter_of must be"), (dict(of=p["of"].long()), "adapter_of i32"), (dict(sc=p["sc"].double()), "bank_scales must be f32"),
+                         (dict(a_=p["a_"].float()), "must be bf16"), (dict(a_=p["a_"][:, :12], b_=p["b_"][:, :, :12]), "multiple of 8"),
+                         (dict(of=p["of"].cpu()), "must be on"), (dict(a_=p["a_"][0]), "a bank is"), (dict(x=p["x"].half()), "a must be bf16"), (dict(g=64), "groupsize")):
+        for call in (forward, backward):
+            with pytest.raises(marlin_gemm.MarlinGemmError, match=text):
+                call({**p, **change})
+    with pytest.raises(marlin_gemm.MarlinGemmError, match="dy must be"):
+        backward({**p, "dy": p["dy"][:, :256]})
+    with pytest.raises(marlin_gemm.MarlinGemmError, match="out must be"):
+        forward(p, out=torch.empty(6, 256, dtype=torch.bfloat16, device="cuda"))
