@@ -19,20 +19,24 @@ inline size_t bank_up256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 // first[a] .. first[a + 1] are adapter a's positions, those of rows without an adapter come last.
 struct BankRows {
     const int *of;      // [rows] adapter of a row; outside [0, count): none
-    const int *order;   // [rows], or null
-    const int *first;   // [count + 2], or null
+    int *order;         // [rows], or null
+    int *first;         // [count + 2], or null
     int rows, count;
 };
 
 bool bank_ok(const kiln_w4a16_adapter_bank &bank);
 size_t bank_order_bytes(int rows, int count);
-// launches the ordering (calls of kBankOrderedFrom rows and more, or `always`); `at`: bank_order_bytes of scratch
-BankRows bank_order(const int *of, int rows, int count, bool always, void *at, hipStream_t stream);
+BankRows bank_rows(const int *of, int rows, int count, void *at);  // with order and first in bank_order_bytes of scratch from `at` on
 
 // slices of K that a projection of `rows` rows is cut into
 int bank_slices(int rows, int K);
-size_t bank_projected_rows(int rows, int K);
+size_t bank_projected_rows(int rows, int K);  // slices * rows at most, and not falling with rows
 // t[slice][position][rank] = the slice's share of src[row, K] * mat[adapter of row][rank, K]^T, f32; positions without an adapter are not written
-void bank_project(const void *src, const void *mat, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream);
+struct BankProjection {
+    const void *src, *mat;
+    float *t;
+    int K, slices;
+};
+void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream);
 
 }  // namespace kiln

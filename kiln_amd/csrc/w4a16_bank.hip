@@ -7,64 +7,17 @@
 // from 257 rows on a launch in front puts them so.  The reference serves one adapter set per process
 // (crates/kiln-model/src/lora_loader.rs:213-232); this is its formula with the adapter a row's own.
 #include "bank.h"
+#include "bank_order.h"
 #include "device_common.h"
 
 namespace kiln {
 namespace {
 
-// order[] and first[]: a block per adapter (and one for the rows without) counts the rows of lower adapters and places its own, 64 rows
-// per ballot, its sixteen wavefronts a sixteenth of the rows each: no block waits for another and rows keep their order inside an
-// adapter.  Up to 8192 rows a wavefront's part is in registers and read once.  2048 rows, 8 adapters: a wavefront for each took 14 us.
-constexpr int kOrderWaves = 16, kOrderUnroll = 8;
+constexpr int kOrderWaves = 16;
 __global__ __launch_bounds__(kOrderWaves * 64) void bank_order_kernel(const int *__restrict__ of, int *__restrict__ order, int *__restrict__ first,
                                                                       int rows, int count) {
-    __shared__ int less_of[kOrderWaves], mine_of[kOrderWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = blockIdx.x;
-    const int each = (rows + kOrderWaves * 64 - 1) / (kOrderWaves * 64) * 64;
-    const int begin = wave * each, end = min(rows, begin + each);
-    int key[kOrderUnroll];
-    auto read = [&](int r0) {
-#pragma unroll
-        for (int u = 0; u < kOrderUnroll; ++u) {
-            const int r = r0 + 64 * u + lane;
-            key[u] = r < end ? of[r] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < kOrderUnroll; ++u) {
-            if ((unsigned)key[u] >= (unsigned)count) key[u] = count;
-            if (r0 + 64 * u + lane >= end) key[u] = INT32_MAX;
-        }
-    };
-    int less = 0, mine = 0;
-    for (int r0 = begin; r0 < end; r0 += 64 * kOrderUnroll) {
-        read(r0);
-#pragma unroll
-        for (int u = 0; u < kOrderUnroll; ++u) {
-            less += __popcll(__ballot(key[u] < a));
-            mine += __popcll(__ballot(key[u] == a));
-        }
-    }
-    if (lane == 0) {
-        less_of[wave] = less;
-        mine_of[wave] = mine;
-    }
-    __syncthreads();
-    int at = 0;
-    for (int w = 0; w < kOrderWaves; ++w) at += less_of[w];
-    if (threadIdx.x == 0) {
-        first[a] = at;
-        if (a == count) first[count + 1] = rows;
-    }
-    for (int w = 0; w < wave; ++w) at += mine_of[w];
-    for (int r0 = begin; r0 < end; r0 += 64 * kOrderUnroll) {
-        if (each > 64 * kOrderUnroll) read(r0);
-#pragma unroll
-        for (int u = 0; u < kOrderUnroll; ++u) {
-            const unsigned long long all = __ballot(key[u] == a);
-            if (key[u] == a) order[at + __popcll(all & ((1ull << lane) - 1))] = r0 + 64 * u + lane;
-            at += __popcll(all);
-        }
-    }
+    __shared__ OrderLds<kOrderWaves> lds;
+    order_rows(of, order, first, rows, count, blockIdx.x, lds);
 }
 
 __device__ __forceinline__ bf16x8 load_bf16x8(const uint16_t *p) {
@@ -106,11 +59,16 @@ __device__ __forceinline__ void project_pieces(const uint16_t *const (&x)[RT], c
 
 // T: a block takes 16 RT positions, one slice of K, and of the adapters present among them those whose turn (in the order they are met)
 // is blockIdx.z modulo gridDim.z.  Its W wavefronts take every W-th 64 of K and meet in LDS.  Blocks go through the slices first, so
-// that with eight of them a die's blocks share one, whose part of the adapters' matrices its L2 then holds.
+// that with eight of them a die's blocks share one, whose part of the adapters' matrices its L2 then holds.  Two projections of the same
+// rows share a launch: the second one's slices are behind the first one's.
 template <int JT, int RT, int W>
-__global__ __launch_bounds__(W * 64) void bank_project_kernel(const uint16_t *__restrict__ src, const uint16_t *__restrict__ mat, BankRows rows,
-                                                           float *__restrict__ t, int K, int steps, int rank) {
+__global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one, BankProjection two, BankRows rows, int rank) {
     constexpr int P = 16 * RT, kAhead = JT + RT <= 4 ? 4 : 2;
+    const bool second = (int)blockIdx.x >= one.slices;
+    const uint16_t *__restrict__ src = (const uint16_t *)(second ? two.src : one.src), *__restrict__ mat = (const uint16_t *)(second ? two.mat : one.mat);
+    float *__restrict__ t = second ? two.t : one.t;
+    const int K = second ? two.K : one.K, slices = second ? two.slices : one.slices, slice = second ? blockIdx.x - one.slices : blockIdx.x;
+    const int steps = (K / 128 + slices - 1) / slices;
     __shared__ float part[W][P][JT * 16 + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
     const int p0 = blockIdx.y * P;
@@ -118,7 +76,7 @@ __global__ __launch_bounds__(W * 64) void bank_project_kernel(const uint16_t *__
     row_at(rows, p0 + (lane & (P - 1)), row, a);
     constexpr unsigned long long kAll = P == 64 ? ~0ull : (1ull << P) - 1;
     unsigned long long left = __ballot(a >= 0) & kAll;
-    const int k0 = blockIdx.x * steps * 128, k1 = min(K, k0 + steps * 128), own = k0 + 64 * wave;
+    const int k0 = slice * steps * 128, k1 = min(K, k0 + steps * 128), own = k0 + 64 * wave;
     const int pieces = own < k1 ? (k1 - own + 64 * W - 1) / (64 * W) : 0;
     const uint16_t *x[RT];
 #pragma unroll
@@ -146,7 +104,7 @@ __global__ __launch_bounds__(W * 64) void bank_project_kernel(const uint16_t *__
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][16 * r + 4 * q + i][16 * j + c] = acc[r][j][i];
         __syncthreads();
-        float *out = t + ((size_t)blockIdx.x * rows.rows + p0) * rank;
+        float *out = t + ((size_t)slice * rows.rows + p0) * rank;
         for (int e = tid; e < P * rank; e += 64 * W) {
             const int r = e / rank, j = e - r * rank;
             float v = 0.f;
@@ -368,13 +326,21 @@ constexpr int kLongContraction = 8192;
 bool long_ordered(int rows, int K) { return rows >= kBankOrderedFrom && K >= kLongContraction; }
 
 template <int JT, int RT, int W>
-void launch_project(const uint16_t *s, const uint16_t *m, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream) {
-    const int groups = K / 128, steps = (groups + slices - 1) / slices, tiles = tiles_of(r.rows, 16 * RT);
+void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream) {
+    const int tiles = tiles_of(r.rows, 16 * RT);
     // the adapters that a tile may hold side by side: as many as it has rows, but where they are together few tiles have more than one
     int turns = r.order ? 1 + r.count / tiles : 16;
     if (turns > 16) turns = 16;
     if (turns > r.count) turns = r.count;
-    bank_project_kernel<JT, RT, W><<<dim3(slices, tiles, turns), W * 64, 0, stream>>>(s, m, r, t, K, steps, rank);
+    bank_project_kernel<JT, RT, W><<<dim3(one.slices + two.slices, tiles, turns), W * 64, 0, stream>>>(one, two, r, rank);
+}
+template <int RT, int W>
+void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream) {
+    const int jt = (rank + 15) / 16;
+    if (jt == 1) launch_project<1, RT, W>(one, two, r, rank, stream);
+    else if (jt == 2) launch_project<2, RT, W>(one, two, r, rank, stream);
+    else if (jt == 3) launch_project<3, RT, W>(one, two, r, rank, stream);
+    else launch_project<4, RT, W>(one, two, r, rank, stream);
 }
 
 }  // namespace
@@ -385,15 +351,8 @@ bool bank_ok(const kiln_w4a16_adapter_bank &bank) {
 
 size_t bank_order_bytes(int rows, int count) { return bank_up256((size_t)rows * 4) + bank_up256(((size_t)count + 2) * 4); }
 
-BankRows bank_order(const int *of, int rows, int count, bool always, void *at, hipStream_t stream) {
-    BankRows r{of, nullptr, nullptr, rows, count};
-    if (rows < kBankOrderedFrom && !always) return r;
-    int *order = reinterpret_cast<int *>(at);
-    int *first = reinterpret_cast<int *>(reinterpret_cast<char *>(at) + bank_up256((size_t)rows * 4));
-    bank_order_kernel<<<count + 1, kOrderWaves * 64, 0, stream>>>(of, order, first, rows, count);
-    r.order = order;
-    r.first = first;
-    return r;
+BankRows bank_rows(const int *of, int rows, int count, void *at) {
+    return BankRows{of, reinterpret_cast<int *>(at), reinterpret_cast<int *>(reinterpret_cast<char *>(at) + bank_up256((size_t)rows * 4)), rows, count};
 }
 
 // Slices are 512 of K at least: two pieces to a wavefront, whose loads are in flight together; shorter ones leave whoever sums them more
@@ -414,25 +373,11 @@ size_t bank_projected_rows(int rows, int K) {
     return here > below ? here : below;
 }
 
-void bank_project(const void *src, const void *mat, const BankRows &r, float *t, int K, int rank, int slices, hipStream_t stream) {
-    const uint16_t *s = (const uint16_t *)src, *m = (const uint16_t *)mat;
-    const int jt = (rank + 15) / 16;
-    if (!r.order || r.rows < kBankOrderedFrom) {
-        if (jt == 1) launch_project<1, 1, 4>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 2) launch_project<2, 1, 4>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 3) launch_project<3, 1, 4>(s, m, r, t, K, rank, slices, stream);
-        else launch_project<4, 1, 4>(s, m, r, t, K, rank, slices, stream);
-    } else if (long_ordered(r.rows, K)) {
-        if (jt == 1) launch_project<1, 2, 4>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 2) launch_project<2, 2, 4>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 3) launch_project<3, 2, 4>(s, m, r, t, K, rank, slices, stream);
-        else launch_project<4, 2, 4>(s, m, r, t, K, rank, slices, stream);
-    } else {
-        if (jt == 1) launch_project<1, 1, 8>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 2) launch_project<2, 1, 8>(s, m, r, t, K, rank, slices, stream);
-        else if (jt == 3) launch_project<3, 1, 8>(s, m, r, t, K, rank, slices, stream);
-        else launch_project<4, 1, 8>(s, m, r, t, K, rank, slices, stream);
-    }
+void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream) {
+    const BankProjection none{}, &other = two ? *two : none;
+    if (!r.order || r.rows < kBankOrderedFrom) launch_project<1, 4>(one, other, r, rank, stream);
+    else if (two || long_ordered(r.rows, one.K)) launch_project<2, 4>(one, other, r, rank, stream);
+    else launch_project<1, 8>(one, other, r, rank, stream);
 }
 
 namespace {
@@ -479,10 +424,12 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     if (st != KILN_W4A16_OK) return st;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     char *at = reinterpret_cast<char *>(scratch);
-    const BankRows rows = bank_order(adapter_of, prob_m, bank->count, false, at, hs);
+    BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
+    if (prob_m < kBankOrderedFrom) rows.order = rows.first = nullptr;
+    else bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
     const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
-    bank_project(A, bank->lora_a, rows, t, prob_k, rank, slices, hs);
+    bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
     uint16_t *y = (uint16_t *)C;
     const uint16_t *m = (const uint16_t *)bank->lora_b;
     if (rank <= 32) launch_expand<1>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);

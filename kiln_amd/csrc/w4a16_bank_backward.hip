@@ -9,69 +9,116 @@
 // rows of an adapter.  Rows are taken in the order of their adapters throughout.
 #include "async_loads.h"
 #include "bank.h"
+#include "bank_order.h"
 #include "device_common.h"
 
 namespace kiln {
 namespace {
 
-// ---- W, row by row ---------------------------------------------------------------------------------------------
-// out[k][n] = bf16((code - 8) * scale): a block takes one scale group (128 rows) x 128 columns, a chunk to each of its eight
-// wavefronts, and turns it through LDS.  The rounding of a weight to 8 bits is what every 16-bit product of the unpacked weight has
-// (the reference's own bar is against bf16(dequant): crates/kiln-marlin-gemm/tests/parity.rs:150-157); the codes themselves would be exact,
-// but the scales run along the contraction here and cannot be pulled out of it.
-constexpr int kTurnPitch = 128 + 8;
-__global__ __launch_bounds__(512) void dequant_rows_kernel(const u32x4 *__restrict__ B, const uint16_t *__restrict__ S, uint16_t *__restrict__ out, int K,
-                                                           int N, int Gs) {
-    __shared__ __align__(16) uint16_t tile[128 * kTurnPitch];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, kq = lane >> 4;
-    const int G = K / kGroupK, g = blockIdx.y, nt = blockIdx.x * 8 + wave;
-    const u32x4 w = B[((size_t)nt * G + g) * 64 + lane];
-    const float s = f16_bits_to_f32(S[scale_index(Gs == 1 ? 0 : g, nt * kTileN + c, Gs)]);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+// ---- what the products read ----------------------------------------------------------------------------------------
+// One launch for what depends on the call's operands alone: the rows' order, the adapters' matrices turned, and W unpacked row by row.
+struct PrepareArgs {
+    const u32x4 *B;        // the packed weight
+    const uint16_t *S;
+    uint16_t *wt;          // bf16 [K, N]
+    const uint16_t *a, *b;  // the bank's matrices, [count, rank, K] and [count, N, rank]
+    uint16_t *at, *bt;      // ... turned: [count, K, rank] and [count, rank, N]
+    uint8_t *odd;           // [count, K / 64]
+    BankRows rows;
+    int K, N, Gs, rank;
+    int order_blocks, turn_blocks;
+};
+constexpr int kPrepareThreads = 512, kTurnPitch = 128 + 8;
+union PrepareLds {
+    uint16_t weight[128 * kTurnPitch];
+    uint16_t bank[64][kBankMaxRank + 2];
+    OrderLds<kPrepareThreads / 64> order;
+};
+
+// wt[k][n] = bf16((code - 8) * scale): a block takes one scale group (128 rows) x 128 columns, a chunk to each of its eight wavefronts.  The
+// rounding of a weight to 8 bits is what every 16-bit product of the unpacked weight has (the reference's own bar is against
+// bf16(dequant): crates/kiln-marlin-gemm/tests/parity.rs:150-157); the codes themselves would be exact, but the scales run along the
+// contraction here and cannot be pulled out of it.
+// A word has eight rows of one column and a row of wt wants many columns: the codes are turned, eight lanes' words of eight nibbles each,
+// in three exchanges between lanes one, two and four apart, and a lane then has eight columns of one row, one 16-byte piece of LDS (as
+// 32 pieces of 2 bytes these writes bounded the kernel: 2560 x 18432 22 us).
+template <int S>
+__device__ __forceinline__ uint32_t exchange_nibbles(uint32_t w, int lane) {
+    constexpr uint32_t kLow = S == 1 ? 0x0F0F0F0Fu : S == 2 ? 0x00FF00FFu : 0x0000FFFFu;
+    const bool lower = (lane & S) == 0;
+    int other = (int)w;
+    if constexpr (S == 1) other = __builtin_amdgcn_update_dpp(0, other, 0xB1, 0xF, 0xF, true);
+    if constexpr (S == 2) other = __builtin_amdgcn_update_dpp(0, other, 0x4E, 0xF, 0xF, true);
+    if constexpr (S == 4) {  // 7 - i, then 3 - i within four: four apart
+        other = __builtin_amdgcn_update_dpp(0, other, 0x141, 0xF, 0xF, true);
+        other = __builtin_amdgcn_update_dpp(0, other, 0x1B, 0xF, 0xF, true);
+    }
+    const uint32_t keep = lower ? kLow : ~kLow, turned = __builtin_amdgcn_alignbit(other, other, lower ? 32 - 4 * S : 4 * S);
+    return (w & keep) | (turned & ~keep);
+}
+__device__ __forceinline__ void unpack_weight(const PrepareArgs &p, int block, PrepareLds &lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 7, h = lane >> 3 & 1, kq = lane >> 4;
+    const int G = p.K / kGroupK, tiles = p.N / 128, g = block / tiles, n0 = block % tiles * 128, nt = n0 / kTileN + wave;
+    const u32x4 w = p.B[((size_t)nt * G + g) * 64 + lane];
+    const u32x4 scales = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, nt * kTileN + 8 * h, p.Gs));
+    const int j = i < 4 ? 2 * i : 2 * i - 7;  // the row in nibble i
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
+        const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(w[t], lane), lane), lane);
+        bf16x8 o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int code = (words[t] >> (4 * nibble_pos(j))) & 0xF;
-            tile[(32 * t + 8 * kq + j) * kTurnPitch + 16 * wave + c] = f32_to_bf16_bits((float)(code - 8) * s);
+        for (int c = 0; c < 8; ++c) {
+            const uint32_t pair = scales[c >> 1];
+            o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? pair >> 16 : pair)));
         }
+        *reinterpret_cast<bf16x8 *>(lds.weight + (32 * t + 8 * kq + j) * kTurnPitch + 16 * wave + 8 * h) = o;
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 32 * i + (tid >> 4), at = 8 * (tid & 15);
-        *reinterpret_cast<u32x4 *>(out + (size_t)(g * kGroupK + row) * N + blockIdx.x * 128 + at) =
-            *reinterpret_cast<const u32x4 *>(tile + row * kTurnPitch + at);
+    for (int r = 0; r < 4; ++r) {
+        const int row = 32 * r + (tid >> 4), at = 8 * (tid & 15);
+        *reinterpret_cast<u32x4 *>(p.wt + (size_t)(g * kGroupK + row) * p.N + n0 + at) = *reinterpret_cast<const u32x4 *>(lds.weight + row * kTurnPitch + at);
     }
 }
 
-// ---- the adapters' matrices turned -------------------------------------------------------------------------------
-// z = 0: at[a][k][rank] of a[a][rank][k]; z = 1: bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows
-// of several adapters at once, zeros for those of others, so it holds finite values alone; where A holds others, odd[a][k / 64] is set and
+// at[a][k][rank] of a[a][rank][k], or bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows of several
+// adapters at once, zeros for those of others, so it holds finite values alone; where A holds others, odd[a][k / 64] is set and
 // bank_grad_kernel adds their products for the rows of that adapter.
-__global__ __launch_bounds__(256) void turn_bank_kernel(const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, uint16_t *__restrict__ at,
-                                                        uint16_t *__restrict__ bt, uint8_t *__restrict__ odd, int K, int N, int rank) {
-    __shared__ uint16_t tile[64][kBankMaxRank + 2];
-    const int tid = threadIdx.x, which = blockIdx.z, len = which ? N : K, l0 = blockIdx.x * 64;
-    if (l0 >= len) return;
-    const size_t base = (size_t)blockIdx.y * rank * len;
-    if (which == 0) {
+__device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, PrepareLds &lds) {
+    const int tid = threadIdx.x, rank = p.rank, of_a = p.K / 64, parts = of_a + p.N / 64, a = block / parts, part = block % parts;
+    const bool is_a = part < of_a;
+    const int len = is_a ? p.K : p.N, l0 = (is_a ? part : part - of_a) * 64;
+    const size_t base = (size_t)a * rank * len;
+    if (is_a) {
         bool any = false;
-        for (int e = tid; e < rank * 64; e += 256) {
-            uint16_t v = a[base + (size_t)(e >> 6) * len + l0 + (e & 63)];
+        for (int e = tid; e < rank * 64; e += kPrepareThreads) {
+            uint16_t v = p.a[base + (size_t)(e >> 6) * len + l0 + (e & 63)];
             if ((v & 0x7F80u) == 0x7F80u) {
                 any = true;
                 v = 0;
             }
-            tile[e & 63][e >> 6] = v;
+            lds.bank[e & 63][e >> 6] = v;
         }
         any = __syncthreads_or(any);
-        if (tid == 0) odd[(size_t)blockIdx.y * (K / 64) + blockIdx.x] = any;
-        for (int e = tid; e < 64 * rank; e += 256) at[base + (size_t)l0 * rank + e] = tile[e / rank][e % rank];
+        if (tid == 0) p.odd[(size_t)a * of_a + part] = any;
+        for (int e = tid; e < 64 * rank; e += kPrepareThreads) p.at[base + (size_t)l0 * rank + e] = lds.bank[e / rank][e % rank];
     } else {
-        for (int e = tid; e < 64 * rank; e += 256) tile[e / rank][e % rank] = b[base + (size_t)l0 * rank + e];
+        for (int e = tid; e < 64 * rank; e += kPrepareThreads) lds.bank[e / rank][e % rank] = p.b[base + (size_t)l0 * rank + e];
         __syncthreads();
-        for (int e = tid; e < rank * 64; e += 256) bt[base + (size_t)(e >> 6) * len + l0 + (e & 63)] = tile[e & 63][e >> 6];
+        for (int e = tid; e < rank * 64; e += kPrepareThreads) p.bt[base + (size_t)(e >> 6) * len + l0 + (e & 63)] = lds.bank[e & 63][e >> 6];
     }
+}
+
+__global__ __launch_bounds__(kPrepareThreads) void bank_prepare_kernel(PrepareArgs p) {
+    __shared__ __align__(16) PrepareLds lds;
+    int block = blockIdx.x;
+    if (block < p.order_blocks) {
+        order_rows(p.rows.of, p.rows.order, p.rows.first, p.rows.rows, p.rows.count, block, lds.order);
+        return;
+    }
+    block -= p.order_blocks;
+    if (block < p.turn_blocks) turn_bank(p, block, lds);
+    else unpack_weight(p, block - p.turn_blocks, lds);
 }
 
 // sums over slices: x[0][i] += x[1][i] + ... (both projections in one launch)
@@ -144,29 +191,45 @@ __global__ __launch_bounds__(WM * WN * 64) void bank_dx_kernel(DxArgs p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
     const int r = lane & 31, h = lane >> 5;
-    auto product = [&](const char *stage) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf16x8 x[TM], w[TN];
-#pragma unroll
-            for (int i = 0; i < TM; ++i) x[i] = *reinterpret_cast<const bf16x8 *>(stage + unit_at(32 * (TM * wm + i) + r, 2 * kk + h));
-#pragma unroll
-            for (int j = 0; j < TN; ++j) w[j] = *reinterpret_cast<const bf16x8 *>(stage + BM * 64 + unit_at(32 * (TN * wn + j) + r, 2 * kk + h));
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], x[i], acc[j][i], 0, 0, 0);
-        }
+    struct Operands {
+        bf16x8 x[TM], w[TN];
     };
+    auto read = [&](const char *stage, int kk, Operands &o) {
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) fetch(first + s);
+        for (int i = 0; i < TM; ++i) o.x[i] = *reinterpret_cast<const bf16x8 *>(stage + unit_at(32 * (TM * wm + i) + r, 2 * kk + h));
+#pragma unroll
+        for (int j = 0; j < TN; ++j) o.w[j] = *reinterpret_cast<const bf16x8 *>(stage + BM * 64 + unit_at(32 * (TN * wn + j) + r, 2 * kk + h));
+    };
+    auto multiply = [&](const Operands &o) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.w[j], o.x[i], acc[j][i], 0, 0, 0);
+    };
+    // Operands are read half a step ahead, and the wavefronts meet in mid-step, where the second half's are in registers and the
+    // first half's products run: behind that, the present step's place is free for the step kStages on.
+    Operands now, then;
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(first + s);
+    wait_vector_loads<(kStages - 1) * (LM + LN)>();
+    __builtin_amdgcn_s_barrier();
+    read(lds, 0, now);
     for (int step = first; step < last; ++step) {
+        const int buffer = (step - first) % kStages;
+        read(lds + buffer * kStage, 1, then);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(now);
+        __builtin_amdgcn_sched_barrier(0);
         wait_vector_loads<(kStages - 2) * (LM + LN)>();
-        __builtin_amdgcn_s_barrier();
-        fetch(step + kStages - 1);
-        product(lds + (step - first) % kStages * kStage);
         wait_lds_reads();
+        __builtin_amdgcn_s_barrier();
+        fetch(step + kStages);
+        read(lds + (buffer + 1) % kStages * kStage, 0, now);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(then);
+        __builtin_amdgcn_sched_barrier(0);
     }
+    wait_lds_reads();
     wait_vector_loads<0>();
     if (p.u && slice == 0) {
         // U A: the runs of rows of one adapter among the block's positions, 32 of the rank at a time, U's bf16 value and then what that
@@ -200,7 +263,10 @@ __global__ __launch_bounds__(WM * WN * 64) void bank_dx_kernel(DxArgs p) {
                             *reinterpret_cast<u32x4 *>(lds + BM * 64 + unit_at(row, unit)) = v;
                         }
                     __syncthreads();
-                    product(lds);
+                    read(lds, 0, now);
+                    read(lds, 1, then);
+                    multiply(now);
+                    multiply(then);
                 }
             q0 = q1;
         }
@@ -474,18 +540,32 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     dx.K = k;
     dx.N = n;
     GradArgs grad{};
-    if (m > 0)
-        dequant_rows_kernel<<<dim3(n / 128, k / 128), 512, 0, hs>>>((const u32x4 *)B, (const uint16_t *)s, wt, k, n, groupsize == -1 ? 1 : k / 128);
+    PrepareArgs prepare{};
+    prepare.B = (const u32x4 *)B;
+    prepare.S = (const uint16_t *)s;
+    prepare.wt = wt;
+    prepare.K = k;
+    prepare.N = n;
+    prepare.Gs = groupsize == -1 ? 1 : k / 128;
     if (bank) {
         uint16_t *a_t = reinterpret_cast<uint16_t *>(at + w.at), *b_t = reinterpret_cast<uint16_t *>(at + w.bt);
         uint8_t *odd = reinterpret_cast<uint8_t *>(at + w.odd);
         float *t = reinterpret_cast<float *>(at + w.t), *u = reinterpret_cast<float *>(at + w.u);
         const uint16_t *lora_a = (const uint16_t *)bank->lora_a;
-        dx.rows = bank_order(adapter_of, m, count, true, at + w.order, hs);
+        dx.rows = bank_rows(adapter_of, m, count, at + w.order);
+        prepare.a = lora_a;
+        prepare.b = (const uint16_t *)bank->lora_b;
+        prepare.at = a_t;
+        prepare.bt = b_t;
+        prepare.odd = odd;
+        prepare.rows = dx.rows;
+        prepare.rank = rank;
+        prepare.order_blocks = count + 1;
+        prepare.turn_blocks = m > 0 ? count * (k / 64 + n / 64) : 0;
+        bank_prepare_kernel<<<prepare.order_blocks + prepare.turn_blocks + (m > 0 ? (n / 128) * (k / 128) : 0), kPrepareThreads, 0, hs>>>(prepare);
         if (m > 0) {
-            turn_bank_kernel<<<dim3((k > n ? k : n) / 64, count, 2), 256, 0, hs>>>(lora_a, (const uint16_t *)bank->lora_b, a_t, b_t, odd, k, n, rank);
-            bank_project(A, lora_a, dx.rows, t, k, rank, w.t_slices, hs);
-            bank_project(dC, b_t, dx.rows, u, n, rank, w.u_slices, hs);
+            const BankProjection of_x{A, lora_a, t, k, w.t_slices};
+            bank_project(BankProjection{dC, b_t, u, n, w.u_slices}, &of_x, dx.rows, rank, hs);
             if (w.t_slices > 1 || w.u_slices > 1)
                 sum_slices_kernel<<<dim3((unsigned)(((size_t)m * rank + 255) / 256), 2), 256, 0, hs>>>(t, w.t_slices, u, w.u_slices, (size_t)m * rank);
         }
@@ -495,6 +575,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
         dx.u = u;
         dx.scales = bank->scales;
         dx.rank = rank;
+    } else {
+        bank_prepare_kernel<<<(n / 128) * (k / 128), kPrepareThreads, 0, hs>>>(prepare);
     }
     if (m > 0) {
         switch (w.dx.kind) {
