@@ -297,11 +297,12 @@ typedef struct {
  * C[i] = A[i] * dequant(B, s) + scales[a] * (A[i] * lora_a[a]^T) * lora_b[a]^T with a = adapter_of[i]: rows of many requests, each
  * with an adapter of its own, beside one shared projection (the reference's formula for one adapter of all rows:
  * crates/kiln-model/src/lora_loader.rs:213-232).  Any m, rows of an adapter anywhere among the others.
- *   adapter_of  int32 [m], device memory; a value outside [0, count) is no adapter: the row is the plain GEMM's
+ *   adapter_of  int32 [m], device memory; a value outside [0, count) is no adapter: the row is the plain product
  *   workspace   as for the plain GEMM of the same sizes (kiln_w4a16_workspace_bytes)
  *   scratch     kiln_w4a16_gemm_bank_scratch_bytes, on 16 bytes; never decreases with m; holds nothing between calls
- * The low-rank term is summed in f32 (the projection kept to 2^-17 of itself) and added to the plain GEMM's result in bf16, which
- * is rounded once more: as the reference adds a delta to its bf16 base.
+ * The low-rank term is summed in f32 (the projection kept to 2^-17 of itself).  Up to 16 rows it lands on the f32 sums of the
+ * product, rounded once; beyond that on the plain GEMM's result in bf16, which is rounded once more, as the reference adds a delta to its
+ * bf16 base.
  */
 size_t kiln_w4a16_gemm_bank_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank);
 kiln_marlin_status_t kiln_w4a16_gemm_bank(

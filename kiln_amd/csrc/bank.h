@@ -39,4 +39,9 @@ struct BankProjection {
 };
 void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream);
 
+// up to 16 rows as they stand: y = x W + the low-rank term of their projections t, in one launch
+constexpr int kBankFewRows = 16;
+void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, const float *t, int slices,
+              int K, int N, bool per_column, hipStream_t stream);
+
 }  // namespace kiln

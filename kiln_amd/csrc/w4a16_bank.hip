@@ -7,6 +7,7 @@
 // from 257 rows on a launch in front puts them so.  The reference serves one adapter set per process
 // (crates/kiln-model/src/lora_loader.rs:213-232); this is its formula with the adapter a row's own.
 #include "bank.h"
+#include "bank_expand.h"
 #include "bank_order.h"
 #include "device_common.h"
 
@@ -18,17 +19,6 @@ __global__ __launch_bounds__(kOrderWaves * 64) void bank_order_kernel(const int 
                                                                       int rows, int count) {
     __shared__ OrderLds<kOrderWaves> lds;
     order_rows(of, order, first, rows, count, blockIdx.x, lds);
-}
-
-__device__ __forceinline__ bf16x8 load_bf16x8(const uint16_t *p) {
-    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4 *>(p));
-}
-
-// The row and the adapter (-1: none) of position p.
-__device__ __forceinline__ void row_at(const BankRows &r, int p, int &row, int &a) {
-    row = p < r.rows ? (r.order ? r.order[p] : p) : -1;
-    a = row >= 0 ? r.of[row] : -1;
-    if ((unsigned)a >= (unsigned)r.count) a = -1;
 }
 
 // U pieces of a projection's contraction, 64 long each and 256 apart, all their loads in front of their products.  A lane's part of a
@@ -116,53 +106,6 @@ __global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one
     }
 }
 
-// y[row] += s_a T[row] B_a^T, formed as B_a (its rows the columns of y) times T^T, so that a lane holds consecutive columns of one row:
-// two products of 16 columns, whose rows of B_a are dealt out such that their results are eight columns side by side.  T goes in as two
-// bf16 parts whose sum is within 2^-17 of it, one product each with the same rows of B.  S: the contraction's steps of 32.
-// A product's result is taken by the rows of its adapter alone (a lane has one row): what another adapter holds that is no number
-// stays with its own rows.
-__device__ __forceinline__ int column_of(int tile, int c) { return 32 * (tile >> 1) + 8 * (c >> 2) + 4 * (tile & 1) + (c & 3); }
-
-template <int S>
-struct ExpandRow {  // this lane's part of its row's T
-    bf16x8 hi[S], lo[S];
-    __device__ __forceinline__ void set(const float *t, float scale, bool live, int q, int rank) {
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int at = 32 * s + 8 * q;
-            hi[s] = lo[s] = bf16x8_zero();
-            if (live && at < rank)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float f = t[at + i] * scale;
-                    hi[s][i] = (__bf16)f;
-                    lo[s][i] = (__bf16)(f - (float)hi[s][i]);
-                }
-        }
-    }
-};
-// 16 TILES columns from n0 on, of adapter `mat`'s rows of B (past the rank: the last eight again, times zeros)
-template <int S, int TILES>
-__device__ __forceinline__ void expand_rows(const uint16_t *__restrict__ mat, int c, int q, int rank, bf16x8 (&b)[TILES][S]) {
-#pragma unroll
-    for (int tile = 0; tile < TILES; ++tile)
-#pragma unroll
-        for (int s = 0; s < S; ++s) b[tile][s] = load_bf16x8(mat + (size_t)column_of(tile, c) * rank + min(32 * s + 8 * q, rank - 8));
-}
-template <int S, int TILES>
-__device__ __forceinline__ void expand_product(const bf16x8 (&b)[TILES][S], const ExpandRow<S> &t, bool own, f32x4 (&acc)[TILES]) {
-#pragma unroll
-    for (int tile = 0; tile < TILES; ++tile) {
-        f32x4 v = acc[tile];
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[tile][s], t.hi[s], v, 0, 0, 0);
-            v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[tile][s], t.lo[s], v, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[tile][i] = own ? v[i] : acc[tile][i];
-    }
-}
 // eight columns of y to the accumulators of two tiles, and back
 __device__ __forceinline__ void take_columns(u32x4 v, f32x4 &even, f32x4 &odd) {
     even = f32x4{__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xFFFF0000u), __builtin_bit_cast(float, v.y << 16),
@@ -174,28 +117,6 @@ __device__ __forceinline__ u32x4 give_columns(const f32x4 &even, const f32x4 &od
     auto pair = [](float lo, float hi) { return f32_to_bf16_bits(lo) | (uint32_t)f32_to_bf16_bits(hi) << 16; };
     return u32x4{pair(even[0], even[1]), pair(even[2], even[3]), pair(odd[0], odd[1]), pair(odd[2], odd[3])};
 }
-// T's slices summed, [positions][rank] of this block's from p0 on
-template <int P>
-__device__ __forceinline__ void sum_projected(const float *__restrict__ t, const BankRows &rows, int p0, int rank, int slices, int tid,
-                                              float (&ts)[P][kBankMaxRank + 4]) {
-    const size_t stride = (size_t)rows.rows * rank;
-    for (int e = tid; e < P * rank; e += 256) {
-        const int r = e / rank;
-        const float *from = t + (size_t)p0 * rank + e;
-        float v = 0.f;
-        if (p0 + r < rows.rows) {
-            int s = 0;
-            for (; s + 4 <= slices; s += 4) {
-                const float v0 = from[s * stride], v1 = from[(s + 1) * stride], v2 = from[(s + 2) * stride], v3 = from[(s + 3) * stride];
-                v += (v0 + v1) + (v2 + v3);
-            }
-            for (; s < slices; ++s) v += from[s * stride];
-        }
-        ts[r][e - r * rank] = v;
-    }
-    __syncthreads();
-}
-
 // Rows as they stand: 16 of them x 64 columns to a block, the adapters met dealt out to its four wavefronts, each of which takes the
 // rows of its own: nothing to add up, and with an adapter per row (a decode step) the loads of four adapters' rows of B go out together.
 // Bound by those loads' latency.  16 rows of 16 adapters, 18432 columns, rank 16: 27 us with the adapters one after the other.
@@ -239,7 +160,7 @@ __global__ __launch_bounds__(256) void bank_expand_kernel(uint16_t *__restrict__
             expand_rows<S, 4>(mat + ((size_t)mine[first + g] * N + n0) * rank, c, q, rank, b[g]);
         }
         if (first == 0) {
-            sum_projected<16>(t, rows, p0, rank, slices, tid, ts);
+            sum_projected<16>(t, rows, p0, rank, slices, tid, 256, ts);
             tv.set(ts[c], scale, live, q, rank);
 #pragma unroll
             for (int i = 0; i < 2; ++i) take_columns(was[i], acc[2 * i], acc[2 * i + 1]);
@@ -282,7 +203,7 @@ __global__ __launch_bounds__(256) void bank_expand_ordered_kernel(uint16_t *__re
 #pragma unroll
         for (int i = 0; i < 2; ++i) was[r][i] = *reinterpret_cast<const u32x4 *>(dst[r] + min(n0, end - 64) + 32 * i);
     }
-    sum_projected<64>(t, rows, p0, rank, slices, tid, ts);
+    sum_projected<64>(t, rows, p0, rank, slices, tid, 256, ts);
     ExpandRow<S> tv[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) tv[r].set(ts[16 * r + c], __shfl(scale, 16 * r + c), a_of[r] >= 0, q, rank);
@@ -342,6 +263,14 @@ void launch_project(const BankProjection &one, const BankProjection &two, const 
     else if (jt == 3) launch_project<3, RT, W>(one, two, r, rank, stream);
     else launch_project<4, RT, W>(one, two, r, rank, stream);
 }
+
+// Base product and low-rank term in one launch (bank_few), or the plain GEMM and the term behind it?  The one saves a launch and the
+// result's way through memory, the other's base product is the faster one on wide outputs.  1 / 8 / 16 rows of as many adapters, rank 16, us:
+// 2560 -> 2560 7.4 / 9.6 / 11.7 against 11.0 / 12.4 / 14.4, 4096 -> 4096 8.0 / 10.6 / 13.1 against 11.1 / 13.0 / 15.3, 2560 -> 8192 8.8 / 11.0 / 13.3
+// against 11.2 / 13.3 / 15.5, 8192 -> 8192 13.4 / 16.9 / 21.2 against 15.0 / 17.9 / 21.1; but 9216 -> 2560 10.5 / 15.0 / 19.3 against 13.3 / 15.7 / 18.2,
+// 14336 -> 4096 13.5 / 18.3 / 24.8 against 16.0 / 19.0 / 22.2, 2560 -> 18432 13.3 / 16.4 / 20.7 against 12.8 / 15.7 / 18.6, 5120 -> 27648 27.7 / 37.5 / 48.9
+// against 21.9 / 26.5 / 30.8.
+bool takes_few(int m, int n, int k) { return m <= kBankFewRows && n <= 8192 && (m <= 8 || k <= 8192); }
 
 }  // namespace
 
@@ -418,17 +347,27 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     if (!bank->lora_a || !bank->lora_b || !bank->scales) return KILN_W4A16_ERR_ARGUMENT;
     for (const void *p : {bank->lora_a, bank->lora_b, static_cast<const void *>(scratch)})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    char *at = reinterpret_cast<char *>(scratch);
+    BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
+    float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
+    const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
+    if (takes_few(prob_m, prob_n, prob_k)) {
+        if (prob_n % 256 != 0 || prob_k % 128 != 0 || (groupsize != -1 && groupsize != 128)) return KILN_W4A16_ERR_PROB_SHAPE;
+        if (!A || !B || !C || !s || !workspace) return KILN_W4A16_ERR_ARGUMENT;
+        for (const void *p : {A, B, static_cast<const void *>(C), s, static_cast<const void *>(workspace)})
+            if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+        rows.order = rows.first = nullptr;
+        bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
+        bank_few(A, B, s, C, *bank, rows, t, slices, prob_k, prob_n, groupsize == -1, hs);
+        return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
+    }
     // the plain GEMM's checks and its launches first: nothing is launched for a call that it refuses
     const kiln_marlin_status_t st =
         kiln_marlin_w4a16_gemm(A, B, C, const_cast<void *>(s), prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, -1, -1, -1, 16);
     if (st != KILN_W4A16_OK) return st;
-    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    char *at = reinterpret_cast<char *>(scratch);
-    BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
     if (prob_m < kBankOrderedFrom) rows.order = rows.first = nullptr;
     else bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
-    float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
-    const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
     bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
     uint16_t *y = (uint16_t *)C;
     const uint16_t *m = (const uint16_t *)bank->lora_b;

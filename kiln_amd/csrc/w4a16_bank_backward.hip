@@ -9,6 +9,7 @@
 // rows of an adapter.  Rows are taken in the order of their adapters throughout.
 #include "async_loads.h"
 #include "bank.h"
+#include "bank_expand.h"
 #include "bank_order.h"
 #include "device_common.h"
 
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(WM * WN * 64) void bank_dx_kernel(DxArgs p) {
                             for (int i = 0; i < 8; ++i) {
                                 const float f = u[i] * scale;
                                 const __bf16 hi = (__bf16)f;
-                                v[i] = side ? (__bf16)(f - (float)hi) : hi;
+                                v[i] = side ? lower_part(f, hi) : hi;
                             }
                         }
                         *reinterpret_cast<bf16x8 *>(lds + unit_at(row, unit)) = v;
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
             for (int i = 0; i < 8; ++i) {
                 const float x = at + 8 * q + i < end ? w[j][i] : 0.f;
                 hi[j][i] = (__bf16)x;
-                lo[j][i] = (__bf16)(x - (float)hi[j][i]);
+                lo[j][i] = lower_part(x, hi[j][i]);
             }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

@@ -1,7 +1,7 @@
 // The experts of a mixture-of-experts MLP for a few tokens, and the router's choice of them.
 //
-// Bound by the packs of the experts that have rows, read once (a token of 8 experts of 64 reads an eighth of the layer).  Three launches:
-// gate, up and silu(gate) * up of every (token, expert) pair, the down projection of every pair, and the sum over a token's pairs.  A
+// Bound by the packs of the experts that have rows, read once (a token of 8 experts of 64 reads an eighth of the layer).  Two launches or
+// three: gate, up and silu(gate) * up of every (token, expert) pair, then the down projection of every pair and the sum over a token's.  A
 // block works out by itself which experts are present and which pairs are theirs: the ids of a run, 64 tokens at most, are a few KB,
 // and a launch in front that sorts them costs more than reading them in every block.
 #include <hip/hip_runtime.h>
@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "device_common.h"
+#include "few_rows.h"
 #include "kiln_w4a16.h"
 
 namespace kiln {
@@ -96,13 +97,9 @@ __device__ __forceinline__ int pairs_of(const MoeArgs &p, const MoePairs *lds, i
     return count;
 }
 
-// Up to 16 rows of one expert times S column tiles of its pack.  The groups of K are dealt out to W wavefronts, GW to each, whose part of
-// the rows stays in registers while the columns go by: per tile nothing is read but its chunks (GW KB a wavefront, the next tile's asked
-// for before the present one is multiplied) and their scales.  The rows' sums over the groups, which the zero-point and the bias of the
-// expanded codes are taken off with, come out of products with ones, once, and go in as what the products start from.  K beyond W GW
-// groups: in passes, the sums kept.  The wavefronts meet in LDS at the end.
-// With the rows read again for every tile or two (64 tokens, 8 of 64 experts, 2560 -> 1024 -> 2560) the two launches took 54 and 51 us: the
-// wavefronts waited for rows, 4 KB of them to a KB of codes.
+// Up to 16 rows of one expert times S column tiles of its pack (few_rows.h); the wavefronts meet in LDS at the end.
+// With the rows read again for every tile or two (64 tokens, 8 of 64 experts, 2560 -> 1024 -> 2560) the two launches took 54 and 51 us, not
+// 39 and 25: the wavefronts waited for rows, 4 KB of them to a KB of codes.
 template <bool IN, bool FEW, int W, int GW, int S>
 __global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
     __shared__ MoePairs pairs;
@@ -126,58 +123,11 @@ __global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
     const int nt0 = blockIdx.x * S;
     const u32x4 *b = (IN ? p.b_in : p.b_out) + ((size_t)e * (N / kTileN) + nt0) * G * 64 + lane;
     const uint16_t *s = (IN ? p.s_in : p.s_out) + ((size_t)e * (N / kTileN) + nt0) * Gs * kTileN + c;
-    const bf16x8 ones = bf16x8_splat_one();
     for (int r0 = 0; r0 < count; r0 += 16) {
         const int pair = list[min(r0 + c, count - 1)];
         const uint16_t *row = (IN ? p.x + (size_t)(pair / p.top) * K : p.h + (size_t)pair * K) + 8 * q;
         f32x4 total[S];
-#pragma unroll
-        for (int i = 0; i < S; ++i) total[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int first = wave * GW; first < G; first += W * GW) {
-            // groups past the last: the last again, with a scale of zero
-            auto group = [&](int u) { return min(first + u, G - 1); };
-            u32x4 w[2][GW];
-            uint16_t scale[2][GW];
-            auto fetch = [&](int tile) {
-#pragma unroll
-                for (int u = 0; u < GW; ++u) {
-                    w[tile & 1][u] = b[(size_t)(tile * G + group(u)) * 64];
-                    scale[tile & 1][u] = s[(size_t)(tile * Gs + (p.per_column ? 0 : group(u))) * kTileN];
-                }
-            };
-            fetch(0);
-            bf16x8 x[GW][4];
-            f32x4 start[GW];
-#pragma unroll
-            for (int u = 0; u < GW; ++u)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) x[u][t] = *reinterpret_cast<const bf16x8 *>(row + group(u) * kGroupK + 32 * t);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int u = 0; u < GW; ++u) {
-                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int t = 0; t < 4; ++t) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][t], ones, sum, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) start[u][i] = -kCodeBias * sum[i];
-            }
-#pragma unroll
-            for (int tile = 0; tile < S; ++tile) {
-                if (tile + 1 < S) fetch(tile + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < GW; ++u) {
-                    const u32x4 &v = w[tile & 1][u];
-                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][0], codes_to_bf16x8(v.x, dc), start[u], 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][1], codes_to_bf16x8(v.y, dc), acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][2], codes_to_bf16x8(v.z, dc), acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u][3], codes_to_bf16x8(v.w, dc), acc, 0, 0, 0);
-                    const float sc = first + u < G ? f16_bits_to_f32(scale[tile & 1][u]) : 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) total[tile][i] += sc * acc[i];
-                }
-            }
-        }
+        few_rows_product<GW, S>(row, b, s, G, p.per_column, wave, W, dc, total, [] {});
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -203,6 +153,56 @@ __global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
             }
         }
         __syncthreads();
+    }
+}
+
+// The down projection and the sum in one launch, for a few pairs: a block takes one column tile for all tokens, its wavefronts share out the
+// experts present (and, where those are fewer, parts of their groups), each with an f32 sum per token and column in LDS, added up in
+// the wavefronts' order.  Rows are read once per column tile here, and experts beyond the wavefronts come one after the other: 8 pairs
+// (2560 -> 1024 -> 2560) 13.9 us a call against 15.7 with the two launches, 52 pairs (2048 -> 1280 -> 2048) 31 against 24.
+constexpr int kJoinWaves = 8, kMoeJoinedPairs = 16;
+template <int GW>
+__global__ __launch_bounds__(kJoinWaves * 64) void moe_join_kernel(MoeArgs p) {
+    __shared__ int lists[kJoinWaves][kMoeRun];
+    __shared__ float sums[kJoinWaves][kMoeRun][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
+    const DequantConsts dc = dequant_consts();
+    const int pairs = p.tokens * p.top, id = id_of(p, lane, pairs);
+    const float weight = lane < pairs ? p.weights[lane] : 0.f;
+    for (int i = lane; i < p.tokens * 16; i += 64) sums[wave][i >> 4][i & 15] = 0.f;
+    int present = 0;
+    for (unsigned long long left = __ballot(id >= 0); left; ++present) left &= ~__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(left)));
+    const int G = p.n_out / kGroupK, Gs = p.per_column ? 1 : G, nt = blockIdx.x, tiles = p.n_down / kTileN;
+    const int parts = present ? min((G + GW - 1) / GW, (kJoinWaves + present - 1) / present) : 1;
+    int *list = lists[wave];
+    for (int unit = wave; unit < present * parts; unit += kJoinWaves) {
+        const int e = expert_in_lanes(id, unit / parts), count = pairs_of(p, nullptr, id, e, lane, list);
+        const unsigned long long named = __ballot(id == e);
+        for (int r0 = 0; r0 < count; r0 += 16) {
+            f32x4 total[1];
+            few_rows_product<GW, 1>(p.h + (size_t)list[min(r0 + c, count - 1)] * p.n_out + 8 * q, p.b_out + ((size_t)e * tiles + nt) * G * 64 + lane,
+                                    p.s_out + ((size_t)e * tiles + nt) * Gs * kTileN + c, G, p.per_column, unit % parts, parts, dc, total, [] {});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int pair = list[min(r0 + 4 * q + i, count - 1)], token = pair / p.top;
+                float w = __shfl(weight, pair);
+                if (__popcll(named) != count)  // some token names the expert again: its weights together
+                    for (int j = 1; j < p.top; ++j) {
+                        const int other = min(pair + j, 63);
+                        const float more = __shfl(weight, other);
+                        if (pair + j < (token + 1) * p.top && (named >> other & 1)) w += more;
+                    }
+                if (r0 + 4 * q + i < count) sums[wave][token][c] += w * total[0][i];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    for (int i = tid; i < p.tokens * 16; i += kJoinWaves * 64) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w) v += sums[w][i >> 4][i & 15];
+        p.y[(size_t)(i >> 4) * p.n_down + nt * 16 + (i & 15)] = f32_to_bf16_bits(v);
     }
 }
 
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs p) {
 }
 
 // Column tiles to a block: many where the blocks are enough all the same (their rows and lists are read once each), two where the experts
-// present are few.  Wavefronts and groups by K: five groups to a wavefront at most.
+// present are few.
 template <bool IN, bool FEW, int W, int GW>
 void launch_expert(const MoeArgs &a, int slots, hipStream_t stream) {
     constexpr int kMany = W == 4 ? 8 : 4;
@@ -248,13 +248,8 @@ void launch_expert(const MoeArgs &a, int slots, hipStream_t stream) {
 }
 template <bool IN, bool FEW>
 void launch_experts(const MoeArgs &a, int slots, hipStream_t stream) {
-    const int G = (IN ? a.hidden : a.n_out) / kGroupK;
-    if (G <= 8) launch_expert<IN, FEW, 4, 2>(a, slots, stream);
-    else if (G <= 12) launch_expert<IN, FEW, 4, 3>(a, slots, stream);
-    else if (G <= 16) launch_expert<IN, FEW, 4, 4>(a, slots, stream);
-    else if (G <= 20) launch_expert<IN, FEW, 4, 5>(a, slots, stream);
-    else if (G <= 32) launch_expert<IN, FEW, 8, 4>(a, slots, stream);
-    else launch_expert<IN, FEW, 8, 5>(a, slots, stream);
+    with_few_rows_split((IN ? a.hidden : a.n_out) / kGroupK,
+                        [&](auto waves, auto groups) { launch_expert<IN, FEW, decltype(waves)::value, decltype(groups)::value>(a, slots, stream); });
 }
 
 // ---- the router's choice -------------------------------------------------------------------------------------------
@@ -382,13 +377,19 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
                         (uint16_t *)scratch, reinterpret_cast<float *>(static_cast<char *>(scratch) + moe_h_bytes(prob_m, top_k, n_out)),
                         (uint16_t *)y + (size_t)m0 * n_down, m, top_k, experts, hidden, n_out, n_down, groupsize == -1};
         const int slots = m * top_k < experts ? m * top_k : experts;
-        if (m <= 64 / top_k) {  // whole tokens in a wavefront's lanes
-            launch_experts<true, true>(a, slots, hs);
-            launch_experts<false, true>(a, slots, hs);
-        } else {
-            launch_experts<true, false>(a, slots, hs);
-            launch_experts<false, false>(a, slots, hs);
+        const bool few = m <= 64 / top_k;  // whole tokens in a wavefront's lanes
+        if (few) launch_experts<true, true>(a, slots, hs);
+        else launch_experts<true, false>(a, slots, hs);
+        if (few && m * top_k <= kMoeJoinedPairs) {
+            const int G = n_out / kGroupK;
+            if (G % 8 == 0) moe_join_kernel<8><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
+            else if (G % 6 == 0) moe_join_kernel<6><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
+            else if (G % 5 == 0) moe_join_kernel<5><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
+            else moe_join_kernel<4><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
+            continue;
         }
+        if (few) launch_experts<false, true>(a, slots, hs);
+        else launch_experts<false, false>(a, slots, hs);
         moe_sum_kernel<<<dim3((n_down / 4 + 255) / 256, m), 256, 0, hs>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;

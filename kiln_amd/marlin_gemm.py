@@ -584,7 +584,7 @@ def marlin_w4a16_gemm_bank(a: torch.Tensor, b_packed: torch.Tensor, scales: torc
 
     `bank_a` bf16 `[count, rank, k]`, `bank_b` bf16 `[count, n, rank]`, `bank_scales` f32 `[count]`, `adapter_of` i32 `[m]`; rank a
     multiple of 8 up to 64 (zero rows of A and columns of B for adapters of a lower rank: `lora.make_bank`).  A row whose
-    `adapter_of` is outside `[0, count)` has no adapter and is `marlin_w4a16_gemm`'s row.
+    `adapter_of` is outside `[0, count)` has no adapter and is the plain product's.
     """
     y = _calls.gemm_bank(a, b_packed, scales, groupsize, bank_a, bank_b, bank_scales, adapter_of, out)
     if y is not None:

@@ -3,9 +3,10 @@ against the formulas in 64 bits.
 
 Tolerances.  U = 2^-8 is the most that a rounding to bf16 changes a value by, relative to it; F = 2^-24 the same for f32.  A sum of n
 products in f32 is off by at most n F times the sum of the products' magnitudes, whatever its order.
-* forward: the result is the plain GEMM's bf16 row plus the low-rank term, rounded once: U |y| and, for the term, the projection's f32
-  sum (k F), its two bf16 parts (2^-16: the second part is rounded by U of a part that is U of the value) and the second sum (2 rank F + a few),
-  relative to the sum of magnitudes.
+* forward: the base product in f32, where the kernels multiply 128 + code and take the rest off: (k + 8) F times the sum of |x| * 280 * scale
+  (144 at most + 136); from 17 rows on it is rounded before the low-rank term is added (U of it), which is then rounded (U |y|) in
+  every case.  For the term, the projection's f32 sum (k F), its two bf16 parts (2^-16: the second part is rounded by U of a part that
+  is U of the value) and the second sum (2 rank F + a few), relative to the sum of magnitudes.
 * dx: a weight is rounded to bf16 (U), so U times the sum of |dy| |W|, plus f32 sums (n F) and the low-rank term as above; U |dx| at the end.
 * dA, dB: the inner product in f32 (K F), the sum over rows (rows F), U of the result.
 """
@@ -57,17 +58,22 @@ def check(got, want, bound):
 
 
 def check_forward(p, y):
-    base = marlin_gemm.marlin_w4a16_gemm(p["x"], p["b"], p["s"], p["g"])
-    rows_without = (p["of"] < 0) | (p["of"] >= len(p["sc"]))
-    assert torch.equal(y[rows_without].view(torch.int16), base[rows_without].view(torch.int16))
-    want, size = base.double(), torch.zeros_like(base, dtype=torch.float64)
-    k, rank = p["x"].shape[1], p["a_"].shape[1]
+    (m, k), rank = p["x"].shape, p["a_"].shape[1]
+    if m > 16:                                    # a row without an adapter is the plain GEMM's, to the bit
+        base = marlin_gemm.marlin_w4a16_gemm(p["x"], p["b"], p["s"], p["g"])
+        without = (p["of"] < 0) | (p["of"] >= len(p["sc"]))
+        assert torch.equal(y[without].view(torch.int16), base[without].view(torch.int16))
+    w = marlin_gemm.dequant_f32(p["b"], p["s"], p["g"]).double()
+    tiled = p["s"].reshape(-1, p["s"].shape[0], 16).transpose(0, 1).reshape(p["s"].shape)
+    scale = tiled.double().repeat_interleave(k // tiled.shape[0], 0)
+    want = p["x"].double() @ w
+    bound = (p["x"].double().abs() @ scale) * 280 * (k + 8) * F + (U * want.abs() if m > 16 else 0.0)
     for j in range(len(p["sc"])):
         mine, s, a, b = p["of"] == j, p["sc"][j].double(), p["a_"][j].double(), p["b_"][j].double()
         x = p["x"][mine].double()
         want[mine] += s * ((x @ a.t()) @ b.t())
-        size[mine] = s.abs() * ((x.abs() @ a.abs().t()) @ b.abs().t())
-    check(y, want, size * ((k + 2 * rank + 64) * F + 2.0 ** -16) + base.double().abs() * 4 * F)
+        bound[mine] += s.abs() * ((x.abs() @ a.abs().t()) @ b.abs().t()) * ((k + 2 * rank + 64) * F + 2.0 ** -16)
+    check(y, want, bound * (1 + U))
 
 
 def check_backward(p, da, d_a, d_b):

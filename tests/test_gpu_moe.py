@@ -78,7 +78,8 @@ def check_layer(args, y):
 
 LAYERS = [
     (1, 8, 64, 2560, 1024, 2560, 128, "any"), (1, 1, 1, 128, 128, 256, -1, "any"), (2, 16, 16, 256, 256, 512, 128, "any"),
-    (5, 2, 8, 384, 640, 768, -1, "any"), (13, 4, 32, 2048, 1280, 2048, -1, "any"), (16, 8, 1024, 128, 128, 256, 128, "any"),
+    (5, 2, 8, 384, 640, 768, -1, "any"), (3, 5, 9, 256, 768, 512, 128, "any"), (1, 16, 3, 256, 1152, 256, 128, "twice"), (8, 2, 2, 128, 640, 256, 128, "twice"),
+    (16, 1, 1, 128, 1024, 256, -1, "any"), (2, 2, 4, 11008, 5504, 512, 128, "any"), (13, 4, 32, 2048, 1280, 2048, -1, "any"), (16, 8, 1024, 128, 128, 256, 128, "any"),
     (17, 3, 5, 640, 384, 256, 128, "any"), (33, 1, 4, 256, 256, 256, 128, "one"), (64, 8, 64, 1024, 256, 1024, 128, "any"),
     (65, 5, 7, 256, 128, 512, 128, "any"), (200, 2, 3, 384, 256, 256, -1, "one"), (9, 4, 6, 256, 128, 256, 128, "twice"),
     (64, 16, 24, 128, 128, 256, 128, "twice"), (4, 2, 8, 256, 128, 256, 128, "none"), (70, 3, 8, 256, 128, 256, 128, "beyond"),
@@ -151,3 +152,92 @@ def test_layer_from_bf16_weights():
     mlp = marlin_gemm.marlin_w4a16_mlp(rows, experts.b_gate_up[4], experts.s_gate_up[4], experts.b_down[4], experts.s_down[4], 128)
     scale = mlp.double().abs().max()
     assert ((one.double() - mlp.double()).abs().max() / scale).item() < 4 * U
+
+
+def bits(t):
+    return t.view(torch.int16).clone()
+
+
+@pytest.mark.parametrize("m,top,experts", [(1, 8, 16), (12, 4, 16), (40, 6, 16)])
+def test_same_bits_again_on_views_other_streams_and_into_a_given_tensor(m, top, experts):
+    args = layer(m, top, experts, 256, 256, 512, 128, seed=1)
+    y = bits(marlin_gemm.marlin_w4a16_moe(*args))
+    x, of, weights, *packs = args
+    wide = (torch.cat([x, x], 1)[:, 256:], torch.stack([of, of], 2)[:, :, 1], torch.cat([weights, weights], 1)[:, :top], *packs)
+    assert torch.equal(bits(marlin_gemm.marlin_w4a16_moe(*wide)), y)
+    room = torch.full((m + 2, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        out = marlin_gemm.marlin_w4a16_moe(*args, out=room[1:m + 1])
+    stream.synchronize()
+    assert out.data_ptr() == room[1:].data_ptr() and torch.equal(bits(out), y)
+    assert bool((room[0] == 7).all()) and bool((room[m + 1] == 7).all())
+    logits = torch.randn(m, 2 * experts, device="cuda")
+    a, b = marlin_gemm.moe_route(logits[:, ::2], top), marlin_gemm.moe_route(logits[:, ::2].contiguous(), top)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("m,top", [(1, 8), (12, 4), (70, 2)])
+def test_a_layer_replayed_from_a_graph(m, top):
+    parts = [layer(m, top, 12, 256, 256, 512, 128, seed=s) for s in (2, 3, 4)]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    logits = [torch.randn(m, 12, device="cuda", generator=gen) for _ in parts]
+    live = [t.clone() if torch.is_tensor(t) else t for t in parts[0]]
+    live_logits = logits[0].clone()
+
+    def call(l, a):
+        of, weights = marlin_gemm.moe_route(l, top)
+        return of, weights, marlin_gemm.marlin_w4a16_moe(a[0], of, weights, *a[3:])
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        call(live_logits, live)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            made = call(live_logits, live)
+        for l, a in zip(logits + logits, parts + parts):
+            live_logits.copy_(l)
+            for to, t in zip(live, a):
+                if torch.is_tensor(t):
+                    to.copy_(t)
+            graph.replay()
+            stream.synchronize()
+            got = [t.clone() for t in made]
+            want = call(l, a)
+            stream.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(bits(got[2]), bits(want[2]))
+
+
+def test_what_is_no_number_stays_with_its_token_and_its_expert():
+    x, of, weights, b_in, s_in, b_out, s_out, g = layer(20, 2, 6, 256, 128, 256, 128, seed=6)
+    of[:, 0], of[:, 1] = torch.arange(20, device="cuda") % 6, (torch.arange(20, device="cuda") + 1) % 6
+    y = bits(marlin_gemm.marlin_w4a16_moe(x, of, weights, b_in, s_in, b_out, s_out, g))
+    bad_x, bad_s, bad_w = x.clone(), s_in.clone(), weights.clone()
+    bad_x[3, 5], bad_s[2, 1, 40], bad_w[7, 1] = math.nan, math.nan, math.inf
+    z = marlin_gemm.marlin_w4a16_moe(bad_x, of, bad_w, b_in, bad_s, b_out, s_out, g)
+    hit = (of == 2).any(1)
+    hit[3] = hit[7] = True
+    assert torch.equal(bits(z)[~hit], y[~hit]) and not bool(torch.isfinite(z[3]).any()) and not bool(torch.isfinite(z[7]).all())
+
+
+def test_no_tokens_and_refusals():
+    args = layer(4, 2, 3, 256, 128, 256, 128)
+    x, of, weights, b_in, s_in, b_out, s_out, g = args
+    assert marlin_gemm.marlin_w4a16_moe(x[:0], of[:0], weights[:0], *args[3:]).shape == (0, 256)
+    of_none, w_none = marlin_gemm.moe_route(torch.empty(0, 5, device="cuda"), 2)
+    assert of_none.shape == (0, 2) and w_none.shape == (0, 2)
+    for change, text in (((x.half(), *args[1:]), "x must be bf16"), ((x, of[:3], *args[2:]), "must be \\[m=4"), ((x, of.long(), *args[2:]), "expert_of must be i32"),
+                         ((x, of, weights.half(), *args[3:]), "weights f32"), ((x, of, weights, b_in[:2], *args[4:]), "s_gate_up must be"),
+                         ((x[:, :128], *args[1:]), "b_gate_up must be"), ((x, of, weights, b_in, s_in, b_out, s_out, 64), "groupsize"),
+                         ((x, of, weights, b_in, s_in, b_out.cpu(), s_out, g), "must be on"), ((x, of.repeat(1, 9), weights.repeat(1, 9), *args[3:]), "top_k must be")):
+        with pytest.raises(marlin_gemm.MarlinGemmError, match=text):
+            marlin_gemm.marlin_w4a16_moe(*change)
+    logits = torch.zeros(3, 8, device="cuda")
+    for call, text in (((logits, 0), "top_k"), ((logits, 9), "top_k"), ((logits.double(), 2), "f32, bf16 or f16"), ((logits[0], 2), "must be \\[m"),
+                       ((torch.zeros(2, 1025, device="cuda"), 2), "1 to 1024"), ((logits.cpu(), 2), "on CUDA")):
+        with pytest.raises(marlin_gemm.MarlinGemmError, match=text):
+            marlin_gemm.moe_route(*call)
+    with pytest.raises(moe.MarlinProjError, match="do not match"):
+        moe.pack_experts(torch.zeros(2, 256, 128), torch.zeros(2, 256, 256), torch.zeros(2, 128, 256))
