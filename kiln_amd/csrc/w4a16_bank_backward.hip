@@ -28,10 +28,15 @@ struct PrepareArgs {
     BankRows rows;
     int K, N, Gs, rank;
     int order_blocks, turn_blocks;
+    const uint16_t *dy;     // few rows: [m, N],
+    float *partial;         // [slices, m, K]
+    int m, slices;
 };
-constexpr int kPrepareThreads = 512, kTurnPitch = 128 + 8;
+constexpr int kPrepareThreads = 512, kTurnPitch = 128 + 8, kFewPitch = 128 + 4, kFewDyPitch = 256 + 8;
 union PrepareLds {
+    uint16_t dy[64 * kFewDyPitch];
     uint16_t weight[128 * kTurnPitch];
+    float sums[64 * kFewPitch];
     uint16_t bank[64][kBankMaxRank + 2];
     OrderLds<kPrepareThreads / 64> order;
 };
@@ -82,11 +87,78 @@ __device__ __forceinline__ void unpack_weight(const PrepareArgs &p, int block, P
     }
 }
 
+// Up to 64 rows: partial[slice][row][k] = sum over the slice's columns of dy[row][n] W[k][n], the codes unpacked where they are multiplied.
+// With the codes turned, and the lanes' words of a chunk dealt out for it (lane i + 8 kq + 32 h has column i + 8 h's), a word is the operand of
+// a product of 32 rows of k x 16 columns as it stands: nothing of W goes through memory again or LDS, and of dy a row's 16 values serve 128 of k.
+// A block takes one scale group and slice, a wavefront 32 rows of k and every other eight of sixteen column tiles, whose part of dy is in
+// LDS; the halves meet there.  Bound by its start, and by its instructions' (straight-line code is read from memory once in every
+// launch: four tiles to a turn of the loop, not all eight, took 45 rows of 4096 <- 2560 from 20 us to 16, dy through LDS to 15).
+constexpr int kFewRows = 64, kFewAhead = 4, kFewTiles = 16, kFewColumns = kFewTiles * kTileN;
+template <int RT>
+__device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareLds &lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 7, kq = lane >> 3 & 3, h = lane >> 5, r = lane & 31;
+    const int t = wave & 3, half = wave >> 2, G = p.K / kGroupK, tiles = p.N / kTileN, g = block / p.slices, slice = block % p.slices;
+    const int turns = (tiles + kFewTiles - 1) / kFewTiles, each = (turns + p.slices - 1) / p.slices * kFewTiles;
+    const uint32_t *words = reinterpret_cast<const uint32_t *>(p.B) + ((size_t)g * 64 + i + 8 * h + 16 * kq) * 4 + t;
+    f32x16 acc[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[rt][e] = 0.f;
+    for (int base = slice * each; base < min(tiles, (slice + 1) * each); base += kFewTiles) {
+        __syncthreads();
+        for (int e = tid; e < 32 * RT * (kFewColumns / 8); e += kPrepareThreads) {  // (N is a multiple of kFewColumns)
+            const int row = e / (kFewColumns / 8), at = 8 * (e % (kFewColumns / 8));
+            *reinterpret_cast<u32x4 *>(lds.dy + row * kFewDyPitch + at) =
+                *reinterpret_cast<const u32x4 *>(p.dy + (size_t)min(row, p.m - 1) * p.N + base * kTileN + at);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int u0 = 0; u0 < kFewTiles / 2; u0 += kFewAhead) {
+            const int tile0 = kFewTiles / 2 * half + u0;
+            uint32_t w[kFewAhead];
+            u32x4 s[kFewAhead];
+#pragma unroll
+            for (int u = 0; u < kFewAhead; ++u) {
+                w[u] = words[(size_t)(base + tile0 + u) * G * 256];
+                s[u] = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, (base + tile0 + u) * kTileN + 8 * h, p.Gs));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < kFewAhead; ++u) {
+                const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(w[u], lane), lane), lane);
+                bf16x8 o;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? s[u][c >> 1] >> 16 : s[u][c >> 1])));
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    acc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o, load_bf16x8(lds.dy + (32 * rt + r) * kFewDyPitch + (tile0 + u) * kTileN + 8 * h), acc[rt], 0, 0, 0);
+            }
+        }
+    }
+    for (int w = 0; w < 2; ++w) {
+        __syncthreads();
+        if (half == w)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {  // row 8 (e / 4) + 4 h + e % 4 of the product: rows of k come in the nibbles' order
+                    float *at = lds.sums + (32 * rt + r) * kFewPitch + 32 * t + 8 * (e >> 2) + 2 * (e & 3) + h;
+                    *at = (w ? *at : 0.f) + acc[rt][e];
+                }
+    }
+    __syncthreads();
+    for (int e = tid; e < p.m * 32; e += kPrepareThreads)
+        *reinterpret_cast<f32x4 *>(p.partial + ((size_t)slice * p.m + (e >> 5)) * p.K + g * kGroupK + 4 * (e & 31)) =
+            *reinterpret_cast<const f32x4 *>(lds.sums + (e >> 5) * kFewPitch + 4 * (e & 31));
+}
+
 // at[a][k][rank] of a[a][rank][k], or bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows of several
 // adapters at once, zeros for those of others, so it holds finite values alone; where A holds others, odd[a][k / 64] is set and
 // bank_grad_kernel adds their products for the rows of that adapter.
 __device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, PrepareLds &lds) {
-    const int tid = threadIdx.x, rank = p.rank, of_a = p.K / 64, parts = of_a + p.N / 64, a = block / parts, part = block % parts;
+    const int tid = threadIdx.x, rank = p.rank, of_a = p.at ? p.K / 64 : 0, parts = of_a + p.N / 64, a = block / parts, part = block % parts;
     const bool is_a = part < of_a;
     const int len = is_a ? p.K : p.N, l0 = (is_a ? part : part - of_a) * 64;
     const size_t base = (size_t)a * rank * len;
@@ -110,6 +182,8 @@ __device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, Prepa
     }
 }
 
+// RT: row tiles of a call of few rows, or 0 for a weight unpacked
+template <int RT>
 __global__ __launch_bounds__(kPrepareThreads) void bank_prepare_kernel(PrepareArgs p) {
     __shared__ __align__(16) PrepareLds lds;
     int block = blockIdx.x;
@@ -119,6 +193,7 @@ __global__ __launch_bounds__(kPrepareThreads) void bank_prepare_kernel(PrepareAr
     }
     block -= p.order_blocks;
     if (block < p.turn_blocks) turn_bank(p, block, lds);
+    else if constexpr (RT > 0) few_dx<RT>(p, block - p.turn_blocks, lds);
     else unpack_weight(p, block - p.turn_blocks, lds);
 }
 
@@ -322,16 +397,66 @@ struct GradArgs {
     const uint16_t *a;   // the adapters' A as they lie, [count, rank, K]
     const uint8_t *odd;  // [count, K / 64]: where A holds values that are no finite numbers,
     uint16_t *dx;        // whose products are still to be added here
+    const float *partial;  // few rows: [slices, rows, K], dx's to be summed and joined by U A here
+    int grad_blocks, slices;
 };
+
+// dx of few rows: the slices' sum and the low-rank term, 4 W 64 of k of one position to a block
+__device__ __forceinline__ void finish_dx(const GradArgs &p, int block, int threads) {
+    const int parts = (p.K / 4 + threads - 1) / threads, at = block / parts, k = (block % parts * threads + (int)threadIdx.x) * 4;
+    if (k >= p.K) return;
+    const int row = p.rows.order ? p.rows.order[at] : at;
+    const size_t stride = (size_t)p.rows.rows * p.K;
+    const float *from = p.partial + (size_t)row * p.K + k;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    int s = 0;
+    for (; s + 4 <= p.slices; s += 4) {
+        f32x4 d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = *reinterpret_cast<const f32x4 *>(from + (s + i) * stride);
+        v += (d[0] + d[1]) + (d[2] + d[3]);
+    }
+    for (; s < p.slices; ++s) v += *reinterpret_cast<const f32x4 *>(from + s * stride);
+    const int a = p.rows.order && at < p.rows.first[p.rows.count] ? p.rows.of[row] : -1;
+    if (a >= 0) {
+        const uint16_t *m = p.a + (size_t)a * p.rank * p.K + k;
+        const float *u = p.u + (size_t)at * p.rank;
+        f32x4 low = {0.f, 0.f, 0.f, 0.f};
+        for (int r0 = 0; r0 < p.rank; r0 += 8) {
+            u32x2 d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = *reinterpret_cast<const u32x2 *>(m + (size_t)(r0 + i) * p.K);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = u[r0 + i];
+                low[0] += f * __builtin_bit_cast(float, d[i].x << 16);
+                low[1] += f * __builtin_bit_cast(float, d[i].x & 0xFFFF0000u);
+                low[2] += f * __builtin_bit_cast(float, d[i].y << 16);
+                low[3] += f * __builtin_bit_cast(float, d[i].y & 0xFFFF0000u);
+            }
+        }
+        const float scale = p.scales[a];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += scale * low[i];
+    }
+    u32x2 o;
+    o.x = f32_to_bf16_bits(v[0]) | (uint32_t)f32_to_bf16_bits(v[1]) << 16;
+    o.y = f32_to_bf16_bits(v[2]) | (uint32_t)f32_to_bf16_bits(v[3]) << 16;
+    *reinterpret_cast<u32x2 *>(p.dx + (size_t)row * p.K + k) = o;
+}
 
 constexpr int kGradPitch = 128 + 4;
 template <int JT, int W>
 __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     __shared__ float sum[JT * 16 * kGradPitch];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int a = blockIdx.y;
-    const bool is_b = (int)blockIdx.x < p.N / 128;
-    const int c0 = (is_b ? blockIdx.x : blockIdx.x - p.N / 128) * 128, len = is_b ? p.N : p.K;
+    if ((int)blockIdx.x >= p.grad_blocks) {
+        finish_dx(p, blockIdx.x - p.grad_blocks, W * 64);
+        return;
+    }
+    const int parts = p.N / 128 + p.K / 128, a = blockIdx.x / parts, block = blockIdx.x % parts;
+    const bool is_b = block < p.N / 128;
+    const int c0 = (is_b ? block : block - p.N / 128) * 128, len = is_b ? p.N : p.K;
     const uint16_t *src = (is_b ? p.dy : p.x) + c0 + 8 * c;
     const float *f = is_b ? p.t : p.u;
     const int begin = p.rows.first[a], end = p.rows.first[a + 1];
@@ -409,7 +534,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
         }
         *reinterpret_cast<u32x4 *>(is_b ? out + (size_t)col * p.rank + 8 * r : out + (size_t)r * p.K + 8 * col) = o;
     }
-    if (is_b) return;
+    if (is_b || p.partial) return;
     const uint8_t *odd = p.odd + (size_t)a * (p.K / 64) + c0 / 64;
     if (!(odd[0] | odd[1])) return;
     for (int i = tid; i < (end - begin) * 128; i += W * 64) {
@@ -424,11 +549,16 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     }
 }
 
-template <int JT>
+template <int JT, int W>
 void launch_grad(const GradArgs &g, hipStream_t stream) {
-    const dim3 grid(g.N / 128 + g.K / 128, g.rows.count);
-    if (grid.x * grid.y >= 512) bank_grad_kernel<JT, 4><<<grid, 256, 0, stream>>>(g);
-    else bank_grad_kernel<JT, 8><<<grid, 512, 0, stream>>>(g);
+    const int dx_blocks = g.partial ? g.rows.rows * ((g.K / 4 + W * 64 - 1) / (W * 64)) : 0;
+    bank_grad_kernel<JT, W><<<g.grad_blocks + dx_blocks, W * 64, 0, stream>>>(g);
+}
+template <int JT>
+void launch_grad(GradArgs g, hipStream_t stream) {
+    g.grad_blocks = (g.N / 128 + g.K / 128) * g.rows.count;
+    if (g.grad_blocks >= 512) launch_grad<JT, 4>(g, stream);
+    else launch_grad<JT, 8>(g, stream);
 }
 
 // ---- the plan ----------------------------------------------------------------------------------------------------
@@ -462,6 +592,14 @@ DxPlan dx_plan(int m, int n, int k) {
     return best;
 }
 
+void launch_prepare(const PrepareArgs &p, hipStream_t stream) {
+    const int blocks = p.order_blocks + p.turn_blocks;
+    if (p.m == 0) bank_prepare_kernel<0><<<blocks, kPrepareThreads, 0, stream>>>(p);  // (the order alone)
+    else if (p.m > kFewRows) bank_prepare_kernel<0><<<blocks + (p.N / 128) * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
+    else if (p.m > 32) bank_prepare_kernel<2><<<blocks + p.slices * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
+    else bank_prepare_kernel<1><<<blocks + p.slices * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
+}
+
 template <int WM, int WN, int TM, int TN>
 void launch_dx(DxArgs p, int slices, hipStream_t stream) {
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
@@ -471,9 +609,15 @@ void launch_dx(DxArgs p, int slices, hipStream_t stream) {
     bank_dx_kernel<WM, WN, TM, TN><<<p.m_tiles * p.k_tiles * slices, WM * WN * 64, kStages * (BM + BN) * 64, stream>>>(p);
 }
 
+// Up to 64 rows: slices of the columns, of 256 at least; 16 at most, by what they add up to
+int few_slices(int n) {
+    const int turns = n / kFewColumns, slices = turns < 16 ? turns : 16, each = (turns + slices - 1) / slices;
+    return (turns + each - 1) / each;
+}
+
 struct BackwardScratch {
     size_t wt, at, bt, odd, order, t, u, partial, total;
-    int t_slices, u_slices;
+    int t_slices, u_slices, few;
     DxPlan dx;
 };
 BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
@@ -484,9 +628,10 @@ BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
         at += bank_up256(bytes);
         return here;
     };
-    s.wt = take((size_t)k * n * 2);
+    s.few = m <= kFewRows ? few_slices(n) : 0;
+    s.wt = take(s.few ? 0 : (size_t)k * n * 2);
     if (count > 0) {
-        s.at = take((size_t)count * rank * k * 2);
+        s.at = take(s.few ? 0 : (size_t)count * rank * k * 2);
         s.bt = take((size_t)count * rank * n * 2);
         s.odd = take((size_t)count * (k / 64));
         s.order = take(bank_order_bytes(m, count));
@@ -495,8 +640,8 @@ BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
         s.t = take((size_t)s.t_slices * m * rank * 4);
         s.u = take((size_t)s.u_slices * m * rank * 4);
     }
-    s.dx = dx_plan(m, n, k);
-    s.partial = take(s.dx.slices > 1 ? (size_t)s.dx.slices * m * k * 4 : 0);
+    s.dx = s.few ? DxPlan{0, s.few} : dx_plan(m, n, k);
+    s.partial = take(s.few || s.dx.slices > 1 ? (size_t)s.dx.slices * m * k * 4 : 0);
     s.total = at;
     return s;
 }
@@ -536,7 +681,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     dx.dy = (const uint16_t *)dC;
     dx.wt = wt;
     dx.dx = (uint16_t *)dA;
-    dx.partial = w.dx.slices > 1 ? reinterpret_cast<float *>(at + w.partial) : nullptr;
+    float *partial = w.few || w.dx.slices > 1 ? reinterpret_cast<float *>(at + w.partial) : nullptr;
+    dx.partial = partial;
     dx.rows = BankRows{nullptr, nullptr, nullptr, m, 0};
     dx.K = k;
     dx.N = n;
@@ -548,6 +694,10 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     prepare.K = k;
     prepare.N = n;
     prepare.Gs = groupsize == -1 ? 1 : k / 128;
+    prepare.dy = (const uint16_t *)dC;
+    prepare.partial = partial;
+    prepare.m = m;
+    prepare.slices = w.few;
     if (bank) {
         uint16_t *a_t = reinterpret_cast<uint16_t *>(at + w.at), *b_t = reinterpret_cast<uint16_t *>(at + w.bt);
         uint8_t *odd = reinterpret_cast<uint8_t *>(at + w.odd);
@@ -556,14 +706,14 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
         dx.rows = bank_rows(adapter_of, m, count, at + w.order);
         prepare.a = lora_a;
         prepare.b = (const uint16_t *)bank->lora_b;
-        prepare.at = a_t;
+        prepare.at = w.few ? nullptr : a_t;
         prepare.bt = b_t;
         prepare.odd = odd;
         prepare.rows = dx.rows;
         prepare.rank = rank;
         prepare.order_blocks = count + 1;
-        prepare.turn_blocks = m > 0 ? count * (k / 64 + n / 64) : 0;
-        bank_prepare_kernel<<<prepare.order_blocks + prepare.turn_blocks + (m > 0 ? (n / 128) * (k / 128) : 0), kPrepareThreads, 0, hs>>>(prepare);
+        prepare.turn_blocks = m > 0 ? count * ((w.few ? 0 : k / 64) + n / 64) : 0;
+        launch_prepare(prepare, hs);
         if (m > 0) {
             const BankProjection of_x{A, lora_a, t, k, w.t_slices};
             bank_project(BankProjection{dC, b_t, u, n, w.u_slices}, &of_x, dx.rows, rank, hs);
@@ -571,24 +721,24 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
                 sum_slices_kernel<<<dim3((unsigned)(((size_t)m * rank + 255) / 256), 2), 256, 0, hs>>>(t, w.t_slices, u, w.u_slices, (size_t)m * rank);
         }
         grad = GradArgs{(const uint16_t *)A, (const uint16_t *)dC, t, u, bank->scales, (uint16_t *)d_lora_a, (uint16_t *)d_lora_b,
-                        dx.rows, k, n, rank, lora_a, odd, (uint16_t *)dA};
+                        dx.rows, k, n, rank, lora_a, odd, (uint16_t *)dA, w.few && m > 0 ? partial : nullptr, 0, w.few};
         dx.at = a_t;
         dx.u = u;
         dx.scales = bank->scales;
         dx.rank = rank;
     } else {
-        bank_prepare_kernel<<<(n / 128) * (k / 128), kPrepareThreads, 0, hs>>>(prepare);
+        launch_prepare(prepare, hs);
     }
-    if (m > 0) {
+    if (m > 0 && !w.few) {
         switch (w.dx.kind) {
             case 0: launch_dx<2, 2, 2, 2>(dx, w.dx.slices, hs); break;
             case 1: launch_dx<2, 4, 2, 2>(dx, w.dx.slices, hs); break;
             default: launch_dx<2, 2, 4, 4>(dx, w.dx.slices, hs); break;
         }
-        if (dx.partial) {
-            const size_t units = (size_t)m * k / 4;
-            sum_dx_kernel<<<(unsigned)((units + 255) / 256), 256, 0, hs>>>((const f32x4 *)dx.partial, (u32x2 *)dA, w.dx.slices, units);
-        }
+    }
+    if (m > 0 && (!bank || !w.few) && partial) {
+        const size_t units = (size_t)m * k / 4;
+        sum_dx_kernel<<<(unsigned)((units + 255) / 256), 256, 0, hs>>>((const f32x4 *)partial, (u32x2 *)dA, w.dx.slices, units);
     }
     if (bank) {  // behind dx, to which it adds where an adapter holds what is no finite number
         switch ((rank + 15) / 16) {
