@@ -48,20 +48,21 @@ __device__ __forceinline__ void project_pieces(const uint16_t *const (&x)[RT], c
 }
 
 // T: a block takes 16 RT positions, one slice of K, and of the adapters present among them those whose turn (in the order they are met)
-// is blockIdx.z modulo gridDim.z.  Its W wavefronts take every W-th 64 of K and meet in LDS.  Blocks go through the slices first, so
+// is blockIdx.y modulo gridDim.y.  Its W wavefronts take every W-th 64 of K and meet in LDS.  Blocks go through the slices first, so
 // that with eight of them a die's blocks share one, whose part of the adapters' matrices its L2 then holds.  Two projections of the same
 // rows share a launch: the second one's slices are behind the first one's.
 template <int JT, int RT, int W>
 __global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one, BankProjection two, BankRows rows, int rank) {
     constexpr int P = 16 * RT, kAhead = JT + RT <= 4 ? 4 : 2;
-    const bool second = (int)blockIdx.x >= one.slices;
+    const int all = one.slices + two.slices, place = blockIdx.x % all, tile = blockIdx.x / all;
+    const bool second = place >= one.slices;
     const uint16_t *__restrict__ src = (const uint16_t *)(second ? two.src : one.src), *__restrict__ mat = (const uint16_t *)(second ? two.mat : one.mat);
     float *__restrict__ t = second ? two.t : one.t;
-    const int K = second ? two.K : one.K, slices = second ? two.slices : one.slices, slice = second ? blockIdx.x - one.slices : blockIdx.x;
+    const int K = second ? two.K : one.K, slices = second ? two.slices : one.slices, slice = second ? place - one.slices : place;
     const int steps = (K / 128 + slices - 1) / slices;
     __shared__ float part[W][P][JT * 16 + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int p0 = blockIdx.y * P;
+    const int p0 = tile * P;
     int row, a;
     row_at(rows, p0 + (lane & (P - 1)), row, a);
     constexpr unsigned long long kAll = P == 64 ? ~0ull : (1ull << P) - 1;
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one
         const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
         const unsigned long long mine = __ballot(a == cur) & kAll;
         left &= ~mine;
-        if (turn % gridDim.z != blockIdx.z) continue;
+        if (turn % gridDim.y != blockIdx.y) continue;
         const uint16_t *m[JT];  // rows past the rank: the last one again, their sums are dropped
 #pragma unroll
         for (int j = 0; j < JT; ++j) m[j] = mat + ((size_t)cur * rank + min(16 * j + c, rank - 1)) * K + own + 16 * q;
@@ -185,14 +186,14 @@ __global__ __launch_bounds__(256) void bank_expand_ordered_kernel(uint16_t *__re
                                                                   int N, int rank, int slices, int columns) {
     __shared__ float ts[64][kBankMaxRank + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    const int p0 = blockIdx.y * 64;
+    const int parts = (N + columns - 1) / columns, part = blockIdx.x % parts, p0 = blockIdx.x / parts * 64;
     int row, a;
     row_at(rows, p0 + lane, row, a);
     const unsigned long long present = __ballot(a >= 0);
     if (!present) return;
     const float scale = a >= 0 ? scales[a] : 0.f;
-    const int end = min(N, (int)(blockIdx.x + 1) * columns);
-    int n0 = blockIdx.x * columns + 64 * wave;
+    const int end = min(N, (part + 1) * columns);
+    int n0 = part * columns + 64 * wave;
     int a_of[4];
     uint16_t *dst[4];
     u32x4 was[4][2];
@@ -253,7 +254,7 @@ void launch_project(const BankProjection &one, const BankProjection &two, const 
     int turns = r.order ? 1 + r.count / tiles : 16;
     if (turns > 16) turns = 16;
     if (turns > r.count) turns = r.count;
-    bank_project_kernel<JT, RT, W><<<dim3(one.slices + two.slices, tiles, turns), W * 64, 0, stream>>>(one, two, r, rank);
+    bank_project_kernel<JT, RT, W><<<dim3((one.slices + two.slices) * tiles, turns), W * 64, 0, stream>>>(one, two, r, rank);
 }
 template <int RT, int W>
 void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream) {
@@ -320,7 +321,7 @@ void launch_expand(uint16_t *y, const uint16_t *m, const float *t, const float *
     const int tiles = tiles_of(r.rows, 64);
     int columns = 1024;  // (2048 rows of 18432 columns: 256 60 us, 512 49, 1024 45, 2048 50)
     while (columns > 256 && tiles * ((N + columns - 1) / columns) < 512) columns /= 2;
-    bank_expand_ordered_kernel<S><<<dim3((N + columns - 1) / columns, tiles), 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices, columns);
+    bank_expand_ordered_kernel<S><<<(N + columns - 1) / columns * tiles, 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices, columns);
 }
 
 }  // namespace

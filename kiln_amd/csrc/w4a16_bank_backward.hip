@@ -537,8 +537,8 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     if (is_b || p.partial) return;
     const uint8_t *odd = p.odd + (size_t)a * (p.K / 64) + c0 / 64;
     if (!(odd[0] | odd[1])) return;
-    for (int i = tid; i < (end - begin) * 128; i += W * 64) {
-        const int at = begin + i / 128, k = c0 + i % 128;
+    for (int at = begin + (tid >> 7); at < end; at += W / 2) {
+        const int k = c0 + (tid & 127);
         uint16_t *dx = p.dx + (size_t)p.rows.order[at] * p.K + k;
         float v = __builtin_bit_cast(float, (uint32_t)*dx << 16);
         for (int r = 0; r < p.rank; ++r) {

@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const T *__restrict__ lo
 template <class T>
 void launch_route(const void *logits, int rows, int experts, int top, int renormalise, int *of, float *weights, hipStream_t stream) {
     const T *l = (const T *)logits;
-    const unsigned grid = (unsigned)((rows + 3) / 4);
+    const unsigned grid = ((unsigned)rows + 3) / 4;
     const int per_lane = (experts + 63) / 64;
     if (per_lane <= 1) moe_route_kernel<T, 1><<<grid, 256, 0, stream>>>(l, rows, experts, top, renormalise, of, weights);
     else if (per_lane <= 2) moe_route_kernel<T, 2><<<grid, 256, 0, stream>>>(l, rows, experts, top, renormalise, of, weights);

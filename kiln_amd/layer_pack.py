@@ -29,7 +29,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _calls, marlin_gemm, marlin_proj
-from .lora import fuse_column_blocks, proj_forward, sides_again, swiglu_forward, swiglu_lora_fits
+from .lora import AdapterBank, fuse_column_blocks, proj_forward, proj_forward_bank, sides_again, swiglu_forward, swiglu_lora_fits
 from .marlin_proj import MarlinPackedProj, MarlinProjError
 
 
@@ -101,6 +101,18 @@ class LayerProjections:
         if lora is not None:                                  # unfused, as the reference's bf16 branch
             y = y + ((x @ lora.a.t().to(x.dtype)) @ lora.b.t().to(x.dtype)) * lora_scale
         return y
+
+    def forward_bank(self, kind: PackKind, x: torch.Tensor, bank: AdapterBank, adapter_of: torch.Tensor) -> torch.Tensor:
+        """`forward` for rows of many requests, each with one of `bank`'s adapters or none (`lora.proj_forward_bank`)."""
+        w = self.packed.get(kind)
+        if w is not None:
+            return proj_forward_bank(x, w, bank, adapter_of)
+        y = self.forward(kind, x).reshape(adapter_of.numel(), -1)
+        rows, of = x.reshape(adapter_of.numel(), -1), adapter_of.reshape(-1)
+        for i in range(bank.a.shape[0]):                       # unfused, an adapter at a time
+            delta = (rows @ bank.a[i].t()) @ bank.b[i].t() * bank.scales[i]
+            y = torch.where((of == i)[:, None], y + delta.to(y.dtype), y)
+        return y.reshape(*x.shape[:-1], -1)
 
     def forward_same_input(self, kinds: Sequence[PackKind], x: torch.Tensor, loras: Optional[Dict[PackKind, object]] = None,
                            lora_scale: float = 1.0) -> Tuple[torch.Tensor, ...]:

@@ -6,6 +6,8 @@ crates/kiln-model/src/adapter_merge.rs:639-712 (A row-concatenated, B column-con
 with each block scaled by its adapter weight); `mlp_proj_forward` / `q_proj_forward` take the
 place of `mlp_proj_forward_decode_if` / `q_proj_forward_decode_if`
 (crates/kiln-model/src/forward.rs:2923-2946, :4776-4801) with the delta fused into the GEMM.
+`AdapterBank`, `make_bank`, `proj_forward_bank` and `proj_backward_bank` are for rows of many requests, each with an adapter of its own, and
+for training those adapters; the reference holds one set of adapters for all rows.
 """
 from __future__ import annotations
 
@@ -173,6 +175,56 @@ def fuse_column_blocks(loras: Sequence, widths: Sequence[int], lora_scale: float
     present = [s for s in sides if s is not None]
     return StackedLora(torch.cat([s.a_cat for s in present], dim=0).contiguous(), b_cat,
                        tuple(r for s in present for r in s.ranks), tuple(v for s in present for v in s.scales))
+
+
+@dataclass
+class AdapterBank:
+    """The adapters of one projection that a batch's requests choose from, one rank for all (`make_bank`)."""
+    a: torch.Tensor        # [count, rank, in_features] bf16
+    b: torch.Tensor        # [count, out_features, rank] bf16
+    scales: torch.Tensor   # [count] f32, on the GPU: alpha / rank
+
+
+def make_bank(adapters: Sequence[LoraProjectionWeights], scales: Sequence[float]) -> AdapterBank:
+    """Adapters of any ranks up to 64 as one bank: each rank rounded up to the largest one's next multiple of 8 with zero rows of A and
+    zero columns of B, which add exact zeros."""
+    if not adapters or len(adapters) != len(scales):
+        raise MarlinProjError("make_bank: need one scale per adapter")
+    rank = -(-max(int(p.a.shape[0]) for p in adapters) // 8) * 8
+    k, n, device = adapters[0].a.shape[1], adapters[0].b.shape[0], adapters[0].a.device
+    a = torch.zeros((len(adapters), rank, k), dtype=torch.bfloat16, device=device)
+    b = torch.zeros((len(adapters), n, rank), dtype=torch.bfloat16, device=device)
+    for i, p in enumerate(adapters):
+        r = p.a.shape[0]
+        if tuple(p.a.shape) != (r, k) or tuple(p.b.shape) != (n, r):
+            raise MarlinProjError(f"make_bank: adapter {i} is {tuple(p.a.shape)} / {tuple(p.b.shape)}, not [rank, {k}] / [{n}, rank]")
+        a[i, :r], b[i, :, :r] = p.a, p.b
+    return AdapterBank(a, b, torch.tensor([float(s) for s in scales], dtype=torch.float32, device=device))
+
+
+def proj_forward_bank(x: torch.Tensor, packed: MarlinPackedProj, bank: AdapterBank, adapter_of: torch.Tensor) -> torch.Tensor:
+    """`proj_forward` for rows of many requests, each with an adapter of its own: `x` `[..., k]`, `adapter_of` i32, one of `bank`'s adapters
+    for each of x's rows (any other value: none)."""
+    if x.shape[-1] != packed.k:
+        raise MarlinProjError(f"marlin_proj: x last-dim {x.shape[-1]} != packed weight k {packed.k}")
+    y = marlin_gemm.marlin_w4a16_gemm_bank(x.reshape(-1, packed.k), packed.b_packed, packed.scales, packed.groupsize, bank.a, bank.b, bank.scales,
+                                           adapter_of.reshape(-1))
+    return y.reshape(*x.shape[:-1], packed.n)
+
+
+def proj_backward_bank(dy: torch.Tensor, x: torch.Tensor, packed: MarlinPackedProj, bank: Optional[AdapterBank] = None,
+                       adapter_of: Optional[torch.Tensor] = None):
+    """The gradients of `proj_forward_bank` from `dy` `[..., n]`, the packed weight frozen: `(dx, d_bank_a, d_bank_b)`.  Without a bank, of
+    `matmul_bf16`: `(dx, None, None)`."""
+    if dy.shape[:-1] != x.shape[:-1] or dy.shape[-1] != packed.n or x.shape[-1] != packed.k:
+        raise MarlinProjError(f"marlin_proj: dy {tuple(dy.shape)} and x {tuple(x.shape)} do not match a packed [{packed.k}, {packed.n}]")
+    rows = dy.reshape(-1, packed.n)
+    if bank is None:
+        dx = marlin_gemm.marlin_w4a16_gemm_backward(rows, packed.b_packed, packed.scales, packed.groupsize)
+        return dx.reshape(x.shape), None, None
+    dx, d_a, d_b = marlin_gemm.marlin_w4a16_gemm_bank_backward(rows, x.reshape(-1, packed.k), packed.b_packed, packed.scales, packed.groupsize,
+                                                               bank.a, bank.b, bank.scales, adapter_of.reshape(-1))
+    return dx.reshape(x.shape), d_a, d_b
 
 
 def swiglu_lora_fits(gate_lora, up_lora) -> bool:

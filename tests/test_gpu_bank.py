@@ -57,10 +57,10 @@ def check(got, want, bound):
     assert excess <= 0.0, (excess, (got - want).abs().max().item())
 
 
-def check_forward(p, y):
+def check_forward(p, y, base=None):
     (m, k), rank = p["x"].shape, p["a_"].shape[1]
-    if m > 16:                                    # a row without an adapter is the plain GEMM's, to the bit
-        base = marlin_gemm.marlin_w4a16_gemm(p["x"], p["b"], p["s"], p["g"])
+    if m > 16:                                    # a row without an adapter is the plain GEMM's of as many rows, to the bit
+        base = base if base is not None else marlin_gemm.marlin_w4a16_gemm(p["x"], p["b"], p["s"], p["g"])
         without = (p["of"] < 0) | (p["of"] >= len(p["sc"]))
         assert torch.equal(y[without].view(torch.int16), base[without].view(torch.int16))
     w = marlin_gemm.dequant_f32(p["b"], p["s"], p["g"]).double()
@@ -244,3 +244,74 @@ def test_refusals():
         backward({**p, "dy": p["dy"][:, :256]})
     with pytest.raises(marlin_gemm.MarlinGemmError, match="out must be"):
         forward(p, out=torch.empty(6, 256, dtype=torch.bfloat16, device="cuda"))
+
+
+def test_more_rows_than_a_grid_is_high():
+    """Over 65536 tiles of 16 rows: the rows sampled, at either end and where the count of tiles passes 16 bits."""
+    m, k, n, count, rank = 16 * 65536 + 21, 128, 256, 3, 8
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    b, s = packed(gen, k, n, 128)
+    p = dict(x=torch.randn(m, k, device="cuda", generator=gen).bfloat16(), b=b, s=s, g=128, a_=(torch.randn(count, rank, k, device="cuda", generator=gen) / 11).bfloat16(),
+             b_=(torch.randn(count, n, rank, device="cuda", generator=gen) / 3).bfloat16(), sc=torch.ones(count, device="cuda"),
+             of=torch.randint(-1, count, (m,), device="cuda", generator=gen).to(torch.int32), dy=(torch.randn(m, n, device="cuda", generator=gen) * 0.02).bfloat16())
+    y, (da, d_a, d_b) = forward(p), backward(p)
+    at = torch.cat([torch.arange(40), torch.randint(0, m, (500,)), torch.arange(65536 * 16 - 20, m)]).cuda()
+    few = {**p, "x": p["x"][at], "of": p["of"][at], "dy": p["dy"][at]}
+    check_forward(few, y[at], marlin_gemm.marlin_w4a16_gemm(p["x"], b, s, 128)[at])
+    want = few["dy"].double() @ marlin_gemm.dequant_f32(b, s, 128).double().t()
+    bound = (few["dy"].double().abs() @ marlin_gemm.dequant_f32(b, s, 128).double().abs().t()) * (U + (n + 2 * rank) * F)
+    for j in range(count):
+        mine, a, bb = few["of"] == j, p["a_"][j].double(), p["b_"][j].double()
+        g = few["dy"][mine].double()
+        want[mine] += (g @ bb) @ a
+        bound[mine] += (g.abs() @ bb.abs()) @ a.abs() * ((2 * n + 2 * rank + 64) * F + 2.0 ** -16)
+        rows = p["of"] == j
+        x, g = p["x"][rows].double(), p["dy"][rows].double()
+        check(d_a[j], (g @ bb).t() @ x, ((g.abs() @ bb.abs()).t() @ x.abs()) * ((n + m + 64) * F))
+        check(d_b[j], g.t() @ (x @ a.t()), (g.abs().t() @ (x.abs() @ a.abs().t())) * ((k + m + 64) * F))
+    check(da[at], want, bound)
+
+
+def test_a_step_of_many_requests_through_a_layer():
+    """Requests with adapters of their own through a layer's packed projections and its experts, then the gradients of the adapters, each part
+    held to its formula on what the part before it gave."""
+    from kiln_amd import layer_pack, lora, moe
+    from kiln_amd.layer_pack import LayerProjections, PackKind
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    rand = lambda *shape: torch.randn(shape, device="cuda", generator=gen)
+    weight = lambda k, n: (rand(k, n) / k ** 0.5).bfloat16()
+    layer = LayerProjections({PackKind.QProj: weight(256, 512), PackKind.OProj: weight(512, 256)})
+    layer_pack.pack_layers([layer])
+    adapters = lambda k, n: lora.make_bank([lora.LoraProjectionWeights((rand(r, k) / k ** 0.5).bfloat16(), (rand(n, r) / r ** 0.5).bfloat16()) for r in (8, 12, 3)], (0.5, 1.0, 2.0))
+    bank_q, bank_o = adapters(256, 512), adapters(512, 256)
+    of = torch.tensor([0, 0, 2, -1, 1, 1, 1, 0, 2, 3] * 3, dtype=torch.int32, device="cuda")
+
+    def as_problem(x, kind, bank, dy=None):
+        w = layer.packed[kind]
+        return dict(x=x, b=w.b_packed, s=w.scales, g=w.groupsize, a_=bank.a, b_=bank.b, sc=bank.scales, of=of, dy=dy)
+
+    x = rand(3, 10, 256).bfloat16()
+    q = layer.forward_bank(PackKind.QProj, x, bank_q, of)
+    assert q.shape == (3, 10, 512)
+    check_forward(as_problem(x.reshape(30, 256), PackKind.QProj, bank_q), q.reshape(30, 512))
+    o = lora.proj_forward_bank(q, layer.packed[PackKind.OProj], bank_o, of.reshape(3, 10))
+    check_forward(as_problem(q.reshape(30, 512), PackKind.OProj, bank_o), o.reshape(30, 256))
+    experts = moe.pack_experts(*(torch.stack([weight(k, n) for _ in range(4)]) for k, n in ((256, 256), (256, 256), (256, 256))))
+    y = x + o + moe.moe_forward(x + o, weight(256, 4), experts, 2)
+    assert bool(torch.isfinite(y).all())
+    dy = (rand(3, 10, 256) * 0.1).bfloat16()
+    dq, d_a, d_b = lora.proj_backward_bank(dy, q, layer.packed[PackKind.OProj], bank_o, of.reshape(3, 10))
+    check_backward(as_problem(q.reshape(30, 512), PackKind.OProj, bank_o, dy.reshape(30, 256)), dq.reshape(30, 512), d_a, d_b)
+    dx, e_a, e_b = lora.proj_backward_bank(dq, x, layer.packed[PackKind.QProj], bank_q, of)
+    check_backward(as_problem(x.reshape(30, 256), PackKind.QProj, bank_q, dq.reshape(30, 512)), dx.reshape(30, 256), e_a, e_b)
+    alone, none_a, none_b = lora.proj_backward_bank(dq, x, layer.packed[PackKind.QProj])
+    assert alone.shape == x.shape and none_a is None and none_b is None
+    # a projection that stayed on bf16 takes the same call
+    plain = LayerProjections({PackKind.QProj: weight(256, 512)})
+    z = plain.forward_bank(PackKind.QProj, x, bank_q, of).reshape(30, 512).double()
+    w = plain.weights_t[PackKind.QProj].double()
+    want = x.reshape(30, 256).double() @ w
+    for j in range(3):
+        mine = of == j
+        want[mine] += bank_q.scales[j].double() * ((x.reshape(30, 256)[mine].double() @ bank_q.a[j].double().t()) @ bank_q.b[j].double().t())
+    assert ((z - want).abs().max() / want.abs().max()).item() < 8 * U
