@@ -14,9 +14,11 @@ namespace kiln {
 //   row  this lane's row (lane & 15), 8 * (lane / 16) values in
 //   b    chunk 0 of tile 0, this lane's word of it;  s  scale 0 of tile 0, this lane's column
 //   meanwhile()  is called once, behind the first loads
-template <int GW, int S, class F>
+//   also(x, first)  is called for every GW groups that this wavefront has, with its part of the rows; groups first + u, of which those from
+//                   G on are none (x then holds the last one's)
+template <int GW, int S, class F, class R>
 __device__ __forceinline__ void few_rows_product(const uint16_t *__restrict__ row, const u32x4 *__restrict__ b, const uint16_t *__restrict__ s, int G,
-                                                 bool per_column, int turn, int turns, const DequantConsts &dc, f32x4 (&total)[S], F &&meanwhile) {
+                                                 bool per_column, int turn, int turns, const DequantConsts &dc, f32x4 (&total)[S], F &&meanwhile, R &&also) {
     const bf16x8 ones = bf16x8_splat_one();
     const int Gs = per_column ? 1 : G;
 #pragma unroll
@@ -66,7 +68,13 @@ __device__ __forceinline__ void few_rows_product(const uint16_t *__restrict__ ro
                 for (int i = 0; i < 4; ++i) total[tile][i] += sc * acc[i];
             }
         }
+        also(x, first);
     }
+}
+template <int GW, int S>
+__device__ __forceinline__ void few_rows_product(const uint16_t *__restrict__ row, const u32x4 *__restrict__ b, const uint16_t *__restrict__ s, int G,
+                                                 bool per_column, int turn, int turns, const DequantConsts &dc, f32x4 (&total)[S]) {
+    few_rows_product<GW, S>(row, b, s, G, per_column, turn, turns, dc, total, [] {}, [](const bf16x8(&)[GW][4], int) {});
 }
 
 // f(W, GW) as integral constants for G groups: five of them to a wavefront at most.

@@ -271,6 +271,10 @@ void launch_project(const BankProjection &one, const BankProjection &two, const 
 // against 11.2 / 13.3 / 15.5, 8192 -> 8192 13.4 / 16.9 / 21.2 against 15.0 / 17.9 / 21.1; but 9216 -> 2560 10.5 / 15.0 / 19.3 against 13.3 / 15.7 / 18.2,
 // 14336 -> 4096 13.5 / 18.3 / 24.8 against 16.0 / 19.0 / 22.2, 2560 -> 18432 13.3 / 16.4 / 20.7 against 12.8 / 15.7 / 18.6, 5120 -> 27648 27.7 / 37.5 / 48.9
 // against 21.9 / 26.5 / 30.8.
+// ... and there, may every block project the rows by itself, out of up to 96 KB of their adapters?  One row of rank 16: 2560 -> 2560 6.3 us
+// against 7.4 and more with the launch in front, 2560 -> 8192 7.8 against 8.8, 1024 -> 4096 5.3 against 7.0 and two rows 5.5 against 6.9; but 4096 -> 2560
+// 7.6 against 7.3, two rows of 2560 -> 8192 10.1 against 9.3.
+bool projects_itself(int m, int k, int rank) { return m <= 2 && (int64_t)m * rank * k <= 48 * 1024; }
 bool takes_few(int m, int n, int k) { return m <= kBankFewRows && n <= 8192 && (m <= 8 || k <= 8192); }
 
 }  // namespace
@@ -359,8 +363,9 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
         for (const void *p : {A, B, static_cast<const void *>(C), s, static_cast<const void *>(workspace)})
             if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
         rows.order = rows.first = nullptr;
-        bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
-        bank_few(A, B, s, C, *bank, rows, t, slices, prob_k, prob_n, groupsize == -1, hs);
+        const bool own = projects_itself(prob_m, prob_k, rank);
+        if (!own) bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
+        bank_few(A, B, s, C, *bank, rows, own ? nullptr : t, slices, prob_k, prob_n, groupsize == -1, hs);
         return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
     }
     // the plain GEMM's checks and its launches first: nothing is launched for a call that it refuses

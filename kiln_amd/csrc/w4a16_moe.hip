@@ -127,7 +127,7 @@ __global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
         const int pair = list[min(r0 + c, count - 1)];
         const uint16_t *row = (IN ? p.x + (size_t)(pair / p.top) * K : p.h + (size_t)pair * K) + 8 * q;
         f32x4 total[S];
-        few_rows_product<GW, S>(row, b, s, G, p.per_column, wave, W, dc, total, [] {});
+        few_rows_product<GW, S>(row, b, s, G, p.per_column, wave, W, dc, total);
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void moe_join_kernel(MoeArgs p) {
         for (int r0 = 0; r0 < count; r0 += 16) {
             f32x4 total[1];
             few_rows_product<GW, 1>(p.h + (size_t)list[min(r0 + c, count - 1)] * p.n_out + 8 * q, p.b_out + ((size_t)e * tiles + nt) * G * 64 + lane,
-                                    p.s_out + ((size_t)e * tiles + nt) * Gs * kTileN + c, G, p.per_column, unit % parts, parts, dc, total, [] {});
+                                    p.s_out + ((size_t)e * tiles + nt) * Gs * kTileN + c, G, p.per_column, unit % parts, parts, dc, total);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int pair = list[min(r0 + 4 * q + i, count - 1)], token = pair / p.top;
