@@ -97,7 +97,8 @@ SHAPES = [
     (16, 2560, 2560, 128, 16, 16, "any"), (17, 640, 768, 128, 40, 64, "any"), (33, 9216, 2560, -1, 5, 40, "runs"), (64, 1024, 256, 128, 64, 48, "any"),
     (65, 128, 1024, 128, 9, 56, "any"), (77, 4096, 512, -1, 3, 32, "runs"), (128, 256, 256, 128, 1, 64, "one"), (129, 896, 1792, 128, 200, 8, "any"),
     (300, 2560, 1024, 128, 6, 16, "runs"), (777, 384, 2560, -1, 11, 24, "any"), (1030, 256, 512, 128, 2, 32, "runs"),
-    (9, 256, 256, 128, 3, 8, "none"), (90, 256, 256, 128, 3, 16, "beyond"), (70, 256, 256, -1, 3, 8, "below"),
+    (1, 640, 512, -1, 3, 64, "any"), (2, 384, 256, 128, 2, 40, "any"), (2, 128, 8192, 128, 5, 24, "runs"), (1, 5760, 256, 128, 3, 8, "one"), (2, 256, 8448, 128, 3, 16, "any"),
+    (1, 5120, 512, 128, 2, 8, "below"), (11, 9216, 256, 128, 6, 16, "any"), (9, 256, 256, 128, 3, 8, "none"), (90, 256, 256, 128, 3, 16, "beyond"), (70, 256, 256, -1, 3, 8, "below"),
 ]
 
 
