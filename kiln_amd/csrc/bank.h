@@ -13,6 +13,12 @@ constexpr int kBankRowTile = 16;
 constexpr int kBankOrderedFrom = 257;  // calls of fewer rows take them as they stand
 constexpr int kBankMaxSlices = 32;     // of the contraction of a projection
 
+// do [a, a + a_bytes) and [b, b + b_bytes) share memory?
+inline bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t i = reinterpret_cast<uintptr_t>(a), j = reinterpret_cast<uintptr_t>(b);
+    return i < j + b_bytes && j < i + a_bytes;
+}
+
 inline size_t bank_up256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 // The rows of a call by position: position p is row order[p] (p itself without `order`), rows of one adapter together.

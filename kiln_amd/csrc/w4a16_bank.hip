@@ -349,19 +349,21 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
         return kiln_marlin_w4a16_gemm(A, B, C, const_cast<void *>(s), prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, -1, -1, -1, 16);
     if (!bank || !adapter_of || !scratch) return KILN_W4A16_ERR_ARGUMENT;
     if (!bank_ok(*bank)) return KILN_W4A16_ERR_KERN_SHAPE;
-    if (!bank->lora_a || !bank->lora_b || !bank->scales) return KILN_W4A16_ERR_ARGUMENT;
-    for (const void *p : {bank->lora_a, bank->lora_b, static_cast<const void *>(scratch)})
+    if (prob_n % 256 != 0 || prob_k % 128 != 0 || (groupsize != -1 && groupsize != 128)) return KILN_W4A16_ERR_PROB_SHAPE;
+    if (!A || !B || !C || !s || !workspace || !bank->lora_a || !bank->lora_b || !bank->scales) return KILN_W4A16_ERR_ARGUMENT;
+    for (const void *p : {A, B, static_cast<const void *>(C), s, static_cast<const void *>(workspace), bank->lora_a, bank->lora_b,
+                          static_cast<const void *>(scratch)})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t adapters = (size_t)bank->count * bank->rank * 2;
+    if (meet(C, (size_t)prob_m * prob_n * 2, A, (size_t)prob_m * prob_k * 2) || meet(C, (size_t)prob_m * prob_n * 2, bank->lora_a, adapters * prob_k) ||
+        meet(C, (size_t)prob_m * prob_n * 2, bank->lora_b, adapters * prob_n))
+        return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     char *at = reinterpret_cast<char *>(scratch);
     BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
     const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
     if (takes_few(prob_m, prob_n, prob_k)) {
-        if (prob_n % 256 != 0 || prob_k % 128 != 0 || (groupsize != -1 && groupsize != 128)) return KILN_W4A16_ERR_PROB_SHAPE;
-        if (!A || !B || !C || !s || !workspace) return KILN_W4A16_ERR_ARGUMENT;
-        for (const void *p : {A, B, static_cast<const void *>(C), s, static_cast<const void *>(workspace)})
-            if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
         rows.order = rows.first = nullptr;
         const bool own = projects_itself(prob_m, prob_k, rank);
         if (!own) bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);

@@ -521,7 +521,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
                 }
         __syncthreads();
     }
-    const float scale = p.scales[a];
+    const float scale = begin < end ? p.scales[a] : 0.f;  // without rows: zeros, whatever the scale
     uint16_t *out = is_b ? p.db + ((size_t)a * p.N + c0) * p.rank : p.da + (size_t)a * p.rank * p.K + c0;
     for (int e = tid; e < p.rank * 16; e += W * 64) {  // eight results each
         const int r = is_b ? e % (p.rank / 8) : e >> 4, col = is_b ? e / (p.rank / 8) : e & 15;
@@ -672,8 +672,19 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     for (const void *p : {dC, A, B, s, static_cast<const void *>(dA), static_cast<const void *>(scratch),
                           bank ? bank->lora_a : nullptr, bank ? bank->lora_b : nullptr, static_cast<const void *>(d_lora_a), static_cast<const void *>(d_lora_b)})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
-    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const int m = prob_m, n = prob_n, k = prob_k, count = bank ? bank->count : 0, rank = bank ? bank->rank : 0;
+    const struct {
+        const void *p;
+        size_t bytes;
+    } results[3] = {{dA, (size_t)m * k * 2}, {d_lora_a, (size_t)count * rank * k * 2}, {d_lora_b, (size_t)count * rank * n * 2}},
+      operands[4] = {{dC, (size_t)m * n * 2}, {A, bank ? (size_t)m * k * 2 : 0}, {bank ? bank->lora_a : nullptr, results[1].bytes},
+                     {bank ? bank->lora_b : nullptr, results[2].bytes}};
+    for (const auto &r : results) {
+        if (r.bytes)
+            for (const auto &o : operands)
+                if (o.bytes && meet(r.p, r.bytes, o.p, o.bytes)) return KILN_W4A16_ERR_ARGUMENT;
+    }
+    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const BackwardScratch w = backward_scratch(m > 0 ? m : 1, n, k, count, rank);
     char *at = reinterpret_cast<char *>(scratch);
     uint16_t *wt = reinterpret_cast<uint16_t *>(at + w.wt);

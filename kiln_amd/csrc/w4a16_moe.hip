@@ -9,6 +9,7 @@
 
 #include <type_traits>
 
+#include "bank.h"
 #include "device_common.h"
 #include "few_rows.h"
 #include "kiln_w4a16.h"
@@ -369,6 +370,7 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
     if (!x || !expert_of || !weights || !b_gate_up || !s_gate_up || !b_down || !s_down || !y || !scratch) return KILN_W4A16_ERR_ARGUMENT;
     for (const void *p : {x, b_gate_up, s_gate_up, b_down, s_down, static_cast<const void *>(y), static_cast<const void *>(scratch)})
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    if (meet(y, (size_t)prob_m * n_down * 2, x, (size_t)prob_m * hidden * 2)) return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     for (int m0 = 0; m0 < prob_m; m0 += kMoeRun) {
         const int m = prob_m - m0 < kMoeRun ? prob_m - m0 : kMoeRun;

@@ -222,6 +222,8 @@ def proj_backward_bank(dy: torch.Tensor, x: torch.Tensor, packed: MarlinPackedPr
     if bank is None:
         dx = marlin_gemm.marlin_w4a16_gemm_backward(rows, packed.b_packed, packed.scales, packed.groupsize)
         return dx.reshape(x.shape), None, None
+    if adapter_of is None:
+        raise MarlinProjError("marlin_proj: a bank needs adapter_of")
     dx, d_a, d_b = marlin_gemm.marlin_w4a16_gemm_bank_backward(rows, x.reshape(-1, packed.k), packed.b_packed, packed.scales, packed.groupsize,
                                                                bank.a, bank.b, bank.scales, adapter_of.reshape(-1))
     return dx.reshape(x.shape), d_a, d_b

@@ -6,25 +6,26 @@ import pytest
 import torch
 
 from kiln_amd import _lib, lora, marlin_gemm
-from kiln_amd.marlin_proj import MarlinProjError
+from kiln_amd.marlin_proj import MarlinPackedProj, MarlinProjError
 
 P = ctypes.c_void_p(1 << 20)
 ODD = ctypes.c_void_p((1 << 20) + 8)
+Y, Y2, Y3 = (ctypes.c_void_p(i << 40) for i in (1, 2, 3))      # results, which share no memory with operands
 
 
 def bank(a=P, b=P, scales=P, count=3, rank=16):
     return ctypes.byref(_lib.AdapterBank(a, b, scales, count, rank))
 
 
-def forward(m=4, n=512, k=256, g=128, x=P, w=P, y=P, s=P, ws=P, bk=None, of=P, scratch=P):
+def forward(m=4, n=512, k=256, g=128, x=P, w=P, y=Y, s=P, ws=P, bk=None, of=P, scratch=P):
     return _lib.load().kiln_w4a16_gemm_bank(x, w, y, s, m, n, k, ws, g, 0, None, bank() if bk is None else bk, of, scratch)
 
 
-def backward(m=4, n=512, k=256, g=128, dy=P, x=P, w=P, s=P, bk=None, of=P, dx=P, da=P, db=P, scratch=P):
+def backward(m=4, n=512, k=256, g=128, dy=P, x=P, w=P, s=P, bk=None, of=P, dx=Y, da=Y2, db=Y3, scratch=P):
     return _lib.load().kiln_w4a16_gemm_bank_backward(dy, x, w, s, m, n, k, g, 0, None, bank() if bk is None else bk, of, dx, da, db, scratch)
 
 
-def experts(m=4, top=2, count=8, hidden=256, n_out=128, n_down=256, g=128, x=P, of=P, weights=P, packs=(P, P, P, P), y=P, scratch=P):
+def experts(m=4, top=2, count=8, hidden=256, n_out=128, n_down=256, g=128, x=P, of=P, weights=P, packs=(P, P, P, P), y=Y, scratch=P):
     return _lib.load().kiln_w4a16_moe(x, of, weights, *packs, y, m, top, count, hidden, n_out, n_down, g, 0, None, scratch)
 
 
@@ -49,6 +50,26 @@ def test_a_bank_call_refuses(call):
             (dict(dy=None), dict(dx=None), dict(da=None), dict(db=None), dict(dy=ODD), dict(dx=ODD), dict(da=ODD), dict(db=ODD))
         for kw in own:
             assert call(m=m, **kw) == _lib.ERR_ARGUMENT, kw
+
+
+def test_results_that_share_memory_with_operands_are_refused():
+    at = lambda base, bytes: ctypes.c_void_p(base.value + bytes)
+    for m in (4, 40, 400):
+        last = at(P, 2 * m * 256 - 16)                 # the last 16 bytes of x
+        for kw in (dict(y=P), dict(y=last), dict(x=at(Y, 2 * m * 512 - 16)), dict(y=at(P, 2 * 3 * 16 * 512 - 16), x=Y2), dict(bk=bank(a=at(Y, 16)))):
+            assert forward(m=m, **kw) == _lib.ERR_ARGUMENT, kw
+        for kw in (dict(dx=P), dict(dx=last), dict(da=P), dict(db=P), dict(dy=at(Y, 16)), dict(dy=Y2), dict(x=Y3), dict(bk=bank(b=Y2)), dict(bk=bank(a=at(Y3, 32)))):
+            assert backward(m=m, **kw) == _lib.ERR_ARGUMENT, kw
+        for kw in (dict(y=P), dict(y=last), dict(x=at(Y, 2 * m * 256 - 16))):
+            assert experts(m=m, **kw) == _lib.ERR_ARGUMENT, kw
+
+
+def test_a_gradient_of_a_bank_needs_the_rows_adapters():
+    x, dy = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(2, 512, dtype=torch.bfloat16)
+    packed = MarlinPackedProj(torch.zeros(16, 1024, dtype=torch.int32), torch.zeros(2, 512, dtype=torch.float16), 128, 256, 512)
+    made = lora.AdapterBank(torch.zeros(1, 8, 256, dtype=torch.bfloat16), torch.zeros(1, 512, 8, dtype=torch.bfloat16), torch.ones(1))
+    with pytest.raises(MarlinProjError, match="adapter_of"):
+        lora.proj_backward_bank(dy, x, packed, made)
 
 
 def test_calls_without_work_are_no_errors():

@@ -201,6 +201,15 @@ def test_no_rows_and_the_plain_gradient():
         assert torch.equal(marlin_gemm.marlin_w4a16_gemm_backward(p["dy"], p["b"], p["s"], -1).view(torch.int16), backward(p)[0].view(torch.int16))
 
 
+@pytest.mark.parametrize("m", [0, 6, 90])
+def test_a_scale_that_is_no_number_stays_with_its_adapter(m):
+    """An adapter without rows has gradients of zero, whatever its scale."""
+    p = problem(m, 256, 512, 128, 4, 16, "one", seed=11)          # every row the last one's
+    want_y, want = bits(forward(p)), bits(backward(p))
+    p["sc"][0], p["sc"][1] = float("inf"), float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(want_y + want, bits(forward(p)) + bits(backward(p))))
+
+
 def test_gradients_against_differences():
     """d(sum y * dy) along a direction of x, A and B, by the forward in steps either way, against the gradients."""
     p = problem(24, 256, 256, 128, 3, 8, "any", seed=9)
