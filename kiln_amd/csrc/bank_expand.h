@@ -68,24 +68,25 @@ __device__ __forceinline__ void expand_product(const bf16x8 (&b)[TILES][S], cons
     }
 }
 
-// T's slices summed, [positions][rank] of this block's from p0 on
+// T's slices summed, [positions][rank] of this block's from p0 on: four of the rank at a time, eight slices' loads in flight together
 template <int P>
 __device__ __forceinline__ void sum_projected(const float *__restrict__ t, const BankRows &rows, int p0, int rank, int slices, int tid, int threads,
                                               float (&ts)[P][kBankMaxRank + 4]) {
     const size_t stride = (size_t)rows.rows * rank;
-    for (int e = tid; e < P * rank; e += threads) {
+    for (int e = 4 * tid; e < P * rank; e += 4 * threads) {
         const int r = e / rank;
-        const float *from = t + (size_t)p0 * rank + e;
-        float v = 0.f;
-        if (p0 + r < rows.rows) {
-            int s = 0;
-            for (; s + 4 <= slices; s += 4) {
-                const float v0 = from[s * stride], v1 = from[(s + 1) * stride], v2 = from[(s + 2) * stride], v3 = from[(s + 3) * stride];
-                v += (v0 + v1) + (v2 + v3);
-            }
-            for (; s < slices; ++s) v += from[s * stride];
+        const float *from = t + (size_t)min(p0 + r, rows.rows - 1) * rank + (e - r * rank);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < slices; s += 8) {
+            f32x4 d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = *reinterpret_cast<const f32x4 *>(from + min(s + i, slices - 1) * stride);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s + i < slices) v += d[i];
         }
-        ts[r][e - r * rank] = v;
+        *reinterpret_cast<f32x4 *>(&ts[r][e - r * rank]) = v;
     }
     __syncthreads();
 }

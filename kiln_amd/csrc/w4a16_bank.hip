@@ -125,7 +125,7 @@ template <int S>
 __global__ __launch_bounds__(256) void bank_expand_kernel(uint16_t *__restrict__ y, const uint16_t *__restrict__ mat, const float *__restrict__ t,
                                                           const float *__restrict__ scales, BankRows rows, int N, int rank, int slices) {
     constexpr int kTogether = S == 1 ? 4 : 2;
-    __shared__ float ts[16][kBankMaxRank + 4];
+    __shared__ __align__(16) float ts[16][kBankMaxRank + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
     const int p0 = blockIdx.y * kBankRowTile, n0 = blockIdx.x * 64;
     int row, a;
@@ -184,7 +184,7 @@ template <int S>
 __global__ __launch_bounds__(256) void bank_expand_ordered_kernel(uint16_t *__restrict__ y, const uint16_t *__restrict__ mat,
                                                                   const float *__restrict__ t, const float *__restrict__ scales, BankRows rows,
                                                                   int N, int rank, int slices, int columns) {
-    __shared__ float ts[64][kBankMaxRank + 4];
+    __shared__ __align__(16) float ts[64][kBankMaxRank + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
     const int parts = (N + columns - 1) / columns, part = blockIdx.x % parts, p0 = blockIdx.x / parts * 64;
     int row, a;

@@ -105,7 +105,19 @@ __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareL
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[rt][e] = 0.f;
-    for (int base = slice * each; base < min(tiles, (slice + 1) * each); base += kFewTiles) {
+    uint32_t w[kFewAhead];
+    u32x4 s[kFewAhead];
+    auto fetch = [&](int tile0) {
+#pragma unroll
+        for (int u = 0; u < kFewAhead; ++u) {
+            const int tile = min(tile0 + u, tiles - 1);
+            w[u] = words[(size_t)tile * G * 256];
+            s[u] = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, tile * kTileN + 8 * h, p.Gs));
+        }
+    };
+    const int last = min(tiles, (slice + 1) * each);
+    fetch(slice * each + kFewTiles / 2 * half);  // a turn's weights are asked for one turn ahead
+    for (int base = slice * each; base < last; base += kFewTiles) {
         __syncthreads();
         for (int e = tid; e < 32 * RT * (kFewColumns / 8); e += kPrepareThreads) {  // (N is a multiple of kFewColumns)
             const int row = e / (kFewColumns / 8), at = 8 * (e % (kFewColumns / 8));
@@ -116,21 +128,22 @@ __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareL
 #pragma unroll 1
         for (int u0 = 0; u0 < kFewTiles / 2; u0 += kFewAhead) {
             const int tile0 = kFewTiles / 2 * half + u0;
-            uint32_t w[kFewAhead];
-            u32x4 s[kFewAhead];
+            uint32_t w_now[kFewAhead];
+            u32x4 s_now[kFewAhead];
 #pragma unroll
             for (int u = 0; u < kFewAhead; ++u) {
-                w[u] = words[(size_t)(base + tile0 + u) * G * 256];
-                s[u] = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, (base + tile0 + u) * kTileN + 8 * h, p.Gs));
+                w_now[u] = w[u];
+                s_now[u] = s[u];
             }
+            fetch(base + tile0 + kFewAhead + (u0 + kFewAhead < kFewTiles / 2 ? 0 : kFewTiles / 2));
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < kFewAhead; ++u) {
-                const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(w[u], lane), lane), lane);
+                const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(w_now[u], lane), lane), lane);
                 bf16x8 o;
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? s[u][c >> 1] >> 16 : s[u][c >> 1])));
+                    o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? s_now[u][c >> 1] >> 16 : s_now[u][c >> 1])));
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
                     acc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o, load_bf16x8(lds.dy + (32 * rt + r) * kFewDyPitch + (tile0 + u) * kTileN + 8 * h), acc[rt], 0, 0, 0);

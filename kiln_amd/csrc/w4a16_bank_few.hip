@@ -61,7 +61,7 @@ template <int W, int GW, int S, int SR, bool OWN>
 __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
     constexpr int kMost = 16 / W, kPitch = S * 16 + 4;
     __shared__ __align__(16) float part[W][16][kPitch];
-    __shared__ float ts[16][kBankMaxRank + 4];
+    __shared__ __align__(16) float ts[16][kBankMaxRank + 4];
     __shared__ float parts_of_t[OWN ? W : 1][kOwnRows][32 * SR];
     if constexpr (OWN) {  // (this wavefront's own, until the block meets)
         for (int e = threadIdx.x & 63; e < kOwnRows * 32 * SR; e += 64) (&parts_of_t[threadIdx.x >> 6][0][0])[e] = 0.f;
