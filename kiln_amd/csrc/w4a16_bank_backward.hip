@@ -16,6 +16,14 @@
 namespace kiln {
 namespace {
 
+// Column e of eight rows of eight bf16 values each, as an operand of a product over the rows.
+__device__ __forceinline__ bf16x8 column_of_rows(const u32x4 (&v)[8], int e) {
+    u32x4 pairs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pairs[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(bf16x8, pairs);
+}
+
 // ---- what the products read ----------------------------------------------------------------------------------------
 // One launch for what depends on the call's operands alone: the rows' order, the adapters' matrices turned, and W unpacked row by row.
 struct PrepareArgs {
@@ -28,15 +36,17 @@ struct PrepareArgs {
     BankRows rows;
     int K, N, Gs, rank;
     int order_blocks, turn_blocks;
-    const uint16_t *dy;     // few rows: [m, N],
-    float *partial;         // [slices, m, K]
-    int m, slices;
+    const uint16_t *dy, *x;  // few rows: [m, N] and [m, K],
+    float *partial;          // [slices, m, K],
+    float *t, *u;            // ... and T and U, [slices, m, rank]
+    int m, slices, t_slices, u_slices, turns;
 };
 constexpr int kPrepareThreads = 512, kTurnPitch = 128 + 8, kFewPitch = 128 + 4, kFewDyPitch = 256 + 8;
 union PrepareLds {
     uint16_t dy[64 * kFewDyPitch];
     uint16_t weight[128 * kTurnPitch];
     float sums[64 * kFewPitch];
+    float projected[kPrepareThreads / 64][16][kBankMaxRank + 4];
     uint16_t bank[64][kBankMaxRank + 2];
     OrderLds<kPrepareThreads / 64> order;
 };
@@ -93,6 +103,7 @@ __device__ __forceinline__ void unpack_weight(const PrepareArgs &p, int block, P
 // A block takes one scale group and slice, a wavefront 32 rows of k and every other eight of sixteen column tiles, whose part of dy is in
 // LDS; the halves meet there.  Bound by its start, and by its instructions' (straight-line code is read from memory once in every
 // launch: four tiles to a turn of the loop, not all eight, took 45 rows of 4096 <- 2560 from 20 us to 16, dy through LDS to 15).
+constexpr int kFewProjected = 8;  // slices of T's and U's contraction at most
 constexpr int kFewRows = 64, kFewAhead = 4, kFewTiles = 16, kFewColumns = kFewTiles * kTileN;
 template <int RT>
 __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareLds &lds) {
@@ -167,11 +178,89 @@ __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareL
             *reinterpret_cast<const f32x4 *>(lds.sums + (e >> 5) * kFewPitch + 4 * (e & 31));
 }
 
+// Up to 64 rows: T = x A^T or U = dy B of 16 rows and one slice of the contraction, for the adapters met among them whose turn is `turn0`
+// modulo p.turns.  A's rows are contiguous along the contraction; of B, [n, rank], a lane reads eight of the rank for each of its eight n
+// and pairs the n's values (v_perm), one product for each of the eight, as bank_grad_kernel does for its rows.
+__device__ __forceinline__ void few_project(const PrepareArgs &p, bool of_x, int slice, int tile, unsigned turn0, PrepareLds &lds) {
+    constexpr int W = kPrepareThreads / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4, p0 = 16 * tile, rank = p.rank;
+    const int len = of_x ? p.K : p.N, slices = of_x ? p.t_slices : p.u_slices;
+    const int each = (len / 128 + slices - 1) / slices * 128, begin = slice * each + 32 * wave, end = min(len, (slice + 1) * each);
+    int a = p0 + c < p.m ? p.rows.of[p0 + c] : -1;
+    if ((unsigned)a >= (unsigned)p.rows.count) a = -1;
+    unsigned left = (unsigned)__ballot(a >= 0) & 0xFFFFu;
+    const uint16_t *src = (of_x ? p.x : p.dy) + (size_t)min(p0 + c, p.m - 1) * len + 8 * q;
+    for (unsigned turn = 0; left; ++turn) {
+        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
+        const unsigned mine = (unsigned)__ballot(a == cur) & 0xFFFFu;
+        left &= ~mine;
+        if (turn % p.turns != turn0) continue;
+        if (of_x) {
+            for (int j0 = 0; j0 < rank; j0 += 16) {  // rows past the rank: the last one again, their sums are dropped
+                const uint16_t *mat = p.a + ((size_t)cur * rank + min(j0 + c, rank - 1)) * len + 8 * q;
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                for (int at = begin; at < end; at += 4 * 32 * W) {
+                    bf16x8 x[4], m[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        x[u] = load_bf16x8(src + min(at + 32 * W * u, len - 32));
+                        m[u] = load_bf16x8(mat + min(at + 32 * W * u, len - 32));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (at + 32 * W * u < end) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], m[u], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lds.projected[wave][4 * q + i][j0 + c] = acc[i];
+            }
+        } else {
+            const int r8 = 8 * min(c, rank / 8 - 1);
+            const uint16_t *mat = p.b + ((size_t)cur * len + 8 * q) * rank + r8;
+            f32x4 acc[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int at = begin; at < end; at += 2 * 32 * W) {
+                bf16x8 x[2];
+                u32x4 v[2][8];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int n = min(at + 32 * W * u, len - 32);
+                    x[u] = load_bf16x8(src + n);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[u][i] = *reinterpret_cast<const u32x4 *>(mat + (size_t)(n + i) * rank);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (at + 32 * W * u < end)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], column_of_rows(v[u], e), acc[e], 0, 0, 0);
+            }
+            if (c < rank / 8)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) lds.projected[wave][4 * q + i][8 * c + e] = acc[e][i];
+        }
+        __syncthreads();
+        float *out = (of_x ? p.t : p.u) + ((size_t)slice * p.m + p0) * rank;
+        for (int e = tid; e < 16 * rank; e += kPrepareThreads) {
+            const int r = e / rank, j = e - r * rank;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v += lds.projected[w][r][j];
+            if (mine >> r & 1) out[e] = v;
+        }
+        __syncthreads();
+    }
+}
+
 // at[a][k][rank] of a[a][rank][k], or bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows of several
 // adapters at once, zeros for those of others, so it holds finite values alone; where A holds others, odd[a][k / 64] is set and
 // bank_grad_kernel adds their products for the rows of that adapter.
 __device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, PrepareLds &lds) {
-    const int tid = threadIdx.x, rank = p.rank, of_a = p.at ? p.K / 64 : 0, parts = of_a + p.N / 64, a = block / parts, part = block % parts;
+    const int tid = threadIdx.x, rank = p.rank, of_a = p.K / 64, parts = of_a + p.N / 64, a = block / parts, part = block % parts;
     const bool is_a = part < of_a;
     const int len = is_a ? p.K : p.N, l0 = (is_a ? part : part - of_a) * 64;
     const size_t base = (size_t)a * rank * len;
@@ -195,19 +284,29 @@ __device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, Prepa
     }
 }
 
-// RT: row tiles of a call of few rows, or 0 for a weight unpacked
+// RT: row tiles of a call of few rows, whose projections are here too, or 0 for a weight unpacked
 template <int RT>
-__global__ __launch_bounds__(kPrepareThreads) void bank_prepare_kernel(PrepareArgs p) {
+__global__ __launch_bounds__(kPrepareThreads, 4) void bank_prepare_kernel(PrepareArgs p) {
     __shared__ __align__(16) PrepareLds lds;
     int block = blockIdx.x;
-    if (block < p.order_blocks) {
-        order_rows(p.rows.of, p.rows.order, p.rows.first, p.rows.rows, p.rows.count, block, lds.order);
-        return;
+    if constexpr (RT > 0) {
+        if (block < p.slices * (p.K / kGroupK)) {
+            few_dx<RT>(p, block, lds);
+            return;
+        }
+        block -= p.slices * (p.K / kGroupK);
+        const int all = p.t_slices + p.u_slices, place = block % all, rest = block / all;
+        const bool of_x = place >= p.u_slices;
+        few_project(p, of_x, of_x ? place - p.u_slices : place, rest / p.turns, rest % p.turns, lds);
+    } else {
+        if (block < p.order_blocks) {
+            order_rows(p.rows.of, p.rows.order, p.rows.first, p.rows.rows, p.rows.count, block, lds.order);
+            return;
+        }
+        block -= p.order_blocks;
+        if (block < p.turn_blocks) turn_bank(p, block, lds);
+        else unpack_weight(p, block - p.turn_blocks, lds);
     }
-    block -= p.order_blocks;
-    if (block < p.turn_blocks) turn_bank(p, block, lds);
-    else if constexpr (RT > 0) few_dx<RT>(p, block - p.turn_blocks, lds);
-    else unpack_weight(p, block - p.turn_blocks, lds);
 }
 
 // sums over slices: x[0][i] += x[1][i] + ... (both projections in one launch)
@@ -410,15 +509,39 @@ struct GradArgs {
     const uint16_t *a;   // the adapters' A as they lie, [count, rank, K]
     const uint8_t *odd;  // [count, K / 64]: where A holds values that are no finite numbers,
     uint16_t *dx;        // whose products are still to be added here
-    const float *partial;  // few rows: [slices, rows, K], dx's to be summed and joined by U A here
-    int grad_blocks, slices;
+    const float *partial;  // few rows: [slices, rows, K], dx's to be summed and joined by U A here,
+    int grad_blocks, slices, t_slices, u_slices;  // as are T's and U's slices
 };
 
-// dx of few rows: the slices' sum and the low-rank term, 4 W 64 of k of one position to a block
-__device__ __forceinline__ void finish_dx(const GradArgs &p, int block, int threads) {
-    const int parts = (p.K / 4 + threads - 1) / threads, at = block / parts, k = (block % parts * threads + (int)threadIdx.x) * 4;
+// T or U of few rows, their slices summed: ts[i] = row list[i]'s
+__device__ __forceinline__ void sum_few(const GradArgs &p, bool of_t, const int *list, int count, int threads, float (&ts)[kFewRows][kBankMaxRank + 4]) {
+    const size_t stride = (size_t)p.rows.rows * p.rank;
+    const int slices = of_t ? p.t_slices : p.u_slices;
+    for (int e = 4 * (int)threadIdx.x; e < count * p.rank; e += 4 * threads) {
+        const int i = e / p.rank, col = e - i * p.rank;
+        const float *from = (of_t ? p.t : p.u) + (size_t)list[i] * p.rank + col;
+        f32x4 d[kFewProjected], v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kFewProjected; ++s) d[s] = *reinterpret_cast<const f32x4 *>(from + min(s, slices - 1) * stride);
+#pragma unroll
+        for (int s = 0; s < kFewProjected; ++s)
+            if (s < slices) v += d[s];
+        *reinterpret_cast<f32x4 *>(&ts[i][col]) = v;
+    }
+    __syncthreads();
+}
+
+// dx of few rows: the slices' sum and the low-rank term, 4 W 64 of k of one row to a block
+__device__ __forceinline__ void finish_dx(const GradArgs &p, int block, int threads, int *list, float (&ts)[kFewRows][kBankMaxRank + 4]) {
+    const int parts = (p.K / 4 + threads - 1) / threads, row = block / parts, k = (block % parts * threads + (int)threadIdx.x) * 4;
+    int a = p.rows.of[row];
+    if ((unsigned)a >= (unsigned)p.rows.count) a = -1;
+    if (a >= 0) {
+        if (threadIdx.x == 0) list[0] = row;
+        __syncthreads();
+        sum_few(p, false, list, 1, threads, ts);
+    }
     if (k >= p.K) return;
-    const int row = p.rows.order ? p.rows.order[at] : at;
     const size_t stride = (size_t)p.rows.rows * p.K;
     const float *from = p.partial + (size_t)row * p.K + k;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -430,10 +553,9 @@ __device__ __forceinline__ void finish_dx(const GradArgs &p, int block, int thre
         v += (d[0] + d[1]) + (d[2] + d[3]);
     }
     for (; s < p.slices; ++s) v += *reinterpret_cast<const f32x4 *>(from + s * stride);
-    const int a = p.rows.order && at < p.rows.first[p.rows.count] ? p.rows.of[row] : -1;
     if (a >= 0) {
         const uint16_t *m = p.a + (size_t)a * p.rank * p.K + k;
-        const float *u = p.u + (size_t)at * p.rank;
+        const float *u = ts[0];
         f32x4 low = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < p.rank; r0 += 8) {
             u32x2 d[8];
@@ -459,20 +581,35 @@ __device__ __forceinline__ void finish_dx(const GradArgs &p, int block, int thre
 }
 
 constexpr int kGradPitch = 128 + 4;
-template <int JT, int W>
+// FEW: rows as they stand, 64 at most, T and U still in slices
+template <int JT, int W, bool FEW>
 __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     __shared__ float sum[JT * 16 * kGradPitch];
+    __shared__ int list[FEW ? kFewRows : 1];
+    __shared__ __align__(16) float ts[FEW ? kFewRows : 1][kBankMaxRank + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4;
-    if ((int)blockIdx.x >= p.grad_blocks) {
-        finish_dx(p, blockIdx.x - p.grad_blocks, W * 64);
-        return;
+    if constexpr (FEW) {
+        if ((int)blockIdx.x >= p.grad_blocks) {
+            finish_dx(p, blockIdx.x - p.grad_blocks, W * 64, list, ts);
+            return;
+        }
     }
     const int parts = p.N / 128 + p.K / 128, a = blockIdx.x / parts, block = blockIdx.x % parts;
     const bool is_b = block < p.N / 128;
     const int c0 = (is_b ? block : block - p.N / 128) * 128, len = is_b ? p.N : p.K;
     const uint16_t *src = (is_b ? p.dy : p.x) + c0 + 8 * c;
     const float *f = is_b ? p.t : p.u;
-    const int begin = p.rows.first[a], end = p.rows.first[a + 1];
+    int begin = 0, end;
+    if constexpr (FEW) {
+        const bool mine = lane < p.rows.rows && p.rows.of[lane] == a;
+        const unsigned long long all = __ballot(mine);
+        end = __popcll(all);
+        if (wave == 0 && mine) list[__popcll(all & ((1ull << lane) - 1))] = lane;
+        __syncthreads();
+        sum_few(p, is_b, list, end, W * 64, ts);
+    } else {
+        begin = p.rows.first[a], end = p.rows.first[a + 1];
+    }
     int col[JT];  // past the rank: the last again, dropped at the end
 #pragma unroll
     for (int j = 0; j < JT; ++j) col[j] = min(16 * j + c, p.rank - 1);
@@ -484,7 +621,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
     int row[8];
     auto rows_at = [&](int at) {  // positions past the last: the last again, times zeros
 #pragma unroll
-        for (int i = 0; i < 8; ++i) row[i] = p.rows.order[min(at + 8 * q + i, end - 1)];
+        for (int i = 0; i < 8; ++i) row[i] = FEW ? list[min(at + 8 * q + i, end - 1)] : p.rows.order[min(at + 8 * q + i, end - 1)];
     };
     int at = begin + 32 * wave;
     if (at < end) rows_at(at);
@@ -496,7 +633,8 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < JT; ++j) w[j][i] = f[(size_t)min(at + 8 * q + i, end - 1) * p.rank + col[j]];
+            for (int j = 0; j < JT; ++j)
+                w[j][i] = FEW ? ts[FEW ? min(at + 8 * q + i, end - 1) : 0][col[j]] : f[(size_t)min(at + 8 * q + i, end - 1) * p.rank + col[j]];
         rows_at(at + 32 * W);
         __builtin_amdgcn_sched_barrier(0);
         bf16x8 hi[JT], lo[JT];
@@ -510,11 +648,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
             }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            u32x4 pairs;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                pairs[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-            const bf16x8 b = __builtin_bit_cast(bf16x8, pairs);
+            const bf16x8 b = column_of_rows(v, e);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 acc[e][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi[j], b, acc[e][j], 0, 0, 0);
@@ -547,7 +681,7 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
         }
         *reinterpret_cast<u32x4 *>(is_b ? out + (size_t)col * p.rank + 8 * r : out + (size_t)r * p.K + 8 * col) = o;
     }
-    if (is_b || p.partial) return;
+    if (FEW || is_b) return;
     const uint8_t *odd = p.odd + (size_t)a * (p.K / 64) + c0 / 64;
     if (!(odd[0] | odd[1])) return;
     for (int at = begin + (tid >> 7); at < end; at += W / 2) {
@@ -563,15 +697,19 @@ __global__ __launch_bounds__(W * 64) void bank_grad_kernel(GradArgs p) {
 }
 
 template <int JT, int W>
-void launch_grad(const GradArgs &g, hipStream_t stream) {
-    const int dx_blocks = g.partial ? g.rows.rows * ((g.K / 4 + W * 64 - 1) / (W * 64)) : 0;
-    bank_grad_kernel<JT, W><<<g.grad_blocks + dx_blocks, W * 64, 0, stream>>>(g);
+void launch_grad(const GradArgs &g, bool few, hipStream_t stream) {
+    if (few) {
+        const int dx_blocks = g.rows.rows * ((g.K / 4 + W * 64 - 1) / (W * 64));
+        bank_grad_kernel<JT, W, true><<<g.grad_blocks + dx_blocks, W * 64, 0, stream>>>(g);
+    } else {
+        bank_grad_kernel<JT, W, false><<<g.grad_blocks, W * 64, 0, stream>>>(g);
+    }
 }
 template <int JT>
-void launch_grad(GradArgs g, hipStream_t stream) {
+void launch_grad(GradArgs g, bool few, hipStream_t stream) {
     g.grad_blocks = (g.N / 128 + g.K / 128) * g.rows.count;
-    if (g.grad_blocks >= 512) launch_grad<JT, 4>(g, stream);
-    else launch_grad<JT, 8>(g, stream);
+    if (g.grad_blocks >= 512) launch_grad<JT, 4>(g, few, stream);
+    else launch_grad<JT, 8>(g, few, stream);
 }
 
 // ---- the plan ----------------------------------------------------------------------------------------------------
@@ -606,11 +744,14 @@ DxPlan dx_plan(int m, int n, int k) {
 }
 
 void launch_prepare(const PrepareArgs &p, hipStream_t stream) {
-    const int blocks = p.order_blocks + p.turn_blocks;
-    if (p.m == 0) bank_prepare_kernel<0><<<blocks, kPrepareThreads, 0, stream>>>(p);  // (the order alone)
-    else if (p.m > kFewRows) bank_prepare_kernel<0><<<blocks + (p.N / 128) * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
-    else if (p.m > 32) bank_prepare_kernel<2><<<blocks + p.slices * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
-    else bank_prepare_kernel<1><<<blocks + p.slices * (p.K / 128), kPrepareThreads, 0, stream>>>(p);
+    const int groups = p.K / kGroupK;
+    if (p.m > kFewRows) {
+        bank_prepare_kernel<0><<<p.order_blocks + p.turn_blocks + (p.N / 128) * groups, kPrepareThreads, 0, stream>>>(p);
+        return;
+    }
+    const int blocks = p.slices * groups + (p.t_slices + p.u_slices) * ((p.m + 15) / 16) * p.turns;
+    if (p.m > 32) bank_prepare_kernel<2><<<blocks, kPrepareThreads, 0, stream>>>(p);
+    else bank_prepare_kernel<1><<<blocks, kPrepareThreads, 0, stream>>>(p);
 }
 
 template <int WM, int WN, int TM, int TN>
@@ -626,6 +767,12 @@ void launch_dx(DxArgs p, int slices, hipStream_t stream) {
 int few_slices(int n) {
     const int turns = n / kFewColumns, slices = turns < 16 ? turns : 16, each = (turns + slices - 1) / slices;
     return (turns + each - 1) / each;
+}
+
+// ... and of their projections' contraction, of 1024 at least
+int few_project_slices(int len) {
+    const int groups = len / 128, slices = (groups + 7) / 8 < kFewProjected ? (groups + 7) / 8 : kFewProjected, each = (groups + slices - 1) / slices;
+    return (groups + each - 1) / each;
 }
 
 struct BackwardScratch {
@@ -644,12 +791,17 @@ BackwardScratch backward_scratch(int m, int n, int k, int count, int rank) {
     s.few = m <= kFewRows ? few_slices(n) : 0;
     s.wt = take(s.few ? 0 : (size_t)k * n * 2);
     if (count > 0) {
-        s.at = take(s.few ? 0 : (size_t)count * rank * k * 2);
-        s.bt = take((size_t)count * rank * n * 2);
-        s.odd = take((size_t)count * (k / 64));
-        s.order = take(bank_order_bytes(m, count));
-        s.t_slices = bank_slices(m, k);
-        s.u_slices = bank_slices(m, n);
+        if (s.few) {
+            s.t_slices = few_project_slices(k);
+            s.u_slices = few_project_slices(n);
+        } else {
+            s.at = take((size_t)count * rank * k * 2);
+            s.bt = take((size_t)count * rank * n * 2);
+            s.odd = take((size_t)count * (k / 64));
+            s.order = take(bank_order_bytes(m, count));
+            s.t_slices = bank_slices(m, k);
+            s.u_slices = bank_slices(m, n);
+        }
         s.t = take((size_t)s.t_slices * m * rank * 4);
         s.u = take((size_t)s.u_slices * m * rank * 4);
     }
@@ -723,29 +875,37 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     prepare.m = m;
     prepare.slices = w.few;
     if (bank) {
-        uint16_t *a_t = reinterpret_cast<uint16_t *>(at + w.at), *b_t = reinterpret_cast<uint16_t *>(at + w.bt);
-        uint8_t *odd = reinterpret_cast<uint8_t *>(at + w.odd);
         float *t = reinterpret_cast<float *>(at + w.t), *u = reinterpret_cast<float *>(at + w.u);
         const uint16_t *lora_a = (const uint16_t *)bank->lora_a;
-        dx.rows = bank_rows(adapter_of, m, count, at + w.order);
+        uint16_t *a_t = reinterpret_cast<uint16_t *>(at + w.at), *b_t = reinterpret_cast<uint16_t *>(at + w.bt);
+        uint8_t *odd = reinterpret_cast<uint8_t *>(at + w.odd);
+        dx.rows = w.few ? BankRows{adapter_of, nullptr, nullptr, m, count} : bank_rows(adapter_of, m, count, at + w.order);
         prepare.a = lora_a;
         prepare.b = (const uint16_t *)bank->lora_b;
-        prepare.at = w.few ? nullptr : a_t;
-        prepare.bt = b_t;
-        prepare.odd = odd;
         prepare.rows = dx.rows;
         prepare.rank = rank;
-        prepare.order_blocks = count + 1;
-        prepare.turn_blocks = m > 0 ? count * ((w.few ? 0 : k / 64) + n / 64) : 0;
-        launch_prepare(prepare, hs);
-        if (m > 0) {
+        if (w.few) {
+            prepare.x = (const uint16_t *)A;
+            prepare.t = t;
+            prepare.u = u;
+            prepare.t_slices = w.t_slices;
+            prepare.u_slices = w.u_slices;
+            prepare.turns = count < 16 ? count : 16;  // the adapters that 16 rows may have
+            if (m > 0) launch_prepare(prepare, hs);
+        } else {
+            prepare.at = a_t;
+            prepare.bt = b_t;
+            prepare.odd = odd;
+            prepare.order_blocks = count + 1;
+            prepare.turn_blocks = count * (k / 64 + n / 64);
+            launch_prepare(prepare, hs);
             const BankProjection of_x{A, lora_a, t, k, w.t_slices};
             bank_project(BankProjection{dC, b_t, u, n, w.u_slices}, &of_x, dx.rows, rank, hs);
             if (w.t_slices > 1 || w.u_slices > 1)
                 sum_slices_kernel<<<dim3((unsigned)(((size_t)m * rank + 255) / 256), 2), 256, 0, hs>>>(t, w.t_slices, u, w.u_slices, (size_t)m * rank);
         }
         grad = GradArgs{(const uint16_t *)A, (const uint16_t *)dC, t, u, bank->scales, (uint16_t *)d_lora_a, (uint16_t *)d_lora_b,
-                        dx.rows, k, n, rank, lora_a, odd, (uint16_t *)dA, w.few && m > 0 ? partial : nullptr, 0, w.few};
+                        dx.rows, k, n, rank, lora_a, odd, (uint16_t *)dA, partial, 0, w.few, w.t_slices, w.u_slices};
         dx.at = a_t;
         dx.u = u;
         dx.scales = bank->scales;
@@ -766,10 +926,10 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
     }
     if (bank) {  // behind dx, to which it adds where an adapter holds what is no finite number
         switch ((rank + 15) / 16) {
-            case 1: launch_grad<1>(grad, hs); break;
-            case 2: launch_grad<2>(grad, hs); break;
-            case 3: launch_grad<3>(grad, hs); break;
-            default: launch_grad<4>(grad, hs); break;
+            case 1: launch_grad<1>(grad, w.few, hs); break;
+            case 2: launch_grad<2>(grad, w.few, hs); break;
+            case 3: launch_grad<3>(grad, w.few, hs); break;
+            default: launch_grad<4>(grad, w.few, hs); break;
         }
     }
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
