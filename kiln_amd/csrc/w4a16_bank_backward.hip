@@ -7,6 +7,8 @@
 // Steps: W as bf16 with its columns contiguous (what a product over the columns reads), the adapters' matrices transposed, T = x A^T and
 // U = dy B in f32, then dx as one matrix product into which U A goes as further steps of the contraction, and dA, dB as sums over the
 // rows of an adapter.  Rows are taken in the order of their adapters throughout.
+#include <type_traits>
+
 #include "async_loads.h"
 #include "bank.h"
 #include "bank_expand.h"
@@ -42,13 +44,20 @@ struct PrepareArgs {
     int m, slices, t_slices, u_slices, turns;
 };
 constexpr int kPrepareThreads = 512, kTurnPitch = 128 + 8, kFewPitch = 128 + 4, kFewDyPitch = 256 + 8;
+constexpr int kFewTiles = 16, kFewColumns = kFewTiles * kTileN;
 union PrepareLds {
-    uint16_t dy[64 * kFewDyPitch];
     uint16_t weight[128 * kTurnPitch];
-    float sums[64 * kFewPitch];
-    float projected[kPrepareThreads / 64][16][kBankMaxRank + 4];
     uint16_t bank[64][kBankMaxRank + 2];
     OrderLds<kPrepareThreads / 64> order;
+};
+union FewLds {
+    struct {
+        uint16_t dy[64 * kFewDyPitch];
+        u32x4 codes[kFewTiles * 64];
+        uint16_t scales[kFewColumns];
+    } in;
+    float sums[64 * kFewPitch];
+    float projected[kPrepareThreads / 64][16][kBankMaxRank + 4];
 };
 
 // wt[k][n] = bf16((code - 8) * scale): a block takes one scale group (128 rows) x 128 columns, a chunk to each of its eight wavefronts.  The
@@ -104,61 +113,50 @@ __device__ __forceinline__ void unpack_weight(const PrepareArgs &p, int block, P
 // LDS; the halves meet there.  Bound by its start, and by its instructions' (straight-line code is read from memory once in every
 // launch: four tiles to a turn of the loop, not all eight, took 45 rows of 4096 <- 2560 from 20 us to 16, dy through LDS to 15).
 constexpr int kFewProjected = 8;  // slices of T's and U's contraction at most
-constexpr int kFewRows = 64, kFewAhead = 4, kFewTiles = 16, kFewColumns = kFewTiles * kTileN;
+constexpr int kFewRows = 64;
 template <int RT>
-__device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareLds &lds) {
+__device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, FewLds &lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 7, kq = lane >> 3 & 3, h = lane >> 5, r = lane & 31;
     const int t = wave & 3, half = wave >> 2, G = p.K / kGroupK, tiles = p.N / kTileN, g = block / p.slices, slice = block % p.slices;
     const int turns = (tiles + kFewTiles - 1) / kFewTiles, each = (turns + p.slices - 1) / p.slices * kFewTiles;
-    const uint32_t *words = reinterpret_cast<const uint32_t *>(p.B) + ((size_t)g * 64 + i + 8 * h + 16 * kq) * 4 + t;
+    const uint32_t *words = reinterpret_cast<const uint32_t *>(lds.in.codes) + (i + 8 * h + 16 * kq) * 4 + t;
     f32x16 acc[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[rt][e] = 0.f;
-    uint32_t w[kFewAhead];
-    u32x4 s[kFewAhead];
-    auto fetch = [&](int tile0) {
+    u32x4 codes[kFewTiles / 8], scales = {0u, 0u, 0u, 0u}, dy[2 * RT];
+    auto fetch = [&](int base) {  // (N is a multiple of kFewColumns)
 #pragma unroll
-        for (int u = 0; u < kFewAhead; ++u) {
-            const int tile = min(tile0 + u, tiles - 1);
-            w[u] = words[(size_t)tile * G * 256];
-            s[u] = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, tile * kTileN + 8 * h, p.Gs));
-        }
+        for (int u = 0; u < kFewTiles / 8; ++u) codes[u] = p.B[((size_t)(base + 8 * u + wave) * G + g) * 64 + lane];
+        if (tid < 2 * kFewTiles)
+            scales = *reinterpret_cast<const u32x4 *>(p.S + scale_index(p.Gs == 1 ? 0 : g, (base + (tid >> 1)) * kTileN + 8 * (tid & 1), p.Gs));
+#pragma unroll
+        for (int u = 0; u < 2 * RT; ++u)
+            dy[u] = *reinterpret_cast<const u32x4 *>(p.dy + (size_t)min(16 * u + (tid >> 5), p.m - 1) * p.N + base * kTileN + 8 * (tid & 31));
     };
     const int last = min(tiles, (slice + 1) * each);
-    fetch(slice * each + kFewTiles / 2 * half);  // a turn's weights are asked for one turn ahead
+    fetch(slice * each);
     for (int base = slice * each; base < last; base += kFewTiles) {
         __syncthreads();
-        for (int e = tid; e < 32 * RT * (kFewColumns / 8); e += kPrepareThreads) {  // (N is a multiple of kFewColumns)
-            const int row = e / (kFewColumns / 8), at = 8 * (e % (kFewColumns / 8));
-            *reinterpret_cast<u32x4 *>(lds.dy + row * kFewDyPitch + at) =
-                *reinterpret_cast<const u32x4 *>(p.dy + (size_t)min(row, p.m - 1) * p.N + base * kTileN + at);
-        }
+#pragma unroll
+        for (int u = 0; u < kFewTiles / 8; ++u) lds.in.codes[(8 * u + wave) * 64 + lane] = codes[u];
+        if (tid < 2 * kFewTiles) *reinterpret_cast<u32x4 *>(lds.in.scales + 8 * tid) = scales;
+#pragma unroll
+        for (int u = 0; u < 2 * RT; ++u) *reinterpret_cast<u32x4 *>(lds.in.dy + (16 * u + (tid >> 5)) * kFewDyPitch + 8 * (tid & 31)) = dy[u];
         __syncthreads();
+        fetch(min(base + kFewTiles, tiles - kFewTiles));
 #pragma unroll 1
-        for (int u0 = 0; u0 < kFewTiles / 2; u0 += kFewAhead) {
-            const int tile0 = kFewTiles / 2 * half + u0;
-            uint32_t w_now[kFewAhead];
-            u32x4 s_now[kFewAhead];
+        for (int tile = kFewTiles / 2 * half; tile < kFewTiles / 2 * (half + 1); ++tile) {
+            const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(words[tile * 256], lane), lane), lane);
+            const u32x4 s = *reinterpret_cast<const u32x4 *>(lds.in.scales + tile * kTileN + 8 * h);
+            bf16x8 o;
 #pragma unroll
-            for (int u = 0; u < kFewAhead; ++u) {
-                w_now[u] = w[u];
-                s_now[u] = s[u];
-            }
-            fetch(base + tile0 + kFewAhead + (u0 + kFewAhead < kFewTiles / 2 ? 0 : kFewTiles / 2));
-            __builtin_amdgcn_sched_barrier(0);
+            for (int c = 0; c < 8; ++c)
+                o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? s[c >> 1] >> 16 : s[c >> 1])));
 #pragma unroll
-            for (int u = 0; u < kFewAhead; ++u) {
-                const uint32_t v = exchange_nibbles<4>(exchange_nibbles<2>(exchange_nibbles<1>(w_now[u], lane), lane), lane);
-                bf16x8 o;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    o[c] = (__bf16)((float)((int)(v >> (4 * c) & 0xF) - 8) * f16_bits_to_f32((uint16_t)(c & 1 ? s_now[u][c >> 1] >> 16 : s_now[u][c >> 1])));
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    acc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o, load_bf16x8(lds.dy + (32 * rt + r) * kFewDyPitch + (tile0 + u) * kTileN + 8 * h), acc[rt], 0, 0, 0);
-            }
+            for (int rt = 0; rt < RT; ++rt)
+                acc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o, load_bf16x8(lds.in.dy + (32 * rt + r) * kFewDyPitch + tile * kTileN + 8 * h), acc[rt], 0, 0, 0);
         }
     }
     for (int w = 0; w < 2; ++w) {
@@ -181,7 +179,7 @@ __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, PrepareL
 // Up to 64 rows: T = x A^T or U = dy B of 16 rows and one slice of the contraction, for the adapters met among them whose turn is `turn0`
 // modulo p.turns.  A's rows are contiguous along the contraction; of B, [n, rank], a lane reads eight of the rank for each of its eight n
 // and pairs the n's values (v_perm), one product for each of the eight, as bank_grad_kernel does for its rows.
-__device__ __forceinline__ void few_project(const PrepareArgs &p, bool of_x, int slice, int tile, unsigned turn0, PrepareLds &lds) {
+__device__ __forceinline__ void few_project(const PrepareArgs &p, bool of_x, int slice, int tile, unsigned turn0, FewLds &lds) {
     constexpr int W = kPrepareThreads / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4, p0 = 16 * tile, rank = p.rank;
     const int len = of_x ? p.K : p.N, slices = of_x ? p.t_slices : p.u_slices;
@@ -287,7 +285,7 @@ __device__ __forceinline__ void turn_bank(const PrepareArgs &p, int block, Prepa
 // RT: row tiles of a call of few rows, whose projections are here too, or 0 for a weight unpacked
 template <int RT>
 __global__ __launch_bounds__(kPrepareThreads, 4) void bank_prepare_kernel(PrepareArgs p) {
-    __shared__ __align__(16) PrepareLds lds;
+    __shared__ __align__(16) std::conditional_t<(RT > 0), FewLds, PrepareLds> lds;
     int block = blockIdx.x;
     if constexpr (RT > 0) {
         if (block < p.slices * (p.K / kGroupK)) {
