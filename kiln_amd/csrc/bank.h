@@ -45,9 +45,14 @@ struct BankProjection {
 };
 void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream);
 
-// up to 16 rows as they stand: y = x W + the low-rank term of their projections t, in one launch
+// up to 16 rows as they stand: y = x W, and their projection (bank_base_slices of it) in the same launch
 constexpr int kBankFewRows = 16;
-void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, const float *t, int slices,
-              int K, int N, bool per_column, hipStream_t stream);
+int bank_base_slices(int K);
+void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column,
+               hipStream_t stream);
+// ... or a row or two with their low-rank term in one launch
+bool bank_projects_itself(int m, int n, int k, int rank);
+void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, int K, int N, bool per_column,
+              hipStream_t stream);
 
 }  // namespace kiln

@@ -1,7 +1,8 @@
 // A packed projection whose rows have low-rank adapters of their own out of a bank:
 // y[i] = x[i] W + s_a (x[i] A_a^T) B_a^T, a = adapter_of[i].
 //
-// Three steps: T = x A^T (w4a16_bank project, f32), the plain GEMM, and y += s T B^T in place.  Rows are handled in tiles of 16
+// Three steps: T = x A^T (f32), the plain GEMM, and y += s T B^T in place; up to 16 rows the first two share a launch where that is faster,
+// and a row or two on few adapters take one launch for everything (w4a16_bank_few.hip).  Rows are handled in tiles of 16
 // positions or 64; a tile multiplies with each adapter that is present among its rows, once, and rows of other adapters are left out
 // of the product, so any order of the rows is right and one in which an adapter's rows are together reads its matrices least often:
 // from 257 rows on a launch in front puts them so.  The reference serves one adapter set per process
@@ -265,17 +266,12 @@ void launch_project(const BankProjection &one, const BankProjection &two, const 
     else launch_project<4, RT, W>(one, two, r, rank, stream);
 }
 
-// Base product and low-rank term in one launch (bank_few), or the plain GEMM and the term behind it?  The one saves a launch and the
-// result's way through memory, the other's base product is the faster one on wide outputs.  1 / 8 / 16 rows of as many adapters, rank 16, us:
-// 2560 -> 2560 7.4 / 9.6 / 11.7 against 11.0 / 12.4 / 14.4, 4096 -> 4096 8.0 / 10.6 / 13.1 against 11.1 / 13.0 / 15.3, 2560 -> 8192 8.8 / 11.0 / 13.3
-// against 11.2 / 13.3 / 15.5, 8192 -> 8192 13.4 / 16.9 / 21.2 against 15.0 / 17.9 / 21.1; but 9216 -> 2560 10.5 / 15.0 / 19.3 against 13.3 / 15.7 / 18.2,
-// 14336 -> 4096 13.5 / 18.3 / 24.8 against 16.0 / 19.0 / 22.2, 2560 -> 18432 13.3 / 16.4 / 20.7 against 12.8 / 15.7 / 18.6, 5120 -> 27648 27.7 / 37.5 / 48.9
-// against 21.9 / 26.5 / 30.8.
-// ... and there, may every block project the rows by itself, out of up to 96 KB of their adapters?  One row of rank 16: 2560 -> 2560 6.3 us
-// against 7.4 and more with the launch in front, 2560 -> 8192 7.8 against 8.8, 1024 -> 4096 5.3 against 7.0 and two rows 5.5 against 6.9; but 4096 -> 2560
-// 7.6 against 7.3, two rows of 2560 -> 8192 10.1 against 9.3.
-bool projects_itself(int m, int k, int rank) { return m <= 2 && (int64_t)m * rank * k <= 48 * 1024; }
-bool takes_few(int m, int n, int k) { return m <= kBankFewRows && n <= 8192 && (m <= 8 || k <= 8192); }
+// Up to 16 rows: may the base product be the one with the projection beside it (bank_base)?  It saves a launch; the plain GEMM is the faster
+// product of many rows on the largest weights and of a long K.  1 / 8 / 16 rows of as many adapters, rank 16, us, against the plain GEMM
+// with the projection behind it: 2560 -> 10240 8.6 / 10.6 / 12.6 against 11.4 / 13.6 / 16.0, 2560 -> 18432 11.5 / 13.9 / 17.0 against 12.5 / 15.4 / 18.7,
+// 4096 -> 14336 10.3 / 12.1 / 14.6 against 14.0 / 16.0 / 18.9, 5120 -> 5120 8.7 / 11.1 / 13.8 against 12.3 / 15.5 / 17.3; but 4096 -> 24576 14.8 / 18.1 / 23.8
+// against 17.5 / 20.3 / 23.1, 5120 -> 27648 20.7 / 25.2 / 33.4 against 22.9 / 26.6 / 30.9, 9216 -> 2560 10.3 / 17.1 / 22.2 against 13.1 / 15.5 / 17.7.
+bool takes_base(int m, int n, int k) { return m <= kBankFewRows && (k <= 5120 ? m <= 8 || (int64_t)n * k <= 64 << 20 : m <= 4); }
 
 }  // namespace
 
@@ -362,21 +358,27 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     char *at = reinterpret_cast<char *>(scratch);
     BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
-    const int slices = bank_slices(prob_m, prob_k), rank = bank->rank;
-    if (takes_few(prob_m, prob_n, prob_k)) {
+    const int rank = bank->rank;
+    if (bank_projects_itself(prob_m, prob_n, prob_k, rank)) {
         rows.order = rows.first = nullptr;
-        const bool own = projects_itself(prob_m, prob_k, rank);
-        if (!own) bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
-        bank_few(A, B, s, C, *bank, rows, own ? nullptr : t, slices, prob_k, prob_n, groupsize == -1, hs);
+        bank_few(A, B, s, C, *bank, rows, prob_k, prob_n, groupsize == -1, hs);
         return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
     }
-    // the plain GEMM's checks and its launches first: nothing is launched for a call that it refuses
-    const kiln_marlin_status_t st =
-        kiln_marlin_w4a16_gemm(A, B, C, const_cast<void *>(s), prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, -1, -1, -1, 16);
-    if (st != KILN_W4A16_OK) return st;
-    if (prob_m < kBankOrderedFrom) rows.order = rows.first = nullptr;
-    else bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
-    bank_project(BankProjection{A, bank->lora_a, t, prob_k, slices}, nullptr, rows, rank, hs);
+    const bool base = takes_base(prob_m, prob_n, prob_k);
+    const int slices = base ? bank_base_slices(prob_k) : bank_slices(prob_m, prob_k);
+    const BankProjection of_x{A, bank->lora_a, t, prob_k, slices};
+    if (base) {
+        rows.order = rows.first = nullptr;
+        bank_base(A, B, s, C, of_x, rows, rank, prob_k, prob_n, groupsize == -1, hs);
+    } else {
+        // the plain GEMM's checks and its launches first: nothing is launched for a call that it refuses
+        const kiln_marlin_status_t st =
+            kiln_marlin_w4a16_gemm(A, B, C, const_cast<void *>(s), prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, -1, -1, -1, 16);
+        if (st != KILN_W4A16_OK) return st;
+        if (prob_m < kBankOrderedFrom) rows.order = rows.first = nullptr;
+        else bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
+        bank_project(of_x, nullptr, rows, rank, hs);
+    }
     uint16_t *y = (uint16_t *)C;
     const uint16_t *m = (const uint16_t *)bank->lora_b;
     if (rank <= 32) launch_expand<1>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);

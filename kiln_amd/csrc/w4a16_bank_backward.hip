@@ -13,6 +13,7 @@
 #include "bank.h"
 #include "bank_expand.h"
 #include "bank_order.h"
+#include "bank_project.h"
 #include "device_common.h"
 
 namespace kiln {
@@ -176,82 +177,42 @@ __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, FewLds &
             *reinterpret_cast<const f32x4 *>(lds.sums + (e >> 5) * kFewPitch + 4 * (e & 31));
 }
 
-// Up to 64 rows: T = x A^T or U = dy B of 16 rows and one slice of the contraction, for the adapters met among them whose turn is `turn0`
-// modulo p.turns.  A's rows are contiguous along the contraction; of B, [n, rank], a lane reads eight of the rank for each of its eight n
-// and pairs the n's values (v_perm), one product for each of the eight, as bank_grad_kernel does for its rows.
-__device__ __forceinline__ void few_project(const PrepareArgs &p, bool of_x, int slice, int tile, unsigned turn0, FewLds &lds) {
+// Up to 64 rows: U = dy B of 16 rows and one slice of the columns (T: project_rows).  A lane reads eight of B's rank, [n, rank], for each of
+// its eight n and pairs the n's values (v_perm), one product for each of the eight, as bank_grad_kernel does for its rows.
+__device__ __forceinline__ void few_project_dy(const PrepareArgs &p, int slice, int tile, unsigned turn0, FewLds &lds) {
     constexpr int W = kPrepareThreads / 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, q = lane >> 4, p0 = 16 * tile, rank = p.rank;
-    const int len = of_x ? p.K : p.N, slices = of_x ? p.t_slices : p.u_slices;
-    const int each = (len / 128 + slices - 1) / slices * 128, begin = slice * each + 32 * wave, end = min(len, (slice + 1) * each);
-    int a = p0 + c < p.m ? p.rows.of[p0 + c] : -1;
-    if ((unsigned)a >= (unsigned)p.rows.count) a = -1;
-    unsigned left = (unsigned)__ballot(a >= 0) & 0xFFFFu;
-    const uint16_t *src = (of_x ? p.x : p.dy) + (size_t)min(p0 + c, p.m - 1) * len + 8 * q;
-    for (unsigned turn = 0; left; ++turn) {
-        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
-        const unsigned mine = (unsigned)__ballot(a == cur) & 0xFFFFu;
-        left &= ~mine;
-        if (turn % p.turns != turn0) continue;
-        if (of_x) {
-            for (int j0 = 0; j0 < rank; j0 += 16) {  // rows past the rank: the last one again, their sums are dropped
-                const uint16_t *mat = p.a + ((size_t)cur * rank + min(j0 + c, rank - 1)) * len + 8 * q;
-                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-                for (int at = begin; at < end; at += 4 * 32 * W) {
-                    bf16x8 x[4], m[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4, p0 = 16 * tile, rank = p.rank;
+    const int each = (p.N / 128 + p.u_slices - 1) / p.u_slices * 128, begin = slice * each + 32 * wave, end = min(p.N, (slice + 1) * each);
+    const uint16_t *src = p.dy + (size_t)min(p0 + c, p.m - 1) * p.N + 8 * q;
+    adapters_of_turn(p.rows, p0, c, turn0, p.turns, [&](int adapter, unsigned mine) {
+        const uint16_t *mat = p.b + ((size_t)adapter * p.N + 8 * q) * rank + 8 * min(c, rank / 8 - 1);
+        f32x4 acc[8];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        x[u] = load_bf16x8(src + min(at + 32 * W * u, len - 32));
-                        m[u] = load_bf16x8(mat + min(at + 32 * W * u, len - 32));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int at = begin; at < end; at += 2 * 32 * W) {
+            bf16x8 x[2];
+            u32x4 v[2][8];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (at + 32 * W * u < end) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], m[u], acc, 0, 0, 0);
-                }
+            for (int u = 0; u < 2; ++u) {
+                const int n = min(at + 32 * W * u, p.N - 32);
+                x[u] = load_bf16x8(src + n);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds.projected[wave][4 * q + i][j0 + c] = acc[i];
+                for (int i = 0; i < 8; ++i) v[u][i] = *reinterpret_cast<const u32x4 *>(mat + (size_t)(n + i) * rank);
             }
-        } else {
-            const int r8 = 8 * min(c, rank / 8 - 1);
-            const uint16_t *mat = p.b + ((size_t)cur * len + 8 * q) * rank + r8;
-            f32x4 acc[8];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int at = begin; at < end; at += 2 * 32 * W) {
-                bf16x8 x[2];
-                u32x4 v[2][8];
+            for (int u = 0; u < 2; ++u)
+                if (at + 32 * W * u < end)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int n = min(at + 32 * W * u, len - 32);
-                    x[u] = load_bf16x8(src + n);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[u][i] = *reinterpret_cast<const u32x4 *>(mat + (size_t)(n + i) * rank);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (at + 32 * W * u < end)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], column_of_rows(v[u], e), acc[e], 0, 0, 0);
-            }
-            if (c < rank / 8)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) lds.projected[wave][4 * q + i][8 * c + e] = acc[e][i];
+                    for (int e = 0; e < 8; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[u], column_of_rows(v[u], e), acc[e], 0, 0, 0);
         }
-        __syncthreads();
-        float *out = (of_x ? p.t : p.u) + ((size_t)slice * p.m + p0) * rank;
-        for (int e = tid; e < 16 * rank; e += kPrepareThreads) {
-            const int r = e / rank, j = e - r * rank;
-            float v = 0.f;
+        if (c < rank / 8)
 #pragma unroll
-            for (int w = 0; w < W; ++w) v += lds.projected[w][r][j];
-            if (mine >> r & 1) out[e] = v;
-        }
-        __syncthreads();
-    }
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lds.projected[wave][4 * q + i][8 * c + e] = acc[e][i];
+        join_projected<W>(lds.projected, p.u, p.rows, p0, slice, rank, mine);
+    });
 }
 
 // at[a][k][rank] of a[a][rank][k], or bt[a][rank][n] of b[a][n][rank]; 64 of k or n to a block.  `at` is multiplied with rows of several
@@ -294,8 +255,9 @@ __global__ __launch_bounds__(kPrepareThreads, 4) void bank_prepare_kernel(Prepar
         }
         block -= p.slices * (p.K / kGroupK);
         const int all = p.t_slices + p.u_slices, place = block % all, rest = block / all;
-        const bool of_x = place >= p.u_slices;
-        few_project(p, of_x, of_x ? place - p.u_slices : place, rest / p.turns, rest % p.turns, lds);
+        const int tile = rest / p.turns, turn0 = rest % p.turns;
+        if (place < p.u_slices) few_project_dy(p, place, tile, turn0, lds);
+        else project_rows<kPrepareThreads / 64>(BankProjection{p.x, p.a, p.t, p.K, p.t_slices}, p.rows, p.rank, place - p.u_slices, tile, turn0, p.turns, lds.projected);
     } else {
         if (block < p.order_blocks) {
             order_rows(p.rows.of, p.rows.order, p.rows.first, p.rows.rows, p.rows.count, block, lds.order);

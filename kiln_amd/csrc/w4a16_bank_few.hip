@@ -1,13 +1,14 @@
-// A packed projection of up to 16 rows with low-rank adapters of their own, base product and low-rank term in one launch behind the
-// projection of the rows onto their adapters (w4a16_bank.hip): the term lands on the f32 sums, and the result is rounded once.
+// A packed projection of up to 16 rows with low-rank adapters of their own (w4a16_bank.hip): base product, projection and low-rank term of a
+// row or two in one launch, or base product and projection in one and the term behind it.
 #include "bank.h"
 #include "bank_expand.h"
+#include "bank_project.h"
 #include "few_rows.h"
 
 namespace kiln {
 namespace {
 
-constexpr int kOwnRows = 2;
+constexpr int kOwnRows = 2, kUnits = 256;
 struct FewArgs {
     const uint16_t *x;
     const u32x4 *b;
@@ -15,10 +16,9 @@ struct FewArgs {
     uint16_t *y;
     const uint16_t *mat;   // [count, N, rank]
     const uint16_t *mat_a;  // [count, rank, K]
-    const float *t;        // [slices, rows, rank], or null: the blocks project the rows by themselves
     const float *scales;
     BankRows rows;
-    int K, N, rank, slices, per_column;
+    int K, N, rank, per_column;
 };
 
 // One row or two onto their adapters, over the groups that a wavefront has of them: t[row][rank] += x A^T.  The loops are left as they are,
@@ -52,20 +52,18 @@ __device__ __forceinline__ void project_own(const FewArgs &p, const bf16x8 (&x)[
     }
 }
 
-// S column tiles to a block of W wavefronts, which meet in LDS after the base product.  The adapters met among the rows are dealt out
-// to the wavefronts; each finishes and stores the rows of its own (those without an adapter are the first one's).  What that needs of
-// memory is touched while the first weights are on their way -- a lane a line or a few of its row's adapter -- and comes out of a cache.
-// OWN: one row or two, and every block projects them onto their adapters by itself, out of the part of the rows that its wavefronts hold:
-// the adapters' A read by every block is less than the launch in front that it saves.
-template <int W, int GW, int S, int SR, bool OWN>
+// One launch for a row or two.  S column tiles to a block of W wavefronts, which meet in LDS after the base product; every block projects the
+// rows onto their adapters by itself, out of the part of the rows that its wavefronts hold: the adapters' A read by every block is less
+// than a launch that it saves.  The first wavefront finishes and stores the rows of the first one's adapter (or of none), the second the other's, on
+// the f32 sums.  What that needs of memory is touched while the first weights are on their way -- a lane a line or a few of its row's
+// adapter -- and comes out of a cache.
+template <int W, int GW, int S, int SR>
 __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
-    constexpr int kMost = 16 / W, kPitch = S * 16 + 4;
+    constexpr int kPitch = S * 16 + 4;
     __shared__ __align__(16) float part[W][16][kPitch];
-    __shared__ __align__(16) float ts[16][kBankMaxRank + 4];
-    __shared__ float parts_of_t[OWN ? W : 1][kOwnRows][32 * SR];
-    if constexpr (OWN) {  // (this wavefront's own, until the block meets)
-        for (int e = threadIdx.x & 63; e < kOwnRows * 32 * SR; e += 64) (&parts_of_t[threadIdx.x >> 6][0][0])[e] = 0.f;
-    }
+    __shared__ __align__(16) float ts[kOwnRows][32 * SR];
+    __shared__ float parts_of_t[W][kOwnRows][32 * SR];
+    for (int e = threadIdx.x & 63; e < kOwnRows * 32 * SR; e += 64) (&parts_of_t[threadIdx.x >> 6][0][0])[e] = 0.f;  // (this wavefront's own, until the block meets)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
     const DequantConsts dc = dequant_consts();
     const int nt0 = blockIdx.x * S, G = p.K / kGroupK, Gs = p.per_column ? 1 : G, n0 = nt0 * kTileN;
@@ -83,52 +81,35 @@ __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
                                    for (int i = 0; i < kLines; ++i)
                                        touched[i] = mat[at * p.N * p.rank + min((4 * (W * i + wave) + q) * 64, S * 16 * p.rank - 1)];
                                },
-                               [&](const bf16x8(&x)[GW][4], int first) {
-                                   if constexpr (OWN) project_own<W, GW, SR>(p, x, first, G, a, lane, parts_of_t[wave]);
-                               });
+                               [&](const bf16x8(&x)[GW][4], int first) { project_own<W, GW, SR>(p, x, first, G, a, lane, parts_of_t[wave]); });
 #pragma unroll
     for (int i = 0; i < kLines; ++i) asm volatile("" : : "v"(touched[i]));
     if (c >= p.rows.rows || (unsigned)a >= (unsigned)p.rows.count) a = -1;
-    unsigned left = (unsigned)__ballot(a >= 0) & 0xFFFFu;
-    int mine[kMost], count = 0;
-    bool live = c < p.rows.rows && a < 0 && wave == 0;
-    for (int turn = 0; left; ++turn) {
-        const int cur = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
-        left &= ~((unsigned)__ballot(a == cur) & 0xFFFFu);
-        if (turn % W != wave) continue;
-#pragma unroll
-        for (int i = 0; i < kMost; ++i)
-            if (i == count) mine[i] = cur;
-        ++count;
-        live |= a == cur;
-    }
+    const int mine = __builtin_amdgcn_readlane(a, wave & 1);
+    const bool other = wave == 1 && mine == __builtin_amdgcn_readlane(a, 0);  // the first wavefront's
+    const bool live = wave < kOwnRows && c < p.rows.rows && !other && (a == mine || (wave == 0 && a < 0));
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) part[wave][4 * q + r][16 * i + c] = total[i][r];
-    auto rows_of_b = [&](int adapter, bf16x8 (&b)[S][SR]) {
+    bf16x8 b[S][SR];
+    if (wave < kOwnRows && mine >= 0)
 #pragma unroll
         for (int tile = 0; tile < S; ++tile)
 #pragma unroll
             for (int s = 0; s < SR; ++s)
-                b[tile][s] = load_bf16x8(mat + (size_t)adapter * p.N * p.rank + (size_t)(16 * tile + c) * p.rank + min(32 * s + 8 * q, p.rank - 8));
-    };
-    bf16x8 b[2][S][SR];
-    if (count > 0) rows_of_b(mine[0], b[0]);
-    if constexpr (OWN) {
-        __syncthreads();
-        for (int e = tid; e < kOwnRows * 32 * SR; e += W * 64) {
-            float v = 0.f;
+                b[tile][s] = load_bf16x8(mat + (size_t)mine * p.N * p.rank + (size_t)(16 * tile + c) * p.rank + min(32 * s + 8 * q, p.rank - 8));
+    __syncthreads();
+    for (int e = tid; e < kOwnRows * 32 * SR; e += W * 64) {
+        float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) v += parts_of_t[w][e / (32 * SR)][e % (32 * SR)];
-            ts[e / (32 * SR)][e % (32 * SR)] = v;
-        }
-        __syncthreads();
-    } else {
-        sum_projected<16>(p.t, p.rows, 0, p.rank, p.slices, tid, W * 64, ts);
+        for (int w = 0; w < W; ++w) v += parts_of_t[w][e / (32 * SR)][e % (32 * SR)];
+        ts[e / (32 * SR)][e % (32 * SR)] = v;
     }
+    __syncthreads();
+    if (wave >= kOwnRows) return;
     ExpandRow<SR> tv;
-    tv.set(ts[c], scale, live && a >= 0, q, p.rank);
+    tv.set(ts[min(c, kOwnRows - 1)], scale, live && a >= 0, q, p.rank);
     f32x4 acc[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -136,12 +117,7 @@ __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
 #pragma unroll
         for (int w = 1; w < W; ++w) acc[i] += *reinterpret_cast<const f32x4 *>(&part[w][c][16 * i + 4 * q]);
     }
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-        if (i >= count) break;
-        if (i + 1 < kMost && i + 1 < count) rows_of_b(mine[i + 1], b[(i + 1) & 1]);
-        expand_product<SR, S>(b[i & 1], tv, a == mine[i], acc);
-    }
+    if (mine >= 0) expand_product<SR, S>(b, tv, a == mine, acc);
     if (!live) return;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -152,29 +128,89 @@ __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
     }
 }
 
+// The base product of up to 16 rows, and beside it in the same launch the rows' projections, which the launch behind it (w4a16_bank.hip)
+// multiplies: the first `projecting` blocks, a slice of the contraction and a turn of the adapters each.  Tiles to a block: as many as leave
+// 128 blocks, the rows are read once for all (2560 -> 18432, 16 rows: 4 17.0 us a call, 2 18.0, 1 21.6; 4096 -> 4096: 2 12.7, 4 13.5).
+template <int W, int GW, int S>
+__global__ __launch_bounds__(W * 64) void bank_base_kernel(FewArgs p, BankProjection of_x, int projecting, int turns) {
+    constexpr int kPitch = S * 16 + 4;
+    union Lds {
+        float projected[W][16][kBankMaxRank + 4];
+        float part[W][16][kPitch];
+    };
+    __shared__ __align__(16) Lds lds;
+    if ((int)blockIdx.x < projecting) {
+        project_rows<W>(of_x, p.rows, p.rank, blockIdx.x / turns, 0, blockIdx.x % turns, turns, lds.projected);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
+    const DequantConsts dc = dequant_consts();
+    const int nt0 = (blockIdx.x - projecting) * S, G = p.K / kGroupK, Gs = p.per_column ? 1 : G;
+    f32x4 total[S];
+    few_rows_product<GW, S>(p.x + (size_t)min(c, p.rows.rows - 1) * p.K + 8 * q, p.b + (size_t)nt0 * G * 64 + lane, p.s + (size_t)nt0 * Gs * kTileN + c, G,
+                            p.per_column, wave, W, dc, total);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds.part[wave][4 * q + r][16 * i + c] = total[i][r];
+    __syncthreads();
+    for (int e = tid; e < p.rows.rows * S * 8; e += W * 64) {
+        const int r = e / (S * 8), col = e % (S * 8) * 2;
+        float lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            lo += lds.part[w][r][col];
+            hi += lds.part[w][r][col + 1];
+        }
+        *reinterpret_cast<uint32_t *>(p.y + (size_t)r * p.N + nt0 * kTileN + col) = f32_to_bf16_bits(lo) | (uint32_t)f32_to_bf16_bits(hi) << 16;
+    }
+}
+
 template <int W, int GW, int S>
 void launch_few(const FewArgs &a, hipStream_t stream) {
     const int blocks = a.N / (16 * S);
-    if (!a.t) {
-        if (a.rank <= 32) bank_few_kernel<W, GW, S, 1, true><<<blocks, W * 64, 0, stream>>>(a);
-        else bank_few_kernel<W, GW, S, 2, true><<<blocks, W * 64, 0, stream>>>(a);
-    } else {
-        if (a.rank <= 32) bank_few_kernel<W, GW, S, 1, false><<<blocks, W * 64, 0, stream>>>(a);
-        else bank_few_kernel<W, GW, S, 2, false><<<blocks, W * 64, 0, stream>>>(a);
-    }
+    if (a.rank <= 32) bank_few_kernel<W, GW, S, 1><<<blocks, W * 64, 0, stream>>>(a);
+    else bank_few_kernel<W, GW, S, 2><<<blocks, W * 64, 0, stream>>>(a);
+}
+// Blocks of the projection are an adapter each; where those would be one round too many, up to four adapters each.
+template <int W, int GW, int S>
+void launch_base(const FewArgs &a, const BankProjection &of_x, hipStream_t stream) {
+    const int blocks = a.N / (16 * S), room = kUnits * (W == 4 ? 2 : 1) - blocks, met = a.rows.count < a.rows.rows ? a.rows.count : a.rows.rows;
+    int turns = met;
+    if (room > 0 && of_x.slices * turns > room) turns = room / of_x.slices > (met + 3) / 4 ? room / of_x.slices : (met + 3) / 4;
+    bank_base_kernel<W, GW, S><<<of_x.slices * turns + blocks, W * 64, 0, stream>>>(a, of_x, of_x.slices * turns, turns);
 }
 
 }  // namespace
 
-void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, const float *t, int slices,
-              int K, int N, bool per_column, hipStream_t stream) {
-    const FewArgs a{(const uint16_t *)x, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, (const uint16_t *)bank.lora_b, (const uint16_t *)bank.lora_a, t, bank.scales,
-                    rows, K, N, bank.rank, slices, per_column};
-    // two tiles to a block where that leaves a block to every compute unit
+// One row of rank 16, us, against two launches: 2560 -> 2560 6.0 to 7.1, 2560 -> 8192 7.6 to 8.5, 1024 -> 4096 4.6 to 7.0 (two rows 5.1); but 4096 -> 2560
+// 7.6 to 7.1, two rows of 2560 -> 8192 10.1 to 8.6.
+bool bank_projects_itself(int m, int n, int k, int rank) { return m <= kOwnRows && n <= 8192 && (int64_t)m * rank * k <= 48 * 1024; }
+
+int bank_base_slices(int K) {  // one turn of a block's wavefronts each
+    const int groups = K / kGroupK, each = groups <= 20 ? 4 : 8, slices = (groups + each - 1) / each;
+    return slices < kBankMaxSlices ? slices : kBankMaxSlices;
+}
+
+void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column,
+               hipStream_t stream) {
+    const FewArgs a{(const uint16_t *)x, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, nullptr, nullptr, nullptr, rows, K, N, rank, per_column};
     with_few_rows_split(K / kGroupK, [&](auto waves, auto groups) {
         constexpr int W = decltype(waves)::value, GW = decltype(groups)::value;
         const int tiles = N / kTileN;
-        if (tiles >= 512) launch_few<W, GW, 2>(a, stream);
+        if (tiles >= 512) launch_base<W, GW, 4>(a, of_x, stream);
+        else if (tiles >= 256) launch_base<W, GW, 2>(a, of_x, stream);
+        else launch_base<W, GW, 1>(a, of_x, stream);
+    });
+}
+
+void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, int K, int N, bool per_column,
+              hipStream_t stream) {
+    const FewArgs a{(const uint16_t *)x, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, (const uint16_t *)bank.lora_b, (const uint16_t *)bank.lora_a,
+                    bank.scales, rows, K, N, bank.rank, per_column};
+    with_few_rows_split(K / kGroupK, [&](auto waves, auto groups) {
+        constexpr int W = decltype(waves)::value, GW = decltype(groups)::value;
+        if (N / kTileN >= 512) launch_few<W, GW, 2>(a, stream);
         else launch_few<W, GW, 1>(a, stream);
     });
 }

@@ -4,8 +4,8 @@ against the formulas in 64 bits.
 Tolerances.  U = 2^-8 is the most that a rounding to bf16 changes a value by, relative to it; F = 2^-24 the same for f32.  A sum of n
 products in f32 is off by at most n F times the sum of the products' magnitudes, whatever its order.
 * forward: the base product in f32, where the kernels multiply 128 + code and take the rest off: (k + 8) F times the sum of |x| * 280 * scale
-  (144 at most + 136); from 17 rows on it is rounded before the low-rank term is added (U of it), which is then rounded (U |y|) in
-  every case.  For the term, the projection's f32 sum (k F), its two bf16 parts (2^-16: the second part is rounded by U of a part that
+  (144 at most + 136); it may be rounded before the low-rank term is added (U of it: two steps of rounding instead of one), and the sum is
+  rounded (U |y|) in every case.  For the term, the projection's f32 sum (k F), its two bf16 parts (2^-16: the second part is rounded by U of a part that
   is U of the value) and the second sum (2 rank F + a few), relative to the sum of magnitudes.
 * dx: a weight is rounded to bf16 (U), so U times the sum of |dy| |W|, plus f32 sums (n F) and the low-rank term as above; U |dx| at the end.
 * dA, dB: the inner product in f32 (K F), the sum over rows (rows F), U of the result.
@@ -67,7 +67,7 @@ def check_forward(p, y, base=None):
     tiled = p["s"].reshape(-1, p["s"].shape[0], 16).transpose(0, 1).reshape(p["s"].shape)
     scale = tiled.double().repeat_interleave(k // tiled.shape[0], 0)
     want = p["x"].double() @ w
-    bound = (p["x"].double().abs() @ scale) * 280 * (k + 8) * F + (U * want.abs() if m > 16 else 0.0)
+    bound = (p["x"].double().abs() @ scale) * 280 * (k + 8) * F + U * want.abs()
     for j in range(len(p["sc"])):
         mine, s, a, b = p["of"] == j, p["sc"][j].double(), p["a_"][j].double(), p["b_"][j].double()
         x = p["x"][mine].double()
