@@ -43,7 +43,15 @@ struct BankProjection {
     float *t;
     int K, slices;
 };
-void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream);
+// Rows put in order beside a projection, for gemm_with_bank: x[row, K] to ordered[position, K], sums[K / 128][position] and adapters[position] (-1: none)
+struct BankGather {
+    const uint16_t *x;
+    uint16_t *ordered;
+    float *sums;
+    int *adapters;
+    int K, blocks;
+};
+void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream, BankGather gather = {});
 
 // up to 16 rows as they stand: y = x W, and their projection (bank_base_slices of it) in the same launch
 constexpr int kBankFewRows = 16;
@@ -54,5 +62,12 @@ void bank_base(const void *x, const void *b, const void *s, void *y, const BankP
 bool bank_projects_itself(int m, int n, int k, int rank);
 void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w4a16_adapter_bank &bank, const BankRows &rows, int K, int N, bool per_column,
               hipStream_t stream);
+
+// many rows: the plain GEMM with a bank's term in it (launch.h), for the sizes where it can
+struct PrefillBank;
+bool bank_in_product(int m, int n, int k, int dev);
+// A: rows in the order of their adapters; row_sums: -136 times their sums, f32 [K/128][m]
+kiln_marlin_status_t gemm_with_bank(const void *A, const void *B, void *C, const void *s, int m, int n, int k, void *workspace, int groupsize, int dev,
+                                    void *stream, float *row_sums, const PrefillBank &bank);
 
 }  // namespace kiln

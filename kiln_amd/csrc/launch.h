@@ -214,6 +214,13 @@ hipError_t launch_mid_own2(const MidArgs &a, hipStream_t stream);
 hipError_t launch_mid_sides(const MidArgs &a, hipStream_t stream);  // ... of unstacked adapters
 
 // One launch of the prefill path (row-sum pre-pass + MFMA kernel), any M >= 1.
+// A bank of adapters for rows that lie in their adapters' order (bank.h): C[order[p]] = A[p] W + T[p] lora_b[a]^T, a the adapter of position p
+struct PrefillBank {
+    const uint16_t *b;              // bf16 [count, N, rank]
+    const uint16_t *t;              // scales[a] T in two bf16 parts by position: [M][rank / 8][2][8]
+    const int *order, *adapters;    // by position: the row, and its adapter (-1: none, at the end)
+    int rank;
+};
 struct PrefillArgs {
     const void *A;   // bf16 [M, K]
     const void *B;   // packed weights, tile layout
@@ -245,6 +252,7 @@ struct PrefillArgs {
     void *next_aext = nullptr;      // swiglu, prefill_forms_next_sums(): prefill_aext_bytes(M, N / 2) bytes, the row sums
                                     // of C for a GEMM over it
     bool next_plain = false;        // ... in the form that GEMM takes: its sums_in_loop
+    const PrefillBank *bank = nullptr;  // sums_in_loop and aext_ready, 128 x 256 blocks whose wavefronts do not share K
 };
 
 size_t prefill_aext_bytes(int m, int k);

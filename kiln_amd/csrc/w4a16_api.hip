@@ -9,6 +9,7 @@
 #include "kiln_w4a16.h"
 #include "async_loads.h"
 #include "device_common.h"
+#include "bank.h"
 #include "launch.h"
 
 namespace kiln {
@@ -1162,7 +1163,7 @@ bool first_blocks_take_sides(int m, int n, int k, int cus) {
 kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void *s, int prob_m, int prob_n,
                               int prob_k, void *workspace, int groupsize, int dev, void *stream, int thread_k,
                               int thread_n, int sms, const LoraSpec *lora, bool swiglu = false,
-                              const MlpSums &sums = MlpSums{}) {
+                              const MlpSums &sums = MlpSums{}, const PrefillBank *bank = nullptr) {
     if (prob_m < 0 || prob_n < 0 || prob_k < 0) return KILN_W4A16_ERR_PROB_SHAPE;
     if (!shape_ok(prob_n, prob_k, groupsize)) return KILN_W4A16_ERR_PROB_SHAPE;
     if (thread_k > 0 && thread_k % 128 != 0) return KILN_W4A16_ERR_PROB_SHAPE;
@@ -1213,6 +1214,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
             pa.aext = sums.read;
             pa.aext_ready = true;
         }
+        pa.bank = bank;
         pa.cus = cus;
         pa.KS = gp.pf.ks;
         pa.bn = gp.pf.bn;
@@ -1223,6 +1225,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
         return launch_prefill(pa, st) == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
     }
 
+    if (bank) return KILN_W4A16_ERR_KERN_SHAPE;
     if (gp.mid) {
         MidArgs ma = mid_args(gp.mp, prob_m, prob_n, prob_k);
         ma.A = A;
@@ -1355,6 +1358,19 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
 }
 
 }  // namespace
+
+// Can the product of so many rows add a bank's term itself (PrefillBank)?  It takes the row sums as f32 then, and 128 x 256 blocks.
+bool bank_in_product(int m, int n, int k, int dev) {
+    const int cus = compute_units(dev);
+    const auto plan = plan_call(m, n, k, cus, -1, -1, 0);
+    return plan->gp.prefill && plan->gp.sums_in_loop && plan->gp.pf.bn == 256 && plan->gp.pf.bm == 128 && !prefill_halves_k(m, n, k, plan->gp.pf, cus);
+}
+kiln_marlin_status_t gemm_with_bank(const void *A, const void *B, void *C, const void *s, int m, int n, int k, void *workspace, int groupsize, int dev,
+                                    void *stream, float *row_sums, const PrefillBank &bank) {
+    MlpSums sums;
+    sums.read = row_sums;
+    return gemm_any(A, B, C, s, m, n, k, workspace, groupsize, dev, stream, -1, -1, -1, nullptr, false, sums, &bank);
+}
 }  // namespace kiln
 
 extern "C" {

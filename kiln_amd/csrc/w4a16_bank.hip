@@ -2,7 +2,8 @@
 // y[i] = x[i] W + s_a (x[i] A_a^T) B_a^T, a = adapter_of[i].
 //
 // Three steps: T = x A^T (f32), the plain GEMM, and y += s T B^T in place; up to 16 rows the first two share a launch where that is faster,
-// and a row or two on few adapters take one launch for everything (w4a16_bank_few.hip).  Rows are handled in tiles of 16
+// and a row or two on few adapters take one launch for everything (w4a16_bank_few.hip).  Thousands of rows on wide outputs: rows are put in
+// the order of their adapters and the product adds the term where it stores a tile (w4a16_prefill.hip).  Rows are handled in tiles of 16
 // positions or 64; a tile multiplies with each adapter that is present among its rows, once, and rows of other adapters are left out
 // of the product, so any order of the rows is right and one in which an adapter's rows are together reads its matrices least often:
 // from 257 rows on a launch in front puts them so.  The reference serves one adapter set per process
@@ -11,6 +12,8 @@
 #include "bank_expand.h"
 #include "bank_order.h"
 #include "device_common.h"
+#include "launch.h"
+#include "lora_project.h"
 
 namespace kiln {
 namespace {
@@ -20,6 +23,69 @@ __global__ __launch_bounds__(kOrderWaves * 64) void bank_order_kernel(const int 
                                                                       int rows, int count) {
     __shared__ OrderLds<kOrderWaves> lds;
     order_rows(of, order, first, rows, count, blockIdx.x, lds);
+}
+
+// Rows put in order for the product, and their sums over a group times the codes' bias, in the order of additions that the plain GEMM has:
+// 16 lanes to a group, a position to a wavefront, 20 of its groups in flight together.
+constexpr int kGatherRows = 8;
+__device__ __forceinline__ void gather_rows(const BankGather &p, const BankRows &rows, int block, int waves) {
+    constexpr int U = 5;
+    const int G = p.K / kGroupK, lane = threadIdx.x & 63, sub = lane & 15, end = min(rows.rows, (block + 1) * kGatherRows);
+    for (int at = block * kGatherRows + (int)(threadIdx.x >> 6); at < end; at += waves) {
+        const int row = rows.order[at], a = rows.of[row];
+        if (lane == 0) p.adapters[at] = (unsigned)a < (unsigned)rows.count ? a : -1;
+        for (int g0 = lane >> 4; g0 < G; g0 += 4 * U) {
+            u32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u32x4 *>(p.x + (size_t)row * p.K + (size_t)min(g0 + 4 * u, G - 1) * kGroupK + sub * 8);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int g = g0 + 4 * u;
+                float sum = sum_bf16x8(v[u]);
+#pragma unroll
+                for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 16);
+                if (g >= G) break;
+                *reinterpret_cast<u32x4 *>(p.ordered + (size_t)at * p.K + (size_t)g * kGroupK + sub * 8) = v[u];
+                if (sub == 0) store_row_sum(reinterpret_cast<u32x4 *>(p.sums), (size_t)g * rows.rows + at, sum, true);
+            }
+        }
+    }
+}
+
+// s_a T, its slices summed, as the product takes it: eight of the rank to a thread, two bf16 parts in place of the first slice's f32.
+__global__ __launch_bounds__(64) void bank_split_kernel(float *__restrict__ t, const float *__restrict__ scales, const int *__restrict__ adapters, int rows, int rank,
+                                                        int slices) {
+    const size_t unit = (size_t)blockIdx.x * 64 + threadIdx.x, stride = (size_t)rows * rank;
+    const int per_row = rank / 8;
+    if (unit >= (size_t)rows * per_row) return;
+    const int a = adapters[unit / per_row];
+    float *at = t + unit * 8;
+    f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    for (int s = 0; s < slices; s += 2) {
+        f32x4 d[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) d[u][i] = *reinterpret_cast<const f32x4 *>(at + min(s + u, slices - 1) * stride + 4 * i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (s + u < slices)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) v[i] += d[u][i];
+    }
+    if (a < 0) return;
+    const float scale = scales[a];
+    bf16x8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = v[i >> 2][i & 3] * scale;
+        hi[i] = (__bf16)f;
+        lo[i] = lower_part(f, hi[i]);
+    }
+    reinterpret_cast<bf16x8 *>(at)[0] = hi;
+    reinterpret_cast<bf16x8 *>(at)[1] = lo;
 }
 
 // U pieces of a projection's contraction, 64 long each and 256 apart, all their loads in front of their products.  A lane's part of a
@@ -53,9 +119,13 @@ __device__ __forceinline__ void project_pieces(const uint16_t *const (&x)[RT], c
 // that with eight of them a die's blocks share one, whose part of the adapters' matrices its L2 then holds.  Two projections of the same
 // rows share a launch: the second one's slices are behind the first one's.
 template <int JT, int RT, int W>
-__global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one, BankProjection two, BankRows rows, int rank) {
+__global__ __launch_bounds__(W * 64) void bank_project_kernel(BankProjection one, BankProjection two, BankRows rows, int rank, BankGather gather) {
     constexpr int P = 16 * RT, kAhead = JT + RT <= 4 ? 4 : 2;
     const int all = one.slices + two.slices, place = blockIdx.x % all, tile = blockIdx.x / all;
+    if (tile * P >= rows.rows) {  // behind the projection's blocks
+        if (blockIdx.y == 0) gather_rows(gather, rows, blockIdx.x - (rows.rows + P - 1) / P * all, W);
+        return;
+    }
     const bool second = place >= one.slices;
     const uint16_t *__restrict__ src = (const uint16_t *)(second ? two.src : one.src), *__restrict__ mat = (const uint16_t *)(second ? two.mat : one.mat);
     float *__restrict__ t = second ? two.t : one.t;
@@ -249,21 +319,21 @@ constexpr int kLongContraction = 8192;
 bool long_ordered(int rows, int K) { return rows >= kBankOrderedFrom && K >= kLongContraction; }
 
 template <int JT, int RT, int W>
-void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream) {
+void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream, const BankGather &gather) {
     const int tiles = tiles_of(r.rows, 16 * RT);
     // the adapters that a tile may hold side by side: as many as it has rows, but where they are together few tiles have more than one
     int turns = r.order ? 1 + r.count / tiles : 16;
     if (turns > 16) turns = 16;
     if (turns > r.count) turns = r.count;
-    bank_project_kernel<JT, RT, W><<<dim3((one.slices + two.slices) * tiles, turns), W * 64, 0, stream>>>(one, two, r, rank);
+    bank_project_kernel<JT, RT, W><<<dim3((one.slices + two.slices) * tiles + gather.blocks, turns), W * 64, 0, stream>>>(one, two, r, rank, gather);
 }
 template <int RT, int W>
-void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream) {
+void launch_project(const BankProjection &one, const BankProjection &two, const BankRows &r, int rank, hipStream_t stream, const BankGather &gather) {
     const int jt = (rank + 15) / 16;
-    if (jt == 1) launch_project<1, RT, W>(one, two, r, rank, stream);
-    else if (jt == 2) launch_project<2, RT, W>(one, two, r, rank, stream);
-    else if (jt == 3) launch_project<3, RT, W>(one, two, r, rank, stream);
-    else launch_project<4, RT, W>(one, two, r, rank, stream);
+    if (jt == 1) launch_project<1, RT, W>(one, two, r, rank, stream, gather);
+    else if (jt == 2) launch_project<2, RT, W>(one, two, r, rank, stream, gather);
+    else if (jt == 3) launch_project<3, RT, W>(one, two, r, rank, stream, gather);
+    else launch_project<4, RT, W>(one, two, r, rank, stream, gather);
 }
 
 // Up to 16 rows: may the base product be the one with the projection beside it (bank_base)?  It saves a launch; the plain GEMM is the faster
@@ -278,6 +348,8 @@ bool takes_base(int m, int n, int k) { return m <= kBankFewRows && (k <= 5120 ? 
 bool bank_ok(const kiln_w4a16_adapter_bank &bank) {
     return bank.count >= 1 && bank.count <= 4096 && bank.rank >= 8 && bank.rank <= kBankMaxRank && bank.rank % 8 == 0;
 }
+
+static size_t bank_ordered_x_bytes(int rows, int K) { return bank_up256((size_t)rows * K * 2); }
 
 size_t bank_order_bytes(int rows, int count) { return bank_up256((size_t)rows * 4) + bank_up256(((size_t)count + 2) * 4); }
 
@@ -303,11 +375,11 @@ size_t bank_projected_rows(int rows, int K) {
     return here > below ? here : below;
 }
 
-void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream) {
+void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream, BankGather gather) {
     const BankProjection none{}, &other = two ? *two : none;
-    if (!r.order || r.rows < kBankOrderedFrom) launch_project<1, 4>(one, other, r, rank, stream);
-    else if (two || long_ordered(r.rows, one.K)) launch_project<2, 4>(one, other, r, rank, stream);
-    else launch_project<1, 8>(one, other, r, rank, stream);
+    if (!r.order || r.rows < kBankOrderedFrom) launch_project<1, 4>(one, other, r, rank, stream, gather);
+    else if (two || long_ordered(r.rows, one.K)) launch_project<2, 4>(one, other, r, rank, stream, gather);
+    else launch_project<1, 8>(one, other, r, rank, stream, gather);
 }
 
 namespace {
@@ -334,7 +406,8 @@ extern "C" {
 
 size_t kiln_w4a16_gemm_bank_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank) {
     if (prob_m < 1 || prob_n < 1 || prob_k < 128 || count < 1 || rank < 1) return 256;
-    return bank_order_bytes(prob_m, count) + bank_up256(bank_projected_rows(prob_m, prob_k) * rank * 4);
+    const size_t ordered = prob_m < kBankOrderedFrom ? 0 : bank_ordered_x_bytes(prob_m, prob_k) + (size_t)prob_m * (prob_k / 128 + 1) * 4;
+    return bank_order_bytes(prob_m, count) + bank_up256(bank_projected_rows(prob_m, prob_k) * rank * 4) + ordered;
 }
 
 kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C, const void *s, int prob_m, int prob_n, int prob_k,
@@ -367,6 +440,19 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     const bool base = takes_base(prob_m, prob_n, prob_k);
     const int slices = base ? bank_base_slices(prob_k) : bank_slices(prob_m, prob_k);
     const BankProjection of_x{A, bank->lora_a, t, prob_k, slices};
+    // (2048 rows of rank 32, 8 adapters, 2560 -> 18432: 186 us a call against 215 with the term behind the product, 4096 -> 14336 222 against 244; on
+    // narrow outputs the rows' copy costs what it saves: 4096 rows 14336 -> 4096 459 against 449)
+    if (prob_m >= kBankOrderedFrom && prob_n >= prob_k && bank_in_product(prob_m, prob_n, prob_k, dev)) {
+        char *ordered = at + bank_order_bytes(prob_m, bank->count) + bank_up256(bank_projected_rows(prob_m, prob_k) * rank * 4);
+        float *sums = reinterpret_cast<float *>(ordered + bank_ordered_x_bytes(prob_m, prob_k));
+        bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
+        int *adapters = reinterpret_cast<int *>(sums + (size_t)prob_m * (prob_k / 128));
+        bank_project(of_x, nullptr, rows, rank, hs,
+                     BankGather{(const uint16_t *)A, (uint16_t *)ordered, sums, adapters, prob_k, (prob_m + kGatherRows - 1) / kGatherRows});
+        bank_split_kernel<<<(unsigned)(((size_t)prob_m * (rank / 8) + 63) / 64), 64, 0, hs>>>(t, bank->scales, adapters, prob_m, rank, slices);
+        const PrefillBank term{(const uint16_t *)bank->lora_b, (const uint16_t *)t, rows.order, adapters, rank};
+        return gemm_with_bank(ordered, B, C, s, prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, sums, term);
+    }
     if (base) {
         rows.order = rows.first = nullptr;
         bank_base(A, B, s, C, of_x, rows, rank, prob_k, prob_n, groupsize == -1, hs);

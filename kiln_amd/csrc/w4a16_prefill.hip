@@ -302,12 +302,17 @@ __device__ __forceinline__ void prefill_fold_done(const PrefillFold &pf, int con
 // 41 -> 36.5 / 33.7 -> 28.4, 4096 -> 2560 at 1100 45.5 -> 35.2, 4096 -> 4096 at 777 46 -> 37, 2560 -> 2560 at 777 30 -> 24,
 // 1536 -> 1536 at 1300 25.6 -> 17.0.  The sums of K are two shorter ones: error beyond the bf16 rounding 1.79e-4 -> 1.48e-4 of
 // the result's norm at 777 x 9216 -> 2560, 14 to 25 % less in each of eight shapes.)
-template <int NWN, int WM, int MI, bool SWIGLU, bool RS, bool FOLD = false, bool INC = false, int WK = 1>
+//
+// BANK: rows of A in the order of their adapters out of a bank, whose term is added like the LoRA term, run by run of one
+// adapter's rows, and C's rows are stored where they belong.  A launch behind the product read and wrote all of C for it:
+// 2048 rows, 2560 -> 18432, rank 32, 41 us.
+template <int NWN, int WM, int MI, bool SWIGLU, bool RS, bool FOLD = false, bool INC = false, int WK = 1, bool BANK = false>
 __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) void w4a16_prefill_kernel(
     const uint16_t *__restrict__ A, const u32x4 *__restrict__ B, const uint16_t *__restrict__ S,
     uint16_t *__restrict__ C, const u32x4 *__restrict__ aext, int M, int N, int K, int Gs, int m_blocks,
     const uint16_t *__restrict__ lora_t, const uint16_t *__restrict__ lora_b, int r_total, int RP, int nb_full,
-    int KS, int GSb, float *partial, int *counters, int die_rows, u32x4 *next_aext, bool next_plain, PrefillFold pf) {
+    int KS, int GSb, float *partial, int *counters, int die_rows, u32x4 *next_aext, bool next_plain,
+    std::conditional_t<BANK, PrefillBank, PrefillFold> pf) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];  // the A ring; reused by the store
     static_assert(!FOLD || WM * NWN == 4, "the projection's blocks have four wavefronts");
     static_assert(!INC || (!RS && WM == 1 && MI == 4), "the row sums come from in front");
@@ -415,6 +420,7 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
     constexpr int kBehindRings = WK * kAStages * kAStageBytes + (WK == 2 && FOLD ? 1024 : 0);
     [[maybe_unused]] constexpr int kPeekAt = WK == 1 ? kFoldPeekOffset : WK * kAStages * kAStageBytes + (INC ? WK * 2 * NW * 256 : 0);
 
+    __shared__ int s_bank[BANK ? 2 : 1][BANK ? BM : 1];  // a bank's rows: where C has them, and their adapters (-1: none)
     __shared__ uint32_t s_meeting[2];
     if constexpr (WK == 2) {
         if (tid < 2) s_meeting[tid] = 0;
@@ -527,6 +533,11 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
     [[maybe_unused]] const uint32_t c_off = (uint32_t)min(m0 + (wave % (BM / 64)) * 64 + lane, M - 1) * 4u;
     [[maybe_unused]] int c_to = c_slots + wave * 256;              // offsets: the slots' bit is theirs, not the base's
     if constexpr (INC) c_ptr = uniform(reinterpret_cast<const char *>(aext) + (size_t)g_begin * M * 4);
+    if constexpr (BANK) {  // two wavefronts each, ahead of what the main loop waits for
+        const int part = wave & 1;
+        load_to_lds_b32(uniform(reinterpret_cast<const char *>(wave < 2 ? pf.order : pf.adapters)), (uint32_t)min(m0 + 64 * part + lane, M - 1) * 4u,
+                        (unsigned)(size_t)(lds_ptr_t)&s_bank[wave >> 1][64 * part]);
+    }
     request_b(bw, b_ptr, s_ptr);
     if constexpr (INC) load_to_lds_b32(c_ptr, c_off, lds_base + c_to);
 #pragma unroll
@@ -731,7 +742,9 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
                         }
                     }
                     if constexpr (LAST && !INC) request_ext(q, q);
-                    if constexpr (PEEK && q == 0) prefill_fold_peek(pf, m0, min(BM, M - m0), lane, lds_base + kPeekAt + wave * 256);
+                    if constexpr (FOLD) {
+                        if constexpr (PEEK && q == 0) prefill_fold_peek(pf, m0, min(BM, M - m0), lane, lds_base + kPeekAt + wave * 256);
+                    }
                 }
                 if constexpr (INC && q == 0 && mi == MI - 1 && !LAST) {
                     // three phases later than without INC: the registers are c's until then
@@ -917,6 +930,67 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
         }
     }
 
+    // --- a bank's term: for every run of rows of one adapter among the block's, T in two bf16 parts (T within 2^-17) times the
+    // adapter's rows of B.  A run that ends inside a row tile: the products of its rows alone are taken, so that what another
+    // adapter holds that is no number does not reach them.
+    if constexpr (BANK) {
+        static_assert(WM == 1 && MI == 4 && WK == 1 && !SWIGLU, "every wavefront has all of the block's 128 rows");
+        const int a_low = m0 + lane < M ? s_bank[1][lane] : -1, a_high = m0 + 64 + lane < M ? s_bank[1][64 + lane] : -1;
+        for (int q0 = 0; q0 < BM && ks == 0;) {
+            const int a = q0 < 64 ? __builtin_amdgcn_readlane(a_low, q0) : __builtin_amdgcn_readlane(a_high, q0 - 64);
+            if (a < 0) break;  // rows without an adapter are the last
+            const int q1 = q0 + __popcll(__ballot(a_low == a)) + __popcll(__ballot(a_high == a));
+            const uint16_t *b = pf.b + ((size_t)a * N + n0 + wn * 64 + l32) * pf.rank;
+            for (int j0 = 0; j0 < pf.rank; j0 += 32) {  // 32 of the rank a turn, their loads in flight together
+                bf16x8 lb[2][2], parts[2][MI][2];
+                bool has[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    has[u] = j0 + 16 * u + 8 * h < pf.rank;
+                    const int j8 = has[u] ? j0 + 16 * u + 8 * h : 0;
+#pragma unroll
+                    for (int ni = 0; ni < 2; ++ni) lb[u][ni] = *reinterpret_cast<const bf16x8 *>(b + (size_t)ni * 32 * pf.rank + j8);
+#pragma unroll
+                    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            parts[u][mi][i] = *reinterpret_cast<const bf16x8 *>(pf.t + ((size_t)min(m0 + mi * 32 + l32, M - 1) * pf.rank + j8) * 2 + 8 * i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int ni = 0; ni < 2; ++ni)
+                        if (!has[u]) lb[u][ni] = bf16x8_zero();
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) {
+                    const int r0 = mi * 32;
+                    if (r0 + 32 <= q0 || r0 >= q1) continue;
+                    const bool own = r0 + l32 >= q0 && r0 + l32 < q1, whole = r0 >= q0 && r0 + 32 <= q1;
+#pragma unroll
+                    for (int ni = 0; ni < 2; ++ni) {
+                        f32x16 v = acc[mi][ni];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                v = __builtin_amdgcn_mfma_f32_32x32x16_bf16(own && has[u] ? parts[u][mi][i] : bf16x8_zero(), lb[u][ni], v, 0, 0, 0);
+                        if (whole) {
+                            acc[mi][ni] = v;
+                        } else {
+                            int first = q0 - r0 - 4 * h;
+                            asm volatile("" : "+v"(first));  // compared where it is used: 128 masks kept would not fit the scalar registers
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[mi][ni][r] = (unsigned)(8 * (r >> 2) + (r & 3) - first) < (unsigned)(q1 - q0) ? v[r] : acc[mi][ni][r];
+                        }
+                    }
+                }
+            }
+            q0 = q1;
+        }
+    }
+
     // --- the halves of K meet in LDS: a wavefront hands the other half's wavefront of its columns that one's rows and
     // adds what it gets to its own, the earlier groups' sum first (a + b is b + a)
     constexpr int MIS = MI / WK;  // row tiles a wavefront goes on with
@@ -1096,9 +1170,11 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
         for (int p = 0; p < MIS * 4; ++p) {
             const int row = p * 8 + (lane >> 3), unit = lane & 7;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(tile + row * 64 + ((unit ^ (row & 7)) << 3));
-            const int grow = m0 + row_first + row;
-            if (grow < M)
+            int grow = m0 + row_first + row;
+            if (grow < M) {
+                if constexpr (BANK) grow = s_bank[0][row];
                 *reinterpret_cast<u32x4 *>(C + (size_t)grow * N + n0 + wn * 64 + unit * 8) = v;
+            }
         }
     }
     KILN_TL(5);
@@ -1348,9 +1424,9 @@ constexpr int kMaxRowSumBytes = 24 * 1024;
 static int row_sum_bytes(int groups) { return groups * 64 * (int)sizeof(float); }
 
 
-template <int NWN, int WM, int MI, bool SWIGLU, bool RS, bool FOLD = false, bool INC = false, int WK = 1>
+template <int NWN, int WM, int MI, bool SWIGLU, bool RS, bool FOLD = false, bool INC = false, int WK = 1, bool BANK = false>
 hipError_t launch_shape_as(const PrefillArgs &a, int grid, int m_blocks, int RP, int KS, int GSb, int max_groups,
-                           hipStream_t stream, const PrefillFold &pf = PrefillFold{}) {
+                           hipStream_t stream, const std::conditional_t<BANK, PrefillBank, PrefillFold> &pf = {}) {
     constexpr int BM = WM * MI * 32, NW = WM * NWN;
     // the A rings, behind them the groups' c or the extension's scales
     constexpr int kRing = WK * (kAStages * BM * 64 + (INC ? 2 * NW * 256 : RS ? 0 : kAStages * NW * 512)) + (WK == 2 && FOLD ? 1024 : 0);
@@ -1368,14 +1444,18 @@ hipError_t launch_shape_as(const PrefillArgs &a, int grid, int m_blocks, int RP,
     constexpr int kLdsSolo0 = (WM == 2 && NWN == 2) ? 96 * 1024 : kLdsMax;
     constexpr int kProjectLds = WK == 2 ? stream_lds_bytes(32, RS ? 0 : kStreamMaxSums) : kProjectLdsBytes16;
     constexpr int kLdsSolo = FOLD && kLdsSolo0 < kProjectLds ? kProjectLds : kLdsSolo0;
-    const hipError_t attr = allow_dynamic_lds<&w4a16_prefill_kernel<NWN, WM, MI, SWIGLU, RS, FOLD, INC, WK>>(kLdsSolo);
+    const hipError_t attr = allow_dynamic_lds<&w4a16_prefill_kernel<NWN, WM, MI, SWIGLU, RS, FOLD, INC, WK, BANK>>(kLdsSolo);
     if (attr != hipSuccess) return attr;
     if (WM == 2 && NWN == 2 && grid <= a.cus) lds_bytes = kLdsSolo;
-    // the projection's blocks stage more
-    const int project_lds = WK == 1 ? kProjectLdsBytes16
-                            : pf.a_cat ? stream_lds_bytes(RP, RS ? 0 : pf.steps_per_slice / 4) : 0;
-    if (FOLD && lds_bytes < project_lds) lds_bytes = project_lds;
-    w4a16_prefill_kernel<NWN, WM, MI, SWIGLU, RS, FOLD, INC, WK><<<grid + (FOLD ? pf.producers : 0), 64 * NW * WK, lds_bytes, stream>>>(
+    int producers = 0;
+    if constexpr (FOLD) {
+        // the projection's blocks stage more
+        const int project_lds = WK == 1 ? kProjectLdsBytes16
+                                : pf.a_cat ? stream_lds_bytes(RP, RS ? 0 : pf.steps_per_slice / 4) : 0;
+        if (lds_bytes < project_lds) lds_bytes = project_lds;
+        producers = pf.producers;
+    }
+    w4a16_prefill_kernel<NWN, WM, MI, SWIGLU, RS, FOLD, INC, WK, BANK><<<grid + producers, 64 * NW * WK, lds_bytes, stream>>>(
         (const uint16_t *)a.A, (const u32x4 *)a.B, (const uint16_t *)a.S, (uint16_t *)a.C, (const u32x4 *)a.aext,
         a.M, a.N, a.K, a.Gs, m_blocks, (const uint16_t *)a.lora_t, (const uint16_t *)a.lora_b, a.r_total, RP,
         a.nb_full, KS, GSb, a.partial, a.counters,
@@ -1730,6 +1810,10 @@ hipError_t launch_prefill(const PrefillArgs &a, hipStream_t stream) {
     if (KS > 1 && (!a.partial || !a.counters || (KS - 1) * GSb >= G)) return hipErrorInvalidValue;
     if (a.nb_full < 0 || a.nb_full > a.N / a.bn) return hipErrorInvalidValue;
     const int grid = prefill_grid(a.M, a.N, shape, a.cus);
+    if (a.bank) {
+        if (!inc || halves || fold || a.bm != 128 || a.bn != 256 || a.r_total != 0 || a.swiglu || !a.aext_ready) return hipErrorInvalidValue;
+        return launch_shape_as<4, 1, 4, false, false, false, true, 1, true>(a, grid, m_blocks, 0, KS, GSb, max_groups, stream, *a.bank);
+    }
     if (fold) {
         pf.consumers = grid;
         if (inc)

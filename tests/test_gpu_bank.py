@@ -114,6 +114,18 @@ def test_backward(m, k, n, g, count, rank, pattern):
     check_backward(p, *backward(p))
 
 
+# from thousands of rows on, wide outputs: the product adds the term itself
+MANY = [(2100, 2560, 8192, 128, 40, 24, "any"), (2048, 2560, 8192, -1, 3, 64, "runs"), (2177, 2560, 8192, 128, 300, 8, "any"), (2050, 2560, 8192, 128, 5, 40, "none")]
+
+
+@pytest.mark.parametrize("m,k,n,g,count,rank,pattern", MANY)
+def test_forward_of_many_rows(m, k, n, g, count, rank, pattern):
+    p = problem(m, k, n, g, count, rank, pattern)
+    y = forward(p)
+    check_forward(p, y)
+    assert torch.equal(bits(y)[0], bits(forward({**p, "x": p["x"].t().contiguous().t()}))[0])
+
+
 def bits(ts):
     return [t.view(torch.int16).clone() for t in (ts if isinstance(ts, tuple) else (ts,))]
 
@@ -149,6 +161,20 @@ def test_an_adapter_that_holds_no_numbers_stays_with_its_own_rows(m):
     assert torch.equal(y[keep].view(torch.int16), z[keep].view(torch.int16)) and bool(torch.isnan(z[1]).all())
 
 
+def test_an_adapter_that_holds_no_numbers_stays_with_its_own_of_many_rows():
+    p = problem(2100, 2560, 8192, 128, 37, 24, "any", seed=3)
+    bad = {**p, "a_": p["a_"].clone(), "b_": p["b_"].clone(), "x": p["x"].clone()}
+    bad["a_"][20, 3, 17], bad["b_"][2, 400, 1], bad["b_"][3, 8000, 20] = float("nan"), float("-inf"), float("nan")
+    row = int((p["of"] == 5).nonzero()[0])
+    bad["x"][row, 7] = float("inf")
+    y, z = forward(p), forward(bad)
+    odd = (p["of"] == 2) | (p["of"] == 3) | (p["of"] == 20)
+    odd[row] = True
+    assert torch.equal(bits(y[~odd])[0], bits(z[~odd])[0])
+    assert not bool(torch.isfinite(z[p["of"] == 20]).any()) and not bool(torch.isfinite(z[p["of"] == 2][:, 400]).any())
+    assert not bool(torch.isfinite(z[p["of"] == 3][:, 8000]).any()) and not bool(torch.isfinite(z[row]).all())
+
+
 @pytest.mark.parametrize("m", [7, 130, 400])
 def test_same_bits_again_on_views_other_streams_and_into_a_given_tensor(m):
     p = problem(m, 384, 512, 128, 6, 16, "any", seed=3)
@@ -166,10 +192,10 @@ def test_same_bits_again_on_views_other_streams_and_into_a_given_tensor(m):
         assert all(torch.equal(a, b) for a, b in zip(got[0] + got[1], y + g))
 
 
-@pytest.mark.parametrize("m", [5, 300])
-def test_replayed_from_a_graph(m):
+@pytest.mark.parametrize("m,k,n", [(5, 256, 512), (50, 256, 512), (300, 256, 512), (4200, 512, 8192)])
+def test_replayed_from_a_graph(m, k, n):
     """Captured calls replayed with other contents in the same tensors, eager calls and synchronisations between the replays."""
-    parts = [problem(m, 256, 512, 128, 4, 8, "any", seed=s) for s in (4, 5, 6)]
+    parts = [problem(m, k, n, 128, 4, 8, "any", seed=s) for s in (4, 5, 6)]
     live = {k: v.clone() if torch.is_tensor(v) else v for k, v in parts[0].items()}
     stream = torch.cuda.Stream()
     with torch.cuda.stream(stream):
