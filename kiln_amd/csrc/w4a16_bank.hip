@@ -337,11 +337,11 @@ void launch_project(const BankProjection &one, const BankProjection &two, const 
 }
 
 // Up to 16 rows: may the base product be the one with the projection beside it (bank_base)?  It saves a launch; the plain GEMM is the faster
-// product of many rows on the largest weights and of a long K.  1 / 8 / 16 rows of as many adapters, rank 16, us, against the plain GEMM
-// with the projection behind it: 2560 -> 10240 8.6 / 10.6 / 12.6 against 11.4 / 13.6 / 16.0, 2560 -> 18432 11.5 / 13.9 / 17.0 against 12.5 / 15.4 / 18.7,
-// 4096 -> 14336 10.3 / 12.1 / 14.6 against 14.0 / 16.0 / 18.9, 5120 -> 5120 8.7 / 11.1 / 13.8 against 12.3 / 15.5 / 17.3; but 4096 -> 24576 14.8 / 18.1 / 23.8
-// against 17.5 / 20.3 / 23.1, 5120 -> 27648 20.7 / 25.2 / 33.4 against 22.9 / 26.6 / 30.9, 9216 -> 2560 10.3 / 17.1 / 22.2 against 13.1 / 15.5 / 17.7.
-bool takes_base(int m, int n, int k) { return m <= kBankFewRows && (k <= 5120 ? m <= 8 || (int64_t)n * k <= 64 << 20 : m <= 4); }
+// product of many rows of a long K.  1 / 8 / 16 rows of as many adapters, rank 16, us, against the plain GEMM with the projection behind it:
+// 2560 -> 10240 8.2 / 10.2 / 13.1 against 11.4 / 13.6 / 16.0, 2560 -> 18432 9.6 / 12.9 / 15.6 against 12.5 / 15.4 / 18.7, 4096 -> 14336
+// 10.3 / 12.0 / 14.6 against 14.0 / 16.0 / 18.9, 5120 -> 27648 17.5 / 24.8 / 29.8 against 22.9 / 26.6 / 30.9; but 9216 -> 2560 10.3 / 17.1 / 22.2 against
+// 13.1 / 15.5 / 17.7.
+bool takes_base(int m, int n, int k) { return m <= kBankFewRows && (k <= 5120 || m <= 4); }
 
 }  // namespace
 

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(W * 64) void bank_few_kernel(FewArgs p) {
 
 // The base product of up to 16 rows, and beside it in the same launch the rows' projections, which the launch behind it (w4a16_bank.hip)
 // multiplies: the first `projecting` blocks, a slice of the contraction and a turn of the adapters each.  Tiles to a block: as many as leave
-// 128 blocks, the rows are read once for all (2560 -> 18432, 16 rows: 4 17.0 us a call, 2 18.0, 1 21.6; 4096 -> 4096: 2 12.7, 4 13.5).
+// a block to every compute unit, the rows are read once for all of them (2560 -> 18432, 16 rows: 5 15.6 us a call, 4 17.0, 2 18.0, 1 21.6).
 template <int W, int GW, int S>
 __global__ __launch_bounds__(W * 64) void bank_base_kernel(FewArgs p, BankProjection of_x, int projecting, int turns) {
     constexpr int kPitch = S * 16 + 4;
@@ -145,7 +145,8 @@ __global__ __launch_bounds__(W * 64) void bank_base_kernel(FewArgs p, BankProjec
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
     const DequantConsts dc = dequant_consts();
-    const int nt0 = (blockIdx.x - projecting) * S, G = p.K / kGroupK, Gs = p.per_column ? 1 : G;
+    // (the last block's tiles may be the one's before it too: the same values twice)
+    const int nt0 = min((int)(blockIdx.x - projecting) * S, p.N / kTileN - S), G = p.K / kGroupK, Gs = p.per_column ? 1 : G;
     f32x4 total[S];
     few_rows_product<GW, S>(p.x + (size_t)min(c, p.rows.rows - 1) * p.K + 8 * q, p.b + (size_t)nt0 * G * 64 + lane, p.s + (size_t)nt0 * Gs * kTileN + c, G,
                             p.per_column, wave, W, dc, total);
@@ -174,11 +175,26 @@ void launch_few(const FewArgs &a, hipStream_t stream) {
 }
 // Blocks of the projection are an adapter each; where those would be one round too many, up to four adapters each.
 template <int W, int GW, int S>
-void launch_base(const FewArgs &a, const BankProjection &of_x, hipStream_t stream) {
-    const int blocks = a.N / (16 * S), room = kUnits * (W == 4 ? 2 : 1) - blocks, met = a.rows.count < a.rows.rows ? a.rows.count : a.rows.rows;
+void launch_base(const FewArgs &a, const BankProjection &of_x, int met, hipStream_t stream) {
+    const int blocks = (a.N / 16 + S - 1) / S, room = kUnits * (W == 4 ? 2 : 1) - blocks;
     int turns = met;
     if (room > 0 && of_x.slices * turns > room) turns = room / of_x.slices > (met + 3) / 4 ? room / of_x.slices : (met + 3) / 4;
     bank_base_kernel<W, GW, S><<<of_x.slices * turns + blocks, W * 64, 0, stream>>>(a, of_x, of_x.slices * turns, turns);
+}
+template <int W, int GW>
+void launch_base(const FewArgs &a, const BankProjection &of_x, hipStream_t stream) {
+    const int met = a.rows.count < a.rows.rows ? a.rows.count : a.rows.rows, tiles = a.N / kTileN;
+    // a unit holds one block of eight wavefronts, or two of four
+    const int units = W == 4 ? kUnits : kUnits - of_x.slices * ((met + 1) / 2);
+    int each = (tiles + units - 1) / units;
+    if (W == 8 && each >= 7 && (tiles + 6) / 7 + of_x.slices * ((met + 3) / 4) > kUnits) each = 4;  // several rounds: small ones
+    if (each <= 1) launch_base<W, GW, 1>(a, of_x, met, stream);
+    else if (each == 2) launch_base<W, GW, 2>(a, of_x, met, stream);
+    else if (each == 3) launch_base<W, GW, 3>(a, of_x, met, stream);
+    else if (each == 4) launch_base<W, GW, 4>(a, of_x, met, stream);
+    else if (each == 5) launch_base<W, GW, 5>(a, of_x, met, stream);
+    else if (each == 6) launch_base<W, GW, 6>(a, of_x, met, stream);
+    else launch_base<W, GW, 7>(a, of_x, met, stream);
 }
 
 }  // namespace
@@ -197,10 +213,7 @@ void bank_base(const void *x, const void *b, const void *s, void *y, const BankP
     const FewArgs a{(const uint16_t *)x, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, nullptr, nullptr, nullptr, rows, K, N, rank, per_column};
     with_few_rows_split(K / kGroupK, [&](auto waves, auto groups) {
         constexpr int W = decltype(waves)::value, GW = decltype(groups)::value;
-        const int tiles = N / kTileN;
-        if (tiles >= 512) launch_base<W, GW, 4>(a, of_x, stream);
-        else if (tiles >= 256) launch_base<W, GW, 2>(a, of_x, stream);
-        else launch_base<W, GW, 1>(a, of_x, stream);
+        launch_base<W, GW>(a, of_x, stream);
     });
 }
 
