@@ -157,15 +157,15 @@ __global__ __launch_bounds__(W * 64) void moe_expert_kernel(MoeArgs p) {
     }
 }
 
-// The down projection and the sum in one launch, for a few pairs: a block takes one column tile for all tokens, its wavefronts share out the
-// experts present (and, where those are fewer, parts of their groups), each with an f32 sum per token and column in LDS, added up in
-// the wavefronts' order.  Rows are read once per column tile here, and experts beyond the wavefronts come one after the other: 8 pairs
-// (2560 -> 1024 -> 2560) 13.9 us a call against 15.7 with the two launches, 52 pairs (2048 -> 1280 -> 2048) 31 against 24.
-constexpr int kJoinWaves = 8, kMoeJoinedPairs = 16;
+// The down projection and the sum in one launch, for as many pairs as a block has wavefronts: a block takes one column tile for all tokens, its
+// wavefronts share out the experts present (and, where those are fewer, parts of their groups), each with an f32 sum per token and column in
+// LDS, added up in the wavefronts' order.  8 pairs (2560 -> 1024 -> 2560) 13.5 us a call against 15.4 with the two launches; experts beyond the
+// wavefronts would come one after the other: 16 pairs 21.6 against 20.5.
+constexpr int kJoinWaves = 8, kMoeJoinedPairs = kJoinWaves;
 template <int GW>
 __global__ __launch_bounds__(kJoinWaves * 64) void moe_join_kernel(MoeArgs p) {
     __shared__ int lists[kJoinWaves][kMoeRun];
-    __shared__ float sums[kJoinWaves][kMoeRun][16];
+    __shared__ float sums[kJoinWaves][kMoeJoinedPairs][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4;
     const DequantConsts dc = dequant_consts();
     const int pairs = p.tokens * p.top, id = id_of(p, lane, pairs);
@@ -238,13 +238,14 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs p) {
     *reinterpret_cast<u32x2 *>(p.y + (size_t)token * p.n_down + col) = o;
 }
 
-// Column tiles to a block: many where the blocks are enough all the same (their rows and lists are read once each), two where the experts
-// present are few.
+// Column tiles to a block: many where the blocks are enough all the same (their rows and lists are read once each), where the experts present
+// are few as leave a block to every compute unit (two tokens of 8 experts, 2560 -> 1024 -> 2560: four 20.5 us, two 22.5; a token: 13.5, 13.8, one 15.9).
 template <bool IN, bool FEW, int W, int GW>
 void launch_expert(const MoeArgs &a, int slots, hipStream_t stream) {
     constexpr int kMany = W == 4 ? 8 : 4;
     const int tiles = (IN ? 2 * a.n_out : a.n_down) / kTileN;
     if (slots * (tiles / kMany) >= 512) moe_expert_kernel<IN, FEW, W, GW, kMany><<<dim3(tiles / kMany, slots), W * 64, 0, stream>>>(a);
+    else if (slots * (tiles / 4) >= 256) moe_expert_kernel<IN, FEW, W, GW, 4><<<dim3(tiles / 4, slots), W * 64, 0, stream>>>(a);
     else moe_expert_kernel<IN, FEW, W, GW, 2><<<dim3(tiles / 2, slots), W * 64, 0, stream>>>(a);
 }
 template <bool IN, bool FEW>
