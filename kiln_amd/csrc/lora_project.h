@@ -16,6 +16,10 @@ __device__ __forceinline__ u32x4 extension_operand(float sum) {
     const uint32_t lo = __builtin_bit_cast(uint32_t, r2) & 0xFFFF0000u;
     return u32x4{(hi >> 16) | hi, (mid >> 16) | mid, (lo >> 16) | lo, 0u};
 }
+// Rows from one group of the extension operand to the next, where the launch that reads it writes it too: whole 128-byte lines, so that row tiles have
+// no line in common.  A block that reads its own rows would otherwise bring a line into its L2 in which the neighbouring tile's rows are not
+// there yet, and that tile's blocks on the same die would read them from it.  (An operand from a launch in front has M.)
+__host__ __device__ __forceinline__ int aext_rows(int M) { return (M + 7) & ~7; }
 // c = -136 * sum as the matrix-core kernel takes it: f32 (`plain`) where it is added at the groups' changes, else the
 // extension contraction's operand
 __device__ __forceinline__ void store_row_sum(u32x4 *__restrict__ aext, size_t at, float sum, bool plain) {
@@ -258,7 +262,7 @@ __device__ __forceinline__ void lora_project_block(unsigned char *lds, const uin
                     if constexpr (PLAIN) {
                         store_row_sum(aext, (size_t)(c0 / 4 + half) * M + m0 + row, sum, true);
                     } else {
-                        u32x4 *dst = aext + (size_t)(c0 / 4 + half) * M + m0 + row;
+                        u32x4 *dst = aext + (size_t)(c0 / 4 + half) * (done ? aext_rows(M) : M) + m0 + row;
                         if (done) store_b128_through(dst, extension_operand(sum));
                         else *dst = extension_operand(sum);
                     }
@@ -417,7 +421,7 @@ __device__ __forceinline__ void lora_project_stream(unsigned char *lds, const ui
     if (aext)
         for (int i = tid; i < (g1 - g0) * kStreamRows; i += W * 64)
             if (i % kStreamRows < rows)
-                store_b128_through(aext + (size_t)(g0 + i / kStreamRows) * M + m0 + i % kStreamRows, extension_operand(sums[i]));
+                store_b128_through(aext + (size_t)(g0 + i / kStreamRows) * (done ? aext_rows(M) : M) + m0 + i % kStreamRows, extension_operand(sums[i]));
     project_store<kStreamRows, W, IT, 8>(acc, sc_lds, T, M, RP, r_total, m0, items, JT, partial, counters, row_tile, slice, KZ, done, 1, 0);
 }
 

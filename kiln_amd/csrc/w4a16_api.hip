@@ -1766,7 +1766,7 @@ static size_t mlp_h_offset(int m, int k1, int n_out, int n2) {
 size_t kiln_w4a16_mlp_workspace_bytes(int prob_m, int hidden, int n_out, int n_down) {
     if (prob_m < 1) prob_m = 1;
     if (hidden <= 0 || n_out <= 0 || n_down <= 0 || n_out > INT32_MAX / 2) return kZeroedBytes;
-    return mlp_h_offset(prob_m, hidden, n_out, n_down) + (size_t)prob_m * n_out * 2 + prefill_aext_bytes(prob_m, n_out);
+    return mlp_h_offset(prob_m, hidden, n_out, n_down) + (size_t)prob_m * n_out * 2 + (size_t)prob_m * (n_out / kGroupK) * 16;
 }
 
 kiln_marlin_status_t kiln_w4a16_mlp(const void *x, const void *b_gate_up, const void *s_gate_up, const void *b_down,

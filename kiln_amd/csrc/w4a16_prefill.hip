@@ -224,7 +224,7 @@ __device__ __forceinline__ void rowsum_producer_block(const uint16_t *__restrict
             const int L = base + u * SLOTS + slot;
             if (sub == 0 && L < items) {
                 const int row = L / G, g = L - row * G;
-                store_b128_through(aext + (size_t)g * M + r0 + row, extension_operand(sum[u]));
+                store_b128_through(aext + (size_t)g * aext_rows(M) + r0 + row, extension_operand(sum[u]));
             }
         }
     }
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(64 * WM * NWN * WK, (WM == 2 && NWN == 4) ? 1 : 2) 
 #pragma unroll
             for (int p = 0; p < APW; ++p) {
                 const int i = wave + NW * p, g = g_begin + min(4 * e + i / (BM / 64), ng - 1);
-                load_to_lds_b128(uniform(reinterpret_cast<const char *>(aext + (size_t)g * M)), ext_off,
+                load_to_lds_b128(uniform(reinterpret_cast<const char *>(aext + (size_t)g * (FOLD ? aext_rows(M) : M))), ext_off,
                                  ring_base + slot * kAStageBytes + i * 1024);
             }
         }
@@ -1188,7 +1188,7 @@ extern "C" int kiln_w4a16_debug_timeline(long long *buf) {
 }
 #endif
 
-size_t prefill_aext_bytes(int m, int k) { return (size_t)m * (k / kGroupK) * sizeof(u32x4); }
+size_t prefill_aext_bytes(int m, int k) { return (size_t)aext_rows(m) * (k / kGroupK) * sizeof(u32x4); }
 
 // Scratch of the projection.  For the small-M kernels (few_rows): up to 16 K slices of T in bf16.
 // For the matrix-core kernel: T once and behind it the f32 tiles in which the slices meet (at most

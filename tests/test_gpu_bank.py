@@ -99,6 +99,9 @@ SHAPES = [
     (300, 2560, 1024, 128, 6, 16, "runs"), (777, 384, 2560, -1, 11, 24, "any"), (1030, 256, 512, 128, 2, 32, "runs"),
     (1, 640, 512, -1, 3, 64, "any"), (2, 384, 256, 128, 2, 40, "any"), (2, 128, 8192, 128, 5, 24, "runs"), (1, 5760, 256, 128, 3, 8, "one"), (2, 256, 8448, 128, 3, 16, "any"),
     (1, 5120, 512, 128, 2, 8, "below"), (11, 9216, 256, 128, 6, 16, "any"), (9, 256, 256, 128, 3, 8, "none"), (90, 256, 256, 128, 3, 16, "beyond"), (70, 256, 256, -1, 3, 8, "below"),
+    # column tiles that no count of them to a block divides; rows of one adapter each
+    (16, 256, 9472, 128, 20, 16, "any"), (7, 384, 18688, -1, 3, 40, "any"), (3, 256, 25600, 128, 4, 8, "any"), (13, 4224, 4352, 128, 13, 24, "any"),
+    (16, 5120, 6912, 128, 40, 64, "any"), (6, 3200, 28160, 128, 2, 56, "runs"), (4, 7296, 1280, 128, 9, 16, "any"),
 ]
 
 
