@@ -476,6 +476,9 @@ int kiln_w4a16_layout_version(void);
  *   out[capacity] = {0 another path takes the call, 1 small-M kernel, 2 mid-M kernel; tiles of a block; K slices; tiles of 16
  *   rank columns that every block projects x onto by itself, 0: the launch's first blocks do}, then {first tile, end of its
  *   own tiles} for every column block.  Returns their count, -1 for sizes or sides that no call may have.
+ * kiln_w4a16_debug_bank_plan: how kiln_w4a16_gemm_bank goes, out[2] = {0 one launch for everything, 1 the projection onto the
+ *   adapters beside the base product, 2 behind the plain GEMM, 3 the term inside the GEMM; slices of k that the scratch
+ *   holds the projection in}.  Returns 0, or 1 for sizes that no call may have.
  */
 int kiln_w4a16_debug_gemm_plan(int prob_m, int prob_n, int prob_k, int cus, int *out);
 int kiln_w4a16_debug_decode_plan(int prob_m, int prob_n, int prob_k, int cus, int *out);
@@ -483,6 +486,7 @@ int kiln_w4a16_debug_prefill_rowsum_producers(int prob_m, int prob_n, int prob_k
 int kiln_w4a16_debug_prefill_projection_blocks(int prob_m, int prob_n, int prob_k, int cus);
 int kiln_w4a16_debug_adapter_blocks(int prob_m, int prob_n, int prob_k, int cus, const kiln_w4a16_adapter_side *sides, int n_sides,
                                     int swiglu, int n_adapters, int *out, int capacity);
+int kiln_w4a16_debug_bank_plan(int prob_m, int prob_n, int prob_k, int rank, int cus, int *out);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,12 @@ inline bool meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     return i < j + b_bytes && j < i + a_bytes;
 }
 
+// `groups` in at most `most` slices of the same number of groups, the last one's perhaps fewer: as many as none is left empty
+inline int bank_level_slices(int groups, int most) {
+    const int each = (groups + most - 1) / most;
+    return (groups + each - 1) / each;
+}
+
 inline size_t bank_up256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 // The rows of a call by position: position p is row order[p] (p itself without `order`), rows of one adapter together.
@@ -34,9 +40,16 @@ bool bank_ok(const kiln_w4a16_adapter_bank &bank);
 size_t bank_order_bytes(int rows, int count);
 BankRows bank_rows(const int *of, int rows, int count, void *at);  // with order and first in bank_order_bytes of scratch from `at` on
 
-// slices of K that a projection of `rows` rows is cut into
+// how a call on a bank goes, and the slices of K that its projection is cut into
+enum class BankMethod { kOneLaunch, kBase, kBehind, kInProduct };
+struct BankPlan {
+    BankMethod method;
+    int slices;
+};
+BankPlan bank_plan(int m, int n, int k, int rank, int cus);
+// slices of K that a projection of `rows` rows is cut into in a launch of its own
 int bank_slices(int rows, int K);
-size_t bank_projected_rows(int rows, int K);  // slices * rows at most, and not falling with rows
+size_t bank_projected_rows(int rows, int K);  // slices * rows of any plan for up to `rows` rows
 // t[slice][position][rank] = the slice's share of src[row, K] * mat[adapter of row][rank, K]^T, f32; positions without an adapter are not written
 struct BankProjection {
     const void *src, *mat;
@@ -65,7 +78,7 @@ void bank_few(const void *x, const void *b, const void *s, void *y, const kiln_w
 
 // many rows: the plain GEMM with a bank's term in it (launch.h), for the sizes where it can
 struct PrefillBank;
-bool bank_in_product(int m, int n, int k, int dev);
+bool bank_in_product(int m, int n, int k, int cus);
 // A: rows in the order of their adapters; row_sums: -136 times their sums, f32 [K/128][m]
 kiln_marlin_status_t gemm_with_bank(const void *A, const void *B, void *C, const void *s, int m, int n, int k, void *workspace, int groupsize, int dev,
                                     void *stream, float *row_sums, const PrefillBank &bank);

@@ -33,6 +33,8 @@ enum WaitGaveUp : unsigned {
     kGaveUpPrefillMeeting = 32u, // there: wavefronts that share a half of their block's K
 };
 
+int compute_units(int dev);  // of a device, read once
+
 // One launch of the decode kernel: M <= 16 rows of A against the whole weight.
 constexpr int kDecodeFlaggedMaxSlices = 4;
 
@@ -213,7 +215,6 @@ hipError_t launch_mid_own1(const MidArgs &a, hipStream_t stream);   // ... with 
 hipError_t launch_mid_own2(const MidArgs &a, hipStream_t stream);
 hipError_t launch_mid_sides(const MidArgs &a, hipStream_t stream);  // ... of unstacked adapters
 
-// One launch of the prefill path (row-sum pre-pass + MFMA kernel), any M >= 1.
 // A bank of adapters for rows that lie in their adapters' order (bank.h): C[order[p]] = A[p] W + T[p] lora_b[a]^T, a the adapter of position p
 struct PrefillBank {
     const uint16_t *b;              // bf16 [count, N, rank]
@@ -221,6 +222,7 @@ struct PrefillBank {
     const int *order, *adapters;    // by position: the row, and its adapter (-1: none, at the end)
     int rank;
 };
+// One launch of the prefill path (row-sum pre-pass + MFMA kernel), any M >= 1.
 struct PrefillArgs {
     const void *A;   // bf16 [M, K]
     const void *B;   // packed weights, tile layout

@@ -33,6 +33,8 @@ struct DeviceInfo {
 };
 DeviceInfo g_dev[kMaxDevices];
 
+}  // namespace
+
 // Device properties are read once per device; the reference asks the driver
 // on every call (marlin_kernel.cu:753).
 int compute_units(int dev) {
@@ -45,6 +47,8 @@ int compute_units(int dev) {
     });
     return d.cus;
 }
+
+namespace {
 
 bool shape_ok(int n, int k, int groupsize) {
     return k % 128 == 0 && n % 256 == 0 && (groupsize == -1 || groupsize == 128);
@@ -1360,8 +1364,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
 }  // namespace
 
 // Can the product of so many rows add a bank's term itself (PrefillBank)?  It takes the row sums as f32 then, and 128 x 256 blocks.
-bool bank_in_product(int m, int n, int k, int dev) {
-    const int cus = compute_units(dev);
+bool bank_in_product(int m, int n, int k, int cus) {
     const auto plan = plan_call(m, n, k, cus, -1, -1, 0);
     return plan->gp.prefill && plan->gp.sums_in_loop && plan->gp.pf.bn == 256 && plan->gp.pf.bm == 128 && !prefill_halves_k(m, n, k, plan->gp.pf, cus);
 }

@@ -364,15 +364,24 @@ int bank_slices(int rows, int K) {
     int slices;
     if (rows < kBankOrderedFrom) slices = (groups + 3) / 4 < kBankMaxSlices ? (groups + 3) / 4 : kBankMaxSlices;
     else slices = long_ordered(rows, K) ? 8 : (groups + 11) / 12;
-    const int steps = (groups + slices - 1) / slices;
-    return (groups + steps - 1) / steps;
+    return bank_level_slices(groups, slices);
 }
 
-// slices * rows <= this, and it does not fall with `rows`
+// slices * rows <= this for the slices of every plan (bank_plan), and it does not fall with `rows`
 size_t bank_projected_rows(int rows, int K) {
-    const size_t below = (size_t)(rows < kBankOrderedFrom ? rows : kBankOrderedFrom) * bank_slices(1, K);
+    const int as_they_stand = bank_slices(1, K) > bank_base_slices(K) ? bank_slices(1, K) : bank_base_slices(K);
+    const size_t below = (size_t)(rows < kBankOrderedFrom ? rows : kBankOrderedFrom) * as_they_stand;
     const size_t here = (size_t)rows * bank_slices(rows, K);
     return here > below ? here : below;
+}
+
+// (2048 rows of rank 32, 8 adapters, 2560 -> 18432: 186 us a call with the term in the product against 215 behind it, 4096 -> 14336 222 against 244; on
+// narrow outputs the rows' copy costs what it saves: 4096 rows 14336 -> 4096 459 against 449)
+BankPlan bank_plan(int m, int n, int k, int rank, int cus) {
+    if (bank_projects_itself(m, n, k, rank)) return {BankMethod::kOneLaunch, 0};
+    if (takes_base(m, n, k)) return {BankMethod::kBase, bank_base_slices(k)};
+    const bool inside = m >= kBankOrderedFrom && n >= k && bank_in_product(m, n, k, cus);
+    return {inside ? BankMethod::kInProduct : BankMethod::kBehind, bank_slices(m, k)};
 }
 
 void bank_project(const BankProjection &one, const BankProjection *two, const BankRows &r, int rank, hipStream_t stream, BankGather gather) {
@@ -410,6 +419,14 @@ size_t kiln_w4a16_gemm_bank_scratch_bytes(int prob_m, int prob_n, int prob_k, in
     return bank_order_bytes(prob_m, count) + bank_up256(bank_projected_rows(prob_m, prob_k) * rank * 4) + ordered;
 }
 
+int kiln_w4a16_debug_bank_plan(int prob_m, int prob_n, int prob_k, int rank, int cus, int *out) {
+    if (prob_m < 1 || prob_n < 256 || prob_n % 256 != 0 || prob_k < 128 || prob_k % 128 != 0 || rank < 8 || rank > kBankMaxRank || rank % 8 != 0 || cus < 1) return 1;
+    const BankPlan plan = bank_plan(prob_m, prob_n, prob_k, rank, cus);
+    out[0] = static_cast<int>(plan.method);
+    out[1] = plan.slices;
+    return 0;
+}
+
 kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C, const void *s, int prob_m, int prob_n, int prob_k,
                                           void *workspace, int groupsize, int dev, void *stream, const kiln_w4a16_adapter_bank *bank,
                                           const int *adapter_of, void *scratch) {
@@ -432,17 +449,15 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
     const int rank = bank->rank;
-    if (bank_projects_itself(prob_m, prob_n, prob_k, rank)) {
+    const BankPlan plan = bank_plan(prob_m, prob_n, prob_k, rank, compute_units(dev));
+    if (plan.method == BankMethod::kOneLaunch) {
         rows.order = rows.first = nullptr;
         bank_few(A, B, s, C, *bank, rows, prob_k, prob_n, groupsize == -1, hs);
         return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
     }
-    const bool base = takes_base(prob_m, prob_n, prob_k);
-    const int slices = base ? bank_base_slices(prob_k) : bank_slices(prob_m, prob_k);
+    const int slices = plan.slices;
     const BankProjection of_x{A, bank->lora_a, t, prob_k, slices};
-    // (2048 rows of rank 32, 8 adapters, 2560 -> 18432: 186 us a call against 215 with the term behind the product, 4096 -> 14336 222 against 244; on
-    // narrow outputs the rows' copy costs what it saves: 4096 rows 14336 -> 4096 459 against 449)
-    if (prob_m >= kBankOrderedFrom && prob_n >= prob_k && bank_in_product(prob_m, prob_n, prob_k, dev)) {
+    if (plan.method == BankMethod::kInProduct) {
         char *ordered = at + bank_order_bytes(prob_m, bank->count) + bank_up256(bank_projected_rows(prob_m, prob_k) * rank * 4);
         float *sums = reinterpret_cast<float *>(ordered + bank_ordered_x_bytes(prob_m, prob_k));
         bank_order_kernel<<<bank->count + 1, kOrderWaves * 64, 0, hs>>>(adapter_of, rows.order, rows.first, prob_m, bank->count);
@@ -453,7 +468,7 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
         const PrefillBank term{(const uint16_t *)bank->lora_b, (const uint16_t *)t, rows.order, adapters, rank};
         return gemm_with_bank(ordered, B, C, s, prob_m, prob_n, prob_k, workspace, groupsize, dev, stream, sums, term);
     }
-    if (base) {
+    if (plan.method == BankMethod::kBase) {
         rows.order = rows.first = nullptr;
         bank_base(A, B, s, C, of_x, rows, rank, prob_k, prob_n, groupsize == -1, hs);
     } else {

@@ -205,7 +205,7 @@ bool bank_projects_itself(int m, int n, int k, int rank) { return m <= kOwnRows 
 
 int bank_base_slices(int K) {  // one turn of a block's wavefronts each
     const int groups = K / kGroupK, each = groups <= 20 ? 4 : 8, slices = (groups + each - 1) / each;
-    return slices < kBankMaxSlices ? slices : kBankMaxSlices;
+    return bank_level_slices(groups, slices < kBankMaxSlices ? slices : kBankMaxSlices);
 }
 
 void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column,
