@@ -24,6 +24,7 @@ constexpr size_t kWsFlaggedBytes = 4 * 1024 * 1024;
 constexpr size_t kWsFoldFlagBytes = 16 * 4096;
 constexpr size_t kWsFoldFlagOffset = kWsCounterBytes + kWsFlaggedBytes - kWsFoldFlagBytes;
 constexpr size_t kWsZeroedBytes = kWsCounterBytes + kWsFlaggedBytes;
+constexpr size_t kLineBytes = 128;  // of a cache: what one launch's blocks write and others of it read has lines of its own
 enum WaitGaveUp : unsigned {
     kGaveUpDecodeExchange = 1u,  // K slices of a launch of up to 16 rows
     kGaveUpMidExchange = 2u,     // K slices of a launch of the mid-M kernel (17 rows up to 1024)

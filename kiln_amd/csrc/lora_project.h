@@ -3,6 +3,7 @@
 #pragma once
 #include "async_loads.h"
 #include "device_common.h"
+#include "launch.h"
 
 namespace kiln {
 
@@ -18,8 +19,10 @@ __device__ __forceinline__ u32x4 extension_operand(float sum) {
 }
 // Rows from one group of the extension operand to the next, where the launch that reads it writes it too: whole 128-byte lines, so that row tiles have
 // no line in common.  A block that reads its own rows would otherwise bring a line into its L2 in which the neighbouring tile's rows are not
-// there yet, and that tile's blocks on the same die would read them from it.  (An operand from a launch in front has M.)
-__host__ __device__ __forceinline__ int aext_rows(int M) { return (M + 7) & ~7; }
+// there yet, and that tile's blocks on the same die would read them from it.  (The operand begins on a line: the workspace's layout sees to it.  One
+// from a launch in front has M.)
+constexpr int kAextRowsOfALine = (int)(kLineBytes / sizeof(u32x4));
+__host__ __device__ __forceinline__ int aext_rows(int M) { return (M + kAextRowsOfALine - 1) / kAextRowsOfALine * kAextRowsOfALine; }
 // c = -136 * sum as the matrix-core kernel takes it: f32 (`plain`) where it is added at the groups' changes, else the
 // extension contraction's operand
 __device__ __forceinline__ void store_row_sum(u32x4 *__restrict__ aext, size_t at, float sum, bool plain) {

@@ -892,10 +892,19 @@ void plan_gemm(int m, int n, int k, int cus, int thread_k, int thread_n, int lor
 
 // workspace of one call: counters | small-M partial tiles | LoRA projection             (small-M path)
 //                        counters | row-sum operands | partial tiles | LoRA projection (matrix-core path)
+// (counters: the whole prefix that is zero between calls)
 // The LoRA projection's scratch comes last: a call without adapters needs `plain` bytes only.
+// What a launch writes and reads itself lies in there, row tile by row tile on whole lines (aext_rows), so everything behind the zeroed
+// prefix begins on one (behind_prefix), wherever the caller's 16-byte boundary is: `total` has room for that, `plain` has not (the
+// static array begins on a line).
+constexpr size_t kWorkspaceAlign = 16;
 struct WorkspaceLayout {
     size_t decode_partial, aext, lora_t, prefill_partial, plain, total;
 };
+char *behind_prefix(void *workspace, size_t off) {  // off >= kZeroedBytes
+    const uintptr_t ws = reinterpret_cast<uintptr_t>(workspace);
+    return reinterpret_cast<char *>((ws + kLineBytes - 1) / kLineBytes * kLineBytes + off);
+}
 WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k) {
     WorkspaceLayout w{};
     size_t off = kZeroedBytes;
@@ -909,8 +918,7 @@ WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k) {
         w.decode_partial = off;
         if (gp.mid) {
             const MidArgs ma = mid_args(gp.mp, m, n, k);
-            if (ma.flagged) w.decode_partial = kCounterBytes;  // in the zeroed region, nothing behind it
-            else off += mid_partial_bytes(ma);
+            if (!ma.flagged) off += mid_partial_bytes(ma);  // (flagged: in the zeroed region)
         } else {
             off += gp.decode_partial;
         }
@@ -919,7 +927,7 @@ WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k) {
     off = (off + 255) & ~(size_t)255;
     w.lora_t = off;
     off += prefill_lora_t_bytes(m, !gp.prefill);
-    w.total = off;
+    w.total = off + kLineBytes - kWorkspaceAlign;
     return w;
 }
 
@@ -1176,7 +1184,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
     if (!A || !B || !C || !s || !workspace) return KILN_W4A16_ERR_ARGUMENT;
     // the kernels move every operand in 16-byte pieces (rows of A and C are multiples of 256 and 512 bytes)
     for (const void *p : {A, B, static_cast<const void *>(C), s, static_cast<const void *>(workspace)})
-        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+        if (reinterpret_cast<uintptr_t>(p) % kWorkspaceAlign != 0) return KILN_W4A16_ERR_ARGUMENT;
 
     const int cus = sms > 0 ? sms : compute_units(dev);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -1185,7 +1193,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
     const GemmPlan &gp = planned->gp;
     const WorkspaceLayout &wl = planned->wl;
     char *ws = reinterpret_cast<char *>(workspace);
-    char *lora_t = ws + wl.lora_t;
+    char *lora_t = behind_prefix(ws, wl.lora_t);
     if (lora && lora->sides && !sides_in_launch(gp, prob_m, prob_n, prob_k, cus, *lora, lora_t, ws)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (gp.prefill) {
         PrefillArgs pa{};
@@ -1193,7 +1201,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
         pa.B = B;
         pa.S = s;
         pa.C = C;
-        pa.aext = ws + wl.aext;
+        pa.aext = behind_prefix(ws, wl.aext);
         pa.M = prob_m;
         pa.N = prob_n;
         pa.K = prob_k;
@@ -1225,7 +1233,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
         pa.bm = gp.pf.bm;
         pa.nb_full = gp.pf.nb_full;
         pa.counters = reinterpret_cast<int *>(workspace);
-        pa.partial = reinterpret_cast<float *>(ws + wl.prefill_partial);
+        pa.partial = reinterpret_cast<float *>(behind_prefix(ws, wl.prefill_partial));
         return launch_prefill(pa, st) == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
     }
 
@@ -1239,7 +1247,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
         ma.Gs = (groupsize == -1) ? 1 : prob_k / kGroupK;
         ma.swiglu = swiglu;
         ma.counters = reinterpret_cast<int *>(workspace);
-        ma.partial = reinterpret_cast<float *>(ws + wl.decode_partial);
+        ma.partial = reinterpret_cast<float *>(ma.flagged ? ws + kCounterBytes : behind_prefix(ws, wl.decode_partial));
         if (lora) {  // the scaled projection of all rows onto the adapters, in K slices
             ma.lora_t = lora_t;
             ma.lora_b = lora->b;
@@ -1306,7 +1314,6 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
     a.B = B;
     a.S = s;
     a.counters = reinterpret_cast<int *>(workspace);
-    a.partial = reinterpret_cast<float *>(ws + wl.decode_partial);
     a.N = prob_n;
     a.K = prob_k;
     a.Gs = (groupsize == -1) ? 1 : prob_k / kGroupK;
@@ -1354,7 +1361,7 @@ kiln_marlin_status_t gemm_any(const void *A, const void *B, void *C, const void 
         a.gm_tiles = l.plan.gm_tiles;
         a.gmp = l.plan.gmp;
         a.flagged = launch_flagged(l, prob_n);
-        a.partial = reinterpret_cast<float *>(ws + (a.flagged ? kCounterBytes : wl.decode_partial));
+        a.partial = reinterpret_cast<float *>(a.flagged ? ws + kCounterBytes : behind_prefix(ws, wl.decode_partial));
         a.group_major = g_tune.decode_group_major;
         if ((a.gmp ? launch_decode_gmp(a, st) : launch_decode(a, st)) != hipSuccess) return KILN_W4A16_ERR_LAUNCH;
     }
@@ -1482,6 +1489,21 @@ kiln_marlin_status_t kiln_w4a16_workspace_reset(void *workspace, void *stream) {
     if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
     zero_fill_kernel<<<256, 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(reinterpret_cast<u32x4 *>(ws), kZeroedBytes / 16);
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
+}
+
+// Where a call's operands behind the zeroed prefix lie (a pure query, no GPU needed): out = {row sums, partial tiles, T, end}; 0: none.
+int kiln_w4a16_debug_workspace_operands(int m, int n, int k, int cus, int adapters, const void *workspace, size_t *out) {
+    if (m < 1 || n < 256 || k < 128 || cus < 1 || !shape_ok(n, k, 128)) return 1;
+    const auto planned = plan_call(m, n, k, cus, -1, -1, adapters != 0);
+    const WorkspaceLayout &wl = planned->wl;
+    void *ws = const_cast<void *>(workspace);
+    auto at = [&](size_t off) { return reinterpret_cast<size_t>(behind_prefix(ws, off)); };
+    const bool prefill = planned->gp.prefill;
+    out[0] = prefill ? at(wl.aext) : 0;
+    out[1] = at(prefill ? wl.prefill_partial : wl.decode_partial);
+    out[2] = adapters ? at(wl.lora_t) : 0;
+    out[3] = at(adapters ? wl.lora_t + prefill_lora_t_bytes(m, !prefill) : wl.plain);
+    return 0;
 }
 
 // The small-M plan for a run of m rows on a part with `cus` compute units (a pure query, no GPU

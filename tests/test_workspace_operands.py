@@ -1,0 +1,30 @@
+"""Operands that a launch writes and reads itself begin on a cache line wherever in memory the caller's workspace lies, and end inside the
+size that the library asks for.  CPU only: the workspace's address is never followed."""
+import ctypes
+
+import pytest
+
+from kiln_amd import _lib
+
+SIZES = [(1, 256, 128), (16, 2560, 9216), (16, 18432, 2560), (33, 2560, 2560), (77, 2560, 9216), (200, 5120, 13824), (515, 10240, 640), (777, 9216, 2560),
+         (1031, 6144, 1152), (1503, 5888, 2176), (2045, 4096, 1280), (2048, 18432, 2560), (8192, 2560, 9216)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("adapters", [0, 1])
+def test_operands_are_on_lines_inside_the_workspace(m, n, k, adapters):
+    L = _lib.load()
+    size, prefix = L.kiln_w4a16_workspace_bytes(m, n, k), L.kiln_w4a16_workspace_zeroed_bytes()
+    for base in range(1 << 30, (1 << 30) + 256, 16):
+        out = (ctypes.c_size_t * 4)()
+        assert L.kiln_w4a16_debug_workspace_operands(m, n, k, 256, adapters, base, out) == 0
+        *operands, end = out
+        assert any(operands) and end <= base + size, base
+        for at in operands:
+            assert at == 0 or (at % 128 == 0 and base + prefix <= at <= end), (base, list(out))
+
+
+def test_the_query_refuses():
+    out = (ctypes.c_size_t * 4)()
+    for m, n, k in ((0, 256, 128), (1, 128, 128), (1, 256, 64), (1, 300, 128)):
+        assert _lib.load().kiln_w4a16_debug_workspace_operands(m, n, k, 256, 0, 1 << 30, out) == 1
