@@ -25,6 +25,13 @@ constexpr size_t kWsFoldFlagBytes = 16 * 4096;
 constexpr size_t kWsFoldFlagOffset = kWsCounterBytes + kWsFlaggedBytes - kWsFoldFlagBytes;
 constexpr size_t kWsZeroedBytes = kWsCounterBytes + kWsFlaggedBytes;
 constexpr size_t kLineBytes = 128;  // of a cache: what one launch's blocks write and others of it read has lines of its own
+// Rows from one K slice of the projection onto adapters, T, to the next where the launch that reads T writes it: whole lines of the
+// narrowest T, 16 columns of bf16.  (With M rows the last row tile of a slice and the first of the next had a line in common, and in later
+// slices all neighbours had: a block that read its own rows could bring others that were not there yet into its die's L2.)
+constexpr int lora_t_rows(int M) {
+    constexpr int kRowsOfALine = (int)(kLineBytes / (16 * sizeof(uint16_t)));
+    return (M + kRowsOfALine - 1) / kRowsOfALine * kRowsOfALine;
+}
 enum WaitGaveUp : unsigned {
     kGaveUpDecodeExchange = 1u,  // K slices of a launch of up to 16 rows
     kGaveUpMidExchange = 2u,     // K slices of a launch of the mid-M kernel (17 rows up to 1024)
@@ -191,7 +198,7 @@ struct MidArgs {
     int r_total = 0;
     int lora_slices = 1;
     // lora_producers > 0: the projection runs in this launch's first blocks (16-row tiles x lora_slices K slices of
-    // lora_steps_per_slice steps) and lora_t is written here; needs >= 4 wavefronts per block
+    // lora_steps_per_slice steps) and lora_t is written here, slices lora_t_rows(M) rows apart; needs >= 4 wavefronts per block
     int lora_producers = 0;
     int lora_steps_per_slice = 0;
     const void *lora_a = nullptr;    // bf16 [r_total, K]

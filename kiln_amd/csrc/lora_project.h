@@ -85,7 +85,7 @@ __device__ __forceinline__ void project_store(f32x4 (&acc)[IT], const float *sc_
                                               int m0, int items, int JT, float *partial, int *counters, int row_tile, int slice,
                                               int KZ, unsigned *done, int done_copies, int done_stride) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint16_t *Tz = T + (size_t)slice * M * RP;
+    uint16_t *Tz = T + (size_t)slice * (done ? lora_t_rows(M) : M) * RP;
     if (partial && KZ > 1) {
         // One T for all of K: the slices of a row tile meet in `partial` as f32 tiles (device-scope
         // accesses); the last block to arrive adds them in slice order, so the result does not

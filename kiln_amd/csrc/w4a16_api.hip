@@ -1491,10 +1491,13 @@ kiln_marlin_status_t kiln_w4a16_workspace_reset(void *workspace, void *stream) {
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
 
-// Where a call's operands behind the zeroed prefix lie (a pure query, no GPU needed): out = {row sums, partial tiles, T, end}; 0: none.
-int kiln_w4a16_debug_workspace_operands(int m, int n, int k, int cus, int adapters, const void *workspace, size_t *out) {
-    if (m < 1 || n < 256 || k < 128 || cus < 1 || !shape_ok(n, k, 128)) return 1;
-    const auto planned = plan_call(m, n, k, cus, -1, -1, adapters != 0);
+// Where a call's operands behind the zeroed prefix lie (a pure query, no GPU needed): out = {row sums, partial tiles, T, end,
+// T's slices, bytes from one to the next}; 0: none.
+int kiln_w4a16_debug_workspace_operands(int m, int n, int k, int cus, int rank, const void *workspace, size_t *out) {
+    if (m < 1 || n < 256 || k < 128 || cus < 1 || rank < 0 || rank > 64 || rank % 8 != 0 || !shape_ok(n, k, 128)) return 1;
+    const bool adapters = rank > 0;
+    const LoraSpec lora{workspace, workspace, rank, 1, nullptr, nullptr};
+    const auto planned = plan_call(m, n, k, cus, -1, -1, adapters ? lora_kind(&lora, m) : 0);
     const WorkspaceLayout &wl = planned->wl;
     void *ws = const_cast<void *>(workspace);
     auto at = [&](size_t off) { return reinterpret_cast<size_t>(behind_prefix(ws, off)); };
@@ -1503,6 +1506,15 @@ int kiln_w4a16_debug_workspace_operands(int m, int n, int k, int cus, int adapte
     out[1] = at(prefill ? wl.prefill_partial : wl.decode_partial);
     out[2] = adapters ? at(wl.lora_t) : 0;
     out[3] = at(adapters ? wl.lora_t + prefill_lora_t_bytes(m, !prefill) : wl.plain);
+    out[4] = out[5] = 0;
+    const GemmPlan &gp = planned->gp;
+    if (adapters && gp.mid && gp.mp.own == 0) {
+        MidArgs ask = mid_args(gp.mp, m, n, k);
+        if (mid_lora_in_launch(gp, lora, ws, &ask)) {
+            out[4] = ask.lora_slices;
+            out[5] = (size_t)lora_t_rows(m) * ((rank + 15) / 16 * 16) * sizeof(uint16_t);
+        }
+    }
     return 0;
 }
 

@@ -153,12 +153,12 @@ struct MidScheduleOf {
 };
 
 // The low-rank term of a call with adapters (LORA instances): T = the scaled projection of x onto the
-// stacked adapters in `slices` K slices, each rounded on its own, bf16 [slices][rows][rp] (written by
+// stacked adapters in `slices` K slices, each rounded on its own, bf16 [slices][t_rows][rp] (written by
 // a launch in front of this one), B_cat bf16 [N][r_total], r_total % 8 == 0.
 struct MidLora {
     const uint16_t *t;
     const uint16_t *b;
-    int r_total, rp, slices;
+    int r_total, rp, slices, t_rows;
     // producers > 0: the projection runs in this launch's first `producers` blocks (row tiles of 16 rows x
     // the K slices, lora_project_block), which raise a word per (slice, row tile) -- in 16 copies, 4 KiB
     // apart, block b looks at copy b % 16: hundreds of readers of one address are served one by one -- in
@@ -650,7 +650,7 @@ __device__ __forceinline__ void mid_block(
 #pragma unroll
                 for (int rb = 0; rb < RBN; ++rb) {
                     const int row = zr + min(32 * rb + l32, M - 1);
-                    ta[rb] = *reinterpret_cast<const u32x4 *>(lo.t + ((size_t)z * rows + row) * lo.rp + j8);
+                    ta[rb] = *reinterpret_cast<const u32x4 *>(lo.t + ((size_t)z * lo.t_rows + row) * lo.rp + j8);
                 }
 #pragma unroll
                 for (int p = 0; p < TP; ++p) {
@@ -936,6 +936,7 @@ hipError_t launch_mid_tgs(const MidArgs &a, hipStream_t stream) {
     lo.r_total = a.r_total;
     lo.rp = (a.r_total + 15) / 16 * 16;
     lo.slices = a.lora_slices;
+    lo.t_rows = a.lora_producers > 0 ? lora_t_rows(a.M) : a.M;
     const int col_blocks = (NT + 2 * TP - 1) / (2 * TP);
 #if KILN_MID_LORA >= 3
     lo.own = own_args(a);

@@ -1200,7 +1200,7 @@ constexpr int kProjectFoldCounters = 8192;  // folded into the product's launch:
 int lora_project_rows_per_block(int m, int k) { return m > 1024 && k > 4096 ? 64 : 16; }
 int prefill_lora_max_slices(int) { return 16; }
 size_t prefill_lora_t_bytes(int m, bool few_rows) {
-    if (few_rows) return (size_t)prefill_lora_max_slices(m) * m * 64 * sizeof(uint16_t);
+    if (few_rows) return (size_t)prefill_lora_max_slices(m) * lora_t_rows(m) * 64 * sizeof(uint16_t);
     size_t many = 0;
     for (int rb = 16; rb <= 64; rb *= 4) {  // either block height
         const size_t tiles = 256 + 2 * (size_t)((m + rb - 1) / rb);

@@ -11,20 +11,36 @@ SIZES = [(1, 256, 128), (16, 2560, 9216), (16, 18432, 2560), (33, 2560, 2560), (
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
-@pytest.mark.parametrize("adapters", [0, 1])
-def test_operands_are_on_lines_inside_the_workspace(m, n, k, adapters):
+@pytest.mark.parametrize("rank", [0, 8, 40])
+def test_operands_are_on_lines_inside_the_workspace(m, n, k, rank):
     L = _lib.load()
     size, prefix = L.kiln_w4a16_workspace_bytes(m, n, k), L.kiln_w4a16_workspace_zeroed_bytes()
     for base in range(1 << 30, (1 << 30) + 256, 16):
-        out = (ctypes.c_size_t * 4)()
-        assert L.kiln_w4a16_debug_workspace_operands(m, n, k, 256, adapters, base, out) == 0
-        *operands, end = out
+        out = (ctypes.c_size_t * 6)()
+        assert L.kiln_w4a16_debug_workspace_operands(m, n, k, 256, rank, base, out) == 0
+        *operands, end, slices, apart = out
         assert any(operands) and end <= base + size, base
         for at in operands:
             assert at == 0 or (at % 128 == 0 and base + prefix <= at <= end), (base, list(out))
+        assert operands[2] + slices * apart <= end
+
+
+def test_slices_of_a_projection_inside_the_launch_are_lines_apart():
+    """... for every count of rows of a launch whose runs of 64 rows wait for their own rows of it alone."""
+    L, seen = _lib.load(), 0
+    for k, n in ((2560, 2560), (9216, 2560), (2560, 18432), (4096, 14336)):
+        for m in range(17, 257):
+            for rank in (8, 16, 24, 32, 40, 64):
+                out = (ctypes.c_size_t * 6)()
+                assert L.kiln_w4a16_debug_workspace_operands(m, n, k, 256, rank, 1 << 30, out) == 0
+                slices, apart = out[4:]
+                assert apart % 128 == 0 and apart >= slices and (slices == 0 or apart >= 32 * m), (m, n, k, rank)
+                assert out[2] + slices * apart <= out[3]
+                seen += slices > 1 and m > 64
+    assert seen > 1000
 
 
 def test_the_query_refuses():
-    out = (ctypes.c_size_t * 4)()
+    out = (ctypes.c_size_t * 6)()
     for m, n, k in ((0, 256, 128), (1, 128, 128), (1, 256, 64), (1, 300, 128)):
         assert _lib.load().kiln_w4a16_debug_workspace_operands(m, n, k, 256, 0, 1 << 30, out) == 1
