@@ -107,12 +107,15 @@ class LayerProjections:
         w = self.packed.get(kind)
         if w is not None:
             return proj_forward_bank(x, w, bank, adapter_of)
-        y = self.forward(kind, x).reshape(adapter_of.numel(), -1)
-        rows, of = x.reshape(adapter_of.numel(), -1), adapter_of.reshape(-1)
+        if adapter_of.numel() != x.shape[:-1].numel():
+            raise MarlinProjError(f"layer_pack: adapter_of names {adapter_of.numel()} rows' adapters (x has {x.shape[:-1].numel()} rows)")
+        y = self.forward(kind, x)
+        shape = y.shape
+        y, rows, of = y.reshape(-1, shape[-1]), x.reshape(-1, x.shape[-1]), adapter_of.reshape(-1)
         for i in range(bank.a.shape[0]):                       # unfused, an adapter at a time
             delta = (rows @ bank.a[i].t()) @ bank.b[i].t() * bank.scales[i]
             y = torch.where((of == i)[:, None], y + delta.to(y.dtype), y)
-        return y.reshape(*x.shape[:-1], -1)
+        return y.reshape(shape)
 
     def forward_same_input(self, kinds: Sequence[PackKind], x: torch.Tensor, loras: Optional[Dict[PackKind, object]] = None,
                            lora_scale: float = 1.0) -> Tuple[torch.Tensor, ...]:
