@@ -113,7 +113,7 @@ class LayerProjections:
         shape = y.shape
         y, rows, of = y.reshape(-1, shape[-1]), x.reshape(-1, x.shape[-1]), adapter_of.reshape(-1)
         for i in range(bank.a.shape[0]):                       # unfused, an adapter at a time
-            delta = (rows @ bank.a[i].t()) @ bank.b[i].t() * bank.scales[i]
+            delta = (rows @ bank.a[i].t().to(x.dtype)) @ bank.b[i].t().to(x.dtype) * bank.scales[i]
             y = torch.where((of == i)[:, None], y + delta.to(y.dtype), y)
         return y.reshape(shape)
 

@@ -41,3 +41,11 @@ def test_rows_of_several_adapters():
         want[mine] += s * (rows[mine] @ a.t()) @ b.t()
         bound[mine] += s * (rows[mine].abs() @ a.abs().t()) @ b.abs().t() * (3 * 2 ** -8 + (96 + 8) * 2 ** -24)
     assert bool(((y - want).abs() <= (bound + 2 ** -8 * want.abs()) * (1 + 2 ** -6)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_rows_of_another_type_as_forward_takes_them(dtype):
+    layer, bank, rand = layer_and_bank(dtype=dtype)
+    x, of = rand(4, 96).to(dtype), torch.tensor([1, -1, 1, 1], dtype=torch.int32)
+    y, alone = layer.forward_bank(PackKind.QProj, x, bank, of), layer.forward(PackKind.QProj, x, lora.LoraProjectionWeights(bank.a[1], bank.b[1]), 2.0)
+    assert y.dtype == dtype and torch.equal(y[of == 1], alone[of == 1]) and torch.equal(y[1], layer.forward(PackKind.QProj, x)[1])
