@@ -191,6 +191,8 @@ def make_bank(adapters: Sequence[LoraProjectionWeights], scales: Sequence[float]
     if not adapters or len(adapters) != len(scales):
         raise MarlinProjError("make_bank: need one scale per adapter")
     rank = -(-max(int(p.a.shape[0]) for p in adapters) // 8) * 8
+    if not 8 <= rank <= 64:
+        raise MarlinProjError(f"make_bank: the largest rank is 1 to 64 (got {max(int(p.a.shape[0]) for p in adapters)})")
     k, n, device = adapters[0].a.shape[1], adapters[0].b.shape[0], adapters[0].a.device
     a = torch.zeros((len(adapters), rank, k), dtype=torch.bfloat16, device=device)
     b = torch.zeros((len(adapters), n, rank), dtype=torch.bfloat16, device=device)

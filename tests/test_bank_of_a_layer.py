@@ -49,3 +49,11 @@ def test_rows_of_another_type_as_forward_takes_them(dtype):
     x, of = rand(4, 96).to(dtype), torch.tensor([1, -1, 1, 1], dtype=torch.int32)
     y, alone = layer.forward_bank(PackKind.QProj, x, bank, of), layer.forward(PackKind.QProj, x, lora.LoraProjectionWeights(bank.a[1], bank.b[1]), 2.0)
     assert y.dtype == dtype and torch.equal(y[of == 1], alone[of == 1]) and torch.equal(y[1], layer.forward(PackKind.QProj, x)[1])
+
+
+def test_ranks_that_no_call_takes_make_no_bank():
+    adapter = lambda rank: lora.LoraProjectionWeights(torch.zeros(rank, 96, dtype=torch.bfloat16), torch.zeros(40, rank, dtype=torch.bfloat16))
+    for ranks in ((65,), (8, 72), (0,), (0, 0)):
+        with pytest.raises(MarlinProjError, match="rank"):
+            lora.make_bank([adapter(r) for r in ranks], [1.0] * len(ranks))
+    assert lora.make_bank([adapter(64), adapter(0)], [1.0, 1.0]).a.shape == (2, 64, 96)
