@@ -479,6 +479,8 @@ int kiln_w4a16_layout_version(void);
  * kiln_w4a16_debug_bank_plan: how kiln_w4a16_gemm_bank goes, out[2] = {0 one launch for everything, 1 the projection onto the
  *   adapters beside the base product, 2 behind the plain GEMM, 3 the term inside the GEMM; slices of k that the scratch
  *   holds the projection in}.  Returns 0, or 1 for sizes that no call may have.
+ * kiln_w4a16_debug_bank_backward_plan: the product behind kiln_w4a16_gemm_bank_backward's dA, out[3] = {rows and columns of k to a block
+ *   (0: calls of few rows, straight from the codes), slices of n}.  Returns 0, or 1 for sizes that no call may have.
  * kiln_w4a16_debug_workspace_operands: where a GEMM with stacked adapters of `rank` (a multiple of 8; 0: none) that is handed
  *   `workspace` (never followed) has its operands behind the zeroed prefix, out[6] = {row sums (0: none), partial tiles, projection
  *   (0: none), the end of all; of a projection that the mid-M kernel's launch writes and reads, its K slices and the bytes from one
@@ -491,6 +493,7 @@ int kiln_w4a16_debug_prefill_projection_blocks(int prob_m, int prob_n, int prob_
 int kiln_w4a16_debug_adapter_blocks(int prob_m, int prob_n, int prob_k, int cus, const kiln_w4a16_adapter_side *sides, int n_sides,
                                     int swiglu, int n_adapters, int *out, int capacity);
 int kiln_w4a16_debug_bank_plan(int prob_m, int prob_n, int prob_k, int rank, int cus, int *out);
+int kiln_w4a16_debug_bank_backward_plan(int prob_m, int prob_n, int prob_k, int *out);
 int kiln_w4a16_debug_workspace_operands(int prob_m, int prob_n, int prob_k, int cus, int rank, const void *workspace, size_t *out);
 
 #ifdef __cplusplus

@@ -54,6 +54,7 @@ EXPORTS = (
     "kiln_w4a16_debug_prefill_projection_blocks",
     "kiln_w4a16_debug_adapter_blocks",
     "kiln_w4a16_debug_bank_plan",
+    "kiln_w4a16_debug_bank_backward_plan",
     "kiln_w4a16_debug_workspace_operands",
 )
 
@@ -214,6 +215,8 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_debug_adapter_blocks.argtypes = [i, i, i, i, vp, i, i, i, c.POINTER(c.c_int), i]
     L.kiln_w4a16_debug_workspace_operands.restype = i
     L.kiln_w4a16_debug_workspace_operands.argtypes = [i, i, i, i, i, vp, c.POINTER(c.c_size_t)]
+    L.kiln_w4a16_debug_bank_backward_plan.restype = i
+    L.kiln_w4a16_debug_bank_backward_plan.argtypes = [i, i, i, c.POINTER(c.c_int)]
     L.kiln_w4a16_debug_bank_plan.restype = i
     L.kiln_w4a16_debug_bank_plan.argtypes = [i, i, i, i, i, c.POINTER(c.c_int)]
     L.kiln_w4a16_gemm_lora.restype = i

@@ -786,6 +786,15 @@ size_t kiln_w4a16_gemm_bank_backward_scratch_bytes(int prob_m, int prob_n, int p
     return backward_scratch(prob_m < 1 ? 1 : prob_m, prob_n, prob_k, count, rank).total;
 }
 
+int kiln_w4a16_debug_bank_backward_plan(int prob_m, int prob_n, int prob_k, int *out) {
+    if (prob_m < 1 || prob_n < 256 || prob_n % 256 != 0 || prob_k < 128 || prob_k % 128 != 0) return 1;
+    const BackwardScratch w = backward_scratch(prob_m, prob_n, prob_k, 0, 0);
+    out[0] = w.few ? 0 : kDxTileM[w.dx.kind];
+    out[1] = w.few ? 0 : kDxTileK[w.dx.kind];
+    out[2] = w.dx.slices;
+    return 0;
+}
+
 kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A, const void *B, const void *s, int prob_m, int prob_n, int prob_k,
                                                    int groupsize, int dev, void *stream, const kiln_w4a16_adapter_bank *bank, const int *adapter_of,
                                                    void *dA, void *d_lora_a, void *d_lora_b, void *scratch) {
