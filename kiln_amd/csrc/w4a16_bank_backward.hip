@@ -17,6 +17,7 @@
 #include "bank_order.h"
 #include "bank_project.h"
 #include "device_common.h"
+#include "launch.h"
 
 namespace kiln {
 namespace {
@@ -718,12 +719,15 @@ void launch_prepare(const PrepareArgs &p, hipStream_t stream) {
 }
 
 template <int WM, int WN, int TM, int TN>
-void launch_dx(DxArgs p, int slices, hipStream_t stream) {
-    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
+hipError_t launch_dx(DxArgs p, int slices, hipStream_t stream) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, kLds = kStages * (BM + BN) * 64;
+    const hipError_t attr = allow_dynamic_lds<&bank_dx_kernel<WM, WN, TM, TN>>(kLds);
+    if (attr != hipSuccess) return attr;
     p.m_tiles = (p.rows.rows + BM - 1) / BM;
     p.k_tiles = (p.K + BN - 1) / BN;
     p.steps = (p.N / 32 + slices - 1) / slices;
-    bank_dx_kernel<WM, WN, TM, TN><<<p.m_tiles * p.k_tiles * slices, WM * WN * 64, kStages * (BM + BN) * 64, stream>>>(p);
+    bank_dx_kernel<WM, WN, TM, TN><<<p.m_tiles * p.k_tiles * slices, WM * WN * 64, kLds, stream>>>(p);
+    return hipSuccess;
 }
 
 // Up to 64 rows: slices of the columns, of 256 at least; 16 at most, by what they add up to
@@ -886,11 +890,10 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank_backward(const void *dC, const void *A
         launch_prepare(prepare, hs);
     }
     if (m > 0 && !w.few) {
-        switch (w.dx.kind) {
-            case 0: launch_dx<2, 2, 2, 2>(dx, w.dx.slices, hs); break;
-            case 1: launch_dx<2, 4, 2, 2>(dx, w.dx.slices, hs); break;
-            default: launch_dx<2, 2, 4, 4>(dx, w.dx.slices, hs); break;
-        }
+        const hipError_t launched = w.dx.kind == 0   ? launch_dx<2, 2, 2, 2>(dx, w.dx.slices, hs)
+                                    : w.dx.kind == 1 ? launch_dx<2, 4, 2, 2>(dx, w.dx.slices, hs)
+                                                     : launch_dx<2, 2, 4, 4>(dx, w.dx.slices, hs);
+        if (launched != hipSuccess) return KILN_W4A16_ERR_LAUNCH;
     }
     if (m > 0 && (!bank || !w.few) && partial) {
         const size_t units = (size_t)m * k / 4;
