@@ -69,7 +69,7 @@ void bank_project(const BankProjection &one, const BankProjection *two, const Ba
 // up to 16 rows as they stand: y = x W, and their projection (bank_base_slices of it) in the same launch
 constexpr int kBankFewRows = 16;
 int bank_base_slices(int K);
-void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column,
+void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column, int cus,
                hipStream_t stream);
 // ... or a row or two with their low-rank term in one launch
 bool bank_projects_itself(int m, int n, int k, int rank);

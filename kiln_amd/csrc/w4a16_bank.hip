@@ -394,14 +394,15 @@ void bank_project(const BankProjection &one, const BankProjection *two, const Ba
 namespace {
 
 template <int S>
-void launch_expand(uint16_t *y, const uint16_t *m, const float *t, const float *scales, const BankRows &r, int N, int rank, int slices, hipStream_t stream) {
+void launch_expand(uint16_t *y, const uint16_t *m, const float *t, const float *scales, const BankRows &r, int N, int rank, int slices, int cus,
+                   hipStream_t stream) {
     if (!r.order) {
         bank_expand_kernel<S><<<dim3(N / 64, tiles_of(r.rows, 16)), 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices);
         return;
     }
     const int tiles = tiles_of(r.rows, 64);
     int columns = 1024;  // (2048 rows of 18432 columns: 256 60 us, 512 49, 1024 45, 2048 50)
-    while (columns > 256 && tiles * ((N + columns - 1) / columns) < 512) columns /= 2;
+    while (columns > 256 && tiles * ((N + columns - 1) / columns) < 2 * cus) columns /= 2;
     bank_expand_ordered_kernel<S><<<(N + columns - 1) / columns * tiles, 256, 0, stream>>>(y, m, t, scales, r, N, rank, slices, columns);
 }
 
@@ -449,7 +450,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     BankRows rows = bank_rows(adapter_of, prob_m, bank->count, at);
     float *t = reinterpret_cast<float *>(at + bank_order_bytes(prob_m, bank->count));
     const int rank = bank->rank;
-    const BankPlan plan = bank_plan(prob_m, prob_n, prob_k, rank, compute_units(dev));
+    const int cus = compute_units(dev);
+    const BankPlan plan = bank_plan(prob_m, prob_n, prob_k, rank, cus);
     if (plan.method == BankMethod::kOneLaunch) {
         rows.order = rows.first = nullptr;
         bank_few(A, B, s, C, *bank, rows, prob_k, prob_n, groupsize == -1, hs);
@@ -470,7 +472,7 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     }
     if (plan.method == BankMethod::kBase) {
         rows.order = rows.first = nullptr;
-        bank_base(A, B, s, C, of_x, rows, rank, prob_k, prob_n, groupsize == -1, hs);
+        bank_base(A, B, s, C, of_x, rows, rank, prob_k, prob_n, groupsize == -1, cus, hs);
     } else {
         // the plain GEMM's checks and its launches first: nothing is launched for a call that it refuses
         const kiln_marlin_status_t st =
@@ -482,8 +484,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_bank(const void *A, const void *B, void *C,
     }
     uint16_t *y = (uint16_t *)C;
     const uint16_t *m = (const uint16_t *)bank->lora_b;
-    if (rank <= 32) launch_expand<1>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);
-    else launch_expand<2>(y, m, t, bank->scales, rows, prob_n, rank, slices, hs);
+    if (rank <= 32) launch_expand<1>(y, m, t, bank->scales, rows, prob_n, rank, slices, cus, hs);
+    else launch_expand<2>(y, m, t, bank->scales, rows, prob_n, rank, slices, cus, hs);
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
 

@@ -680,7 +680,8 @@ void launch_grad(GradArgs g, bool few, hipStream_t stream) {
 // The block of the product for dx and the slices of its contraction.  A block of 256 x 256 is the fastest by its area (2048 rows of n 18432, k
 // 2560, three slices: 189 us, 1.02 PFLOP/s; 128 x 256 216, 128 x 128 237), a smaller one where those would leave compute units without
 // work (777 rows, 2560 -> 9216: 128 x 256 49 us, 128 x 128 55, 256 x 256 79).  Times by a model: so many rounds of blocks, each its steps
-// at what one takes, measured, and with slices what writing, reading and adding them takes.
+// at what one takes, measured, and with slices what writing, reading and adding them takes.  (Of 256 compute units, the part's: the scratch that
+// holds the slices is asked for without a device, and a plan of another count could need more.)
 struct DxPlan {
     int kind;    // 0: 128 x 128, two blocks to a compute unit; 1: 128 x 256; 2: 256 x 256
     int slices;

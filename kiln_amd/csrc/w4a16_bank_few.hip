@@ -8,7 +8,7 @@
 namespace kiln {
 namespace {
 
-constexpr int kOwnRows = 2, kUnits = 256;
+constexpr int kOwnRows = 2;
 struct FewArgs {
     const uint16_t *x;
     const u32x4 *b;
@@ -175,26 +175,26 @@ void launch_few(const FewArgs &a, hipStream_t stream) {
 }
 // Blocks of the projection are an adapter each; where those would be one round too many, up to four adapters each.
 template <int W, int GW, int S>
-void launch_base(const FewArgs &a, const BankProjection &of_x, int met, hipStream_t stream) {
-    const int blocks = (a.N / 16 + S - 1) / S, room = kUnits * (W == 4 ? 2 : 1) - blocks;
+void launch_base(const FewArgs &a, const BankProjection &of_x, int met, int cus, hipStream_t stream) {
+    const int blocks = (a.N / 16 + S - 1) / S, room = cus * (W == 4 ? 2 : 1) - blocks;
     int turns = met;
     if (room > 0 && of_x.slices * turns > room) turns = room / of_x.slices > (met + 3) / 4 ? room / of_x.slices : (met + 3) / 4;
     bank_base_kernel<W, GW, S><<<of_x.slices * turns + blocks, W * 64, 0, stream>>>(a, of_x, of_x.slices * turns, turns);
 }
 template <int W, int GW>
-void launch_base(const FewArgs &a, const BankProjection &of_x, hipStream_t stream) {
+void launch_base(const FewArgs &a, const BankProjection &of_x, int cus, hipStream_t stream) {
     const int met = a.rows.count < a.rows.rows ? a.rows.count : a.rows.rows, tiles = a.N / kTileN;
     // a unit holds one block of eight wavefronts, or two of four
-    const int units = W == 4 ? kUnits : kUnits - of_x.slices * ((met + 1) / 2);
+    const int left = W == 4 ? cus : cus - of_x.slices * ((met + 1) / 2), units = left > 0 ? left : 1;
     int each = (tiles + units - 1) / units;
-    if (W == 8 && each >= 7 && (tiles + 6) / 7 + of_x.slices * ((met + 3) / 4) > kUnits) each = 4;  // several rounds: small ones
-    if (each <= 1) launch_base<W, GW, 1>(a, of_x, met, stream);
-    else if (each == 2) launch_base<W, GW, 2>(a, of_x, met, stream);
-    else if (each == 3) launch_base<W, GW, 3>(a, of_x, met, stream);
-    else if (each == 4) launch_base<W, GW, 4>(a, of_x, met, stream);
-    else if (each == 5) launch_base<W, GW, 5>(a, of_x, met, stream);
-    else if (each == 6) launch_base<W, GW, 6>(a, of_x, met, stream);
-    else launch_base<W, GW, 7>(a, of_x, met, stream);
+    if (W == 8 && each >= 7 && (tiles + 6) / 7 + of_x.slices * ((met + 3) / 4) > cus) each = 4;  // several rounds: small ones
+    if (each <= 1) launch_base<W, GW, 1>(a, of_x, met, cus, stream);
+    else if (each == 2) launch_base<W, GW, 2>(a, of_x, met, cus, stream);
+    else if (each == 3) launch_base<W, GW, 3>(a, of_x, met, cus, stream);
+    else if (each == 4) launch_base<W, GW, 4>(a, of_x, met, cus, stream);
+    else if (each == 5) launch_base<W, GW, 5>(a, of_x, met, cus, stream);
+    else if (each == 6) launch_base<W, GW, 6>(a, of_x, met, cus, stream);
+    else launch_base<W, GW, 7>(a, of_x, met, cus, stream);
 }
 
 }  // namespace
@@ -208,12 +208,12 @@ int bank_base_slices(int K) {  // one turn of a block's wavefronts each
     return bank_level_slices(groups, slices < kBankMaxSlices ? slices : kBankMaxSlices);
 }
 
-void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column,
+void bank_base(const void *x, const void *b, const void *s, void *y, const BankProjection &of_x, const BankRows &rows, int rank, int K, int N, bool per_column, int cus,
                hipStream_t stream) {
     const FewArgs a{(const uint16_t *)x, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, nullptr, nullptr, nullptr, rows, K, N, rank, per_column};
     with_few_rows_split(K / kGroupK, [&](auto waves, auto groups) {
         constexpr int W = decltype(waves)::value, GW = decltype(groups)::value;
-        launch_base<W, GW>(a, of_x, stream);
+        launch_base<W, GW>(a, of_x, cus, stream);
     });
 }
 

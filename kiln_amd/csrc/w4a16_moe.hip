@@ -13,6 +13,7 @@
 #include "device_common.h"
 #include "few_rows.h"
 #include "kiln_w4a16.h"
+#include "launch.h"
 
 namespace kiln {
 namespace {
@@ -241,17 +242,17 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(MoeArgs p) {
 // Column tiles to a block: many where the blocks are enough all the same (their rows and lists are read once each), where the experts present
 // are few as leave a block to every compute unit (two tokens of 8 experts, 2560 -> 1024 -> 2560: four 20.5 us, two 22.5; a token: 13.5, 13.8, one 15.9).
 template <bool IN, bool FEW, int W, int GW>
-void launch_expert(const MoeArgs &a, int slots, hipStream_t stream) {
+void launch_expert(const MoeArgs &a, int slots, int cus, hipStream_t stream) {
     constexpr int kMany = W == 4 ? 8 : 4;
     const int tiles = (IN ? 2 * a.n_out : a.n_down) / kTileN;
-    if (slots * (tiles / kMany) >= 512) moe_expert_kernel<IN, FEW, W, GW, kMany><<<dim3(tiles / kMany, slots), W * 64, 0, stream>>>(a);
-    else if (slots * (tiles / 4) >= 256) moe_expert_kernel<IN, FEW, W, GW, 4><<<dim3(tiles / 4, slots), W * 64, 0, stream>>>(a);
+    if (slots * (tiles / kMany) >= 2 * cus) moe_expert_kernel<IN, FEW, W, GW, kMany><<<dim3(tiles / kMany, slots), W * 64, 0, stream>>>(a);
+    else if (slots * (tiles / 4) >= cus) moe_expert_kernel<IN, FEW, W, GW, 4><<<dim3(tiles / 4, slots), W * 64, 0, stream>>>(a);
     else moe_expert_kernel<IN, FEW, W, GW, 2><<<dim3(tiles / 2, slots), W * 64, 0, stream>>>(a);
 }
 template <bool IN, bool FEW>
-void launch_experts(const MoeArgs &a, int slots, hipStream_t stream) {
+void launch_experts(const MoeArgs &a, int slots, int cus, hipStream_t stream) {
     with_few_rows_split((IN ? a.hidden : a.n_out) / kGroupK,
-                        [&](auto waves, auto groups) { launch_expert<IN, FEW, decltype(waves)::value, decltype(groups)::value>(a, slots, stream); });
+                        [&](auto waves, auto groups) { launch_expert<IN, FEW, decltype(waves)::value, decltype(groups)::value>(a, slots, cus, stream); });
 }
 
 // ---- the router's choice -------------------------------------------------------------------------------------------
@@ -362,7 +363,6 @@ size_t kiln_w4a16_moe_scratch_bytes(int prob_m, int top_k, int n_out, int n_down
 kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const float *weights, const void *b_gate_up, const void *s_gate_up,
                                     const void *b_down, const void *s_down, void *y, int prob_m, int top_k, int experts, int hidden, int n_out,
                                     int n_down, int groupsize, int dev, void *stream, void *scratch) {
-    (void)dev;
     if (prob_m < 0 || hidden <= 0 || n_out <= 0 || n_down <= 0 || hidden % 128 != 0 || n_out % 128 != 0 || n_down % 256 != 0 ||
         n_out > INT32_MAX / 2 || (groupsize != -1 && groupsize != 128))
         return KILN_W4A16_ERR_PROB_SHAPE;
@@ -373,6 +373,7 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
         if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
     if (meet(y, (size_t)prob_m * n_down * 2, x, (size_t)prob_m * hidden * 2)) return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    const int cus = compute_units(dev);
     for (int m0 = 0; m0 < prob_m; m0 += kMoeRun) {
         const int m = prob_m - m0 < kMoeRun ? prob_m - m0 : kMoeRun;
         const MoeArgs a{(const uint16_t *)x + (size_t)m0 * hidden, expert_of + (size_t)m0 * top_k, weights + (size_t)m0 * top_k,
@@ -381,8 +382,8 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
                         (uint16_t *)y + (size_t)m0 * n_down, m, top_k, experts, hidden, n_out, n_down, groupsize == -1};
         const int slots = m * top_k < experts ? m * top_k : experts;
         const bool few = m <= 64 / top_k;  // whole tokens in a wavefront's lanes
-        if (few) launch_experts<true, true>(a, slots, hs);
-        else launch_experts<true, false>(a, slots, hs);
+        if (few) launch_experts<true, true>(a, slots, cus, hs);
+        else launch_experts<true, false>(a, slots, cus, hs);
         if (few && m * top_k <= kMoeJoinedPairs) {
             const int G = n_out / kGroupK;
             if (G % 8 == 0) moe_join_kernel<8><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
@@ -391,8 +392,8 @@ kiln_marlin_status_t kiln_w4a16_moe(const void *x, const int *expert_of, const f
             else moe_join_kernel<4><<<n_down / 16, kJoinWaves * 64, 0, hs>>>(a);
             continue;
         }
-        if (few) launch_experts<false, true>(a, slots, hs);
-        else launch_experts<false, false>(a, slots, hs);
+        if (few) launch_experts<false, true>(a, slots, cus, hs);
+        else launch_experts<false, false>(a, slots, cus, hs);
         moe_sum_kernel<<<dim3((n_down / 4 + 255) / 256, m), 256, 0, hs>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
