@@ -10,7 +10,11 @@ namespace kiln {
 
 constexpr int kBankMaxRank = 64;
 constexpr int kBankRowTile = 16;
-constexpr int kBankOrderedFrom = 257;  // calls of fewer rows take them as they stand
+// Calls of fewer rows take them as they stand.  Rank 16, us a call as they stand / in order: 32 adapters, rows mixed, 128 / 256 / 300 / 400 rows
+// 2560 -> 18432 50.2 / 54.7, 72.1 / 61.2, 77.1 / 62.0, 98.3 / 71.9; 9216 -> 2560 33.9 / 45.6, 52.3 / 50.9, 57.5 / 53.4, 73.0 / 57.7; 5120 -> 5120
+// 32.9 / 44.7, 47.8 / 46.2, 52.8 / 49.1, 73.6 / 61.9; 2560 -> 2560 19.6 / 34.4, 25.4 / 33.6, 26.1 / 33.4, 36.0 / 37.9.  Four adapters, each one's
+// rows together, lose by order up to 400 rows of narrow outputs (5120 -> 5120 at 300 39.7 / 45.6) and gain beyond 300 on wide ones.
+constexpr int kBankOrderedFrom = 257;
 constexpr int kBankMaxSlices = 32;     // of the contraction of a projection
 
 // do [a, a + a_bytes) and [b, b + b_bytes) share memory?

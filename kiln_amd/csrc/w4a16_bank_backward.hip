@@ -118,6 +118,9 @@ __device__ __forceinline__ void unpack_weight(const PrepareArgs &p, int block, P
 // its instructions and their fetch (straight-line code is read from memory once in every launch): 45 rows of 4096 <- 2560 20 us with eight
 // tiles unrolled, 15 with four and codes from memory, 12 to 14 with a loop of one tile and everything through LDS.
 constexpr int kFewProjected = 8;  // slices of T's and U's contraction at most
+// (rows of a wavefront's ballot and of the tile of dy in LDS; beyond, W is unpacked for a product.  us a call at 64 rows straight from the codes / by that
+// product, four adapters of rank 16: 2560 <- 2560 16.8 / 42.1, 4096 <- 2560 21.5 / 44.5, 9216 <- 2560 28.5 / 56.0, 2560 <- 18432 36.8 / 80.0;
+// at 65 43.0, 46.7, 58.0 and 82)
 constexpr int kFewRows = 64;
 template <int RT>
 __device__ __forceinline__ void few_dx(const PrepareArgs &p, int block, FewLds &lds) {
