@@ -891,7 +891,7 @@ void plan_gemm(int m, int n, int k, int cus, int thread_k, int thread_n, int lor
 }
 
 // workspace of one call: counters | small-M partial tiles | LoRA projection             (small-M path)
-//                        counters | row-sum operands | partial tiles | LoRA projection (matrix-core path)
+//                        counters | partial tiles | row-sum operands | LoRA projection (matrix-core path)
 // (counters: the whole prefix that is zero between calls)
 // The LoRA projection's scratch comes last: a call without adapters needs `plain` bytes only.
 // What a launch writes and reads itself lies in there, row tile by row tile on whole lines (aext_rows), so everything behind the zeroed
@@ -905,15 +905,18 @@ char *behind_prefix(void *workspace, size_t off) {  // off >= kZeroedBytes
     const uintptr_t ws = reinterpret_cast<uintptr_t>(workspace);
     return reinterpret_cast<char *>((ws + kLineBytes - 1) / kLineBytes * kLineBytes + off);
 }
-WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k) {
+WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k, int cus) {
     WorkspaceLayout w{};
     size_t off = kZeroedBytes;
     if (gp.prefill) {
-        w.aext = off;
-        off += prefill_aext_bytes(m, k);
-        off = (off + 255) & ~(size_t)255;
         w.prefill_partial = off;
         off += prefill_partial_bytes(m, n, gp.pf);
+        off = (off + 255) & ~(size_t)255;
+        w.aext = off;
+        // (a plain call's row sums are m rows apart unless its own blocks write them)
+        const bool itself = !gp.sums_in_loop && prefill_rowsum_producers(m, n, k, gp.pf, cus) > 0;
+        w.plain = off + (itself ? prefill_aext_bytes(m, k) : (size_t)m * (k / kGroupK) * sizeof(u32x4));
+        off += prefill_aext_bytes(m, k);
     } else {
         w.decode_partial = off;
         if (gp.mid) {
@@ -922,8 +925,8 @@ WorkspaceLayout workspace_layout(const GemmPlan &gp, int m, int n, int k) {
         } else {
             off += gp.decode_partial;
         }
+        w.plain = off;
     }
-    w.plain = off;
     off = (off + 255) & ~(size_t)255;
     w.lora_t = off;
     off += prefill_lora_t_bytes(m, !gp.prefill);
@@ -943,7 +946,7 @@ std::shared_ptr<const PlannedCall> plan_call(int m, int n, int k, int cus, int t
     auto form = [&]() {
         auto pc = std::make_shared<PlannedCall>();
         plan_gemm(m, n, k, cus, thread_k, thread_n, lora, &pc->gp);
-        pc->wl = workspace_layout(pc->gp, m, n, k);
+        pc->wl = workspace_layout(pc->gp, m, n, k, cus);
         return pc;
     };
 #ifdef KILN_W4A16_TUNING_HOOKS
@@ -1070,7 +1073,7 @@ size_t workspace_bytes_upto(int m, int n, int k, int cus, int thread_k, int thre
         for (int lora = 0; lora < 3; ++lora) {  // a call with adapters may take another path
             GemmPlan gp;
             plan_gemm(mm, n, k, cus, thread_k, thread_n, lora, &gp);
-            const size_t need = workspace_layout(gp, mm, n, k).total;
+            const size_t need = workspace_layout(gp, mm, n, k, cus).total;
             if (need > most) most = need;
         }
     };

@@ -43,3 +43,18 @@ def test_same_bits_as_on_a_line(m, k, n, rank, off):
         assert torch.equal(call(x[i % 2], odd), want[i % 2]), i
     room, first = odd
     assert bool((room[:first] == 0xA5).all()) and bool((room[first + size:] == 0xA5).all())
+
+
+def test_the_static_array_takes_the_rows_that_fill_it():
+    L, m, k, n = _lib.load(), 6451, 5120, 5120
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    b = torch.randint(-2**31, 2**31, (k // 16, 2 * n), dtype=torch.int64, device="cuda", generator=gen).to(torch.int32)
+    s = ((torch.rand(k // 128, n, device="cuda", generator=gen) + 0.5) / (4.6 * k ** 0.5)).half()
+    x = torch.randn(m, k, device="cuda", generator=gen).bfloat16()
+    y, z = (torch.zeros(m, n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ws, stream = torch.zeros(L.kiln_w4a16_workspace_bytes(m, n, k), dtype=torch.uint8, device="cuda"), torch.cuda.current_stream().cuda_stream
+    assert L.kiln_marlin_w4a16_gemm(x.data_ptr(), b.data_ptr(), y.data_ptr(), s.data_ptr(), m, n, k, ws.data_ptr(), 128, 0, stream, -1, -1, -1, 16) == _lib.OK
+    for _ in range(2):
+        assert L.kiln_marlin_w4a16_gemm_static_scratch(x.data_ptr(), b.data_ptr(), z.data_ptr(), s.data_ptr(), m, n, k, 128, 0, stream) == _lib.OK
+    assert bool(y.any()) and torch.equal(y.view(torch.int16), z.view(torch.int16))
+    assert L.kiln_marlin_w4a16_gemm_static_scratch(x.data_ptr(), b.data_ptr(), z.data_ptr(), s.data_ptr(), m + 1, n, k, 128, 0, stream) == _lib.ERR_SCRATCH

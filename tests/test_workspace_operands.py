@@ -44,3 +44,21 @@ def test_the_query_refuses():
     out = (ctypes.c_size_t * 6)()
     for m, n, k in ((0, 256, 128), (1, 128, 128), (1, 256, 64), (1, 300, 128)):
         assert _lib.load().kiln_w4a16_debug_workspace_operands(m, n, k, 256, 0, 1 << 30, out) == 1
+
+
+@pytest.mark.parametrize("m", range(6445, 6454))
+def test_row_sums_of_a_launch_in_front_take_their_rows_alone(m):
+    """... which is what the static array has to hold: 6451 rows of 5120 -> 5120 fill it."""
+    L, out = _lib.load(), (ctypes.c_size_t * 6)()
+    assert L.kiln_w4a16_debug_prefill_rowsum_producers(m, 5120, 5120, 256) <= 0
+    assert L.kiln_w4a16_debug_workspace_operands(m, 5120, 5120, 256, 0, 1 << 30, out) == 0
+    assert (out[3] - (1 << 30) <= _lib.STATIC_SCRATCH_BYTES) == (m <= 6451)
+
+
+def test_plain_calls_need_no_more_than_their_row_sums_and_partial_tiles():
+    L, out = _lib.load(), (ctypes.c_size_t * 6)()
+    for m, n, k in SIZES + [(m, n, k) for m in range(257, 4200, 131) for n, k in ((2560, 9216), (5120, 5120), (18432, 2560))]:
+        assert L.kiln_w4a16_debug_workspace_operands(m, n, k, 256, 0, 1 << 30, out) == 0
+        if out[0]:
+            rows = -(-m // 8) * 8 if L.kiln_w4a16_debug_prefill_rowsum_producers(m, n, k, 256) > 0 else m
+            assert out[1] <= out[0] and out[3] == out[0] + rows * (k // 128) * 16, (m, n, k)
