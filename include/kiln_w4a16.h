@@ -303,7 +303,9 @@ typedef struct {
  *   dev         stream's device, whose compute units the launches are planned for (in the gradients and the router it is not used)
  * The low-rank term is summed in f32 (the projection kept to 2^-17 of itself).  For a row or two of narrow outputs, and from 257 rows on where
  * the product adds it itself (n >= k; kiln_w4a16_debug_bank_plan 0 and 3), it lands on the f32 sums of the product, rounded once;
- * otherwise on the product's bf16 value, which is rounded once more, as the reference adds a delta to its bf16 base.  C shares no memory with A or the bank (refused, as are the gradients below that share it with what they are made of).
+ * otherwise on the product's bf16 value, which is rounded once more, as the reference adds a delta to its bf16 base.  The projection is
+ * multiplied in two bf16 parts: an infinity in a row's own adapter reaches its values as one or as NaN, and no other row's.
+ * C shares no memory with A or the bank (refused, as are the gradients below that share it with what they are made of).
  */
 size_t kiln_w4a16_gemm_bank_scratch_bytes(int prob_m, int prob_n, int prob_k, int count, int rank);
 kiln_marlin_status_t kiln_w4a16_gemm_bank(
