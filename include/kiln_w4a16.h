@@ -360,6 +360,80 @@ kiln_marlin_status_t kiln_w4a16_moe_route(
     int *expert_of, float *weights, int dev, void *stream);
 
 /*
+ * The choices of a router in the order of their experts, for the products of many rows below.  Pair p = i * top_k + j is row i's
+ * choice j, expert_of[i, j]; an id outside [0, experts) is no expert (one held elsewhere).
+ *   order   int32 [m * top_k]   the pairs by expert, in their order inside one, those without an expert last
+ *   place   int32 [m, top_k]    its inverse: a pair's position
+ *   first   int32 [experts + 1] expert e has the positions first[e] ... first[e + 1]; from first[experts] on there is no expert
+ * All in device memory.  Deterministic.  scratch: kiln_w4a16_moe_sort_scratch_bytes, on 4 bytes, holds nothing between calls.  m == 0 writes
+ * `first` alone.  experts 1 ... 1024, top_k 1 ... 16, m * top_k <= 2^30.  No counterpart in the reference, whose model family is dense.
+ */
+size_t kiln_w4a16_moe_sort_scratch_bytes(int experts);
+kiln_marlin_status_t kiln_w4a16_moe_sort(
+    const int *expert_of, int prob_m, int top_k, int experts,
+    int *order, int *first, int *place, int dev, void *stream, void *scratch);
+
+/*
+ * Rows of tokens in that order, and back.  first and place from kiln_w4a16_moe_sort; width % 8 == 0; bf16 rows on 16 bytes; results share no
+ * memory with operands (refused).  A pair without an expert is a row of zeros where rows are written, and is not read.
+ *   gather            rows[place[i, j]] = x[i]                              x bf16 [m, width], rows bf16 [m * top_k, width]
+ *   combine           y[i] = sum_j weights[i, j] * rows[place[i, j]]        weights f32 [m, top_k] or NULL (ones: gather's gradient); summed in f32
+ *                                                                           in the order of j, rounded once; y bf16 [m, width]
+ *   combine_backward  d_rows[place[i, j]] = weights[i, j] * dy[i]           bf16 [m * top_k, width], rounded once
+ *                     d_weights[i, j] = <rows[place[i, j]], dy[i]>          f32 [m, top_k], summed in f32; 0 without an expert
+ * (Positions in `place` outside [0, m * top_k) are passed over.)
+ */
+kiln_marlin_status_t kiln_w4a16_moe_gather(
+    const void *x, const int *first, const int *place, void *rows,
+    int prob_m, int top_k, int experts, int width, int dev, void *stream);
+kiln_marlin_status_t kiln_w4a16_moe_combine(
+    const void *rows, const float *weights, const int *first, const int *place, void *y,
+    int prob_m, int top_k, int experts, int width, int dev, void *stream);
+kiln_marlin_status_t kiln_w4a16_moe_combine_backward(
+    const void *dy, const void *rows, const float *weights, const int *first, const int *place, void *d_rows, float *d_weights,
+    int prob_m, int top_k, int experts, int width, int dev, void *stream);
+
+/*
+ * y[p] = x[p] * dequant(B_e, s_e) for first[e] <= p < first[e + 1]: rows in the order of their experts times their expert's pack, all
+ * experts in one call.
+ *   x      bf16 [x_rows, k]: x_rows == rows; or with `order` (kiln_w4a16_moe_sort's) the tokens, and position p takes row order[p] / top_k of
+ *          them: x_rows * top_k == rows (top_k is not used without `order`)
+ *   first  int32 [experts + 1], device memory, from 0 on and not falling; rows behind first[experts] are zeros in y
+ *   B, s   [experts] packs [k, n], one after the other
+ *   y      bf16 [rows, n], rounded once; with `swiglu` bf16 [rows, n / 2] = silu(gate) * up of packs as for kiln_w4a16_gemm_swiglu; shares no
+ *          memory with x (refused)
+ *   scratch  kiln_w4a16_gemm_experts_scratch_bytes(x_rows, k), on 16 bytes, holds nothing between calls
+ * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024.
+ * The gradient of the rows, the packs frozen: dx[p] = dy[p] * dequant(B_e, s_e)^T, bf16 [rows, k], rounded once; a weight enters the product
+ * rounded to bf16, as in kiln_w4a16_gemm_bank_backward.
+ */
+size_t kiln_w4a16_gemm_experts_scratch_bytes(int x_rows, int prob_k);
+kiln_marlin_status_t kiln_w4a16_gemm_experts(
+    const void *x, const int *first, const int *order, const void *B, const void *s, void *y, int rows, int x_rows, int top_k,
+    int prob_n, int prob_k, int experts, int groupsize, int swiglu, int dev, void *stream, void *scratch);
+kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(
+    const void *dy, const int *first, const void *B, const void *s, void *dx, int rows,
+    int prob_n, int prob_k, int experts, int groupsize, int dev, void *stream);
+
+/*
+ * silu(gate) * up in training (crates/kiln-model/src/forward.rs:2771-2819 is the forward), with gate and up kept in 8 bits for the backward pass.
+ *   gate_up    bf16 [m, 2 * n_out], 8 gate columns and the 8 matching up columns in turn: what the plain GEMM or kiln_w4a16_gemm_experts
+ *              gives on a pack of kiln_w4a16_interleave_gate_up
+ *   h          bf16 [m, n_out] = silu(gate) * up
+ *   whole      int8 [m, 2 * n_out], the same columns;  exponents  uint8 [m, n_out / 32, 2], gate's and up's:
+ *              value = whole * 2^(exponent - 133).  32 gate values, or 32 up values, share an exponent, the bf16 exponent field of the largest
+ *              magnitude (at least 1); whole is rounded to the nearest, ties to even, at most 127 in magnitude.  A block with an infinity or
+ *              NaN has exponent 255 and is NaN.
+ * The backward pass out of them: with s = 1 / (1 + exp(-gate)), d_up = dh * gate * s and d_gate = dh * up * s * (1 + gate * (1 - s)), bf16 in
+ * gate_up's columns, rounded once; h again unless NULL (of the kept values).  n_out % 128 == 0; all on 16 bytes; no result shares memory with
+ * an operand or another result (refused).
+ */
+kiln_marlin_status_t kiln_w4a16_swiglu_keep(
+    const void *gate_up, void *h, void *whole, void *exponents, int prob_m, int n_out, int dev, void *stream);
+kiln_marlin_status_t kiln_w4a16_swiglu_keep_backward(
+    const void *dh, const void *whole, const void *exponents, void *d_gate_up, void *h, int prob_m, int n_out, int dev, void *stream);
+
+/*
  * out[k, n] (f32, row-major) = (code - 8) * f32(scale), read from the tile
  * layout on the device.  The device-side statement of lib.rs:425; used to
  * prove the repack bit-exact.  No counterpart entry point in the reference.

@@ -1,6 +1,7 @@
 """The extension that calls the library without ctypes (`kiln_amd/lib/_torch_calls.so`, built from
 csrc/torch/torch_calls.cpp): `linear`, `linear_lora`, `linear_sides`, `mlp`, `quantize`, `repack`, `gemm_bank`, `gemm_bank_backward`, `moe`,
-`moe_route`.  Each takes the plain case -- contiguous CUDA
+`moe_route`, `moe_sort`, `moe_gather`, `moe_combine`, `moe_combine_backward`, `gemm_experts`, `gemm_experts_backward`, `swiglu_keep`,
+`swiglu_keep_backward`.  Each takes the plain case -- contiguous CUDA
 tensors of the right types, a workspace that is already there -- and returns None for anything else, upon
 which the wrappers here take their checked route (same kernels, the reference's error texts).
 
@@ -23,7 +24,10 @@ _FUNCTIONS = ("kiln_marlin_w4a16_gemm", "kiln_w4a16_gemm_lora", "kiln_w4a16_gemm
               "kiln_w4a16_quantize_and_pack_many_device", "kiln_w4a16_takes_adapter_sides", "kiln_w4a16_gemm_adapter_sides",
               "kiln_w4a16_repack_gptq_device", "kiln_w4a16_takes_rank", "kiln_w4a16_gemm_bank", "kiln_w4a16_gemm_bank_scratch_bytes",
               "kiln_w4a16_gemm_bank_backward", "kiln_w4a16_gemm_bank_backward_scratch_bytes", "kiln_w4a16_moe",
-              "kiln_w4a16_moe_scratch_bytes", "kiln_w4a16_moe_route")
+              "kiln_w4a16_moe_scratch_bytes", "kiln_w4a16_moe_route", "kiln_w4a16_moe_sort", "kiln_w4a16_moe_sort_scratch_bytes",
+              "kiln_w4a16_moe_gather", "kiln_w4a16_moe_combine", "kiln_w4a16_moe_combine_backward", "kiln_w4a16_gemm_experts",
+              "kiln_w4a16_gemm_experts_scratch_bytes", "kiln_w4a16_gemm_experts_backward", "kiln_w4a16_swiglu_keep",
+              "kiln_w4a16_swiglu_keep_backward")
 
 
 _ext = None
@@ -79,5 +83,9 @@ def _stand_in(name: str):
     return first_call
 
 
-_NAMES = ("linear", "linear_lora", "linear_sides", "mlp", "quantize", "repack", "gemm_bank", "gemm_bank_backward", "moe", "moe_route")
-linear, linear_lora, linear_sides, mlp, quantize, repack, gemm_bank, gemm_bank_backward, moe, moe_route = map(_stand_in, _NAMES)
+_NAMES = ("linear", "linear_lora", "linear_sides", "mlp", "quantize", "repack", "gemm_bank", "gemm_bank_backward", "moe", "moe_route",
+          "moe_sort", "moe_gather", "moe_combine", "moe_combine_backward", "gemm_experts", "gemm_experts_backward", "swiglu_keep",
+          "swiglu_keep_backward")
+linear, linear_lora, linear_sides, mlp, quantize, repack, gemm_bank, gemm_bank_backward, moe, moe_route = map(_stand_in, _NAMES[:10])
+(moe_sort, moe_gather, moe_combine, moe_combine_backward, gemm_experts, gemm_experts_backward, swiglu_keep,
+ swiglu_keep_backward) = map(_stand_in, _NAMES[10:])

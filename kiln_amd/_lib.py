@@ -37,6 +37,16 @@ EXPORTS = (
     "kiln_w4a16_moe_scratch_bytes",
     "kiln_w4a16_moe",
     "kiln_w4a16_moe_route",
+    "kiln_w4a16_moe_sort_scratch_bytes",
+    "kiln_w4a16_moe_sort",
+    "kiln_w4a16_moe_gather",
+    "kiln_w4a16_moe_combine",
+    "kiln_w4a16_moe_combine_backward",
+    "kiln_w4a16_gemm_experts_scratch_bytes",
+    "kiln_w4a16_gemm_experts",
+    "kiln_w4a16_gemm_experts_backward",
+    "kiln_w4a16_swiglu_keep",
+    "kiln_w4a16_swiglu_keep_backward",
     "kiln_w4a16_quantize_and_pack_device",
     "kiln_w4a16_quantize_and_pack_many_device",
     "kiln_w4a16_interleave_gate_up_device",
@@ -251,6 +261,26 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_moe.argtypes = [vp] * 8 + [i] * 8 + [vp, vp]
     L.kiln_w4a16_moe_route.restype = i
     L.kiln_w4a16_moe_route.argtypes = [vp, i, i, i, i, i, vp, vp, i, vp]
+    L.kiln_w4a16_moe_sort_scratch_bytes.restype = c.c_size_t
+    L.kiln_w4a16_moe_sort_scratch_bytes.argtypes = [i]
+    L.kiln_w4a16_moe_sort.restype = i
+    L.kiln_w4a16_moe_sort.argtypes = [vp, i, i, i, vp, vp, vp, i, vp, vp]
+    L.kiln_w4a16_moe_gather.restype = i
+    L.kiln_w4a16_moe_gather.argtypes = [vp] * 4 + [i] * 5 + [vp]
+    L.kiln_w4a16_moe_combine.restype = i
+    L.kiln_w4a16_moe_combine.argtypes = [vp] * 5 + [i] * 5 + [vp]
+    L.kiln_w4a16_moe_combine_backward.restype = i
+    L.kiln_w4a16_moe_combine_backward.argtypes = [vp] * 7 + [i] * 5 + [vp]
+    L.kiln_w4a16_gemm_experts_scratch_bytes.restype = c.c_size_t
+    L.kiln_w4a16_gemm_experts_scratch_bytes.argtypes = [i, i]
+    L.kiln_w4a16_gemm_experts.restype = i
+    L.kiln_w4a16_gemm_experts.argtypes = [vp] * 6 + [i] * 9 + [vp, vp]
+    L.kiln_w4a16_gemm_experts_backward.restype = i
+    L.kiln_w4a16_gemm_experts_backward.argtypes = [vp] * 5 + [i] * 6 + [vp]
+    L.kiln_w4a16_swiglu_keep.restype = i
+    L.kiln_w4a16_swiglu_keep.argtypes = [vp] * 4 + [i] * 3 + [vp]
+    L.kiln_w4a16_swiglu_keep_backward.restype = i
+    L.kiln_w4a16_swiglu_keep_backward.argtypes = [vp] * 5 + [i] * 3 + [vp]
     L.kiln_w4a16_stack_adapters.restype = i
     L.kiln_w4a16_stack_adapters.argtypes = [c.POINTER(vp), c.POINTER(vp), c.POINTER(i), c.POINTER(i), c.POINTER(i), i, i, i, i, i,
                                             vp, vp, vp]

@@ -49,6 +49,16 @@ struct Library {
     decltype(&kiln_w4a16_moe) moe = nullptr;
     decltype(&kiln_w4a16_moe_scratch_bytes) moe_scratch_bytes = nullptr;
     decltype(&kiln_w4a16_moe_route) moe_route = nullptr;
+    decltype(&kiln_w4a16_moe_sort) moe_sort = nullptr;
+    decltype(&kiln_w4a16_moe_sort_scratch_bytes) moe_sort_scratch_bytes = nullptr;
+    decltype(&kiln_w4a16_moe_gather) moe_gather = nullptr;
+    decltype(&kiln_w4a16_moe_combine) moe_combine = nullptr;
+    decltype(&kiln_w4a16_moe_combine_backward) moe_combine_backward = nullptr;
+    decltype(&kiln_w4a16_gemm_experts) experts = nullptr;
+    decltype(&kiln_w4a16_gemm_experts_scratch_bytes) experts_scratch_bytes = nullptr;
+    decltype(&kiln_w4a16_gemm_experts_backward) experts_backward = nullptr;
+    decltype(&kiln_w4a16_swiglu_keep) swiglu_keep = nullptr;
+    decltype(&kiln_w4a16_swiglu_keep_backward) swiglu_keep_backward = nullptr;
 };
 Library g_lib;  // written by bind() under the interpreter lock, like everything below
 
@@ -821,6 +831,265 @@ PyObject *py_moe_route(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// the tensors as a tuple, or null with an error
+template <size_t N>
+PyObject *tuple_of(std::array<at::Tensor, N> &&tensors) {
+    PyObject *all = PyTuple_New((Py_ssize_t)N);
+    for (size_t i = 0; all && i < N; ++i) {
+        PyObject *part = THPVariable_Wrap(std::move(tensors[i]));
+        if (!part) {
+            Py_DECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, (Py_ssize_t)i, part);
+    }
+    return all;
+}
+// a positive count that fits an int
+bool count_of(PyObject *o, int64_t most, int *count) {
+    if (!PyLong_CheckExact(o)) return false;
+    const long v = PyLong_AsLong(o);
+    if (v == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (v < 1 || v > most) return false;
+    *count = (int)v;
+    return true;
+}
+constexpr int64_t kMostPairs = 1 << 30;
+// tensors in place of the first N arguments, the first on CUDA
+template <size_t N>
+bool tensors_of(PyObject *const *args, std::array<const at::Tensor *, N> *t) {
+    for (size_t i = 0; i < N; ++i)
+        if (!((*t)[i] = tensor_of(args[i]))) return false;
+    return (*t)[0]->is_cuda();
+}
+// first and place of moe_sort
+struct Sorted {
+    const int *first = nullptr, *place = nullptr;
+    int m = 0, top = 0, experts = 0;
+};
+bool sorted_of(const at::Tensor &first, const at::Tensor &place, c10::Device device, Sorted *s) {
+    if (!plain(first, at::kInt, 1, device) || !plain(place, at::kInt, 2, device)) return false;
+    const int64_t m = place.size(0), top = place.size(1), experts = first.size(0) - 1;
+    if (m < 1 || top < 1 || top > 16 || m * top > kMostPairs || experts < 1 || experts > 1024) return false;
+    *s = {static_cast<const int *>(first.data_ptr()), static_cast<const int *>(place.data_ptr()), (int)m, (int)top, (int)experts};
+    return true;
+}
+bool rows_of(const at::Tensor &rows, int64_t count, c10::Device device) {
+    return plain(rows, at::kBFloat16, 2, device) && rows.size(0) == count && rows.size(1) >= 8 && rows.size(1) % 8 == 0 && rows.size(1) <= INT32_MAX;
+}
+// `given` if it is a result of the right form (false: it is of another), else a new tensor
+bool rows_output(PyObject *given, int64_t rows, int64_t width, c10::Device device, at::Tensor *out) {
+    if (given == Py_None) {
+        *out = empty_bf16({rows, width}, device);
+        return true;
+    }
+    const at::Tensor *t = tensor_of(given);
+    if (!t || !plain(*t, at::kBFloat16, 2, device) || t->size(0) != rows || t->size(1) != width) return false;
+    *out = *t;
+    return true;
+}
+
+// moe_sort(expert_of, experts) -> (order, first, place)
+PyObject *py_moe_sort(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 1> t;
+    int experts;
+    if (nargs != 2 || !g_lib.moe_sort || !tensors_of(args, &t) || !count_of(args[1], 1024, &experts)) Py_RETURN_NONE;
+    const at::Tensor &of = *t[0];
+    const c10::Device device = of.device();
+    if (!plain(of, at::kInt, 2, device)) Py_RETURN_NONE;
+    const int64_t m = of.size(0), top = of.size(1);
+    if (m < 1 || top < 1 || top > 16 || m * top > kMostPairs) Py_RETURN_NONE;
+    Launch at_(device);
+    at::Tensor order = empty_of({m * top}, at::kInt, device), first = empty_of({experts + 1}, at::kInt, device), place = empty_of({m, top}, at::kInt, device);
+    const at::Tensor scratch = empty_of({(int64_t)g_lib.moe_sort_scratch_bytes(experts)}, at::kByte, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe_sort(static_cast<const int *>(of.data_ptr()), (int)m, (int)top, experts, static_cast<int *>(order.data_ptr()),
+                        static_cast<int *>(first.data_ptr()), static_cast<int *>(place.data_ptr()), device.index(), at_.stream, scratch.data_ptr());
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return tuple_of<3>({std::move(order), std::move(first), std::move(place)});
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_gather(x, first, place, out)
+PyObject *py_moe_gather(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 3> t;
+    if (nargs != 4 || !g_lib.moe_gather || !tensors_of(args, &t)) Py_RETURN_NONE;
+    const c10::Device device = t[0]->device();
+    Sorted s;
+    if (!sorted_of(*t[1], *t[2], device, &s) || !rows_of(*t[0], s.m, device)) Py_RETURN_NONE;
+    const int64_t width = t[0]->size(1);
+    Launch at_(device);
+    at::Tensor out;
+    if (!rows_output(args[3], (int64_t)s.m * s.top, width, device, &out)) Py_RETURN_NONE;
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe_gather(t[0]->data_ptr(), s.first, s.place, out.data_ptr(), s.m, s.top, s.experts, (int)width, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+bool weights_of(const at::Tensor &weights, const Sorted &s, c10::Device device) {
+    return plain(weights, at::kFloat, 2, device) && weights.size(0) == s.m && weights.size(1) == s.top;
+}
+
+// moe_combine(rows, weights or None, first, place, out)
+PyObject *py_moe_combine(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 5 || !g_lib.moe_combine) Py_RETURN_NONE;
+    const at::Tensor *rows = tensor_of(args[0]), *weights = tensor_of(args[1]), *first = tensor_of(args[2]), *place = tensor_of(args[3]);
+    if (!rows || !rows->is_cuda() || !first || !place || (!weights && args[1] != Py_None)) Py_RETURN_NONE;
+    const c10::Device device = rows->device();
+    Sorted s;
+    if (!sorted_of(*first, *place, device, &s) || !rows_of(*rows, (int64_t)s.m * s.top, device) || (weights && !weights_of(*weights, s, device)))
+        Py_RETURN_NONE;
+    const int64_t width = rows->size(1);
+    Launch at_(device);
+    at::Tensor out;
+    if (!rows_output(args[4], s.m, width, device, &out)) Py_RETURN_NONE;
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe_combine(rows->data_ptr(), weights ? static_cast<const float *>(weights->data_ptr()) : nullptr, s.first, s.place, out.data_ptr(), s.m,
+                           s.top, s.experts, (int)width, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_combine_backward(dy, rows, weights, first, place) -> (d_rows, d_weights)
+PyObject *py_moe_combine_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 5> t;
+    if (nargs != 5 || !g_lib.moe_combine_backward || !tensors_of(args, &t)) Py_RETURN_NONE;
+    const c10::Device device = t[0]->device();
+    Sorted s;
+    if (!sorted_of(*t[3], *t[4], device, &s) || !rows_of(*t[0], s.m, device) || !rows_of(*t[1], (int64_t)s.m * s.top, device) ||
+        t[0]->size(1) != t[1]->size(1) || !weights_of(*t[2], s, device))
+        Py_RETURN_NONE;
+    const int64_t width = t[0]->size(1);
+    Launch at_(device);
+    at::Tensor d_rows = empty_bf16({(int64_t)s.m * s.top, width}, device), d_weights = empty_of({s.m, s.top}, at::kFloat, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.moe_combine_backward(t[0]->data_ptr(), t[1]->data_ptr(), static_cast<const float *>(t[2]->data_ptr()), s.first, s.place, d_rows.data_ptr(),
+                                    static_cast<float *>(d_weights.data_ptr()), s.m, s.top, s.experts, (int)width, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return tuple_of<2>({std::move(d_rows), std::move(d_weights)});
+    END_HANDLE_TH_ERRORS
+}
+
+// packs [experts, k/16, 2n] and [experts, k/g, n], first [experts + 1]
+bool expert_packs_ok(const at::Tensor &first, const at::Tensor &b, const at::Tensor &s, int g, c10::Device device) {
+    if (!plain(first, at::kInt, 1, device) || !plain(b, at::kInt, 3, device) || !plain(s, at::kHalf, 3, device)) return false;
+    const int64_t experts = b.size(0), k = b.size(1) * 16, n = s.size(2);
+    return experts >= 1 && experts <= 1024 && first.size(0) == experts + 1 && s.size(0) == experts && k >= 128 && k % 128 == 0 && k <= INT32_MAX &&
+           n >= 256 && n % 256 == 0 && n <= INT32_MAX / 2 && b.size(2) == 2 * n && s.size(1) == (g == -1 ? 1 : k / 128);
+}
+
+// gemm_experts(x, first, b, s, groupsize, order or None, top_k, swiglu, out)
+PyObject *py_gemm_experts(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 4> t;
+    int g, top = 1;
+    if (nargs != 9 || !g_lib.experts || !tensors_of(args, &t) || !groupsize_of(args[4], &g) || !PyBool_Check(args[7])) Py_RETURN_NONE;
+    const at::Tensor *order = tensor_of(args[5]);
+    const c10::Device device = t[0]->device();
+    if ((!order && args[5] != Py_None) || (order && !count_of(args[6], INT32_MAX, &top)) || !plain(*t[0], at::kBFloat16, 2, device) ||
+        !expert_packs_ok(*t[1], *t[2], *t[3], g, device))
+        Py_RETURN_NONE;
+    const int64_t x_rows = t[0]->size(0), rows = x_rows * top, k = t[2]->size(1) * 16, n = t[3]->size(2);
+    if (x_rows < 1 || rows > INT32_MAX || t[0]->size(1) != k || (order && (!plain(*order, at::kInt, 1, device) || order->size(0) != rows))) Py_RETURN_NONE;
+    const bool swiglu = args[7] == Py_True;
+    Launch at_(device);
+    at::Tensor out;
+    if (!rows_output(args[8], rows, swiglu ? n / 2 : n, device, &out)) Py_RETURN_NONE;
+    const at::Tensor scratch = empty_of({(int64_t)g_lib.experts_scratch_bytes((int)x_rows, (int)k)}, at::kByte, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.experts(t[0]->data_ptr(), static_cast<const int *>(t[1]->data_ptr()), order ? static_cast<const int *>(order->data_ptr()) : nullptr,
+                       t[2]->data_ptr(), t[3]->data_ptr(), out.data_ptr(), (int)rows, (int)x_rows, top, (int)n, (int)k, (int)t[2]->size(0), g, swiglu,
+                       device.index(), at_.stream, scratch.data_ptr());
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// gemm_experts_backward(dy, first, b, s, groupsize)
+PyObject *py_gemm_experts_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 4> t;
+    int g;
+    if (nargs != 5 || !g_lib.experts_backward || !tensors_of(args, &t) || !groupsize_of(args[4], &g)) Py_RETURN_NONE;
+    const c10::Device device = t[0]->device();
+    if (!plain(*t[0], at::kBFloat16, 2, device) || !expert_packs_ok(*t[1], *t[2], *t[3], g, device)) Py_RETURN_NONE;
+    const int64_t rows = t[0]->size(0), k = t[2]->size(1) * 16, n = t[3]->size(2);
+    if (rows < 1 || rows > INT32_MAX || t[0]->size(1) != n) Py_RETURN_NONE;
+    Launch at_(device);
+    at::Tensor out = empty_bf16({rows, k}, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.experts_backward(t[0]->data_ptr(), static_cast<const int *>(t[1]->data_ptr()), t[2]->data_ptr(), t[3]->data_ptr(), out.data_ptr(), (int)rows,
+                                (int)n, (int)k, (int)t[2]->size(0), g, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// swiglu_keep(gate_up) -> (h, whole, exponents)
+PyObject *py_swiglu_keep(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 1> t;
+    if (nargs != 1 || !g_lib.swiglu_keep || !tensors_of(args, &t)) Py_RETURN_NONE;
+    const c10::Device device = t[0]->device();
+    if (!plain(*t[0], at::kBFloat16, 2, device)) Py_RETURN_NONE;
+    const int64_t m = t[0]->size(0), n = t[0]->size(1) / 2;
+    if (m < 1 || m > INT32_MAX || n < 128 || n > INT32_MAX / 2 || t[0]->size(1) % 256) Py_RETURN_NONE;
+    Launch at_(device);
+    at::Tensor h = empty_bf16({m, n}, device), whole = empty_of({m, 2 * n}, at::kChar, device), exponents = empty_of({m, n / 32, 2}, at::kByte, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.swiglu_keep(t[0]->data_ptr(), h.data_ptr(), whole.data_ptr(), exponents.data_ptr(), (int)m, (int)n, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    return tuple_of<3>({std::move(h), std::move(whole), std::move(exponents)});
+    END_HANDLE_TH_ERRORS
+}
+
+// swiglu_keep_backward(dh, whole, exponents, recompute) -> d_gate_up or (d_gate_up, h)
+PyObject *py_swiglu_keep_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    std::array<const at::Tensor *, 3> t;
+    if (nargs != 4 || !g_lib.swiglu_keep_backward || !tensors_of(args, &t) || !PyBool_Check(args[3])) Py_RETURN_NONE;
+    const c10::Device device = t[0]->device();
+    if (!plain(*t[0], at::kBFloat16, 2, device) || !plain(*t[1], at::kChar, 2, device) || !plain(*t[2], at::kByte, 3, device)) Py_RETURN_NONE;
+    const int64_t m = t[0]->size(0), n = t[0]->size(1);
+    if (m < 1 || m > INT32_MAX || n < 128 || n > INT32_MAX / 2 || n % 128 || t[1]->sizes() != at::IntArrayRef({m, 2 * n}) ||
+        t[2]->sizes() != at::IntArrayRef({m, n / 32, 2}))
+        Py_RETURN_NONE;
+    const bool recompute = args[3] == Py_True;
+    Launch at_(device);
+    at::Tensor d_gate_up = empty_bf16({m, 2 * n}, device), h;
+    if (recompute) h = empty_bf16({m, n}, device);
+    int st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_lib.swiglu_keep_backward(t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), d_gate_up.data_ptr(), recompute ? h.data_ptr() : nullptr, (int)m,
+                                    (int)n, device.index(), at_.stream);
+    Py_END_ALLOW_THREADS
+    if (st != KILN_W4A16_OK) Py_RETURN_NONE;
+    if (!recompute) return THPVariable_Wrap(std::move(d_gate_up));
+    return tuple_of<2>({std::move(d_gate_up), std::move(h)});
+    END_HANDLE_TH_ERRORS
+}
+
 // set_workspaces(marlin_gemm's dictionary of them)
 PyObject *py_set_workspaces(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (nargs != 1 || !PyDict_CheckExact(args[0])) {
@@ -835,12 +1104,12 @@ PyObject *py_set_workspaces(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 
 // bind(addresses of the library's functions, in the order of Library)
 PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    if (nargs != 20) {
-        PyErr_SetString(PyExc_TypeError, "bind takes twenty function addresses");
+    if (nargs != 30) {
+        PyErr_SetString(PyExc_TypeError, "bind takes thirty function addresses");
         return nullptr;
     }
-    void *p[20];
-    for (int i = 0; i < 20; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+    void *p[30];
+    for (int i = 0; i < 30; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
     g_lib.gemm = reinterpret_cast<decltype(g_lib.gemm)>(p[0]);
     g_lib.gemm_lora = reinterpret_cast<decltype(g_lib.gemm_lora)>(p[1]);
@@ -862,6 +1131,16 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     g_lib.moe = reinterpret_cast<decltype(g_lib.moe)>(p[17]);
     g_lib.moe_scratch_bytes = reinterpret_cast<decltype(g_lib.moe_scratch_bytes)>(p[18]);
     g_lib.moe_route = reinterpret_cast<decltype(g_lib.moe_route)>(p[19]);
+    g_lib.moe_sort = reinterpret_cast<decltype(g_lib.moe_sort)>(p[20]);
+    g_lib.moe_sort_scratch_bytes = reinterpret_cast<decltype(g_lib.moe_sort_scratch_bytes)>(p[21]);
+    g_lib.moe_gather = reinterpret_cast<decltype(g_lib.moe_gather)>(p[22]);
+    g_lib.moe_combine = reinterpret_cast<decltype(g_lib.moe_combine)>(p[23]);
+    g_lib.moe_combine_backward = reinterpret_cast<decltype(g_lib.moe_combine_backward)>(p[24]);
+    g_lib.experts = reinterpret_cast<decltype(g_lib.experts)>(p[25]);
+    g_lib.experts_scratch_bytes = reinterpret_cast<decltype(g_lib.experts_scratch_bytes)>(p[26]);
+    g_lib.experts_backward = reinterpret_cast<decltype(g_lib.experts_backward)>(p[27]);
+    g_lib.swiglu_keep = reinterpret_cast<decltype(g_lib.swiglu_keep)>(p[28]);
+    g_lib.swiglu_keep_backward = reinterpret_cast<decltype(g_lib.swiglu_keep_backward)>(p[29]);
     Py_RETURN_NONE;
 }
 
@@ -882,7 +1161,11 @@ PyObject *py_set_adapter_types(PyObject *, PyObject *const *args, Py_ssize_t nar
 PyMethodDef g_methods[] = {FAST("linear", py_linear), FAST("linear_lora", py_linear_lora), FAST("linear_sides", py_linear_sides),
                            FAST("mlp", py_mlp), FAST("quantize", py_quantize), FAST("repack", py_repack),
                            FAST("gemm_bank", py_gemm_bank), FAST("gemm_bank_backward", py_gemm_bank_backward), FAST("moe", py_moe),
-                           FAST("moe_route", py_moe_route), FAST("set_workspaces", py_set_workspaces), FAST("bind", py_bind),
+                           FAST("moe_route", py_moe_route), FAST("moe_sort", py_moe_sort), FAST("moe_gather", py_moe_gather),
+                           FAST("moe_combine", py_moe_combine), FAST("moe_combine_backward", py_moe_combine_backward),
+                           FAST("gemm_experts", py_gemm_experts), FAST("gemm_experts_backward", py_gemm_experts_backward),
+                           FAST("swiglu_keep", py_swiglu_keep), FAST("swiglu_keep_backward", py_swiglu_keep_backward),
+                           FAST("set_workspaces", py_set_workspaces), FAST("bind", py_bind),
                            FAST("set_adapter_types", py_set_adapter_types), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

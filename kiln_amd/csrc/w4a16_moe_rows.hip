@@ -1,0 +1,339 @@
+// A router's choices in the order of their experts, the tokens' rows in that order and back: what stands around products with experts
+// for many tokens (w4a16_experts.hip), and the gradients.
+//   sort              order = the pairs (token, choice) by expert, in their order inside one; place its inverse; first[e] where e begins
+//   gather            rows[place[t, j]] = x[t]                          its gradient: a combine with weights of one
+//   combine           y[t] = sum_j w[t, j] rows[place[t, j]]
+//   combine backward  d_rows[place[t, j]] = w[t, j] dy[t],  d_w[t, j] = <rows[place[t, j]], dy[t]>
+// Pairs without an expert come last, from position first[experts] on: rows of zeros where rows are written, never read.
+// No counterpart in the reference, whose model family is dense.  All but the sort are bound by the rows, read and written once.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "bank.h"
+#include "device_common.h"
+#include "kiln_w4a16.h"
+#include "launch.h"
+
+namespace kiln {
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxTop = 16;
+constexpr int64_t kMaxPairs = 1 << 30;
+
+// ---- the sort ------------------------------------------------------------------------------------------------------
+// By counting: pairs go to blocks and their wavefronts in contiguous parts; a pair's position is where its expert begins, plus the expert's
+// pairs in earlier blocks, earlier wavefronts and earlier turns of its own, plus those in lower lanes.  Nothing depends on who comes
+// first.  Several blocks need their counts from a launch in front; one block's pairs are counted where they are placed.
+constexpr int kSortWaves = 8, kSortThreads = kSortWaves * 64;
+constexpr int kSortMaxBlocks = 256;
+constexpr int kSortBlockPairs = 2048;
+struct SortArgs {
+    const int *of;
+    int *order, *first, *place;
+    int *counts;  // [blocks, experts + 1]
+    int pairs, experts, each;  // pairs to a block, a multiple of kSortThreads
+};
+__device__ __forceinline__ int sort_key(const SortArgs &p, int pair) {
+    const int e = p.of[pair];
+    return (unsigned)e < (unsigned)p.experts ? e : p.experts;
+}
+
+__global__ __launch_bounds__(kSortThreads) void moe_count_kernel(SortArgs p) {
+    __shared__ int count[kMaxExperts + 1];
+    for (int e = threadIdx.x; e <= p.experts; e += kSortThreads) count[e] = 0;
+    __syncthreads();
+    const int begin = blockIdx.x * p.each, end = min(p.pairs, begin + p.each);
+    for (int i = begin + threadIdx.x; i < end; i += kSortThreads) atomicAdd(&count[sort_key(p, i)], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e <= p.experts; e += kSortThreads) p.counts[(size_t)blockIdx.x * (p.experts + 1) + e] = count[e];
+}
+
+__global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(SortArgs p) {
+    __shared__ int count[kSortWaves][kMaxExperts + 1];  // of a wavefront; then where its next pair of the expert goes
+    __shared__ int total[kMaxExperts + 1], before[kMaxExperts + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = p.experts + 1;
+    const int part = p.each / kSortWaves, begin = blockIdx.x * p.each + wave * part, end = min(p.pairs, begin + part);
+    for (int i = tid; i < kSortWaves * keys; i += kSortThreads) count[i / keys][i % keys] = 0;
+    __syncthreads();
+    for (int i = begin + lane; i < end; i += 64) atomicAdd(&count[wave][sort_key(p, i)], 1);
+    __syncthreads();
+    for (int e = tid; e < keys; e += kSortThreads) {
+        int all = 0, earlier = 0;
+        if (gridDim.x == 1) {
+            for (int w = 0; w < kSortWaves; ++w) all += count[w][e];
+        } else {
+#pragma unroll 8
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const int n = p.counts[(size_t)b * keys + e];
+                all += n;
+                earlier += b < (int)blockIdx.x ? n : 0;
+            }
+        }
+        total[e] = all;
+        before[e] = earlier;
+    }
+    __syncthreads();
+    if (wave == 0) {  // where each expert begins: a lane adds up consecutive ones
+        const int per = (keys + 63) / 64, e0 = lane * per, e1 = min(keys, e0 + per);
+        int sum = 0;
+        for (int e = e0; e < e1; ++e) sum += total[e];
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int below = __shfl_up(upto, d);
+            if (lane >= d) upto += below;
+        }
+        int at = upto - sum;
+        for (int e = e0; e < e1; ++e) {
+            if (blockIdx.x == 0) p.first[e] = at;
+            before[e] += at;
+            at += total[e];
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < keys; e += kSortThreads) {
+        int at = before[e];
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = count[w][e];
+            count[w][e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    const int bits = 32 - __builtin_clz(keys - 1);
+    for (int i0 = begin; i0 < end; i0 += 64) {
+        const int i = i0 + lane;
+        const bool here = i < end;
+        const int key = here ? sort_key(p, i) : -1;
+        unsigned long long same = __ballot(here);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long set = __ballot(key >> b & 1);
+            same &= key >> b & 1 ? set : ~set;
+        }
+        const int lower = __popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (here) at = count[wave][key];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (here && lower == 0) count[wave][key] = at + __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (here) {
+            p.order[at + lower] = i;
+            p.place[i] = at + lower;
+        }
+    }
+}
+
+// ---- rows ----------------------------------------------------------------------------------------------------------
+// Units of 16 bytes, a thread for each of a token's: it is read or written once, its rows at `top` places.  Eight of them are in flight together.
+// (A place that no pair has is passed over: nothing is read or written out of bounds whatever `place` holds.)
+struct RowsArgs {
+    const uint16_t *in;      // gather: x; combine: rows; combine backward: dy
+    const uint16_t *rows;    // combine backward
+    const float *weights;    // [tokens, top], or null: one each
+    const int *first, *place;
+    uint16_t *out;
+    float *d_weights;
+    int tokens, top, experts, units;
+};
+
+__global__ __launch_bounds__(256) void moe_gather_kernel(RowsArgs p) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)p.tokens * p.units) return;
+    const int token = (int)(i / p.units), unit = (int)(i - (size_t)token * p.units), placed = p.first[p.experts], pairs = p.tokens * p.top;
+    const u32x4 v = reinterpret_cast<const u32x4 *>(p.in)[i], zero = {0u, 0u, 0u, 0u};
+    for (int j = 0; j < p.top; ++j) {
+        const int at = p.place[(size_t)token * p.top + j];
+        if ((unsigned)at < (unsigned)pairs) reinterpret_cast<u32x4 *>(p.out)[(size_t)at * p.units + unit] = at < placed ? v : zero;
+    }
+}
+
+__device__ __forceinline__ float bf16_low(uint32_t v) { return __builtin_bit_cast(float, v << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t v) { return __builtin_bit_cast(float, v & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t bf16_pair(float low, float high) { return f32_to_bf16_bits(low) | (uint32_t)f32_to_bf16_bits(high) << 16; }
+
+__global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs p) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)p.tokens * p.units) return;
+    const int token = (int)(i / p.units), unit = (int)(i - (size_t)token * p.units), placed = min(p.first[p.experts], p.tokens * p.top);
+    float sum[8] = {};
+    for (int j0 = 0; j0 < p.top; j0 += 8) {
+        u32x4 v[8];
+        bool here[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int at = j0 + u < p.top ? p.place[(size_t)token * p.top + j0 + u] : placed;
+            here[u] = at >= 0 && at < placed;
+            if (here[u]) v[u] = reinterpret_cast<const u32x4 *>(p.in)[(size_t)at * p.units + unit];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (!here[u]) continue;
+            const float w = p.weights ? p.weights[(size_t)token * p.top + j0 + u] : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[2 * e] = fmaf(w, bf16_low(v[u][e]), sum[2 * e]);
+                sum[2 * e + 1] = fmaf(w, bf16_high(v[u][e]), sum[2 * e + 1]);
+            }
+        }
+    }
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = bf16_pair(sum[2 * e], sum[2 * e + 1]);
+    reinterpret_cast<u32x4 *>(p.out)[i] = o;
+}
+
+// W wavefronts to a token, 4 / W tokens to a block: a lane goes over its units of dy and of every row; a row's product is summed in f32 in the lanes,
+// across them and across the wavefronts, in that order.
+template <int W>
+__global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
+    __shared__ float part[4][kMaxTop];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, of = wave % W, pairs = p.tokens * p.top, placed = min(p.first[p.experts], pairs);
+    const int token = blockIdx.x * (4 / W) + wave / W;
+    const bool live = token < p.tokens;
+    const int *place = p.place + (size_t)(live ? token : 0) * p.top;
+    const float *weights = p.weights + (size_t)(live ? token : 0) * p.top;
+    for (int j0 = 0; j0 < (live ? p.top : 0); j0 += 8) {
+        float dot[8] = {};
+        int at[8];
+        float w[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int j = min(j0 + u, p.top - 1);
+            at[u] = (unsigned)place[j] < (unsigned)pairs ? place[j] : -1;
+            w[u] = weights[j];
+        }
+        for (int unit = of * 64 + lane; unit < p.units; unit += W * 64) {
+            const u32x4 d = reinterpret_cast<const u32x4 *>(p.in)[(size_t)token * p.units + unit];
+            u32x4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (j0 + u < p.top && (unsigned)at[u] < (unsigned)placed) v[u] = reinterpret_cast<const u32x4 *>(p.rows)[(size_t)at[u] * p.units + unit];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (j0 + u >= p.top || at[u] < 0) continue;
+                u32x4 o = {0u, 0u, 0u, 0u};
+                if (at[u] < placed) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[e] = bf16_pair(w[u] * bf16_low(d[e]), w[u] * bf16_high(d[e]));
+                        dot[u] = fmaf(bf16_low(d[e]), bf16_low(v[u][e]), dot[u]);
+                        dot[u] = fmaf(bf16_high(d[e]), bf16_high(v[u][e]), dot[u]);
+                    }
+                }
+                reinterpret_cast<u32x4 *>(p.out)[(size_t)at[u] * p.units + unit] = o;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            float s = dot[u];
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+            if (lane == 0 && j0 + u < p.top) part[wave][j0 + u] = s;
+        }
+    }
+    __syncthreads();
+    if (of == 0 && live && lane < p.top) {
+        float s = part[wave][lane];
+#pragma unroll
+        for (int i = 1; i < W; ++i) s += part[wave + i][lane];
+        p.d_weights[(size_t)token * p.top + lane] = s;
+    }
+}
+
+// ---- the entry points' checks --------------------------------------------------------------------------------------
+bool on_16(std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if (!p || reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+    return true;
+}
+// rows of `width` bf16 values for m tokens: KILN_W4A16_OK, or why not
+kiln_marlin_status_t rows_ok(int m, int top_k, int experts, int width) {
+    if (m < 0 || width < 1 || width % 8 != 0) return KILN_W4A16_ERR_PROB_SHAPE;
+    if (top_k < 1 || top_k > kMaxTop || experts < 1 || experts > kMaxExperts || (int64_t)m * top_k > kMaxPairs) return KILN_W4A16_ERR_KERN_SHAPE;
+    if (((int64_t)m * (width / 8) + 255) / 256 > INT32_MAX) return KILN_W4A16_ERR_KERN_SHAPE;
+    return KILN_W4A16_OK;
+}
+int sort_block_pairs(int pairs) {
+    const int each = pairs <= kSortBlockPairs ? pairs : std::max(kSortBlockPairs, (pairs + kSortMaxBlocks - 1) / kSortMaxBlocks);
+    return (each + kSortThreads - 1) / kSortThreads * kSortThreads;
+}
+kiln_marlin_status_t launched() { return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH; }
+unsigned thread_blocks(int m, int units) { return (unsigned)(((size_t)m * units + 255) / 256); }
+
+}  // namespace
+}  // namespace kiln
+
+using namespace kiln;
+
+extern "C" {
+
+size_t kiln_w4a16_moe_sort_scratch_bytes(int experts) {
+    return (size_t)kSortMaxBlocks * ((experts < 1 ? 1 : experts > kMaxExperts ? kMaxExperts : experts) + 1) * sizeof(int);
+}
+
+kiln_marlin_status_t kiln_w4a16_moe_sort(const int *expert_of, int prob_m, int top_k, int experts, int *order, int *first, int *place, int dev,
+                                         void *stream, void *scratch) {
+    (void)dev;
+    if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, 8)) return st;
+    const int pairs = prob_m * top_k;
+    if (!first || !scratch || (pairs && (!expert_of || !order || !place))) return KILN_W4A16_ERR_ARGUMENT;
+    for (const void *p : {static_cast<const void *>(expert_of), static_cast<const void *>(order), static_cast<const void *>(first),
+                          static_cast<const void *>(place), static_cast<const void *>(scratch)})
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t bytes = (size_t)pairs * 4, first_bytes = ((size_t)experts + 1) * 4;
+    if (meet(expert_of, bytes, order, bytes) || meet(expert_of, bytes, place, bytes) || meet(expert_of, bytes, first, first_bytes) ||
+        meet(order, bytes, place, bytes) || meet(order, bytes, first, first_bytes) || meet(place, bytes, first, first_bytes))
+        return KILN_W4A16_ERR_ARGUMENT;
+    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    const int each = pairs ? sort_block_pairs(pairs) : kSortThreads, blocks = pairs ? (pairs + each - 1) / each : 1;
+    const SortArgs a{expert_of, order, first, place, static_cast<int *>(scratch), pairs, experts, each};
+    if (blocks > 1) moe_count_kernel<<<blocks, kSortThreads, 0, hs>>>(a);
+    moe_sort_kernel<<<blocks, kSortThreads, 0, hs>>>(a);
+    return launched();
+}
+
+kiln_marlin_status_t kiln_w4a16_moe_gather(const void *x, const int *first, const int *place, void *rows, int prob_m, int top_k, int experts,
+                                           int width, int dev, void *stream) {
+    (void)dev;
+    if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
+    if (prob_m == 0) return KILN_W4A16_OK;
+    if (!on_16({x, rows}) || !first || !place) return KILN_W4A16_ERR_ARGUMENT;
+    if (meet(rows, (size_t)prob_m * top_k * width * 2, x, (size_t)prob_m * width * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    const RowsArgs a{(const uint16_t *)x, nullptr, nullptr, first, place, (uint16_t *)rows, nullptr, prob_m, top_k, experts, width / 8};
+    moe_gather_kernel<<<thread_blocks(prob_m, width / 8), 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+    return launched();
+}
+
+kiln_marlin_status_t kiln_w4a16_moe_combine(const void *rows, const float *weights, const int *first, const int *place, void *y, int prob_m, int top_k,
+                                            int experts, int width, int dev, void *stream) {
+    (void)dev;
+    if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
+    if (prob_m == 0) return KILN_W4A16_OK;
+    if (!on_16({rows, y}) || !first || !place) return KILN_W4A16_ERR_ARGUMENT;
+    if (meet(y, (size_t)prob_m * width * 2, rows, (size_t)prob_m * top_k * width * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    const RowsArgs a{(const uint16_t *)rows, nullptr, weights, first, place, (uint16_t *)y, nullptr, prob_m, top_k, experts, width / 8};
+    moe_combine_kernel<<<thread_blocks(prob_m, width / 8), 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+    return launched();
+}
+
+kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void *rows, const float *weights, const int *first, const int *place,
+                                                     void *d_rows, float *d_weights, int prob_m, int top_k, int experts, int width, int dev, void *stream) {
+    (void)dev;
+    if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
+    if (prob_m == 0) return KILN_W4A16_OK;
+    if (!on_16({dy, rows, d_rows}) || !weights || !first || !place || !d_weights) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t rows_bytes = (size_t)prob_m * top_k * width * 2, pair_bytes = (size_t)prob_m * top_k * 4;
+    if (meet(d_rows, rows_bytes, rows, rows_bytes) || meet(d_rows, rows_bytes, dy, (size_t)prob_m * width * 2) ||
+        meet(d_weights, pair_bytes, weights, pair_bytes))
+        return KILN_W4A16_ERR_ARGUMENT;
+    const RowsArgs a{(const uint16_t *)dy, (const uint16_t *)rows, weights, first, place, (uint16_t *)d_rows, d_weights, prob_m, top_k, experts, width / 8};
+    hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
+    if (width <= 512) moe_combine_backward_kernel<1><<<(prob_m + 3) / 4, 256, 0, hs>>>(a);
+    else moe_combine_backward_kernel<4><<<prob_m, 256, 0, hs>>>(a);
+    return launched();
+}
+
+}  // extern "C"

@@ -761,3 +761,301 @@ def marlin_w4a16_moe(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Te
         raise MarlinGemmError(f"kiln_w4a16_moe failed with status {status}: {_lib.status_string(status)} "
                               f"(m={m}, top_k={top_k}, experts={experts}, hidden={hidden}, n_out={n_out}, n_down={n_down})")
     return out
+
+
+# ---- a mixture of experts for many tokens, and training through it ------------------------------------------------------------------
+
+def _check_tensor(name: str, t, shape, dtype, device) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+        _bail(f"{name} must be {dtype} {tuple(shape)} on {device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+
+
+def _check_status(status: int, call: str, what: str) -> None:
+    if status != 0:
+        raise MarlinGemmError(f"{call} failed with status {status}: {_lib.status_string(status)} ({what})")
+
+
+def _stream_of(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def moe_sort(expert_of: torch.Tensor, experts: int):
+    """The choices of a router (`moe_route`) in the order of their experts: `(order, first, place)`, i32.
+
+    Pair `p = i * top_k + j` is row i's choice `expert_of[i, j]`; an id outside `[0, experts)` is no expert (one held elsewhere).  `order`
+    `[m * top_k]` holds the pairs by expert, in their order inside one, those without an expert last; `place` `[m, top_k]` is its inverse;
+    expert e has the positions `first[e] ... first[e + 1]`, and from `first[experts]` on there is no expert."""
+    made = _calls.moe_sort(expert_of, experts)
+    if made is not None:
+        return made
+    if not expert_of.is_cuda:
+        _bail("expert_of must be on CUDA")
+    if expert_of.dim() != 2 or expert_of.dtype != torch.int32:
+        _bail(f"expert_of must be i32 [m, top_k] (got {expert_of.dtype} {tuple(expert_of.shape)})")
+    m, top_k = expert_of.shape
+    experts = _check_experts(experts)
+    _check_pairs(m, top_k)
+    device = expert_of.device
+    lib = _lib.load()
+    expert_of = expert_of.contiguous()
+    order = torch.empty(m * top_k, dtype=torch.int32, device=device)
+    first = torch.empty(experts + 1, dtype=torch.int32, device=device)
+    place = torch.empty((m, top_k), dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        scratch = torch.empty(lib.kiln_w4a16_moe_sort_scratch_bytes(experts), dtype=torch.uint8, device=device)
+        status = lib.kiln_w4a16_moe_sort(expert_of.data_ptr(), m, top_k, experts, order.data_ptr(), first.data_ptr(), place.data_ptr(),
+                                         device.index or 0, _stream_of(device), scratch.data_ptr())
+    _check_status(status, "kiln_w4a16_moe_sort", f"m={m}, top_k={top_k}, experts={experts}")
+    return order, first, place
+
+
+def _check_experts(experts) -> int:
+    experts = int(experts)
+    if not 1 <= experts <= 1024:
+        _bail(f"a layer has 1 to 1024 experts (got {experts})")
+    return experts
+
+
+def _check_pairs(m: int, top_k: int) -> None:
+    if not 1 <= top_k <= 16:
+        _bail(f"top_k must be 1 to 16 (got {top_k})")
+    if m * top_k > 1 << 30:
+        _bail(f"m * top_k must be at most 2^30 (got {m} * {top_k})")
+
+
+def _check_sorted(first, place, device):
+    """`first` and `place` of `moe_sort`: `(m, top_k, experts)`."""
+    if first.dim() != 1 or place.dim() != 2:
+        _bail(f"first must be [experts + 1] and place [m, top_k] (got {tuple(first.shape)} and {tuple(place.shape)})")
+    for name, t in (("first", first), ("place", place)):
+        _check_tensor(name, t, t.shape, torch.int32, device)
+    m, top_k = place.shape
+    _check_pairs(m, top_k)
+    return m, top_k, _check_experts(first.shape[0] - 1)
+
+
+def _check_rows(name: str, rows, count: int | None = None) -> int:
+    """bf16 rows on CUDA: their width."""
+    if not rows.is_cuda:
+        _bail(f"{name} must be on CUDA")
+    if rows.dim() != 2 or rows.dtype != torch.bfloat16 or (count is not None and rows.shape[0] != count):
+        _bail(f"{name} must be bf16 [{'rows' if count is None else count}, width] (got {rows.dtype} {tuple(rows.shape)})")
+    width = rows.shape[1]
+    if width == 0 or width % 8:
+        _bail(f"{name}: the width must be a multiple of 8 (got {width})")
+    return width
+
+
+def moe_gather(x: torch.Tensor, first: torch.Tensor, place: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The tokens' rows in the order of `moe_sort`: `rows[place[i, j]] = x[i]`, bf16 `[m, width]` -> `[m * top_k, width]`; zeros for pairs without an
+    expert.  Its gradient is `moe_gather_backward`."""
+    rows = _calls.moe_gather(x, first, place, out)
+    if rows is not None:
+        return rows
+    width = _check_rows("x", x)
+    m, top_k, experts = _check_sorted(first, place, x.device)
+    _check_rows("x", x, m)
+    out = _check_out("out", out, (m * top_k, width), x.device)
+    if m == 0:
+        return out
+    x, first, place = x.contiguous(), first.contiguous(), place.contiguous()
+    with torch.cuda.device(x.device):
+        status = _lib.load().kiln_w4a16_moe_gather(x.data_ptr(), first.data_ptr(), place.data_ptr(), out.data_ptr(), m, top_k, experts, width,
+                                                   x.device.index or 0, _stream_of(x.device))
+    _check_status(status, "kiln_w4a16_moe_gather", f"m={m}, top_k={top_k}, experts={experts}, width={width}")
+    return out
+
+
+def _combine(rows, weights, first, place, out):
+    width = _check_rows("rows", rows)
+    device = rows.device
+    m, top_k, experts = _check_sorted(first, place, device)
+    _check_rows("rows", rows, m * top_k)
+    if weights is not None:
+        _check_tensor("weights", weights, (m, top_k), torch.float32, device)
+        weights = weights.contiguous()
+    out = _check_out("out", out, (m, width), device)
+    if m == 0:
+        return out
+    rows, first, place = rows.contiguous(), first.contiguous(), place.contiguous()
+    with torch.cuda.device(device):
+        status = _lib.load().kiln_w4a16_moe_combine(rows.data_ptr(), None if weights is None else weights.data_ptr(), first.data_ptr(), place.data_ptr(),
+                                                    out.data_ptr(), m, top_k, experts, width, device.index or 0, _stream_of(device))
+    _check_status(status, "kiln_w4a16_moe_combine", f"m={m}, top_k={top_k}, experts={experts}, width={width}")
+    return out
+
+
+def moe_gather_backward(d_rows: torch.Tensor, first: torch.Tensor, place: torch.Tensor) -> torch.Tensor:
+    """The gradient of `moe_gather`'s `x`: `dx[i] = sum_j d_rows[place[i, j]]`, bf16 `[m * top_k, width]` -> `[m, width]`, summed in f32 and rounded
+    once; nothing from pairs without an expert."""
+    dx = _calls.moe_combine(d_rows, None, first, place, None)
+    return dx if dx is not None else _combine(d_rows, None, first, place, None)
+
+
+def moe_combine(rows: torch.Tensor, weights: torch.Tensor, first: torch.Tensor, place: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The experts' rows back to their tokens: `y[i] = sum_j weights[i, j] * rows[place[i, j]]`, bf16 `[m * top_k, width]` -> `[m, width]`, `weights`
+    f32 `[m, top_k]` (`moe_route`), summed in f32 and rounded once; nothing from pairs without an expert."""
+    y = _calls.moe_combine(rows, weights, first, place, out)
+    if y is not None:
+        return y
+    if weights is None:
+        _bail("weights must be f32 [m, top_k]")
+    return _combine(rows, weights, first, place, out)
+
+
+def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, first: torch.Tensor, place: torch.Tensor):
+    """The gradients of `moe_combine(rows, weights, ...)` from `dy` bf16 `[m, width]`: `(d_rows, d_weights)`, `d_rows[place[i, j]] = weights[i, j] dy[i]`
+    bf16 and `d_weights[i, j] = <rows[place[i, j]], dy[i]>` f32; zeros for pairs without an expert."""
+    made = _calls.moe_combine_backward(dy, rows, weights, first, place)
+    if made is not None:
+        return made
+    width = _check_rows("rows", rows)
+    device = rows.device
+    m, top_k, experts = _check_sorted(first, place, device)
+    _check_rows("rows", rows, m * top_k)
+    _check_tensor("dy", dy, (m, width), torch.bfloat16, device)
+    _check_tensor("weights", weights, (m, top_k), torch.float32, device)
+    dy, rows, weights, first, place = (t.contiguous() for t in (dy, rows, weights, first, place))
+    d_rows, d_weights = torch.empty_like(rows), torch.empty_like(weights)
+    if m == 0:
+        return d_rows, d_weights
+    with torch.cuda.device(device):
+        status = _lib.load().kiln_w4a16_moe_combine_backward(
+            dy.data_ptr(), rows.data_ptr(), weights.data_ptr(), first.data_ptr(), place.data_ptr(), d_rows.data_ptr(), d_weights.data_ptr(), m, top_k, experts,
+            width, device.index or 0, _stream_of(device))
+    _check_status(status, "kiln_w4a16_moe_combine_backward", f"m={m}, top_k={top_k}, experts={experts}, width={width}")
+    return d_rows, d_weights
+
+
+def _check_expert_packs(first, b_packed, scales, groupsize: int, device):
+    """The packs of `marlin_w4a16_gemm_experts`: `(experts, k, n)`."""
+    if not (groupsize == -1 or groupsize == 128):
+        _bail(f"groupsize must be -1 or 128 (got {groupsize})")
+    if b_packed.dim() != 3 or scales.dim() != 3:
+        _bail("the experts' packs are 3-D, experts first")
+    experts, k, n = _check_experts(b_packed.shape[0]), b_packed.shape[1] * 16, scales.shape[2]
+    if k == 0 or n == 0 or k % 128 or n % 256:
+        _bail(f"k={k} must be a multiple of 128, n={n} of 256")
+    _check_tensor("b_packed", b_packed, (experts, k // 16, 2 * n), torch.int32, device)
+    _check_tensor("scales", scales, (experts, 1 if groupsize == -1 else k // 128, n), torch.float16, device)
+    _check_tensor("first", first, (experts + 1,), torch.int32, device)
+    return experts, k, n
+
+
+def marlin_w4a16_gemm_experts(x: torch.Tensor, first: torch.Tensor, b_packed: torch.Tensor, scales: torch.Tensor, groupsize: int, *,
+                              order: torch.Tensor | None = None, top_k: int = 1, swiglu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows in the order of their experts times their expert's packed weight, all experts in one call: `y[p] = x[p] @ dequant(b_packed[e])` for
+    `first[e] <= p < first[e + 1]`, bf16 `[rows, k]` -> `[rows, n]`; rows behind `first[experts]` are zero.
+
+    `first` from `moe_sort`.  With `order` (its too) and `top_k`, `x` holds the tokens and position p takes row `order[p] // top_k`: no gathered copy.
+    With `swiglu` the packs are gate and up interleaved (`pack.interleave_gate_up`) and the result is `silu(gate) * up`, `[rows, n / 2]`.
+    `b_packed` `[experts, k/16, 2n]` and `scales` `[experts, k/g, n]` as in `marlin_w4a16_moe`."""
+    y = _calls.gemm_experts(x, first, b_packed, scales, groupsize, order, top_k, swiglu, out)
+    if y is not None:
+        return y
+    if not x.is_cuda:
+        _bail("x must be on CUDA")
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        _bail(f"x must be bf16 [rows, k] (got {x.dtype} {tuple(x.shape)})")
+    device = x.device
+    experts, k, n = _check_expert_packs(first, b_packed, scales, groupsize, device)
+    x_rows = rows = x.shape[0]
+    if x.shape[1] != k:
+        _bail(f"x must be [rows, k={k}] (got {tuple(x.shape)})")
+    if order is not None:
+        top_k = int(top_k)
+        if top_k < 1:
+            _bail(f"top_k must be at least 1 (got {top_k})")
+        rows = x_rows * top_k
+        _check_tensor("order", order, (rows,), torch.int32, device)
+        order = order.contiguous()
+    out = _check_out("out", out, (rows, n // 2 if swiglu else n), device)
+    if rows == 0:
+        return out
+    lib = _lib.load()
+    x, first, b_packed, scales = x.contiguous(), first.contiguous(), b_packed.contiguous(), scales.contiguous()
+    with torch.cuda.device(device):
+        scratch = torch.empty(lib.kiln_w4a16_gemm_experts_scratch_bytes(x_rows, k), dtype=torch.uint8, device=device)
+        status = lib.kiln_w4a16_gemm_experts(x.data_ptr(), first.data_ptr(), None if order is None else order.data_ptr(), b_packed.data_ptr(),
+                                             scales.data_ptr(), out.data_ptr(), rows, x_rows, top_k if order is not None else 1, n, k, experts, groupsize,
+                                             int(bool(swiglu)), device.index or 0, _stream_of(device), scratch.data_ptr())
+    _check_status(status, "kiln_w4a16_gemm_experts", f"rows={rows}, n={n}, k={k}, experts={experts}")
+    return out
+
+
+def marlin_w4a16_gemm_experts_backward(dy: torch.Tensor, first: torch.Tensor, b_packed: torch.Tensor, scales: torch.Tensor, groupsize: int) -> torch.Tensor:
+    """The gradient of `marlin_w4a16_gemm_experts`' rows, the packs frozen: `dx[p] = dy[p] @ dequant(b_packed[e])^T`, bf16 `[rows, n]` -> `[rows, k]`; rows
+    behind `first[experts]` are zero.  (Of a call with `order`: `moe_gather_backward` brings it back to the tokens; with `swiglu`: keep gate
+    and up by `swiglu_keep`.)"""
+    dx = _calls.gemm_experts_backward(dy, first, b_packed, scales, groupsize)
+    if dx is not None:
+        return dx
+    if not dy.is_cuda:
+        _bail("dy must be on CUDA")
+    device = dy.device
+    experts, k, n = _check_expert_packs(first, b_packed, scales, groupsize, device)
+    if dy.dim() != 2:
+        _bail(f"dy must be bf16 [rows, n={n}] (got {tuple(dy.shape)})")
+    rows = dy.shape[0]
+    _check_gradient(dy, rows, n, device)
+    dx = torch.empty((rows, k), dtype=torch.bfloat16, device=device)
+    if rows == 0:
+        return dx
+    dy, first, b_packed, scales = dy.contiguous(), first.contiguous(), b_packed.contiguous(), scales.contiguous()
+    with torch.cuda.device(device):
+        status = _lib.load().kiln_w4a16_gemm_experts_backward(dy.data_ptr(), first.data_ptr(), b_packed.data_ptr(), scales.data_ptr(), dx.data_ptr(), rows, n, k,
+                                                              experts, groupsize, device.index or 0, _stream_of(device))
+    _check_status(status, "kiln_w4a16_gemm_experts_backward", f"rows={rows}, n={n}, k={k}, experts={experts}")
+    return dx
+
+
+def swiglu_keep(gate_up: torch.Tensor):
+    """`h = silu(gate) * up` in training, with gate and up kept in 8 bits for `swiglu_keep_backward`: `gate_up` bf16 `[m, 2 n_out]` in the packed column
+    order (8 gate columns, then the 8 matching up columns: what `marlin_w4a16_gemm` gives on a pack of `pack.interleave_gate_up`) ->
+    `(h bf16 [m, n_out], whole i8 [m, 2 n_out], exponents u8 [m, n_out / 32, 2])`.
+
+    `value = whole * 2^(exponent - 133)`: 32 gate values, or 32 up values, share an exponent, the bf16 exponent field of the largest; at most 2^-7 of that
+    one away, and exact in bf16.  A block with an infinity or NaN is kept as NaN.  (crates/kiln-model/src/forward.rs:2771-2819 is the forward.)"""
+    made = _calls.swiglu_keep(gate_up)
+    if made is not None:
+        return made
+    if not gate_up.is_cuda:
+        _bail("gate_up must be on CUDA")
+    if gate_up.dim() != 2 or gate_up.dtype != torch.bfloat16 or gate_up.shape[1] == 0 or gate_up.shape[1] % 256:
+        _bail(f"gate_up must be bf16 [m, 2 n_out], n_out a multiple of 128 (got {gate_up.dtype} {tuple(gate_up.shape)})")
+    m, n_out, device = gate_up.shape[0], gate_up.shape[1] // 2, gate_up.device
+    gate_up = gate_up.contiguous()
+    h = torch.empty((m, n_out), dtype=torch.bfloat16, device=device)
+    whole = torch.empty((m, 2 * n_out), dtype=torch.int8, device=device)
+    exponents = torch.empty((m, n_out // 32, 2), dtype=torch.uint8, device=device)
+    if m == 0:
+        return h, whole, exponents
+    with torch.cuda.device(device):
+        status = _lib.load().kiln_w4a16_swiglu_keep(gate_up.data_ptr(), h.data_ptr(), whole.data_ptr(), exponents.data_ptr(), m, n_out, device.index or 0,
+                                                    _stream_of(device))
+    _check_status(status, "kiln_w4a16_swiglu_keep", f"m={m}, n_out={n_out}")
+    return h, whole, exponents
+
+
+def swiglu_keep_backward(dh: torch.Tensor, whole: torch.Tensor, exponents: torch.Tensor, *, recompute: bool = False):
+    """The gradient of `swiglu_keep`'s `gate_up` out of what it kept, from `dh` bf16 `[m, n_out]`: bf16 `[m, 2 n_out]`, the same columns; with
+    `recompute` `(d_gate_up, h)`, `h` of the kept values (for the gradients of adapters on what reads it)."""
+    made = _calls.swiglu_keep_backward(dh, whole, exponents, recompute)
+    if made is not None:
+        return made
+    if not dh.is_cuda:
+        _bail("dh must be on CUDA")
+    if dh.dim() != 2 or dh.dtype != torch.bfloat16 or dh.shape[1] == 0 or dh.shape[1] % 128:
+        _bail(f"dh must be bf16 [m, n_out], n_out a multiple of 128 (got {dh.dtype} {tuple(dh.shape)})")
+    (m, n_out), device = dh.shape, dh.device
+    _check_tensor("whole", whole, (m, 2 * n_out), torch.int8, device)
+    _check_tensor("exponents", exponents, (m, n_out // 32, 2), torch.uint8, device)
+    dh, whole, exponents = dh.contiguous(), whole.contiguous(), exponents.contiguous()
+    d_gate_up = torch.empty((m, 2 * n_out), dtype=torch.bfloat16, device=device)
+    h = torch.empty((m, n_out), dtype=torch.bfloat16, device=device) if recompute else None
+    if m:
+        with torch.cuda.device(device):
+            status = _lib.load().kiln_w4a16_swiglu_keep_backward(dh.data_ptr(), whole.data_ptr(), exponents.data_ptr(), d_gate_up.data_ptr(),
+                                                                 h.data_ptr() if recompute else None, m, n_out, device.index or 0, _stream_of(device))
+        _check_status(status, "kiln_w4a16_swiglu_keep_backward", f"m={m}, n_out={n_out}")
+    return (d_gate_up, h) if recompute else d_gate_up
