@@ -365,10 +365,10 @@ kiln_marlin_status_t kiln_w4a16_moe_route(
  *   order   int32 [m * top_k]   the pairs by expert, in their order inside one, those without an expert last
  *   place   int32 [m, top_k]    its inverse: a pair's position
  *   first   int32 [experts + 1] expert e has the positions first[e] ... first[e + 1]; from first[experts] on there is no expert
- * All in device memory.  Deterministic.  scratch: kiln_w4a16_moe_sort_scratch_bytes, on 4 bytes, holds nothing between calls.  m == 0 writes
- * `first` alone.  experts 1 ... 1024, top_k 1 ... 16, m * top_k <= 2^30.  No counterpart in the reference, whose model family is dense.
+ * All in device memory.  Deterministic.  scratch: kiln_w4a16_moe_sort_scratch_bytes, on 4 bytes, holds nothing between calls; NULL where that is 0 (few
+ * pairs).  m == 0 writes `first` alone.  experts 1 ... 1024, top_k 1 ... 16, m * top_k <= 2^30.  No counterpart in the reference, whose model family is dense.
  */
-size_t kiln_w4a16_moe_sort_scratch_bytes(int experts);
+size_t kiln_w4a16_moe_sort_scratch_bytes(int prob_m, int top_k, int experts);
 kiln_marlin_status_t kiln_w4a16_moe_sort(
     const int *expert_of, int prob_m, int top_k, int experts,
     int *order, int *first, int *place, int dev, void *stream, void *scratch);
@@ -558,6 +558,8 @@ int kiln_w4a16_layout_version(void);
  *   holds the projection in}.  Returns 0, or 1 for sizes that no call may have.
  * kiln_w4a16_debug_bank_backward_plan: the product behind kiln_w4a16_gemm_bank_backward's dA, out[3] = {rows and columns of k to a block
  *   (0: calls of few rows, straight from the codes), slices of n}.  Returns 0, or 1 for sizes that no call may have.
+ * kiln_w4a16_debug_experts_plan: the blocks of kiln_w4a16_gemm_experts (`backward`: of its gradient), 0 of 32 rows and few columns whose wavefronts share
+ *   out the contraction, 1, 2, 3 of up to 32, 64, 128 rows x 256 columns; -1 for sizes that no call may have.
  * kiln_w4a16_debug_workspace_operands: where a GEMM with stacked adapters of `rank` (a multiple of 8; 0: none) that is handed
  *   `workspace` (never followed) has its operands behind the zeroed prefix, out[6] = {row sums (0: none), partial tiles, projection
  *   (0: none), the end of all; of a projection that the mid-M kernel's launch writes and reads, its K slices and the bytes from one
@@ -571,6 +573,7 @@ int kiln_w4a16_debug_adapter_blocks(int prob_m, int prob_n, int prob_k, int cus,
                                     int swiglu, int n_adapters, int *out, int capacity);
 int kiln_w4a16_debug_bank_plan(int prob_m, int prob_n, int prob_k, int rank, int cus, int *out);
 int kiln_w4a16_debug_bank_backward_plan(int prob_m, int prob_n, int prob_k, int *out);
+int kiln_w4a16_debug_experts_plan(int rows, int prob_n, int prob_k, int experts, int backward, int cus);
 int kiln_w4a16_debug_workspace_operands(int prob_m, int prob_n, int prob_k, int cus, int rank, const void *workspace, size_t *out);
 
 #ifdef __cplusplus

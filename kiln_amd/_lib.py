@@ -65,6 +65,7 @@ EXPORTS = (
     "kiln_w4a16_debug_adapter_blocks",
     "kiln_w4a16_debug_bank_plan",
     "kiln_w4a16_debug_bank_backward_plan",
+    "kiln_w4a16_debug_experts_plan",
     "kiln_w4a16_debug_workspace_operands",
 )
 
@@ -225,6 +226,8 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_debug_adapter_blocks.argtypes = [i, i, i, i, vp, i, i, i, c.POINTER(c.c_int), i]
     L.kiln_w4a16_debug_workspace_operands.restype = i
     L.kiln_w4a16_debug_workspace_operands.argtypes = [i, i, i, i, i, vp, c.POINTER(c.c_size_t)]
+    L.kiln_w4a16_debug_experts_plan.restype = i
+    L.kiln_w4a16_debug_experts_plan.argtypes = [i] * 6
     L.kiln_w4a16_debug_bank_backward_plan.restype = i
     L.kiln_w4a16_debug_bank_backward_plan.argtypes = [i, i, i, c.POINTER(c.c_int)]
     L.kiln_w4a16_debug_bank_plan.restype = i
@@ -262,7 +265,7 @@ def _load(tuning: bool) -> ctypes.CDLL:
     L.kiln_w4a16_moe_route.restype = i
     L.kiln_w4a16_moe_route.argtypes = [vp, i, i, i, i, i, vp, vp, i, vp]
     L.kiln_w4a16_moe_sort_scratch_bytes.restype = c.c_size_t
-    L.kiln_w4a16_moe_sort_scratch_bytes.argtypes = [i]
+    L.kiln_w4a16_moe_sort_scratch_bytes.argtypes = [i, i, i]
     L.kiln_w4a16_moe_sort.restype = i
     L.kiln_w4a16_moe_sort.argtypes = [vp, i, i, i, vp, vp, vp, i, vp, vp]
     L.kiln_w4a16_moe_gather.restype = i

@@ -58,7 +58,8 @@ __device__ __forceinline__ float from_whole(uint32_t word, int i, int exponent) 
     const float v = __builtin_amdgcn_ldexpf((float)((int)(word << (24 - 8 * i)) >> 24), exponent - 133);
     return exponent == kNoNumber ? __builtin_nanf("") : v;
 }
-__device__ __forceinline__ uint32_t pair_of(float low, float high) { return f32_to_bf16_bits(low) | (uint32_t)f32_to_bf16_bits(high) << 16; }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pair_of(float low, float high) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)low, (__bf16)high}); }
 
 struct KeepArgs {
     const u32x4 *gate_up;   // [rows, n / 8, 2] pieces of eight

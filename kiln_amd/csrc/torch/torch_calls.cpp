@@ -902,11 +902,14 @@ PyObject *py_moe_sort(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (m < 1 || top < 1 || top > 16 || m * top > kMostPairs) Py_RETURN_NONE;
     Launch at_(device);
     at::Tensor order = empty_of({m * top}, at::kInt, device), first = empty_of({experts + 1}, at::kInt, device), place = empty_of({m, top}, at::kInt, device);
-    const at::Tensor scratch = empty_of({(int64_t)g_lib.moe_sort_scratch_bytes(experts)}, at::kByte, device);
+    const size_t scratch_bytes = g_lib.moe_sort_scratch_bytes((int)m, (int)top, experts);
+    at::Tensor scratch;
+    if (scratch_bytes) scratch = empty_of({(int64_t)scratch_bytes}, at::kByte, device);
     int st;
     Py_BEGIN_ALLOW_THREADS
     st = g_lib.moe_sort(static_cast<const int *>(of.data_ptr()), (int)m, (int)top, experts, static_cast<int *>(order.data_ptr()),
-                        static_cast<int *>(first.data_ptr()), static_cast<int *>(place.data_ptr()), device.index(), at_.stream, scratch.data_ptr());
+                        static_cast<int *>(first.data_ptr()), static_cast<int *>(place.data_ptr()), device.index(), at_.stream,
+                        scratch_bytes ? scratch.data_ptr() : nullptr);
     Py_END_ALLOW_THREADS
     if (st != KILN_W4A16_OK) Py_RETURN_NONE;
     return tuple_of<3>({std::move(order), std::move(first), std::move(place)});

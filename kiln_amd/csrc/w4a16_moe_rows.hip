@@ -139,10 +139,22 @@ struct RowsArgs {
     int tokens, top, experts, units;
 };
 
+// a thread's token and unit (32 bits where they do: a division of 64 takes longer than a small call's loads)
+struct Place {
+    int token, unit;
+    size_t at;
+    bool live;
+};
+__device__ __forceinline__ Place place_of(const RowsArgs &p) {
+    const size_t total = (size_t)p.tokens * p.units, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int token = total >> 32 ? (int)(i / p.units) : (int)((unsigned)i / (unsigned)p.units);
+    return {token, (int)(i - (size_t)token * p.units), i, i < total};
+}
+
 __global__ __launch_bounds__(256) void moe_gather_kernel(RowsArgs p) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)p.tokens * p.units) return;
-    const int token = (int)(i / p.units), unit = (int)(i - (size_t)token * p.units), placed = p.first[p.experts], pairs = p.tokens * p.top;
+    const auto [token, unit, i, live] = place_of(p);
+    if (!live) return;
+    const int placed = p.first[p.experts], pairs = p.tokens * p.top;
     const u32x4 v = reinterpret_cast<const u32x4 *>(p.in)[i], zero = {0u, 0u, 0u, 0u};
     for (int j = 0; j < p.top; ++j) {
         const int at = p.place[(size_t)token * p.top + j];
@@ -152,12 +164,13 @@ __global__ __launch_bounds__(256) void moe_gather_kernel(RowsArgs p) {
 
 __device__ __forceinline__ float bf16_low(uint32_t v) { return __builtin_bit_cast(float, v << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t v) { return __builtin_bit_cast(float, v & 0xFFFF0000u); }
-__device__ __forceinline__ uint32_t bf16_pair(float low, float high) { return f32_to_bf16_bits(low) | (uint32_t)f32_to_bf16_bits(high) << 16; }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bf16_pair(float low, float high) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)low, (__bf16)high}); }
 
 __global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs p) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)p.tokens * p.units) return;
-    const int token = (int)(i / p.units), unit = (int)(i - (size_t)token * p.units), placed = min(p.first[p.experts], p.tokens * p.top);
+    const auto [token, unit, i, live] = place_of(p);
+    if (!live) return;
+    const int placed = min(p.first[p.experts], p.tokens * p.top);
     float sum[8] = {};
     for (int j0 = 0; j0 < p.top; j0 += 8) {
         u32x4 v[8];
@@ -257,8 +270,12 @@ kiln_marlin_status_t rows_ok(int m, int top_k, int experts, int width) {
     return KILN_W4A16_OK;
 }
 int sort_block_pairs(int pairs) {
-    const int each = pairs <= kSortBlockPairs ? pairs : std::max(kSortBlockPairs, (pairs + kSortMaxBlocks - 1) / kSortMaxBlocks);
+    const int each = pairs <= kSortBlockPairs ? std::max(pairs, 1) : std::max(kSortBlockPairs, (pairs + kSortMaxBlocks - 1) / kSortMaxBlocks);
     return (each + kSortThreads - 1) / kSortThreads * kSortThreads;
+}
+int sort_blocks(int pairs) {
+    const int each = sort_block_pairs(pairs);
+    return pairs ? (pairs + each - 1) / each : 1;
 }
 kiln_marlin_status_t launched() { return hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH; }
 unsigned thread_blocks(int m, int units) { return (unsigned)(((size_t)m * units + 255) / 256); }
@@ -270,8 +287,10 @@ using namespace kiln;
 
 extern "C" {
 
-size_t kiln_w4a16_moe_sort_scratch_bytes(int experts) {
-    return (size_t)kSortMaxBlocks * ((experts < 1 ? 1 : experts > kMaxExperts ? kMaxExperts : experts) + 1) * sizeof(int);
+size_t kiln_w4a16_moe_sort_scratch_bytes(int prob_m, int top_k, int experts) {
+    if (rows_ok(prob_m, top_k, experts, 8) != KILN_W4A16_OK) return 0;
+    const int blocks = sort_blocks(prob_m * top_k);
+    return blocks == 1 ? 0 : (size_t)blocks * (experts + 1) * sizeof(int);
 }
 
 kiln_marlin_status_t kiln_w4a16_moe_sort(const int *expert_of, int prob_m, int top_k, int experts, int *order, int *first, int *place, int dev,
@@ -279,7 +298,8 @@ kiln_marlin_status_t kiln_w4a16_moe_sort(const int *expert_of, int prob_m, int t
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, 8)) return st;
     const int pairs = prob_m * top_k;
-    if (!first || !scratch || (pairs && (!expert_of || !order || !place))) return KILN_W4A16_ERR_ARGUMENT;
+    const int each = sort_block_pairs(pairs), blocks = sort_blocks(pairs);
+    if (!first || (blocks > 1 && !scratch) || (pairs && (!expert_of || !order || !place))) return KILN_W4A16_ERR_ARGUMENT;
     for (const void *p : {static_cast<const void *>(expert_of), static_cast<const void *>(order), static_cast<const void *>(first),
                           static_cast<const void *>(place), static_cast<const void *>(scratch)})
         if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
@@ -288,7 +308,6 @@ kiln_marlin_status_t kiln_w4a16_moe_sort(const int *expert_of, int prob_m, int t
         meet(order, bytes, place, bytes) || meet(order, bytes, first, first_bytes) || meet(place, bytes, first, first_bytes))
         return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    const int each = pairs ? sort_block_pairs(pairs) : kSortThreads, blocks = pairs ? (pairs + each - 1) / each : 1;
     const SortArgs a{expert_of, order, first, place, static_cast<int *>(scratch), pairs, experts, each};
     if (blocks > 1) moe_count_kernel<<<blocks, kSortThreads, 0, hs>>>(a);
     moe_sort_kernel<<<blocks, kSortThreads, 0, hs>>>(a);

@@ -802,7 +802,7 @@ def moe_sort(expert_of: torch.Tensor, experts: int):
     first = torch.empty(experts + 1, dtype=torch.int32, device=device)
     place = torch.empty((m, top_k), dtype=torch.int32, device=device)
     with torch.cuda.device(device):
-        scratch = torch.empty(lib.kiln_w4a16_moe_sort_scratch_bytes(experts), dtype=torch.uint8, device=device)
+        scratch = torch.empty(lib.kiln_w4a16_moe_sort_scratch_bytes(m, top_k, experts), dtype=torch.uint8, device=device)
         status = lib.kiln_w4a16_moe_sort(expert_of.data_ptr(), m, top_k, experts, order.data_ptr(), first.data_ptr(), place.data_ptr(),
                                          device.index or 0, _stream_of(device), scratch.data_ptr())
     _check_status(status, "kiln_w4a16_moe_sort", f"m={m}, top_k={top_k}, experts={experts}")
