@@ -8,7 +8,8 @@
 * `kiln_amd.lora`         -- stacked LoRA adapters fused into the GEMM epilogue
   (mirror of the call sites in crates/kiln-model/src/forward.rs:2923-2946), and
   banks of adapters that rows choose from, with their gradients
-* `kiln_amd.moe`          -- a mixture-of-experts MLP on packed experts
+* `kiln_amd.moe`          -- a mixture-of-experts MLP on packed experts, for a few
+  tokens and for many, and its gradients
 
 All are thin hosts over the C ABI in include/kiln_w4a16.h; torch is used for
 device memory and streams only.

@@ -272,27 +272,19 @@ __device__ __forceinline__ void few_product(const char *rows, const u32x4 (&w)[2
     const bf16x8 bias = bf16x8_splat(0xC308C308u);  // -136
     static_assert(kCodeBias == 136.f, "");
     const int l32 = lane & 31, h = lane >> 5;
-    // a step's operands are made behind the products of the one before; left to itself the compiler reads all eight steps' first
-    bf16x8 a[2][MI], b[2][2];
-    auto prepare = [&](auto sc) {
-        constexpr int step = decltype(sc)::value;
+    unrolled<0, 8>([&](auto sc) {  // (steps kept apart, each one's operands made behind the one before's products: 96 tokens 48.7 us, not 44.5)
+        constexpr int step = decltype(sc)::value, t = step >> 1, v = step & 1;
+        bf16x8 a[MI];
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-            a[step & 1][mi] = *reinterpret_cast<const bf16x8 *>(rows + (32 * mi + l32) * 256 + (((2 * step + h) ^ (l32 & 15)) << 4));
+        for (int mi = 0; mi < MI; ++mi) a[mi] = *reinterpret_cast<const bf16x8 *>(rows + (32 * mi + l32) * 256 + (((2 * step + h) ^ (l32 & 15)) << 4));
 #pragma unroll
-        for (int ni = 0; ni < 2; ++ni) b[step & 1][ni] = codes_to_bf16x8(w[ni][step & 1][step >> 1], dq);
-    };
-    prepare(std::integral_constant<int, 0>{});
-    unrolled<0, 8>([&](auto sc) {
-        constexpr int step = decltype(sc)::value, now = step & 1;
-        if constexpr (step < 7) prepare(std::integral_constant<int, step + 1>{});
+        for (int mi = 0; mi < MI; ++mi) off[mi] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[mi], bias, step == 0 ? f32x16{} : off[mi], 0, 0, 0);
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-            off[mi] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[now][mi], bias, step == 0 ? f32x16{} : off[mi], 0, 0, 0);
+        for (int ni = 0; ni < 2; ++ni) {
+            const bf16x8 b = codes_to_bf16x8(w[ni][v][t], dq);
 #pragma unroll
-            for (int ni = 0; ni < 2; ++ni) tile.acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[now][mi], b[now][ni], tile.acc[mi][ni], 0, 0, 0);
+            for (int mi = 0; mi < MI; ++mi) tile.acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[mi], b, tile.acc[mi][ni], 0, 0, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
     });
 }
 // the sums without the surplus, in units of the next group's scale

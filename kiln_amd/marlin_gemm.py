@@ -895,11 +895,11 @@ def moe_gather_backward(d_rows: torch.Tensor, first: torch.Tensor, place: torch.
 def moe_combine(rows: torch.Tensor, weights: torch.Tensor, first: torch.Tensor, place: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The experts' rows back to their tokens: `y[i] = sum_j weights[i, j] * rows[place[i, j]]`, bf16 `[m * top_k, width]` -> `[m, width]`, `weights`
     f32 `[m, top_k]` (`moe_route`), summed in f32 and rounded once; nothing from pairs without an expert."""
+    if weights is None:
+        _bail("weights must be f32 [m, top_k]")
     y = _calls.moe_combine(rows, weights, first, place, out)
     if y is not None:
         return y
-    if weights is None:
-        _bail("weights must be f32 [m, top_k]")
     return _combine(rows, weights, first, place, out)
 
 
@@ -1059,3 +1059,17 @@ def swiglu_keep_backward(dh: torch.Tensor, whole: torch.Tensor, exponents: torch
                                                                  h.data_ptr() if recompute else None, m, n_out, device.index or 0, _stream_of(device))
         _check_status(status, "kiln_w4a16_swiglu_keep_backward", f"m={m}, n_out={n_out}")
     return (d_gate_up, h) if recompute else d_gate_up
+
+
+def marlin_w4a16_mlp_keep(x: torch.Tensor, b_gate_up: torch.Tensor, s_gate_up: torch.Tensor, b_down: torch.Tensor, s_down: torch.Tensor, groupsize: int):
+    """`marlin_w4a16_mlp` in training: `(y, whole, exponents)`, the latter two for `marlin_w4a16_mlp_backward` (`swiglu_keep`).  Gate and up are rounded
+    to bf16 before `silu(gate) * up`, as the reference's are (crates/kiln-model/src/forward.rs:2771-2819)."""
+    h, whole, exponents = swiglu_keep(marlin_w4a16_gemm(x, b_gate_up, s_gate_up, groupsize))
+    return marlin_w4a16_gemm(h, b_down, s_down, groupsize), whole, exponents
+
+
+def marlin_w4a16_mlp_backward(dy: torch.Tensor, whole: torch.Tensor, exponents: torch.Tensor, b_gate_up: torch.Tensor, s_gate_up: torch.Tensor,
+                              b_down: torch.Tensor, s_down: torch.Tensor, groupsize: int) -> torch.Tensor:
+    """The gradient of `marlin_w4a16_mlp_keep`'s `x` from `dy` bf16 `[m, n_down]`, the packs frozen: bf16 `[m, hidden]`."""
+    dh = marlin_w4a16_gemm_backward(dy, b_down, s_down, groupsize)
+    return marlin_w4a16_gemm_backward(swiglu_keep_backward(dh, whole, exponents), b_gate_up, s_gate_up, groupsize)

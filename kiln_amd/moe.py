@@ -1,4 +1,5 @@
-"""A mixture-of-experts MLP on packed experts: the router's choice, the experts it names, their sum.
+"""A mixture-of-experts MLP on packed experts: the router's choice, the experts it names, their sum; for a few tokens as one call, for many with their
+rows in the order of the experts, and with its gradients.
 
 The reference's model family is dense (crates/kiln-core/src/config.rs:78-101): its MLP is `marlin_gemm.marlin_w4a16_mlp`
 (crates/kiln-model/src/forward.rs:2723-2848), of which every expert here is one.
@@ -49,3 +50,52 @@ def moe_forward(x: torch.Tensor, router_t: torch.Tensor, experts: MoeExperts, to
     y = marlin_gemm.marlin_w4a16_moe(rows, expert_of, weights, experts.b_gate_up, experts.s_gate_up, experts.b_down, experts.s_down,
                                      experts.groupsize)
     return y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+def experts_many(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Tensor, experts: MoeExperts) -> torch.Tensor:
+    """`marlin_w4a16_moe` for many tokens: the choices sorted by expert, gate, up and `silu(gate) * up` straight from the tokens, the down projection, and
+    the rows back to their tokens with their weights.  `x` bf16 `[m, hidden]`, `expert_of` i32 and `weights` f32 `[m, top_k]`.  (`marlin_w4a16_moe` reads the
+    packs of a run of 64 tokens' experts for every run; here they are read once.  A pair's row is rounded to bf16 before the sum.)"""
+    order, first, place = marlin_gemm.moe_sort(expert_of, experts.b_down.shape[0])
+    h = marlin_gemm.marlin_w4a16_gemm_experts(x, first, experts.b_gate_up, experts.s_gate_up, experts.groupsize, order=order, top_k=expert_of.shape[1],
+                                              swiglu=True)
+    rows = marlin_gemm.marlin_w4a16_gemm_experts(h, first, experts.b_down, experts.s_down, experts.groupsize)
+    return marlin_gemm.moe_combine(rows, weights, first, place)
+
+
+def moe_forward_many(x: torch.Tensor, router_t: torch.Tensor, experts: MoeExperts, top_k: int, renormalise: bool = True) -> torch.Tensor:
+    """`moe_forward` for many tokens (`experts_many`): a prefill.  Worth it from about 33 tokens on; below, `moe_forward` has fewer launches."""
+    rows = x.reshape(-1, x.shape[-1])
+    expert_of, weights = marlin_gemm.moe_route(rows @ router_t, top_k, renormalise)
+    y = experts_many(rows, expert_of, weights, experts)
+    return y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+@dataclass
+class MoeKept:
+    """What `experts_backward` needs of a forward pass: the order, the experts' rows (for the weights' gradient), and gate and up in 8 bits."""
+    first: torch.Tensor
+    place: torch.Tensor
+    weights: torch.Tensor
+    rows: torch.Tensor        # bf16 [m * top_k, n_down]
+    whole: torch.Tensor       # i8 [m * top_k, 2 n_out]
+    exponents: torch.Tensor   # u8 [m * top_k, n_out / 32, 2]
+
+
+def experts_keep(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Tensor, experts: MoeExperts):
+    """`experts_many` in training: `(y, kept)`, `kept` for `experts_backward`.  Gate and up are rounded to bf16 before `silu(gate) * up` (they are a tensor
+    here) and kept in 8 bits (`marlin_gemm.swiglu_keep`)."""
+    order, first, place = marlin_gemm.moe_sort(expert_of, experts.b_down.shape[0])
+    gate_up = marlin_gemm.marlin_w4a16_gemm_experts(x, first, experts.b_gate_up, experts.s_gate_up, experts.groupsize, order=order, top_k=expert_of.shape[1])
+    h, whole, exponents = marlin_gemm.swiglu_keep(gate_up)
+    rows = marlin_gemm.marlin_w4a16_gemm_experts(h, first, experts.b_down, experts.s_down, experts.groupsize)
+    return marlin_gemm.moe_combine(rows, weights, first, place), MoeKept(first, place, weights, rows, whole, exponents)
+
+
+def experts_backward(dy: torch.Tensor, kept: MoeKept, experts: MoeExperts):
+    """The gradients of `experts_keep(x, ..., weights, ...)` from `dy` bf16 `[m, n_down]`, the packs frozen: `(dx bf16 [m, hidden], d_weights f32 [m, top_k])`."""
+    d_rows, d_weights = marlin_gemm.moe_combine_backward(dy, kept.rows, kept.weights, kept.first, kept.place)
+    dh = marlin_gemm.marlin_w4a16_gemm_experts_backward(d_rows, kept.first, experts.b_down, experts.s_down, experts.groupsize)
+    d_gate_up = marlin_gemm.swiglu_keep_backward(dh, kept.whole, kept.exponents)
+    d_rows = marlin_gemm.marlin_w4a16_gemm_experts_backward(d_gate_up, kept.first, experts.b_gate_up, experts.s_gate_up, experts.groupsize)
+    return marlin_gemm.moe_gather_backward(d_rows, kept.first, kept.place), d_weights

@@ -42,6 +42,7 @@ def sorted_by_hand(of, experts):
 
 def silu_times(y):
     """silu(gate) * up of float64 columns in the packed order."""
-    both = y.reshape(len(y), -1, 2, 8)
-    gate, up = both[:, :, 0].reshape(len(y), -1), both[:, :, 1].reshape(len(y), -1)
+    n = y.shape[1] // 2
+    both = y.reshape(len(y), n // 8, 2, 8)
+    gate, up = both[:, :, 0].reshape(len(y), n), both[:, :, 1].reshape(len(y), n)
     return gate * torch.sigmoid(gate) * up
