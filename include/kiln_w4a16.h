@@ -403,7 +403,8 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(
  *   y      bf16 [rows, n], rounded once; with `swiglu` bf16 [rows, n / 2] = silu(gate) * up of packs as for kiln_w4a16_gemm_swiglu; shares no
  *          memory with x (refused)
  *   scratch  kiln_w4a16_gemm_experts_scratch_bytes(x_rows, k), on 16 bytes, holds nothing between calls
- * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024.
+ *   dev      stream's device, whose compute units the launches are planned for (in the other calls on sorted rows it is not used)
+ * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024, x_rows <= 2^29.
  * The gradient of the rows, the packs frozen: dx[p] = dy[p] * dequant(B_e, s_e)^T, bf16 [rows, k], rounded once; a weight enters the product
  * rounded to bf16, as in kiln_w4a16_gemm_bank_backward.
  */
@@ -425,8 +426,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(
  *              magnitude (at least 1); whole is rounded to the nearest, ties to even, at most 127 in magnitude.  A block with an infinity or
  *              NaN has exponent 255 and is NaN.
  * The backward pass out of them: with s = 1 / (1 + exp(-gate)), d_up = dh * gate * s and d_gate = dh * up * s * (1 + gate * (1 - s)), bf16 in
- * gate_up's columns, rounded once; h again unless NULL (of the kept values).  n_out % 128 == 0; all on 16 bytes; no result shares memory with
- * an operand or another result (refused).
+ * gate_up's columns, rounded once; h again unless NULL (of the kept values).  n_out % 128 == 0; all on 16 bytes (exponents on 2); no result shares
+ * memory with an operand or another result (refused).
  */
 kiln_marlin_status_t kiln_w4a16_swiglu_keep(
     const void *gate_up, void *h, void *whole, void *exponents, int prob_m, int n_out, int dev, void *stream);

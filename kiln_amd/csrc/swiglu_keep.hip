@@ -12,12 +12,10 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <initializer_list>
-
-#include "bank.h"
 #include "device_common.h"
 #include "kiln_w4a16.h"
 #include "launch.h"
+#include "pieces.h"
 
 namespace kiln {
 namespace {
@@ -125,25 +123,6 @@ kiln_marlin_status_t shape_ok(int m, int n_out) {
     if (m < 0 || n_out < 1 || n_out % 128 != 0 || n_out > INT32_MAX / 2) return KILN_W4A16_ERR_PROB_SHAPE;
     return ((int64_t)m * (n_out / 8) + 255) / 256 > INT32_MAX ? KILN_W4A16_ERR_KERN_SHAPE : KILN_W4A16_OK;
 }
-bool aligned(std::initializer_list<const void *> pointers) {
-    for (const void *p : pointers)
-        if (!p || reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
-    return true;
-}
-// do any two of these share memory?
-struct Piece {
-    const void *at;
-    size_t bytes;
-};
-bool any_meet(std::initializer_list<Piece> written, std::initializer_list<Piece> read) {
-    for (const Piece *i = written.begin(); i != written.end(); ++i) {
-        for (const Piece *j = i + 1; j != written.end(); ++j)
-            if (meet(i->at, i->bytes, j->at, j->bytes)) return true;
-        for (const Piece &r : read)
-            if (meet(i->at, i->bytes, r.at, r.bytes)) return true;
-    }
-    return false;
-}
 
 }  // namespace
 }  // namespace kiln
@@ -156,7 +135,7 @@ kiln_marlin_status_t kiln_w4a16_swiglu_keep(const void *gate_up, void *h, void *
     (void)dev;
     if (const kiln_marlin_status_t st = shape_ok(prob_m, n_out)) return st;
     if (prob_m == 0) return KILN_W4A16_OK;
-    if (!aligned({gate_up, h, whole, exponents})) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {gate_up, h, whole}) || !all_on(2, {exponents})) return KILN_W4A16_ERR_ARGUMENT;
     const size_t n = (size_t)prob_m * n_out;
     if (any_meet({{h, 2 * n}, {whole, 2 * n}, {exponents, n / 16}}, {{gate_up, 4 * n}})) return KILN_W4A16_ERR_ARGUMENT;
     const KeepArgs a{(const u32x4 *)gate_up, nullptr, (u32x4 *)whole, (uint16_t *)exponents, (u32x4 *)h, nullptr, n / 8};
@@ -169,9 +148,9 @@ kiln_marlin_status_t kiln_w4a16_swiglu_keep_backward(const void *dh, const void 
     (void)dev;
     if (const kiln_marlin_status_t st = shape_ok(prob_m, n_out)) return st;
     if (prob_m == 0) return KILN_W4A16_OK;
-    if (!aligned({dh, whole, exponents, d_gate_up}) || reinterpret_cast<uintptr_t>(h) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {dh, whole, d_gate_up}) || !all_on(2, {exponents}) || reinterpret_cast<uintptr_t>(h) % 16 != 0) return KILN_W4A16_ERR_ARGUMENT;
     const size_t n = (size_t)prob_m * n_out;
-    if (any_meet({{d_gate_up, 4 * n}, {h, h ? 2 * n : 0}}, {{dh, 2 * n}, {whole, 2 * n}, {exponents, n / 16}})) return KILN_W4A16_ERR_ARGUMENT;
+    if (any_meet({{d_gate_up, 4 * n}, {h, 2 * n}}, {{dh, 2 * n}, {whole, 2 * n}, {exponents, n / 16}})) return KILN_W4A16_ERR_ARGUMENT;
     const KeepArgs a{nullptr, (const u32x4 *)dh, (u32x4 *)const_cast<void *>(whole), (uint16_t *)const_cast<void *>(exponents), (u32x4 *)h, (u32x4 *)d_gate_up, n / 8};
     const unsigned grid = (unsigned)((a.pieces + 255) / 256);
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);

@@ -7,24 +7,31 @@
 // experts: the host knows how many rows there are, not whose, so it starts as many blocks as any choice could need and a block finds its
 // expert, rows and columns in `first`; those without work leave.
 //
-// Either way a block is four wavefronts side by side, 32 MI rows x 256 columns of the result (64 to a wavefront: tiles of
-// v_mfma_f32_32x32x16_bf16), 32 of the contraction to a stage.  Everything comes straight to LDS, four stages of the rows in flight.
+// A block is four wavefronts; tiles of v_mfma_f32_32x32x16_bf16, everything straight to LDS in stages of the contraction with several on their way.  By the rows
+// that an expert has (choose_blocks) it takes
+//   128 rows x 256 columns: four row tiles x 64 columns to a wavefront, products scheduled by hand,
+//   64 or 32 rows x 256 columns: larger stages, the loads bound them,
+//   32 rows x 64 columns (the gradient: 128), the wavefronts sharing out the contraction, where the others would leave compute units idle.
+// In blocks of 128 and 64 rows what is left of an expert goes as in the smaller ones.
+//
+// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 185-200, the gradient 215-227: the vector instructions that expand the codes, beside
+// the matrix cores (48 % and 42 % of the cycles busy), and rounds of blocks that do not come out even; 768 rows of 64 experts, 2560 -> 2048: 41-48, 3.6 to 4.3 TB/s of
+// packs; 2331 rows of 24 experts, 1280 -> 2048: 27, a round and a half of blocks, each one's start and latencies.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
-#include <initializer_list>
 
 #include "async_loads.h"
-#include "bank.h"
 #include "device_common.h"
 #include "kiln_w4a16.h"
 #include "launch.h"
+#include "pieces.h"
 
 namespace kiln {
 namespace {
 
-constexpr int kMaxExperts = 1024;
+constexpr int kMaxExperts = 1024, kMaxRows = 1 << 29;  // (a row's sum has a 32-bit offset)
 constexpr int kWaves = 4, kThreads = kWaves * 64, kColumns = kWaves * 64, kStages = 4;
 
 struct ExpertsArgs {
@@ -272,7 +279,7 @@ __device__ __forceinline__ void few_product(const char *rows, const u32x4 (&w)[2
     const bf16x8 bias = bf16x8_splat(0xC308C308u);  // -136
     static_assert(kCodeBias == 136.f, "");
     const int l32 = lane & 31, h = lane >> 5;
-    unrolled<0, 8>([&](auto sc) {  // (steps kept apart, each one's operands made behind the one before's products: 96 tokens 48.7 us, not 44.5)
+    unrolled<0, 8>([&](auto sc) {
         constexpr int step = decltype(sc)::value, t = step >> 1, v = step & 1;
         bf16x8 a[MI];
 #pragma unroll
@@ -1064,11 +1071,9 @@ kiln_marlin_status_t experts_ok(int rows, int n, int k, int experts, int groupsi
     if (experts < 1 || experts > kMaxExperts) return KILN_W4A16_ERR_KERN_SHAPE;
     return most_tiles(rows, experts, 32) * (std::max((int64_t)n, (int64_t)k) / 64 + 1) > INT32_MAX - 8 ? KILN_W4A16_ERR_KERN_SHAPE : KILN_W4A16_OK;
 }
-bool aligned(std::initializer_list<const void *> pointers) {
-    for (const void *p : pointers)
-        if (!p || reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
-    return true;
-}
+// what a call reads of the packs and the order
+Piece pack_of(const void *b, int n, int k, int experts) { return {b, (size_t)experts * k * n / 2}; }
+Piece scales_of(const void *s, int n, int k, int experts, int groupsize) { return {s, (size_t)experts * (groupsize == -1 ? 1 : k / kGroupK) * n * 2}; }
 
 }  // namespace
 }  // namespace kiln
@@ -1085,11 +1090,14 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts(const void *x, const int *first, co
                                              int top_k, int prob_n, int prob_k, int experts, int groupsize, int swiglu, int dev, void *stream, void *scratch) {
     if (const kiln_marlin_status_t st = experts_ok(rows, prob_n, prob_k, experts, groupsize)) return st;
     if (x_rows < 0 || top_k < 1 || (order ? (int64_t)x_rows * top_k != rows : x_rows != rows)) return KILN_W4A16_ERR_KERN_SHAPE;
-    if ((int64_t)x_rows * (prob_k / kGroupK) > (int64_t)INT32_MAX * 16) return KILN_W4A16_ERR_KERN_SHAPE;
+    if (x_rows > kMaxRows || (int64_t)x_rows * (prob_k / kGroupK) > (int64_t)INT32_MAX * 16) return KILN_W4A16_ERR_KERN_SHAPE;
     if (rows == 0) return KILN_W4A16_OK;
-    if (!aligned({x, b, s, y, scratch}) || !first) return KILN_W4A16_ERR_ARGUMENT;
-    const int width = swiglu ? prob_n / 2 : prob_n;
-    if (meet(y, (size_t)rows * width * 2, x, (size_t)x_rows * prob_k * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {x, b, s, y, scratch}) || !all_on(4, {first}) || reinterpret_cast<uintptr_t>(order) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t width = swiglu ? prob_n / 2 : prob_n;
+    if (any_meet({{y, rows * width * 2}, {scratch, kiln_w4a16_gemm_experts_scratch_bytes(x_rows, prob_k)}},
+                 {{x, (size_t)x_rows * prob_k * 2}, {first, ((size_t)experts + 1) * 4}, {order, (size_t)rows * 4}, pack_of(b, prob_n, prob_k, experts),
+                  scales_of(s, prob_n, prob_k, experts, groupsize)}))
+        return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const Blocks blocks = forward_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
     if (blocks == Blocks::kFourTiles) {
@@ -1120,8 +1128,10 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(const void *dy, const int 
                                                       int experts, int groupsize, int dev, void *stream) {
     if (const kiln_marlin_status_t st = experts_ok(rows, prob_n, prob_k, experts, groupsize)) return st;
     if (rows == 0) return KILN_W4A16_OK;
-    if (!aligned({dy, b, s, dx}) || !first) return KILN_W4A16_ERR_ARGUMENT;
-    if (meet(dx, (size_t)rows * prob_k * 2, dy, (size_t)rows * prob_n * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {dy, b, s, dx}) || !all_on(4, {first})) return KILN_W4A16_ERR_ARGUMENT;
+    if (any_meet({{dx, (size_t)rows * prob_k * 2}}, {{dy, (size_t)rows * prob_n * 2}, {first, ((size_t)experts + 1) * 4}, pack_of(b, prob_n, prob_k, experts),
+                                                     scales_of(s, prob_n, prob_k, experts, groupsize)}))
+        return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const Blocks blocks = gradient_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
     ExpertsArgs a{(const uint16_t *)dy, first, nullptr, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)dx, nullptr,

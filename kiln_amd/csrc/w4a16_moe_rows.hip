@@ -10,12 +10,11 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <initializer_list>
 
-#include "bank.h"
 #include "device_common.h"
 #include "kiln_w4a16.h"
 #include "launch.h"
+#include "pieces.h"
 
 namespace kiln {
 namespace {
@@ -257,11 +256,6 @@ __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
 }
 
 // ---- the entry points' checks --------------------------------------------------------------------------------------
-bool on_16(std::initializer_list<const void *> pointers) {
-    for (const void *p : pointers)
-        if (!p || reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
-    return true;
-}
 // rows of `width` bf16 values for m tokens: KILN_W4A16_OK, or why not
 kiln_marlin_status_t rows_ok(int m, int top_k, int experts, int width) {
     if (m < 0 || width < 1 || width % 8 != 0) return KILN_W4A16_ERR_PROB_SHAPE;
@@ -299,13 +293,10 @@ kiln_marlin_status_t kiln_w4a16_moe_sort(const int *expert_of, int prob_m, int t
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, 8)) return st;
     const int pairs = prob_m * top_k;
     const int each = sort_block_pairs(pairs), blocks = sort_blocks(pairs);
-    if (!first || (blocks > 1 && !scratch) || (pairs && (!expert_of || !order || !place))) return KILN_W4A16_ERR_ARGUMENT;
-    for (const void *p : {static_cast<const void *>(expert_of), static_cast<const void *>(order), static_cast<const void *>(first),
-                          static_cast<const void *>(place), static_cast<const void *>(scratch)})
-        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
-    const size_t bytes = (size_t)pairs * 4, first_bytes = ((size_t)experts + 1) * 4;
-    if (meet(expert_of, bytes, order, bytes) || meet(expert_of, bytes, place, bytes) || meet(expert_of, bytes, first, first_bytes) ||
-        meet(order, bytes, place, bytes) || meet(order, bytes, first, first_bytes) || meet(place, bytes, first, first_bytes))
+    if (!all_on(4, {first}) || (blocks > 1 && !all_on(4, {scratch})) || (pairs && !all_on(4, {expert_of, order, place}))) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t bytes = (size_t)pairs * 4;
+    if (any_meet({{order, bytes}, {place, bytes}, {first, ((size_t)experts + 1) * 4}, {scratch, kiln_w4a16_moe_sort_scratch_bytes(prob_m, top_k, experts)}},
+                 {{expert_of, bytes}}))
         return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const SortArgs a{expert_of, order, first, place, static_cast<int *>(scratch), pairs, experts, each};
@@ -319,8 +310,9 @@ kiln_marlin_status_t kiln_w4a16_moe_gather(const void *x, const int *first, cons
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
     if (prob_m == 0) return KILN_W4A16_OK;
-    if (!on_16({x, rows}) || !first || !place) return KILN_W4A16_ERR_ARGUMENT;
-    if (meet(rows, (size_t)prob_m * top_k * width * 2, x, (size_t)prob_m * width * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {x, rows}) || !all_on(4, {first, place})) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t pairs = (size_t)prob_m * top_k, first_bytes = ((size_t)experts + 1) * 4;
+    if (any_meet({{rows, pairs * width * 2}}, {{x, (size_t)prob_m * width * 2}, {first, first_bytes}, {place, pairs * 4}})) return KILN_W4A16_ERR_ARGUMENT;
     const RowsArgs a{(const uint16_t *)x, nullptr, nullptr, first, place, (uint16_t *)rows, nullptr, prob_m, top_k, experts, width / 8};
     moe_gather_kernel<<<thread_blocks(prob_m, width / 8), 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
     return launched();
@@ -331,8 +323,10 @@ kiln_marlin_status_t kiln_w4a16_moe_combine(const void *rows, const float *weigh
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
     if (prob_m == 0) return KILN_W4A16_OK;
-    if (!on_16({rows, y}) || !first || !place) return KILN_W4A16_ERR_ARGUMENT;
-    if (meet(y, (size_t)prob_m * width * 2, rows, (size_t)prob_m * top_k * width * 2)) return KILN_W4A16_ERR_ARGUMENT;
+    if (!all_on(16, {rows, y}) || !all_on(4, {first, place}) || reinterpret_cast<uintptr_t>(weights) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t pairs = (size_t)prob_m * top_k, first_bytes = ((size_t)experts + 1) * 4;
+    if (any_meet({{y, (size_t)prob_m * width * 2}}, {{rows, pairs * width * 2}, {weights, pairs * 4}, {first, first_bytes}, {place, pairs * 4}}))
+        return KILN_W4A16_ERR_ARGUMENT;
     const RowsArgs a{(const uint16_t *)rows, nullptr, weights, first, place, (uint16_t *)y, nullptr, prob_m, top_k, experts, width / 8};
     moe_combine_kernel<<<thread_blocks(prob_m, width / 8), 256, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
     return launched();
@@ -343,10 +337,10 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
     if (prob_m == 0) return KILN_W4A16_OK;
-    if (!on_16({dy, rows, d_rows}) || !weights || !first || !place || !d_weights) return KILN_W4A16_ERR_ARGUMENT;
-    const size_t rows_bytes = (size_t)prob_m * top_k * width * 2, pair_bytes = (size_t)prob_m * top_k * 4;
-    if (meet(d_rows, rows_bytes, rows, rows_bytes) || meet(d_rows, rows_bytes, dy, (size_t)prob_m * width * 2) ||
-        meet(d_weights, pair_bytes, weights, pair_bytes))
+    if (!all_on(16, {dy, rows, d_rows}) || !all_on(4, {weights, first, place, d_weights})) return KILN_W4A16_ERR_ARGUMENT;
+    const size_t pairs = (size_t)prob_m * top_k, first_bytes = ((size_t)experts + 1) * 4;
+    if (any_meet({{d_rows, pairs * width * 2}, {d_weights, pairs * 4}},
+                 {{dy, (size_t)prob_m * width * 2}, {rows, pairs * width * 2}, {weights, pairs * 4}, {first, first_bytes}, {place, pairs * 4}}))
         return KILN_W4A16_ERR_ARGUMENT;
     const RowsArgs a{(const uint16_t *)dy, (const uint16_t *)rows, weights, first, place, (uint16_t *)d_rows, d_weights, prob_m, top_k, experts, width / 8};
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);

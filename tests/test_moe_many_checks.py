@@ -17,7 +17,7 @@ def at(base, bytes):
     return ctypes.c_void_p(base.value + bytes)
 
 
-def sort(of=P, m=600, top=4, experts=8, order=R[0], first=R[1], place=R[2], scratch=P):
+def sort(of=P, m=600, top=4, experts=8, order=R[0], first=R[1], place=R[2], scratch=R[3]):
     return _lib.load().kiln_w4a16_moe_sort(of, m, top, experts, order, first, place, 0, None, scratch)
 
 
@@ -33,7 +33,7 @@ def combine_backward(dy=P, rows=P, weights=P, first=P, place=P, d_rows=R[0], d_w
     return _lib.load().kiln_w4a16_moe_combine_backward(dy, rows, weights, first, place, d_rows, d_weights, m, top, experts, width, 0, None)
 
 
-def experts(x=P, first=P, order=None, b=P, s=P, y=R[0], rows=8, x_rows=8, top=1, n=512, k=256, count=4, g=128, swiglu=0, scratch=P):
+def experts(x=P, first=P, order=None, b=P, s=P, y=R[0], rows=8, x_rows=8, top=1, n=512, k=256, count=4, g=128, swiglu=0, scratch=R[3]):
     return _lib.load().kiln_w4a16_gemm_experts(x, first, order, b, s, y, rows, x_rows, top, n, k, count, g, swiglu, 0, None, scratch)
 
 
@@ -61,7 +61,7 @@ ROUTED = (dict(top=0), dict(top=17), dict(experts=0), dict(experts=1025), dict(m
 def test_sort_refuses():
     refuses(sort, (dict(m=-1),), ROUTED,
             (*(dict([(name, bad)]) for name in ("of", "order", "first", "place", "scratch") for bad in (None, ODD4)),
-             dict(order=P), dict(place=P), dict(first=P), dict(place=R[0]), dict(first=at(R[0], 600 * 4 * 4 - 4)), dict(first=at(R[2], 16))))
+             dict(order=P), dict(place=P), dict(first=P), dict(place=R[0]), dict(first=at(R[0], 600 * 4 * 4 - 4)), dict(first=at(R[2], 16)), dict(scratch=P), dict(scratch=R[0])))
 
 
 def test_rows_refuse():
@@ -69,24 +69,25 @@ def test_rows_refuse():
     for call, pointers, plain in ((gather, ("x", "rows"), ("first", "place")), (combine, ("rows", "y"), ("first", "place")),
                                   (combine_backward, ("dy", "rows", "d_rows"), ("first", "place", "weights", "d_weights"))):
         refuses(call, shape, ROUTED, (*(dict([(name, bad)]) for name in pointers for bad in (None, ODD)), *(dict([(name, None)]) for name in plain)))
-    refuses(gather, (), (), (dict(rows=P), dict(rows=at(P, 4 * 64 * 2 - 16)), dict(x=at(R[0], 4 * 2 * 64 * 2 - 16))))
-    refuses(combine, (), (), (dict(y=P), dict(rows=at(R[0], 16))))
+    refuses(gather, (), (), (dict(place=R[0]), dict(first=R[0]), dict(rows=P), dict(rows=at(P, 4 * 64 * 2 - 16)), dict(x=at(R[0], 4 * 2 * 64 * 2 - 16))))
+    refuses(combine, (), (), (dict(weights=R[0]), dict(place=R[0]), dict(weights=ODD4), dict(y=P), dict(rows=at(R[0], 16))))
     refuses(combine_backward, (), (), (dict(d_rows=P), dict(dy=at(R[0], 16)), dict(d_weights=P)))
 
 
 def test_products_refuse():
     shape = (dict(n=300), dict(k=200), dict(g=64), dict(n=0), dict(k=0), dict(rows=-1))
     refuses(experts, shape, (dict(count=0), dict(count=1025), dict(x_rows=7), dict(order=P, x_rows=8, top=2), dict(order=P, x_rows=4, top=0), dict(x_rows=-1, rows=0)),
-            (*(dict([(name, bad)]) for name in ("x", "b", "s", "y", "scratch") for bad in (None, ODD)), dict(first=None), dict(y=P), dict(x=at(R[0], 8 * 512 * 2 - 16))))
+            (*(dict([(name, bad)]) for name in ("x", "b", "s", "y", "scratch") for bad in (None, ODD)), dict(first=None), dict(first=ODD4), dict(y=P), dict(x=at(R[0], 8 * 512 * 2 - 16)),
+             dict(b=at(R[0], 16)), dict(s=R[0]), dict(first=R[0]), dict(order=R[0], x_rows=4, top=2), dict(scratch=R[0]), dict(order=ODD4, x_rows=4, top=2)))
     refuses(experts_backward, shape, (dict(count=0), dict(count=1025), dict(rows=2 ** 31 - 1, n=1 << 20)),
             (*(dict([(name, bad)]) for name in ("dy", "b", "s", "dx") for bad in (None, ODD)), dict(first=None), dict(dx=P), dict(dy=at(R[0], 16))))
 
 
 def test_kept_activations_refuse():
     shape = (dict(m=-1), dict(n=0), dict(n=64), dict(n=192), dict(n=-128), dict(n=1 << 30))
-    refuses(keep, shape, (), (*(dict([(name, bad)]) for name in ("gate_up", "h", "whole", "exponents") for bad in (None, ODD)),
+    refuses(keep, shape, (), (*(dict([(name, bad)]) for name in ("gate_up", "h", "whole") for bad in (None, ODD)), dict(exponents=None), dict(exponents=at(R[2], 1)),
                               dict(h=P), dict(whole=P), dict(exponents=P), dict(whole=R[0]), dict(exponents=at(R[1], 16))))
-    refuses(keep_backward, shape, (), (*(dict([(name, bad)]) for name in ("dh", "whole", "exponents", "d") for bad in (None, ODD)),
+    refuses(keep_backward, shape, (), (*(dict([(name, bad)]) for name in ("dh", "whole", "d") for bad in (None, ODD)), dict(exponents=None), dict(exponents=at(P, 1)),
                                        dict(h=ODD), dict(d=P), dict(h=P), dict(h=R[0])))
 
 
