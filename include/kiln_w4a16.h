@@ -560,7 +560,8 @@ int kiln_w4a16_layout_version(void);
  * kiln_w4a16_debug_bank_backward_plan: the product behind kiln_w4a16_gemm_bank_backward's dA, out[3] = {rows and columns of k to a block
  *   (0: calls of few rows, straight from the codes), slices of n}.  Returns 0, or 1 for sizes that no call may have.
  * kiln_w4a16_debug_experts_plan: the blocks of kiln_w4a16_gemm_experts (`backward`: of its gradient), 0 of 32 rows and few columns whose wavefronts share
- *   out the contraction, 1, 2, 3 of up to 32, 64, 128 rows x 256 columns; -1 for sizes that no call may have.
+ *   out the contraction, 1, 2, 3 of up to 32, 64, 128 rows x 256 columns, 4, 5 of up to 32, 64 rows with two sets of wavefronts; -1 for sizes
+ *   that no call may have.
  * kiln_w4a16_debug_workspace_operands: where a GEMM with stacked adapters of `rank` (a multiple of 8; 0: none) that is handed
  *   `workspace` (never followed) has its operands behind the zeroed prefix, out[6] = {row sums (0: none), partial tiles, projection
  *   (0: none), the end of all; of a projection that the mid-M kernel's launch writes and reads, its K slices and the bytes from one

@@ -11,12 +11,14 @@
 // that an expert has (choose_blocks) it takes
 //   128 rows x 256 columns: four row tiles x 64 columns to a wavefront, products scheduled by hand,
 //   64 or 32 rows x 256 columns: larger stages, the loads bound them,
+//   the same with two sets of wavefronts, for half of the contraction each, where a compute unit gets one block at most,
 //   32 rows x 64 columns (the gradient: 128), the wavefronts sharing out the contraction, where the others would leave compute units idle.
 // In blocks of 128 and 64 rows what is left of an expert goes as in the smaller ones.
 //
-// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 185-200, the gradient 215-227: the vector instructions that expand the codes, beside
-// the matrix cores (48 % and 42 % of the cycles busy), and rounds of blocks that do not come out even; 768 rows of 64 experts, 2560 -> 2048: 41-48, 3.6 to 4.3 TB/s of
-// packs; 2331 rows of 24 experts, 1280 -> 2048: 27, a round and a half of blocks, each one's start and latencies.
+// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 185-200, the gradient 215-227: rounds of blocks that do not come out even (the same rows in
+// equal parts 167 and 185), and power: on values of this kind the matrix instructions alone reach 1.6 to 1.8 PFLOP/s, not the 2.2 that they do on zeros, and the vector
+// instructions that expand the codes, reads of LDS and loads come on top (each left out for a measurement took 2 to 8 % off); 768 rows of 64 experts, 2560 -> 2048:
+// 41-48, 3.6 to 4.3 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 27, a round and a half of blocks, each one's start and latencies.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -100,7 +102,7 @@ __device__ __forceinline__ Work find_work(const int *__restrict__ first, int exp
 // rows of no expert: zeros in the block's columns
 __device__ __forceinline__ void write_zeros(uint16_t *y, int width, int row0, int rows, int column0, int columns) {
     const int units = columns / 8;
-    for (int i = threadIdx.x; i < rows * units; i += kThreads)
+    for (int i = threadIdx.x; i < rows * units; i += blockDim.x)
         *reinterpret_cast<u32x4 *>(y + (size_t)(row0 + i / units) * width + column0 + 8 * (i % units)) = u32x4{0u, 0u, 0u, 0u};
 }
 
@@ -224,12 +226,11 @@ struct Columns {
     }
 };
 
-// the scaled sums out, 32 rows at a time through the wavefront's own part of LDS, so that a row's columns are written side by side
+constexpr int kStoreBytes = kWaves * 32 * (128 + 16);
+// the scaled sums out, 32 rows at a time through the wavefront's own part of LDS (which nothing else uses any more), so that a row's columns are written
+// side by side
 template <int MI, bool SWIGLU>
 __device__ __forceinline__ void store_tile(const ExpertsArgs &p, const Work &work, char *lds, int lane, int wave, Tile<MI> &tile, const float (&scale)[2]) {
-    wait_vector_loads<0>();
-    wait_lds_reads();
-    __syncthreads();
     constexpr int kPitch = (SWIGLU ? 64 : 128) + 16;
     char *mine = lds + wave * (32 * kPitch);
     const int width = SWIGLU ? p.N / 2 : p.N, column0 = work.column * (SWIGLU ? kColumns / 2 : kColumns), l32 = lane & 31, h = lane >> 5;
@@ -305,9 +306,29 @@ __device__ __forceinline__ void few_rescale(Tile<MI> &tile, const f32x16 (&off)[
             for (int r = 0; r < 16; ++r) tile.acc[mi][ni][r] = (tile.acc[mi][ni][r] + off[mi][r]) * by[ni];
 }
 
-template <int MI, bool SWIGLU>
-__device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &work, char *lds, int lane, int wave) {
+// Where a compute unit gets one block at most, the block has a second set of four wavefronts for every other group (SETS), with LDS of its own; their sums
+// meet there at the end, the first set's before the second's.
+template <int MI>
+__device__ __forceinline__ void add_second_set(char *lds, int lane, int wave, int set, Tile<MI> &tile) {
+    static_assert(kStoreBytes + MI * 32768 <= 2 * FewLds<MI>::kBytes, "");
+    wait_vector_loads<0>();  // stages asked for past the end still write to LDS
+    wait_lds_reads();
+    __syncthreads();
+    float *box = reinterpret_cast<float *>(lds + kStoreBytes) + wave * (MI * 2048) + lane;
+    if (set == 1)
+#pragma unroll
+        for (int i = 0; i < MI * 32; ++i) box[i * 64] = tile.acc[i >> 5][i >> 4 & 1][i & 15];
+    __syncthreads();
+    if (set == 0)
+#pragma unroll
+        for (int i = 0; i < MI * 32; ++i) tile.acc[i >> 5][i >> 4 & 1][i & 15] += box[i * 64];
+}
+
+template <int MI, bool SWIGLU, int SETS>
+__device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &work, char *all_lds, int lane, int wave_of_all) {
     using L = FewLds<MI>;
+    const int wave = wave_of_all % kWaves, set = wave_of_all / kWaves;
+    char *const lds = all_lds + set * L::kBytes;
     constexpr int LR = 2 * MI, LS = LR + 5;  // loads of a wavefront and stage: four rows each; with the words and scales
     const Columns<SWIGLU> cols(p, work.expert, work.column * (kColumns / kTileN) + wave * 4, lane, wave * 4096, wave * 256);
     const int G = p.K / kGroupK;
@@ -318,9 +339,9 @@ __device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &wo
         const int row = 4 * (wave * LR + i) + (lane >> 4);
         rows[i] = reinterpret_cast<const char *>(p.x + (size_t)source_of(p, work, min(row, work.rows - 1)) * p.K) + (((lane & 15) ^ (row & 15)) << 4);
     }
-    auto fetch = [&](int g) {  // past the end: the last one again, so that the count of loads in flight stays what it is
-        const int from = min(g, G - 1);
-        const unsigned to = lds0 + (unsigned)(g % L::kRing) * L::kStage;
+    auto fetch = [&](int turn) {  // past the end: the last one again, so that the count of loads in flight stays what it is
+        const int from = min(SETS * turn + set, G - 1);
+        const unsigned to = lds0 + (unsigned)(turn % L::kRing) * L::kStage;
 #pragma unroll
         for (int i = 0; i < LR; ++i) load_to_lds_b128(rows[i] + (size_t)from * 256, to + (wave * LR + i) * 1024);
         cols.fetch(from, to + L::kRows, to + L::kScales);
@@ -334,15 +355,16 @@ __device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &wo
         for (int r = 0; r < 16; ++r) off[mi][r] = 0.f;
     float scale[2] = {0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < L::kRing - 1; ++g) fetch(g);
+    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch(turn);
 #pragma unroll 1
-    for (int g = 0; g < G; ++g) {
+    for (int turn = 0; SETS * turn < G; ++turn) {
         wait_vector_loads<(L::kRing - 2) * LS>();  // this stage has landed
         wait_lds_reads();
         __builtin_amdgcn_s_barrier();  // ... everywhere, and the one before has been read
         asm volatile("" : : : "memory");
-        fetch(g + L::kRing - 1);
-        const char *stage = lds + (g % L::kRing) * L::kStage;
+        fetch(turn + L::kRing - 1);
+        if (SETS > 1 && SETS * turn + set >= G) break;  // (the last turn of all)
+        const char *stage = lds + (turn % L::kRing) * L::kStage;
         u32x4 w[2][2];
         float by[2];
         cols.read_words(stage + L::kRows, w);
@@ -356,8 +378,16 @@ __device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &wo
         few_product<MI>(stage, w, dq, lane, tile, off);
     }
     few_rescale(tile, off, scale);
+    if constexpr (SETS > 1) {
+        add_second_set<MI>(all_lds, lane, wave, set, tile);
+        if (set == 1) return;
+    } else {
+        wait_vector_loads<0>();
+        wait_lds_reads();
+        __syncthreads();
+    }
     const float done[2] = {1.f, 1.f};
-    store_tile<MI, SWIGLU>(p, work, lds, lane, wave, tile, done);
+    store_tile<MI, SWIGLU>(p, work, all_lds, lane, wave, tile, done);
 }
 
 // Calls whose blocks would not fill the chip: a block takes 32 rows x 64 columns, its wavefronts every fourth group each.  They share nothing until
@@ -605,14 +635,17 @@ __device__ __forceinline__ void experts_many(const ExpertsArgs &p, const Work &w
     };
     for (int g = 0; g + 1 < G; ++g) group(g, std::false_type{});
     group(G - 1, std::true_type{});
+    wait_vector_loads<0>();  // stages asked for past the end still write to LDS
+    wait_lds_reads();
+    __syncthreads();
     store_tile<MI, SWIGLU>(p, work, lds, lane, wave, tile, scale);
 }
 
 // MAX: row tiles of the largest block.  A smaller one -- an expert's last rows -- multiplies no more row tiles than it needs.
-template <int MAX>
-constexpr int kForwardLds = std::max({FewLds<1>::kBytes, MAX >= 2 ? FewLds<2>::kBytes : 0, MAX == 4 ? ManyLds::kBytes : 0});
-template <int MAX, bool SWIGLU>
-__global__ __launch_bounds__(kThreads, 2) void experts_kernel(ExpertsArgs p) {
+template <int MAX, int SETS>
+constexpr int kForwardLds = std::max({SETS * FewLds<1>::kBytes, MAX >= 2 ? SETS * FewLds<2>::kBytes : 0, MAX == 4 ? ManyLds::kBytes : 0});
+template <int MAX, bool SWIGLU, int SETS>
+__global__ __launch_bounds__(SETS * kThreads, 2) void experts_kernel(ExpertsArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Work work = find_work<32 * MAX>(p.first, p.experts, p.rows, p.column_blocks, lane);
@@ -630,11 +663,11 @@ __global__ __launch_bounds__(kThreads, 2) void experts_kernel(ExpertsArgs p) {
     }
     if constexpr (MAX >= 2) {
         if (work.rows > 32) {
-            experts_few<2, SWIGLU>(p, work, lds, lane, wave);
+            experts_few<2, SWIGLU, SETS>(p, work, lds, lane, wave);
             return;
         }
     }
-    experts_few<1, SWIGLU>(p, work, lds, lane, wave);
+    experts_few<1, SWIGLU, SETS>(p, work, lds, lane, wave);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
@@ -712,9 +745,11 @@ __device__ __forceinline__ void store_gradient(const ExpertsArgs &p, const Work 
 }
 
 // Up to 64 rows: a stage is 128 columns of the pack, eight column tiles, as in the forward product; one or two more are on their way.
-template <int MI>
-__device__ __forceinline__ void experts_backward_few(const ExpertsArgs &p, const Work &work, char *lds, int lane, int wave) {
+template <int MI, int SETS>
+__device__ __forceinline__ void experts_backward_few(const ExpertsArgs &p, const Work &work, char *all_lds, int lane, int wave_of_all) {
     using L = FewLds<MI>;
+    const int wave = wave_of_all % kWaves, set = wave_of_all / kWaves;
+    char *const lds = all_lds + set * L::kBytes;
     constexpr int LR = 2 * MI, LS = LR + 5;
     const int l32 = lane & 31, h = lane >> 5, G = p.K / kGroupK, tiles = p.N / kTileN, stages = p.N / 128;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr_t)lds);
@@ -729,9 +764,9 @@ __device__ __forceinline__ void experts_backward_few(const ExpertsArgs &p, const
     const char *const codes = uniform(reinterpret_cast<const char *>(p.b) + (((size_t)work.expert * tiles + tile0) * G + fetched) * 1024);
     const char *const scales = uniform(reinterpret_cast<const char *>(p.s + ((size_t)work.expert * tiles * p.Gs + (p.Gs == 1 ? 0 : group)) * kTileN));
     const uint32_t scale_off = (uint32_t)(lane >> 3) * (uint32_t)p.Gs * (kTileN * 2) + (lane & 7) * 4;
-    auto fetch = [&](int stage) {  // past the end: the last one again, so that the count of loads in flight stays what it is
-        const int from = min(stage, stages - 1);
-        const unsigned to = lds0 + (unsigned)(stage % L::kRing) * L::kStage;
+    auto fetch = [&](int turn) {  // past the end: the last one again, so that the count of loads in flight stays what it is
+        const int from = min(SETS * turn + set, stages - 1);
+        const unsigned to = lds0 + (unsigned)(turn % L::kRing) * L::kStage;
 #pragma unroll
         for (int i = 0; i < LR; ++i) load_to_lds_b128(rows[i] + (size_t)from * 256, to + (wave * LR + i) * 1024);
         // chunks [group][tile]
@@ -745,15 +780,16 @@ __device__ __forceinline__ void experts_backward_few(const ExpertsArgs &p, const
     const TurnedConsts tc = turned_consts();
     Tile<MI> tile;
 #pragma unroll
-    for (int st = 0; st < L::kRing - 1; ++st) fetch(st);
+    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch(turn);
 #pragma unroll 1
-    for (int st = 0; st < stages; ++st) {
+    for (int turn = 0; SETS * turn < stages; ++turn) {
         wait_vector_loads<(L::kRing - 2) * LS>();  // this stage has landed
         wait_lds_reads();
         __builtin_amdgcn_s_barrier();  // ... everywhere, and the one before has been read
         asm volatile("" : : : "memory");
-        fetch(st + L::kRing - 1);
-        const unsigned at = (unsigned)(st % L::kRing) * L::kStage;
+        fetch(turn + L::kRing - 1);
+        if (SETS > 1 && SETS * turn + set >= stages) break;  // (the last turn of all)
+        const unsigned at = (unsigned)(turn % L::kRing) * L::kStage;
         const char *stage = lds + at;
         // k16 steps: a pair of column tiles has two, lanes 32 ... 63 take the second tile.  A step's codes, scales and rows are read two steps ahead and its
         // weights made behind the products of the one before.
@@ -797,7 +833,12 @@ __device__ __forceinline__ void experts_backward_few(const ExpertsArgs &p, const
             __builtin_amdgcn_sched_barrier(0);
         });
     }
-    wait_vector_loads<0>();  // stages asked for past the end still write to LDS
+    if constexpr (SETS > 1) {
+        add_second_set<MI>(all_lds, lane, wave, set, tile);
+        if (set == 1) return;
+    } else {
+        wait_vector_loads<0>();  // stages asked for past the end still write to LDS
+    }
     if (2 * work.column + (wave >> 1) < G) store_gradient<MI>(p, work, lane, work.column * kColumns + 64 * wave, tile);  // (a last block of half the columns)
 }
 
@@ -985,10 +1026,10 @@ __device__ __forceinline__ void experts_backward_many(const ExpertsArgs &p, cons
     if (2 * work.column + (wave >> 1) < G) store_gradient<MI>(p, work, lane, work.column * kColumns + 64 * wave, tile);  // (a last block of half the columns)
 }
 
-template <int MAX>
-constexpr int kBackwardLds = std::max({FewLds<1>::kBytes, MAX >= 2 ? FewLds<2>::kBytes : 0, MAX == 4 ? ManyBackwardLds::kBytes : 0});
-template <int MAX>
-__global__ __launch_bounds__(kThreads, 2) void experts_backward_kernel(ExpertsArgs p) {
+template <int MAX, int SETS>
+constexpr int kBackwardLds = std::max({SETS * FewLds<1>::kBytes, MAX >= 2 ? SETS * FewLds<2>::kBytes : 0, MAX == 4 ? ManyBackwardLds::kBytes : 0});
+template <int MAX, int SETS>
+__global__ __launch_bounds__(SETS * kThreads, 2) void experts_backward_kernel(ExpertsArgs p) {
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Work work = find_work<32 * MAX>(p.first, p.experts, p.rows, p.column_blocks, lane);
@@ -1005,11 +1046,11 @@ __global__ __launch_bounds__(kThreads, 2) void experts_backward_kernel(ExpertsAr
     }
     if constexpr (MAX >= 2) {
         if (work.rows > 32) {
-            experts_backward_few<2>(p, work, lds, lane, wave);
+            experts_backward_few<2, SETS>(p, work, lds, lane, wave);
             return;
         }
     }
-    experts_backward_few<1>(p, work, lds, lane, wave);
+    experts_backward_few<1, SETS>(p, work, lds, lane, wave);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
@@ -1017,29 +1058,32 @@ __global__ __launch_bounds__(kThreads, 2) void experts_backward_kernel(ExpertsAr
 int64_t most_tiles(int rows, int experts, int block_rows) {
     return (int64_t)rows / block_rows + std::min<int64_t>((int64_t)experts + 1, rows);
 }
-// Which blocks a call takes, from what 128 of the contraction cost a block: `alone` on its compute unit, or `busy` where compute units have several (two side by
-// side take twice as long: what they have to issue bounds them, not what they wait for), us; `rest` of a block to an expert for its last rows, `least` of one
-// to an expert of few.  us a call, 32 rows to a block / 64 / 128, and split:
-//   forward   400 rows of 16 experts, 2560 -> 2048   21 /  30 /  33,  27     400 of  4, 2560 -> 1024   20 /  30 /  39, 11
-//            3000 rows of 64 experts, 2560 -> 2048   69 /  54 /  59, 141    4000 of 64, 2560 -> 1024   50 /  48 /  45, 87
-//           16384 rows of 64 experts, 2560 -> 2048  266 / 229 / 200, 577    8000 of  8, 1024 ->  512   17 /  22 /  24, 45
-//   gradient  400 rows of 16 experts, 2560 <- 2048   24 /  25 /  24,  26     400 of 16,  768 <-  768   11 /  11 /  11,  9
-//            3000 rows of 64 experts, 2560 <- 2048   90 /  64 /  66, 127    2331 of 24, 1280 <- 2048   34 /  27 /  38, 48
-//           16384 rows of 64 experts, 2560 <- 2048  333 / 235 / 216, 504    6000 of 32, 2048 <-  768   49 /  39 /  35, 97
-// Split blocks are one to a compute unit (LDS) and taken where one round of them does; with two they lose.
-enum class Blocks { kSplit, kOneTile, kTwoTiles, kFourTiles };
+// Which blocks a call takes, from what 128 of the contraction cost a block, us: `alone` on its compute unit, or `busy` where compute units have several (two side
+// by side take nearly twice as long: what they have to issue bounds them, not what they wait for); `rest` of a block to an expert for its last rows, `least` of
+// one to an expert of few.  us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
+//   forward    400 rows of 16 experts, 2560 -> 2048   22 /  30 /  33,   20 /  26,   28      800 of 32, 1280 -> 2048   19 /  19 /  21,  24 /  17,  34
+//              400 rows of  4 experts, 2560 -> 1024   21 /  30 /  39,   19 /  26,   11     4000 of 64, 2560 -> 1024   50 /  49 /  46,  59 /  55,  92
+//             3000 rows of 64 experts, 2560 -> 2048   73 /  56 /  61,   86 /  64,  143     8000 of  8, 1024 ->  512   18 /  22 /  25,  21 /  27,  47
+//            16384 rows of 64 experts, 2560 -> 2048  263 / 230 / 203,  322 / 267,  585
+//   gradient   400 rows of 16 experts, 2560 <- 2048   24 /  25 /  24,   22 /  22,   27      400 of 16,  768 <-  768   11 /  11 /  11,  10 /  11,   9
+//             2331 rows of 24 experts, 1280 <- 2048   34 /  26 /  38,   40 /  25,   48     6000 of 32, 2048 <-  768   49 /  38 /  34,  67 /  51,  98
+//             3000 rows of 64 experts, 2560 <- 2048   87 /  63 /  65,  107 /  75,  125
+//            16384 rows of 64 experts, 2560 <- 2048  335 / 230 / 218,  412 / 295,  502
+// Two sets and split blocks are one to a compute unit (LDS) and taken where one round of them does.
+enum class Blocks { kSplit, kOneTile, kTwoTiles, kFourTiles, kOneTileTwoSets, kTwoTilesTwoSets };
 struct BlockCost {
     Blocks blocks;
     int rows;
-    float alone, busy, rest, least, launch;
+    float alone, busy, rest, least, launch;  // busy 0: one to a compute unit at most
 };
-Blocks choose_blocks(const BlockCost (&costs)[3], int rows, int experts, int contraction, int column_blocks, int split_columns, int cus) {
+Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int contraction, int column_blocks, int split_columns, int cus) {
     const float present = (float)std::min(rows, experts), each = rows / present, groups = contraction / 128.f;
     if (present * std::max(1.f, each / 32 + 0.5f) * split_columns <= cus) return Blocks::kSplit;
     const BlockCost *best = nullptr;
     float least = 0.f;
     for (const BlockCost &c : costs) {
         const float share = present * std::max(c.least, each / c.rows + c.rest) * column_blocks / cus;
+        if (share > 1.f && c.busy == 0.f) continue;
         const float time = groups * (share <= 1.f ? c.alone : c.busy * std::max(share, 2.f)) + c.launch;
         if (!best || time < least) {
             best = &c;
@@ -1048,21 +1092,25 @@ Blocks choose_blocks(const BlockCost (&costs)[3], int rows, int experts, int con
     }
     return best->blocks;
 }
-constexpr BlockCost kForwardCosts[3] = {{Blocks::kOneTile, 32, 1.0f, 0.83f, 0.5f, 1.f, 0.f},
-                                        {Blocks::kTwoTiles, 64, 2.0f, 1.23f, 0.3f, 0.67f, 0.f},
-                                        {Blocks::kFourTiles, 128, 2.1f, 2.15f, 0.25f, 0.39f, 3.f}};  // (its rows' sums are a launch)
-constexpr BlockCost kGradientCosts[3] = {{Blocks::kOneTile, 32, 1.25f, 1.17f, 0.5f, 1.f, 0.f},
-                                         {Blocks::kTwoTiles, 64, 1.5f, 1.47f, 0.3f, 0.8f, 0.f},
-                                         {Blocks::kFourTiles, 128, 2.2f, 2.5f, 0.3f, 0.47f, 0.f}};
+constexpr BlockCost kForwardCosts[5] = {{Blocks::kOneTile, 32, 0.82f, 0.83f, 0.5f, 1.f, 0.f},
+                                        {Blocks::kTwoTiles, 64, 1.3f, 1.23f, 0.3f, 0.67f, 0.f},
+                                        {Blocks::kFourTiles, 128, 1.9f, 2.15f, 0.25f, 0.39f, 3.f},  // (its rows' sums are a launch)
+                                        {Blocks::kOneTileTwoSets, 32, 0.7f, 0.f, 0.5f, 1.f, 1.f},
+                                        {Blocks::kTwoTilesTwoSets, 64, 1.08f, 0.f, 0.3f, 0.67f, 1.f}};
+constexpr BlockCost kGradientCosts[5] = {{Blocks::kOneTile, 32, 1.1f, 1.17f, 0.5f, 1.f, 0.f},
+                                         {Blocks::kTwoTiles, 64, 1.4f, 1.6f, 0.3f, 0.8f, 0.f},
+                                         {Blocks::kFourTiles, 128, 2.2f, 2.5f, 0.35f, 0.47f, 0.f},
+                                         {Blocks::kOneTileTwoSets, 32, 0.9f, 0.f, 0.5f, 1.f, 1.f},
+                                         {Blocks::kTwoTilesTwoSets, 64, 1.25f, 0.f, 0.3f, 0.8f, 1.f}};
 Blocks forward_blocks(int rows, int n, int k, int experts, int cus) { return choose_blocks(kForwardCosts, rows, experts, k, n / kColumns, n / 64, cus); }
 Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {
     return choose_blocks(kGradientCosts, rows, experts, n, (k + kColumns - 1) / kColumns, k / kGroupK, cus);
 }
 // (Eight blocks more: a die's shares of both lists may be rounded up.)
 template <auto Kernel>
-bool launch(const ExpertsArgs &a, int block_rows, int lds_bytes, hipStream_t stream) {
+bool launch(const ExpertsArgs &a, int block_rows, int lds_bytes, hipStream_t stream, int threads = kThreads) {
     if (allow_dynamic_lds<Kernel>(lds_bytes) != hipSuccess) return false;
-    Kernel<<<(unsigned)(most_tiles(a.rows, a.experts, block_rows) * a.column_blocks + 8), kThreads, lds_bytes, stream>>>(a);
+    Kernel<<<(unsigned)(most_tiles(a.rows, a.experts, block_rows) * a.column_blocks + 8), threads, lds_bytes, stream>>>(a);
     return true;
 }
 
@@ -1107,19 +1155,22 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts(const void *x, const int *first, co
     ExpertsArgs a{(const uint16_t *)x, first, order, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, (const float *)scratch,
                   rows, x_rows, top_k, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, prob_n / kColumns};
     bool ok = false;
-    auto with = [&](auto mc) {
-        constexpr int MI = decltype(mc)::value;
-        ok = swiglu ? launch<experts_kernel<MI, true>>(a, 32 * MI, kForwardLds<MI>, hs)
-                    : launch<experts_kernel<MI, false>>(a, 32 * MI, kForwardLds<MI>, hs);
+    auto with = [&](auto mc, auto sc) {
+        constexpr int MI = decltype(mc)::value, SETS = decltype(sc)::value;
+        ok = swiglu ? launch<experts_kernel<MI, true, SETS>>(a, 32 * MI, kForwardLds<MI, SETS>, hs, SETS * kThreads)
+                    : launch<experts_kernel<MI, false, SETS>>(a, 32 * MI, kForwardLds<MI, SETS>, hs, SETS * kThreads);
     };
+    using std::integral_constant;
     switch (blocks) {
         case Blocks::kSplit:
             a.column_blocks = prob_n / 64;
             ok = swiglu ? launch<experts_split_kernel<true>>(a, 32, SplitLds::kBytes, hs) : launch<experts_split_kernel<false>>(a, 32, SplitLds::kBytes, hs);
             break;
-        case Blocks::kOneTile: with(std::integral_constant<int, 1>{}); break;
-        case Blocks::kTwoTiles: with(std::integral_constant<int, 2>{}); break;
-        case Blocks::kFourTiles: with(std::integral_constant<int, 4>{}); break;
+        case Blocks::kOneTile: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kTwoTiles: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kFourTiles: with(integral_constant<int, 4>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kOneTileTwoSets: with(integral_constant<int, 1>{}, integral_constant<int, 2>{}); break;
+        case Blocks::kTwoTilesTwoSets: with(integral_constant<int, 2>{}, integral_constant<int, 2>{}); break;
     }
     return ok && hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }
@@ -1137,18 +1188,21 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(const void *dy, const int 
     ExpertsArgs a{(const uint16_t *)dy, first, nullptr, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)dx, nullptr,
                   rows, rows, 1, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, (prob_k + kColumns - 1) / kColumns};
     bool ok = false;
-    auto with = [&](auto mc) {
-        constexpr int MI = decltype(mc)::value;
-        ok = launch<experts_backward_kernel<MI>>(a, 32 * MI, kBackwardLds<MI>, hs);
+    auto with = [&](auto mc, auto sc) {
+        constexpr int MI = decltype(mc)::value, SETS = decltype(sc)::value;
+        ok = launch<experts_backward_kernel<MI, SETS>>(a, 32 * MI, kBackwardLds<MI, SETS>, hs, SETS * kThreads);
     };
+    using std::integral_constant;
     switch (blocks) {
         case Blocks::kSplit:
             a.column_blocks = prob_k / kGroupK;
             ok = launch<experts_split_backward_kernel>(a, 32, SplitBackwardLds::kBytes, hs);
             break;
-        case Blocks::kOneTile: with(std::integral_constant<int, 1>{}); break;
-        case Blocks::kTwoTiles: with(std::integral_constant<int, 2>{}); break;
-        case Blocks::kFourTiles: with(std::integral_constant<int, 4>{}); break;
+        case Blocks::kOneTile: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kTwoTiles: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kFourTiles: with(integral_constant<int, 4>{}, integral_constant<int, 1>{}); break;
+        case Blocks::kOneTileTwoSets: with(integral_constant<int, 1>{}, integral_constant<int, 2>{}); break;
+        case Blocks::kTwoTilesTwoSets: with(integral_constant<int, 2>{}, integral_constant<int, 2>{}); break;
     }
     return ok && hipGetLastError() == hipSuccess ? KILN_W4A16_OK : KILN_W4A16_ERR_LAUNCH;
 }

@@ -85,17 +85,18 @@ def test_the_whole_layer_beside_the_call_for_a_few_tokens():
 
 
 def test_every_kind_of_block_is_taken_by_some_size():
-    """The sizes that the tests of products and gradients run, on this part: each of the four kinds in both directions."""
+    """The sizes that the tests of products and gradients run, on this part: each of the six kinds in both directions."""
     from tests import test_gpu_experts_many as t
     cus = torch.cuda.get_device_properties(0).multi_processor_count
     plan = lambda *a: _lib.load().kiln_w4a16_debug_experts_plan(*a, cus)
     sizes = [(sum(c), n, k, len(c) - 1) for c in t.COUNTS for k, n in ((128, 256), (384, 512), (256, 768), (1152, 256))] + \
             [(3000, 2048, 2560, 2), (700, 2560, 2048, 32), (100, 2048, 2560, 64), (4096, 2560, 1024, 8)] + SIZES
     for backward in (0, 1):
-        assert {plan(*s, backward) for s in sizes} == {0, 1, 2, 3}
+        assert {plan(*s, backward) for s in sizes} == {0, 1, 2, 3, 4, 5}
 
 
-SIZES = [(768, 2048, 512, 64), (1600, 512, 2048, 64), (3000, 2048, 512, 64), (3000, 512, 2048, 64), (6000, 1024, 1024, 32), (5000, 512, 512, 4)]
+SIZES = [(768, 2048, 512, 64), (1600, 512, 2048, 64), (3000, 2048, 512, 64), (3000, 512, 2048, 64), (6000, 1024, 1024, 32), (5000, 512, 512, 4),
+         (400, 2048, 2560, 16), (800, 2048, 1280, 32), (1500, 2560, 1024, 64), (2331, 2048, 1280, 24)]
 
 
 @pytest.mark.parametrize("rows,n,k,experts", SIZES)
