@@ -15,7 +15,7 @@
 //   32 rows x 64 columns (the gradient: 128), the wavefronts sharing out the contraction, where the others would leave compute units idle.
 // In blocks of 128 and 64 rows what is left of an expert goes as in the smaller ones.
 //
-// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 185-200, the gradient 215-227: rounds of blocks that do not come out even (the same rows in
+// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 177-185, the gradient 198-207: rounds of blocks that do not come out even (the same rows in
 // equal parts 167 and 185), and power: on values of this kind the matrix instructions alone reach 1.6 to 1.8 PFLOP/s, not the 2.2 that they do on zeros, and the vector
 // instructions that expand the codes, reads of LDS and loads come on top (each left out for a measurement took 2 to 8 % off); 768 rows of 64 experts, 2560 -> 2048:
 // 41-48, 3.6 to 4.3 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 27, a round and a half of blocks, each one's start and latencies.
@@ -48,9 +48,11 @@ struct ExpertsArgs {
     int column_blocks;
 };
 
-// The work of a block: up to BM rows of one expert, and a block of columns.  Whole row tiles come first, then what is left of each expert: the
-// last blocks to start are the short ones.  Blocks go to the eight dies in turn, a die's share of either list is contiguous in (expert, columns,
-// rows), rows first: what it reads at one time is a few blocks of a pack and one expert's rows.
+// The work of a block: up to BM rows of one expert, and a block of columns.  What is left of an expert behind its last whole row tile comes first where that is no more than half
+// a tile: those blocks wait for their loads, and beside others they are no tail (ordered last: 16384 rows of 64
+// experts, 2560 -> 2048 200 us, first 180; the gradient 217 and 203).
+// Blocks go to the eight dies in turn, a die's share of either list is contiguous in (expert, columns, rows), rows first: what it reads at one time is a few
+// blocks of a pack and one expert's rows.
 struct Work {
     int expert, row0, rows, column;  // expert == experts: rows of no expert;  -1: nothing
 };
@@ -59,44 +61,48 @@ __device__ __forceinline__ Work find_work(const int *__restrict__ first, int exp
     const int keys = experts + 1, per = (keys + 63) / 64, e0 = min(keys, lane * per), e1 = min(keys, e0 + per);
     auto begin_of = [&](int e) { return e < keys ? max(0, min(first[e], rows)) : rows; };  // (in bounds whatever `first` holds)
     auto rows_of = [&](int e) { return max(0, begin_of(e + 1) - begin_of(e)); };
-    int whole = 0, part = 0;  // of the lane's experts: whole tiles, tiles that are not
+    auto tiles_of = [](int n) { return (n + BM / 2 - 1) / BM; };                        // of more than half of BM rows
+    auto has_rest = [](int n) { return n % BM != 0 && n % BM <= BM / 2; };
+    int tiles = 0, rests = 0;  // of the lane's experts
     for (int e = e0; e < e1; ++e) {
         const int n = rows_of(e);
-        whole += n / BM;
-        part += n % BM != 0;
+        tiles += tiles_of(n);
+        rests += has_rest(n);
     }
-    int whole_upto = whole, part_upto = part;
+    int tiles_upto = tiles, rests_upto = rests;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int a = __shfl_up(whole_upto, d), b = __shfl_up(part_upto, d);
+        const int a = __shfl_up(tiles_upto, d), b = __shfl_up(rests_upto, d);
         if (lane >= d) {
-            whole_upto += a;
-            part_upto += b;
+            tiles_upto += a;
+            rests_upto += b;
         }
     }
-    const unsigned die = blockIdx.x & 7;
     unsigned seq = blockIdx.x >> 3, id;
-    auto mine = [&](unsigned total) {  // of a list: is this block's place in the die's share of it?
+    auto mine = [&](unsigned total, unsigned die) {  // of a list: is this block's place in the die's share of it?
         const unsigned each = total >> 3, more = total & 7, count = each + (die < more ? 1u : 0u);
         id = die * each + min(die, more) + seq;
         if (seq < count) return true;
         seq -= count;
         return false;
     };
-    const bool is_whole = mine((unsigned)__builtin_amdgcn_readlane(whole_upto, 63) * (unsigned)column_blocks);
-    if (!is_whole && !mine((unsigned)__builtin_amdgcn_readlane(part_upto, 63) * (unsigned)column_blocks)) return {-1, 0, 0, 0};
-    const int tile = (int)(id / (unsigned)column_blocks), upto = is_whole ? whole_upto : part_upto;
+    // (what does not go evenly into eight is the first dies' of one list and the last dies' of the other: as many blocks as compute units are one to each)
+    const unsigned die = blockIdx.x & 7;
+    const bool is_rest = mine((unsigned)__builtin_amdgcn_readlane(rests_upto, 63) * (unsigned)column_blocks, die);
+    if (!is_rest && !mine((unsigned)__builtin_amdgcn_readlane(tiles_upto, 63) * (unsigned)column_blocks, 7 - die)) return {-1, 0, 0, 0};
+    const int tile = (int)(id / (unsigned)column_blocks), upto = is_rest ? rests_upto : tiles_upto;
     const int at = __builtin_ctzll(__ballot(upto > tile));
-    int base = __builtin_amdgcn_readlane(upto - (is_whole ? whole : part), at), e = at * per, count, n;
+    int base = __builtin_amdgcn_readlane(upto - (is_rest ? rests : tiles), at), e = at * per, count, n;
     for (;; ++e) {
         n = __builtin_amdgcn_readfirstlane(rows_of(e));
-        count = is_whole ? n / BM : n % BM != 0;
+        count = is_rest ? has_rest(n) : tiles_of(n);
         if (tile < base + count) break;
         base += count;
     }
     const int inside = (int)(id - (unsigned)base * (unsigned)column_blocks);
-    if (is_whole) return {e, begin_of(e) + inside % count * BM, BM, inside / count};
-    return {e, begin_of(e) + n / BM * BM, n % BM, inside};
+    if (is_rest) return {e, begin_of(e) + n / BM * BM, n % BM, inside};
+    const int t = inside % count;
+    return {e, begin_of(e) + t * BM, min(BM, n - t * BM), inside / count};
 }
 
 // rows of no expert: zeros in the block's columns
@@ -1061,30 +1067,37 @@ int64_t most_tiles(int rows, int experts, int block_rows) {
 // Which blocks a call takes, from what 128 of the contraction cost a block, us: `alone` on its compute unit, or `busy` where compute units have several (two side
 // by side take nearly twice as long: what they have to issue bounds them, not what they wait for); `rest` of a block to an expert for its last rows, `least` of
 // one to an expert of few.  us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
-//   forward    400 rows of 16 experts, 2560 -> 2048   22 /  30 /  33,   20 /  26,   28      800 of 32, 1280 -> 2048   19 /  19 /  21,  24 /  17,  34
-//              400 rows of  4 experts, 2560 -> 1024   21 /  30 /  39,   19 /  26,   11     4000 of 64, 2560 -> 1024   50 /  49 /  46,  59 /  55,  92
-//             3000 rows of 64 experts, 2560 -> 2048   73 /  56 /  61,   86 /  64,  143     8000 of  8, 1024 ->  512   18 /  22 /  25,  21 /  27,  47
-//            16384 rows of 64 experts, 2560 -> 2048  263 / 230 / 203,  322 / 267,  585
-//   gradient   400 rows of 16 experts, 2560 <- 2048   24 /  25 /  24,   22 /  22,   27      400 of 16,  768 <-  768   11 /  11 /  11,  10 /  11,   9
-//             2331 rows of 24 experts, 1280 <- 2048   34 /  26 /  38,   40 /  25,   48     6000 of 32, 2048 <-  768   49 /  38 /  34,  67 /  51,  98
-//             3000 rows of 64 experts, 2560 <- 2048   87 /  63 /  65,  107 /  75,  125
-//            16384 rows of 64 experts, 2560 <- 2048  335 / 230 / 218,  412 / 295,  502
+//   forward    400 rows of 16 experts, 2560 -> 2048   23 /  32 /  34,   20 /  27,   28      800 of 32, 1280 -> 2048   19 /  20 /  22,  24 /  18,  34
+//              400 rows of  4 experts, 2560 -> 1024   21 /  30 /  39,   19 /  26,   11     4000 of 64, 2560 -> 1024   47 /  40 /  45,  54 /  45,  92
+//             3000 rows of 64 experts, 2560 -> 2048   67 /  53 /  56,   75 /  57,  143     8000 of  8, 1024 ->  512   16 /  19 /  24,  20 /  23,  47
+//             8000 rows of 64 experts, 2560 -> 2048  150 / 121 /  97,  162 / 128,  302    10000 of 16,  768 -> 1536   43 /  36 /  32,  62 /  44
+//            16384 rows of 64 experts, 2560 -> 2048  271 / 217 / 177,  308 / 246,  585
+//   gradient   400 rows of 16 experts, 2560 <- 2048   25 /  26 /  26,   23 /  24,   27      400 of 16,  768 <-  768   11 /  11 /  11,  10 /  11,   9
+//             2331 rows of 24 experts, 1280 <- 2048   34 /  26 /  38,   39 /  25,   48     6000 of 32, 2048 <-  768   46 /  33 /  32,  64 /  45,  98
+//             3000 rows of 64 experts, 2560 <- 2048   87 /  60 /  60,   99 /  70,  125     1500 of 64, 1024 <- 2560   41 /  43 /  30,  47 /  50,  44
+//            16384 rows of 64 experts, 2560 <- 2048  328 / 223 / 198,  415 / 265,  502
+// (The costs were fitted to 28 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory: what is
+// chosen is within 1 % of the best on average, 22 % off at the worst, 1000 rows of 8 experts, 512 -> 2048.)
 // Two sets and split blocks are one to a compute unit (LDS) and taken where one round of them does.
 enum class Blocks { kSplit, kOneTile, kTwoTiles, kFourTiles, kOneTileTwoSets, kTwoTilesTwoSets };
 struct BlockCost {
     Blocks blocks;
     int rows;
-    float alone, busy, rest, least, launch;  // busy 0: one to a compute unit at most
+    float alone, few, busy, rest, least, launch;  // few: alone, and up to kFewEach rows to an expert;  busy 0: one to a compute unit at most
 };
+constexpr float kFewEach = 24.f;
 Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int contraction, int column_blocks, int split_columns, int cus) {
     const float present = (float)std::min(rows, experts), each = rows / present, groups = contraction / 128.f;
-    if (present * std::max(1.f, each / 32 + 0.5f) * split_columns <= cus) return Blocks::kSplit;
+    if (present * std::max(1.f, each / 32 + 0.5f) * split_columns <= 1.05f * cus) return Blocks::kSplit;
     const BlockCost *best = nullptr;
     float least = 0.f;
     for (const BlockCost &c : costs) {
-        const float share = present * std::max(c.least, each / c.rows + c.rest) * column_blocks / cus;
-        if (share > 1.f && c.busy == 0.f) continue;
-        const float time = groups * (share <= 1.f ? c.alone : c.busy * std::max(share, 2.f)) + c.launch;
+        float share = present * std::max(c.least, each / c.rows + c.rest) * column_blocks / cus;
+        if (c.busy == 0.f) {  // a block too many takes a second round: an expert in 32 may have four times the rows of another
+            if (each * 4 > c.rows) share += present / 32 * column_blocks / cus;
+            if (share > 1.f) continue;
+        }
+        const float time = groups * (share > 1.f ? c.busy * std::max(share, 2.f) : each <= kFewEach ? c.few : c.alone) + c.launch;
         if (!best || time < least) {
             best = &c;
             least = time;
@@ -1092,16 +1105,17 @@ Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int con
     }
     return best->blocks;
 }
-constexpr BlockCost kForwardCosts[5] = {{Blocks::kOneTile, 32, 0.82f, 0.83f, 0.5f, 1.f, 0.f},
-                                        {Blocks::kTwoTiles, 64, 1.3f, 1.23f, 0.3f, 0.67f, 0.f},
-                                        {Blocks::kFourTiles, 128, 1.9f, 2.15f, 0.25f, 0.39f, 3.f},  // (its rows' sums are a launch)
-                                        {Blocks::kOneTileTwoSets, 32, 0.7f, 0.f, 0.5f, 1.f, 1.f},
-                                        {Blocks::kTwoTilesTwoSets, 64, 1.08f, 0.f, 0.3f, 0.67f, 1.f}};
-constexpr BlockCost kGradientCosts[5] = {{Blocks::kOneTile, 32, 1.1f, 1.17f, 0.5f, 1.f, 0.f},
-                                         {Blocks::kTwoTiles, 64, 1.4f, 1.6f, 0.3f, 0.8f, 0.f},
-                                         {Blocks::kFourTiles, 128, 2.2f, 2.5f, 0.35f, 0.47f, 0.f},
-                                         {Blocks::kOneTileTwoSets, 32, 0.9f, 0.f, 0.5f, 1.f, 1.f},
-                                         {Blocks::kTwoTilesTwoSets, 64, 1.25f, 0.f, 0.3f, 0.8f, 1.f}};
+// (of equals the larger: an expert with more rows than others then takes no second block)
+constexpr BlockCost kForwardCosts[5] = {{Blocks::kTwoTiles, 64, 1.37f, 0.84f, 1.f, 0.3f, 1.f, 0.f},
+                                        {Blocks::kOneTile, 32, 0.84f, 0.84f, 0.96f, 0.53f, 1.f, 0.f},
+                                        {Blocks::kFourTiles, 128, 1.9f, 0.84f, 1.59f, 0.26f, 0.41f, 3.5f},  // (its rows' sums are a launch)
+                                        {Blocks::kTwoTilesTwoSets, 64, 1.25f, 0.71f, 0.f, 0.3f, 1.f, 1.f},
+                                        {Blocks::kOneTileTwoSets, 32, 0.71f, 0.71f, 0.f, 0.53f, 1.f, 1.f}};
+constexpr BlockCost kGradientCosts[5] = {{Blocks::kTwoTiles, 64, 1.54f, 1.16f, 1.36f, 0.3f, 0.8f, 0.f},
+                                         {Blocks::kOneTile, 32, 1.16f, 1.16f, 1.27f, 0.5f, 1.f, 0.f},
+                                         {Blocks::kFourTiles, 128, 2.72f, 1.04f, 2.2f, 0.41f, 0.56f, 0.f},
+                                         {Blocks::kTwoTilesTwoSets, 64, 1.29f, 0.99f, 0.f, 0.3f, 0.8f, 1.f},
+                                         {Blocks::kOneTileTwoSets, 32, 0.99f, 0.99f, 0.f, 0.5f, 1.f, 1.f}};
 Blocks forward_blocks(int rows, int n, int k, int experts, int cus) { return choose_blocks(kForwardCosts, rows, experts, k, n / kColumns, n / 64, cus); }
 Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {
     return choose_blocks(kGradientCosts, rows, experts, n, (k + kColumns - 1) / kColumns, k / kGroupK, cus);
