@@ -381,7 +381,7 @@ kiln_marlin_status_t kiln_w4a16_moe_sort(
  *                                                                           in the order of j, rounded once; y bf16 [m, width]
  *   combine_backward  d_rows[place[i, j]] = weights[i, j] * dy[i]           bf16 [m * top_k, width], rounded once
  *                     d_weights[i, j] = <rows[place[i, j]], dy[i]>          f32 [m, top_k], summed in f32; 0 without an expert
- * (Positions in `place` outside [0, m * top_k) are passed over.)
+ * (Positions in `place` outside [0, m * top_k) are passed over.)  m * width <= 2^35 - 2048, and combine_backward m <= 2^24 - 1, with width <= 512 2^26 - 4.
  */
 kiln_marlin_status_t kiln_w4a16_moe_gather(
     const void *x, const int *first, const int *place, void *rows,
@@ -404,7 +404,7 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(
  *          memory with x (refused)
  *   scratch  kiln_w4a16_gemm_experts_scratch_bytes(x_rows, k), on 16 bytes, holds nothing between calls
  *   dev      stream's device, whose compute units the launches are planned for (in the other calls on sorted rows it is not used)
- * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024, x_rows <= 2^29.
+ * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024, x_rows <= 2^29, x_rows * k <= 2^35 - 2048.
  * The gradient of the rows, the packs frozen: dx[p] = dy[p] * dequant(B_e, s_e)^T, bf16 [rows, k], rounded once; a weight enters the product
  * rounded to bf16, as in kiln_w4a16_gemm_bank_backward.
  */
@@ -426,7 +426,7 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(
  *              magnitude (at least 1); whole is rounded to the nearest, ties to even, at most 127 in magnitude.  A block with an infinity or
  *              NaN has exponent 255 and is NaN.
  * The backward pass out of them: with s = 1 / (1 + exp(-gate)), d_up = dh * gate * s and d_gate = dh * up * s * (1 + gate * (1 - s)), bf16 in
- * gate_up's columns, rounded once; h again unless NULL (of the kept values).  n_out % 128 == 0; all on 16 bytes (exponents on 2); no result shares
+ * gate_up's columns, rounded once; h again unless NULL (of the kept values).  n_out % 128 == 0, m * n_out <= 2^35 - 2048; all on 16 bytes (exponents on 2); no result shares
  * memory with an operand or another result (refused).
  */
 kiln_marlin_status_t kiln_w4a16_swiglu_keep(

@@ -24,6 +24,8 @@ inline bool any_meet(std::initializer_list<Piece> written, std::initializer_list
     }
     return false;
 }
+// may one launch have so many blocks?  (Its work-items are counted in 32 bits.)
+inline bool launchable(int64_t blocks, int threads) { return blocks * threads <= (int64_t)UINT32_MAX; }
 // all there and on `bytes`?
 inline bool all_on(size_t bytes, std::initializer_list<const void *> pointers) {
     for (const void *p : pointers)

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void swiglu_keep_backward_kernel(KeepArgs p) {
 
 kiln_marlin_status_t shape_ok(int m, int n_out) {
     if (m < 0 || n_out < 1 || n_out % 128 != 0 || n_out > INT32_MAX / 2) return KILN_W4A16_ERR_PROB_SHAPE;
-    return ((int64_t)m * (n_out / 8) + 255) / 256 > INT32_MAX ? KILN_W4A16_ERR_KERN_SHAPE : KILN_W4A16_OK;
+    return launchable(((int64_t)m * (n_out / 8) + 255) / 256, 256) ? KILN_W4A16_OK : KILN_W4A16_ERR_KERN_SHAPE;
 }
 
 }  // namespace

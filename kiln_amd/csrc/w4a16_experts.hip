@@ -1120,11 +1120,14 @@ Blocks forward_blocks(int rows, int n, int k, int experts, int cus) { return cho
 Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {
     return choose_blocks(kGradientCosts, rows, experts, n, (k + kColumns - 1) / kColumns, k / kGroupK, cus);
 }
+int rows_of(Blocks blocks) { return blocks == Blocks::kFourTiles ? 128 : blocks == Blocks::kTwoTiles || blocks == Blocks::kTwoTilesTwoSets ? 64 : 32; }
+int threads_of(Blocks blocks) { return blocks == Blocks::kOneTileTwoSets || blocks == Blocks::kTwoTilesTwoSets ? 2 * kThreads : kThreads; }
 // (Eight blocks more: a die's shares of both lists may be rounded up.)
+int64_t blocks_of(Blocks blocks, int rows, int experts, int column_blocks) { return most_tiles(rows, experts, rows_of(blocks)) * column_blocks + 8; }
 template <auto Kernel>
-bool launch(const ExpertsArgs &a, int block_rows, int lds_bytes, hipStream_t stream, int threads = kThreads) {
+bool launch(const ExpertsArgs &a, Blocks blocks, int lds_bytes, hipStream_t stream) {
     if (allow_dynamic_lds<Kernel>(lds_bytes) != hipSuccess) return false;
-    Kernel<<<(unsigned)(most_tiles(a.rows, a.experts, block_rows) * a.column_blocks + 8), threads, lds_bytes, stream>>>(a);
+    Kernel<<<(unsigned)blocks_of(blocks, a.rows, a.experts, a.column_blocks), threads_of(blocks), lds_bytes, stream>>>(a);
     return true;
 }
 
@@ -1152,8 +1155,12 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts(const void *x, const int *first, co
                                              int top_k, int prob_n, int prob_k, int experts, int groupsize, int swiglu, int dev, void *stream, void *scratch) {
     if (const kiln_marlin_status_t st = experts_ok(rows, prob_n, prob_k, experts, groupsize)) return st;
     if (x_rows < 0 || top_k < 1 || (order ? (int64_t)x_rows * top_k != rows : x_rows != rows)) return KILN_W4A16_ERR_KERN_SHAPE;
-    if (x_rows > kMaxRows || (int64_t)x_rows * (prob_k / kGroupK) > (int64_t)INT32_MAX * 16) return KILN_W4A16_ERR_KERN_SHAPE;
+    const int64_t items = (int64_t)x_rows * (prob_k / kGroupK);
+    if (x_rows > kMaxRows || !launchable((items + 15) / 16, 256)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (rows == 0) return KILN_W4A16_OK;
+    const Blocks blocks = forward_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
+    const int column_blocks = blocks == Blocks::kSplit ? prob_n / 64 : prob_n / kColumns;
+    if (!launchable(blocks_of(blocks, rows, experts, column_blocks), threads_of(blocks))) return KILN_W4A16_ERR_KERN_SHAPE;
     if (!all_on(16, {x, b, s, y, scratch}) || !all_on(4, {first}) || reinterpret_cast<uintptr_t>(order) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
     const size_t width = swiglu ? prob_n / 2 : prob_n;
     if (any_meet({{y, rows * width * 2}, {scratch, kiln_w4a16_gemm_experts_scratch_bytes(x_rows, prob_k)}},
@@ -1161,24 +1168,21 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts(const void *x, const int *first, co
                   scales_of(s, prob_n, prob_k, experts, groupsize)}))
         return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    const Blocks blocks = forward_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
     if (blocks == Blocks::kFourTiles) {
-        const size_t items = (size_t)x_rows * (prob_k / kGroupK);
         expert_row_sums_kernel<<<(unsigned)((items + 15) / 16), 256, 0, hs>>>((const uint16_t *)x, (float *)scratch, x_rows, prob_k);
     }
     ExpertsArgs a{(const uint16_t *)x, first, order, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)y, (const float *)scratch,
-                  rows, x_rows, top_k, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, prob_n / kColumns};
+                  rows, x_rows, top_k, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, column_blocks};
     bool ok = false;
     auto with = [&](auto mc, auto sc) {
         constexpr int MI = decltype(mc)::value, SETS = decltype(sc)::value;
-        ok = swiglu ? launch<experts_kernel<MI, true, SETS>>(a, 32 * MI, kForwardLds<MI, SETS>, hs, SETS * kThreads)
-                    : launch<experts_kernel<MI, false, SETS>>(a, 32 * MI, kForwardLds<MI, SETS>, hs, SETS * kThreads);
+        ok = swiglu ? launch<experts_kernel<MI, true, SETS>>(a, blocks, kForwardLds<MI, SETS>, hs)
+                    : launch<experts_kernel<MI, false, SETS>>(a, blocks, kForwardLds<MI, SETS>, hs);
     };
     using std::integral_constant;
     switch (blocks) {
         case Blocks::kSplit:
-            a.column_blocks = prob_n / 64;
-            ok = swiglu ? launch<experts_split_kernel<true>>(a, 32, SplitLds::kBytes, hs) : launch<experts_split_kernel<false>>(a, 32, SplitLds::kBytes, hs);
+            ok = swiglu ? launch<experts_split_kernel<true>>(a, blocks, SplitLds::kBytes, hs) : launch<experts_split_kernel<false>>(a, blocks, SplitLds::kBytes, hs);
             break;
         case Blocks::kOneTile: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
         case Blocks::kTwoTiles: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;
@@ -1193,24 +1197,25 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(const void *dy, const int 
                                                       int experts, int groupsize, int dev, void *stream) {
     if (const kiln_marlin_status_t st = experts_ok(rows, prob_n, prob_k, experts, groupsize)) return st;
     if (rows == 0) return KILN_W4A16_OK;
+    const Blocks blocks = gradient_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
+    const int column_blocks = blocks == Blocks::kSplit ? prob_k / kGroupK : (prob_k + kColumns - 1) / kColumns;
+    if (!launchable(blocks_of(blocks, rows, experts, column_blocks), threads_of(blocks))) return KILN_W4A16_ERR_KERN_SHAPE;
     if (!all_on(16, {dy, b, s, dx}) || !all_on(4, {first})) return KILN_W4A16_ERR_ARGUMENT;
     if (any_meet({{dx, (size_t)rows * prob_k * 2}}, {{dy, (size_t)rows * prob_n * 2}, {first, ((size_t)experts + 1) * 4}, pack_of(b, prob_n, prob_k, experts),
                                                      scales_of(s, prob_n, prob_k, experts, groupsize)}))
         return KILN_W4A16_ERR_ARGUMENT;
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    const Blocks blocks = gradient_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
     ExpertsArgs a{(const uint16_t *)dy, first, nullptr, (const u32x4 *)b, (const uint16_t *)s, (uint16_t *)dx, nullptr,
-                  rows, rows, 1, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, (prob_k + kColumns - 1) / kColumns};
+                  rows, rows, 1, experts, prob_k, prob_n, groupsize == -1 ? 1 : prob_k / kGroupK, column_blocks};
     bool ok = false;
     auto with = [&](auto mc, auto sc) {
         constexpr int MI = decltype(mc)::value, SETS = decltype(sc)::value;
-        ok = launch<experts_backward_kernel<MI, SETS>>(a, 32 * MI, kBackwardLds<MI, SETS>, hs, SETS * kThreads);
+        ok = launch<experts_backward_kernel<MI, SETS>>(a, blocks, kBackwardLds<MI, SETS>, hs);
     };
     using std::integral_constant;
     switch (blocks) {
         case Blocks::kSplit:
-            a.column_blocks = prob_k / kGroupK;
-            ok = launch<experts_split_backward_kernel>(a, 32, SplitBackwardLds::kBytes, hs);
+            ok = launch<experts_split_backward_kernel>(a, blocks, SplitBackwardLds::kBytes, hs);
             break;
         case Blocks::kOneTile: with(integral_constant<int, 1>{}, integral_constant<int, 1>{}); break;
         case Blocks::kTwoTiles: with(integral_constant<int, 2>{}, integral_constant<int, 1>{}); break;

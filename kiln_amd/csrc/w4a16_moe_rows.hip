@@ -260,8 +260,7 @@ __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
 kiln_marlin_status_t rows_ok(int m, int top_k, int experts, int width) {
     if (m < 0 || width < 1 || width % 8 != 0) return KILN_W4A16_ERR_PROB_SHAPE;
     if (top_k < 1 || top_k > kMaxTop || experts < 1 || experts > kMaxExperts || (int64_t)m * top_k > kMaxPairs) return KILN_W4A16_ERR_KERN_SHAPE;
-    if (((int64_t)m * (width / 8) + 255) / 256 > INT32_MAX) return KILN_W4A16_ERR_KERN_SHAPE;
-    return KILN_W4A16_OK;
+    return launchable(((int64_t)m * (width / 8) + 255) / 256, 256) ? KILN_W4A16_OK : KILN_W4A16_ERR_KERN_SHAPE;
 }
 int sort_block_pairs(int pairs) {
     const int each = pairs <= kSortBlockPairs ? std::max(pairs, 1) : std::max(kSortBlockPairs, (pairs + kSortMaxBlocks - 1) / kSortMaxBlocks);
@@ -336,6 +335,9 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
                                                      void *d_rows, float *d_weights, int prob_m, int top_k, int experts, int width, int dev, void *stream) {
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
+    const bool narrow = width <= 512;
+    const int64_t blocks = narrow ? ((int64_t)prob_m + 3) / 4 : prob_m;
+    if (!launchable(blocks, 256)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (prob_m == 0) return KILN_W4A16_OK;
     if (!all_on(16, {dy, rows, d_rows}) || !all_on(4, {weights, first, place, d_weights})) return KILN_W4A16_ERR_ARGUMENT;
     const size_t pairs = (size_t)prob_m * top_k, first_bytes = ((size_t)experts + 1) * 4;
@@ -344,8 +346,8 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
         return KILN_W4A16_ERR_ARGUMENT;
     const RowsArgs a{(const uint16_t *)dy, (const uint16_t *)rows, weights, first, place, (uint16_t *)d_rows, d_weights, prob_m, top_k, experts, width / 8};
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    if (width <= 512) moe_combine_backward_kernel<1><<<(prob_m + 3) / 4, 256, 0, hs>>>(a);
-    else moe_combine_backward_kernel<4><<<prob_m, 256, 0, hs>>>(a);
+    if (narrow) moe_combine_backward_kernel<1><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    else moe_combine_backward_kernel<4><<<(unsigned)blocks, 256, 0, hs>>>(a);
     return launched();
 }
 
