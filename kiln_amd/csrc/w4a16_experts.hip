@@ -18,7 +18,8 @@
 // us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 177-185, the gradient 198-207: rounds of blocks that do not come out even (the same rows in
 // equal parts 167 and 185), and power: on values of this kind the matrix instructions alone reach 1.6 to 1.8 PFLOP/s, not the 2.2 that they do on zeros, and the vector
 // instructions that expand the codes, reads of LDS and loads come on top (each left out for a measurement took 2 to 8 % off); 768 rows of 64 experts, 2560 -> 2048:
-// 41-48, 3.6 to 4.3 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 27, a round and a half of blocks, each one's start and latencies.
+// 42, 4.1 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 25, a round and a half of blocks, each one's start (6 us with its stores), then 1.2 us to 128 of the
+// contraction, 2.1 where two blocks share a compute unit: matrix products 0.5 of it, vector instructions, LDS and loads 0.1 to 0.2 each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -56,28 +57,36 @@ struct ExpertsArgs {
 struct Work {
     int expert, row0, rows, column;  // expert == experts: rows of no expert;  -1: nothing
 };
+// (Nothing else is on its way while a block finds its work: up to 63 experts are a lane's each, loaded together and read from the lanes again.)
+__device__ __forceinline__ int sum_of_lanes_upto(int v) {
+    auto add = [&](auto control, auto rows) { v += __builtin_amdgcn_update_dpp(0, v, decltype(control)::value, decltype(rows)::value, 0xF, false); };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // from 1, 2, 4, 8 lanes below in a row of 16
+    add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // the last lane of the row below to rows 1 and 3
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // lane 31 to rows 2 and 3
+    return v;
+}
 template <int BM>
 __device__ __forceinline__ Work find_work(const int *__restrict__ first, int experts, int rows, int column_blocks, int lane) {
     const int keys = experts + 1, per = (keys + 63) / 64, e0 = min(keys, lane * per), e1 = min(keys, e0 + per);
-    auto begin_of = [&](int e) { return e < keys ? max(0, min(first[e], rows)) : rows; };  // (in bounds whatever `first` holds)
-    auto rows_of = [&](int e) { return max(0, begin_of(e + 1) - begin_of(e)); };
-    auto tiles_of = [](int n) { return (n + BM / 2 - 1) / BM; };                        // of more than half of BM rows
+    auto begin_of = [&](int e) {  // (in bounds whatever `first` holds)
+        const int begin = first[min(e, experts)];
+        return e < keys ? max(0, min(begin, rows)) : rows;
+    };
+    auto tiles_of = [](int n) { return (n + BM / 2 - 1) / BM; };  // of more than half of BM rows
     auto has_rest = [](int n) { return n % BM != 0 && n % BM <= BM / 2; };
-    int tiles = 0, rests = 0;  // of the lane's experts
-    for (int e = e0; e < e1; ++e) {
-        const int n = rows_of(e);
-        tiles += tiles_of(n);
-        rests += has_rest(n);
+    int begin = begin_of(e0), end = begin_of(e0 + 1), n = max(0, end - begin);  // of the lane's first expert
+    int tiles = tiles_of(n), rests = has_rest(n);  // of all of them
+    for (int e = e0 + 1; e < e1; ++e) {
+        const int next = begin_of(e + 1), m = max(0, next - end);
+        tiles += tiles_of(m);
+        rests += has_rest(m);
+        end = next;
     }
-    int tiles_upto = tiles, rests_upto = rests;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int a = __shfl_up(tiles_upto, d), b = __shfl_up(rests_upto, d);
-        if (lane >= d) {
-            tiles_upto += a;
-            rests_upto += b;
-        }
-    }
+    const int tiles_upto = sum_of_lanes_upto(tiles), rests_upto = sum_of_lanes_upto(rests);
     unsigned seq = blockIdx.x >> 3, id;
     auto mine = [&](unsigned total, unsigned die) {  // of a list: is this block's place in the die's share of it?
         const unsigned each = total >> 3, more = total & 7, count = each + (die < more ? 1u : 0u);
@@ -92,17 +101,22 @@ __device__ __forceinline__ Work find_work(const int *__restrict__ first, int exp
     if (!is_rest && !mine((unsigned)__builtin_amdgcn_readlane(tiles_upto, 63) * (unsigned)column_blocks, 7 - die)) return {-1, 0, 0, 0};
     const int tile = (int)(id / (unsigned)column_blocks), upto = is_rest ? rests_upto : tiles_upto;
     const int at = __builtin_ctzll(__ballot(upto > tile));
-    int base = __builtin_amdgcn_readlane(upto - (is_rest ? rests : tiles), at), e = at * per, count, n;
-    for (;; ++e) {
-        n = __builtin_amdgcn_readfirstlane(rows_of(e));
+    int base = __builtin_amdgcn_readlane(upto - (is_rest ? rests : tiles), at), e = at * per;
+    begin = __builtin_amdgcn_readlane(begin, at);
+    n = __builtin_amdgcn_readlane(n, at);
+    int count;
+    for (;;) {
         count = is_rest ? has_rest(n) : tiles_of(n);
         if (tile < base + count) break;
         base += count;
+        ++e;
+        begin = __builtin_amdgcn_readfirstlane(begin_of(e));
+        n = max(0, __builtin_amdgcn_readfirstlane(begin_of(e + 1)) - begin);
     }
     const int inside = (int)(id - (unsigned)base * (unsigned)column_blocks);
-    if (is_rest) return {e, begin_of(e) + n / BM * BM, n % BM, inside};
+    if (is_rest) return {e, begin + n / BM * BM, n % BM, inside};
     const int t = inside % count;
-    return {e, begin_of(e) + t * BM, min(BM, n - t * BM), inside / count};
+    return {e, begin + t * BM, min(BM, n - t * BM), inside / count};
 }
 
 // rows of no expert: zeros in the block's columns
@@ -155,8 +169,8 @@ struct Tile {
 // applied by a running rescale of the sums, (sums so far) / scale(g) times scale(g) / scale(g + 1) at each change of group, in f32.  The
 // surplus of 136 times a row's sum over the group comes off
 //   in blocks of 128 rows at the group's start, in the rescale's own multiply-add, from sums that a launch in front has formed: no work of its own;
-//   in smaller ones at its end, from a third product beside the two column sub-tiles', with -136 throughout: those blocks wait for the
-//   weights, not for the matrix cores, and calls of nothing else need no launch in front.
+//   in smaller ones at its end, by one product more with -136 throughout, of sums that a lane forms of the rows it multiplies (two values to an
+//   instruction): calls of nothing else need no launch in front.  (Eight products, one beside every step's: 2331 rows of 24 experts, 1280 -> 2048 29 us, so 26.)
 // A group's words and scales come to LDS two groups ahead.
 struct ManyLds {
     static constexpr int kStage = 128 * kRowBytes;
@@ -188,8 +202,9 @@ __device__ __forceinline__ uint32_t across_columns(float first, float second, in
     return __builtin_amdgcn_perm(own, other, lane & 1 ? 0x07060302u : 0x01000504u);
 }
 
+__device__ __forceinline__ int source_of(const ExpertsArgs &p, int pair) { return (int)min((unsigned)pair / (unsigned)p.top, (unsigned)p.x_rows - 1); }
 __device__ __forceinline__ int source_of(const ExpertsArgs &p, const Work &work, int row) {
-    return p.order ? (int)min((unsigned)p.order[work.row0 + row] / (unsigned)p.top, (unsigned)p.x_rows - 1) : work.row0 + row;
+    return p.order ? source_of(p, p.order[work.row0 + row]) : work.row0 + row;
 }
 
 // A wavefront's four column tiles of its expert's pack, from tile nt0 on: a group's words and scales to LDS (five loads), and out of it, words_in and
@@ -280,36 +295,52 @@ struct FewLds {
     static constexpr int kRing = MI == 1 ? 3 : 2, kRows = 32 * MI * 256, kScales = kRows + kWaves * 4096, kStage = kScales + kWaves * 256;
     static constexpr int kBytes = kRing * kStage;
 };
-// a group's eight k16 steps: the words' word t holds two of them; off: the rows' surplus
+// a group's eight k16 steps: the words' word t holds two of them.  Behind them the rows' surplus: a lane has summed its half of row lane % 32, and one more
+// product, with -136 throughout, adds up the halves and takes them off -- the sum in three parts of 8 bits, which is all of it.
 template <int MI>
-__device__ __forceinline__ void few_product(const char *rows, const u32x4 (&w)[2][2], const DequantConsts &dq, int lane, Tile<MI> &tile, f32x16 (&off)[MI]) {
+__device__ __forceinline__ void few_product(const char *rows, const u32x4 (&w)[2][2], const DequantConsts &dq, int lane, Tile<MI> &tile) {
     const bf16x8 bias = bf16x8_splat(0xC308C308u);  // -136
     static_assert(kCodeBias == 136.f, "");
     const int l32 = lane & 31, h = lane >> 5;
+    float sum[MI];
     unrolled<0, 8>([&](auto sc) {
         constexpr int step = decltype(sc)::value, t = step >> 1, v = step & 1;
-        bf16x8 a[MI];
+        u32x4 a[MI];
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) a[mi] = *reinterpret_cast<const bf16x8 *>(rows + (32 * mi + l32) * 256 + (((2 * step + h) ^ (l32 & 15)) << 4));
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) off[mi] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[mi], bias, step == 0 ? f32x16{} : off[mi], 0, 0, 0);
+        for (int mi = 0; mi < MI; ++mi) a[mi] = *reinterpret_cast<const u32x4 *>(rows + (32 * mi + l32) * 256 + (((2 * step + h) ^ (l32 & 15)) << 4));
 #pragma unroll
         for (int ni = 0; ni < 2; ++ni) {
             const bf16x8 b = codes_to_bf16x8(w[ni][v][t], dq);
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) tile.acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[mi], b, tile.acc[mi][ni], 0, 0, 0);
+            for (int mi = 0; mi < MI; ++mi)
+                tile.acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[mi]), b, tile.acc[mi][ni], 0, 0, 0);
         }
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sum[mi] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)a[mi][i]), bf16x2{(__bf16)1.f, (__bf16)1.f}, step + i == 0 ? 0.f : sum[mi], false);
     });
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        const uint32_t first = __builtin_bit_cast(uint32_t, sum[mi]);
+        const float behind = sum[mi] - __builtin_bit_cast(float, first & 0xFFFF0000u);
+        const uint32_t second = __builtin_bit_cast(uint32_t, behind);
+        const uint32_t third = __builtin_bit_cast(uint32_t, behind - __builtin_bit_cast(float, second & 0xFFFF0000u));
+        const bf16x8 parts = __builtin_bit_cast(bf16x8, u32x4{__builtin_amdgcn_perm(second, first, 0x07060302u), third >> 16, 0u, 0u});
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni) tile.acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(parts, bias, tile.acc[mi][ni], 0, 0, 0);
+    }
 }
-// the sums without the surplus, in units of the next group's scale
+// the sums in units of the next group's scale
 template <int MI>
-__device__ __forceinline__ void few_rescale(Tile<MI> &tile, const f32x16 (&off)[MI], const float (&by)[2]) {
+__device__ __forceinline__ void few_rescale(Tile<MI> &tile, const float (&by)[2]) {
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
         for (int ni = 0; ni < 2; ++ni)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) tile.acc[mi][ni][r] = (tile.acc[mi][ni][r] + off[mi][r]) * by[ni];
+            for (int r = 0; r < 16; ++r) tile.acc[mi][ni][r] *= by[ni];
 }
 
 // Where a compute unit gets one block at most, the block has a second set of four wavefronts for every other group (SETS), with LDS of its own; their sums
@@ -339,29 +370,35 @@ __device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &wo
     const Columns<SWIGLU> cols(p, work.expert, work.column * (kColumns / kTileN) + wave * 4, lane, wave * 4096, wave * 256);
     const int G = p.K / kGroupK;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr_t)lds);
+    auto group_of = [&](int turn) { return min(SETS * turn + set, G - 1); };  // past the end: the last one again, so that the count of loads in flight stays what it is
+    auto stage_of = [&](int turn) { return lds0 + (unsigned)(turn % L::kRing) * L::kStage; };
+    // The first stages' words wait for nothing, their rows for the order, which goes by the ring's last place.
+    const unsigned spare = (unsigned)(L::kRing - 1) * L::kStage + wave * 256;
+    if (p.order) load_to_lds_b32(uniform(reinterpret_cast<const char *>(p.order + work.row0)), (uint32_t)min(lane, work.rows - 1) * 4u, lds0 + spare);
+#pragma unroll
+    for (int turn = 0; turn < L::kRing - 1; ++turn) cols.fetch(group_of(turn), stage_of(turn) + L::kRows, stage_of(turn) + L::kScales);
+    wait_vector_loads<(L::kRing - 1) * 5>();
     const char *rows[LR];
 #pragma unroll
     for (int i = 0; i < LR; ++i) {
         const int row = 4 * (wave * LR + i) + (lane >> 4);
-        rows[i] = reinterpret_cast<const char *>(p.x + (size_t)source_of(p, work, min(row, work.rows - 1)) * p.K) + (((lane & 15) ^ (row & 15)) << 4);
+        const int source = p.order ? source_of(p, *reinterpret_cast<const int *>(lds + spare + 4 * row)) : work.row0 + min(row, work.rows - 1);
+        rows[i] = reinterpret_cast<const char *>(p.x + (size_t)source * p.K) + (((lane & 15) ^ (row & 15)) << 4);
     }
-    auto fetch = [&](int turn) {  // past the end: the last one again, so that the count of loads in flight stays what it is
-        const int from = min(SETS * turn + set, G - 1);
-        const unsigned to = lds0 + (unsigned)(turn % L::kRing) * L::kStage;
+    auto fetch_rows = [&](int turn) {
 #pragma unroll
-        for (int i = 0; i < LR; ++i) load_to_lds_b128(rows[i] + (size_t)from * 256, to + (wave * LR + i) * 1024);
-        cols.fetch(from, to + L::kRows, to + L::kScales);
+        for (int i = 0; i < LR; ++i) load_to_lds_b128(rows[i] + (size_t)group_of(turn) * 256, stage_of(turn) + (wave * LR + i) * 1024);
+    };
+    auto fetch = [&](int turn) {
+        fetch_rows(turn);
+        cols.fetch(group_of(turn), stage_of(turn) + L::kRows, stage_of(turn) + L::kScales);
     };
     const DequantConsts dq = dequant_consts();
     Tile<MI> tile;
-    f32x16 off[MI];
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) off[mi][r] = 0.f;
     float scale[2] = {0.f, 0.f};
 #pragma unroll
-    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch(turn);
+    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch_rows(turn);
+    wait_vector_loads<(L::kRing - 2) * LR>();  // the words and the first stage's rows; from here on a stage's rows are asked for before its words
 #pragma unroll 1
     for (int turn = 0; SETS * turn < G; ++turn) {
         wait_vector_loads<(L::kRing - 2) * LS>();  // this stage has landed
@@ -380,10 +417,10 @@ __device__ __forceinline__ void experts_few(const ExpertsArgs &p, const Work &wo
             by[ni] = scale[ni] * __builtin_amdgcn_rcpf(next);
             scale[ni] = next;
         }
-        few_rescale(tile, off, by);  // (of the first group: zeros)
-        few_product<MI>(stage, w, dq, lane, tile, off);
+        if (p.Gs != 1) few_rescale(tile, by);  // (of the first group: zeros)
+        few_product<MI>(stage, w, dq, lane, tile);
     }
-    few_rescale(tile, off, scale);
+    few_rescale(tile, scale);
     if constexpr (SETS > 1) {
         add_second_set<MI>(all_lds, lane, wave, set, tile);
         if (set == 1) return;
@@ -416,30 +453,37 @@ __global__ __launch_bounds__(kThreads, 1) void experts_split_kernel(ExpertsArgs 
     }
     const Columns<SWIGLU> cols(p, work.expert, work.column * 4, lane, 0, 0);
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr_t)lds + wave * L::kWave);
+    auto group_of = [&](int turn) { return min(wave + kWaves * turn, G - 1); };  // past the end: the last group again, so that the count of loads in flight stays what it is
+    auto stage_of = [&](int turn) { return lds0 + (unsigned)(turn % L::kRing) * L::kStage; };
+    const unsigned spare = (unsigned)(L::kRing - 1) * L::kStage;  // (as in experts_few)
+    if (p.order) load_to_lds_b32(uniform(reinterpret_cast<const char *>(p.order + work.row0)), (uint32_t)min(lane, work.rows - 1) * 4u, lds0 + spare);
+#pragma unroll
+    for (int turn = 0; turn < L::kRing - 1; ++turn) cols.fetch(group_of(turn), stage_of(turn) + 32 * 256, stage_of(turn) + L::kScales);
+    wait_vector_loads<(L::kRing - 1) * 5>();
     const char *rows[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int row = 4 * i + (lane >> 4);
-        rows[i] = reinterpret_cast<const char *>(p.x + (size_t)source_of(p, work, min(row, work.rows - 1)) * p.K) + (((lane & 15) ^ (row & 15)) << 4);
+        const int source = p.order ? source_of(p, *reinterpret_cast<const int *>(lds + wave * L::kWave + spare + 4 * row)) : work.row0 + min(row, work.rows - 1);
+        rows[i] = reinterpret_cast<const char *>(p.x + (size_t)source * p.K) + (((lane & 15) ^ (row & 15)) << 4);
     }
-    auto fetch = [&](int turn) {  // past the end: the last group again, so that the count of loads in flight stays what it is
-        const int from = min(wave + kWaves * turn, G - 1);
-        const unsigned to = lds0 + (unsigned)(turn % L::kRing) * L::kStage;
+    auto fetch_rows = [&](int turn) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_to_lds_b128(rows[i] + (size_t)from * 256, to + i * 1024);
-        cols.fetch(from, to + 32 * 256, to + L::kScales);
+        for (int i = 0; i < 8; ++i) load_to_lds_b128(rows[i] + (size_t)group_of(turn) * 256, stage_of(turn) + i * 1024);
     };
     const DequantConsts dq = dequant_consts();
     Tile<1> tile;
-    f32x16 off[1] = {};
     float scale[2] = {0.f, 0.f};
 #pragma unroll
-    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch(turn);
+    for (int turn = 0; turn < L::kRing - 1; ++turn) fetch_rows(turn);
 #pragma unroll 1
     for (int turn = 0; wave + kWaves * turn < G; ++turn) {
         wait_lds_reads();  // the stage before has been read
-        fetch(turn + L::kRing - 1);
-        wait_vector_loads<(L::kRing - 1) * LS>();
+        const int next = turn + L::kRing - 1;
+        fetch_rows(next);
+        cols.fetch(group_of(next), stage_of(next) + 32 * 256, stage_of(next) + L::kScales);
+        if (turn == 0) wait_vector_loads<(L::kRing - 2) * 8 + LS>();  // (the first stages' words were asked for before all rows)
+        else wait_vector_loads<(L::kRing - 1) * LS>();
         const char *stage = lds + wave * L::kWave + (turn % L::kRing) * L::kStage;
         u32x4 w[2][2];
         float by[2];
@@ -450,10 +494,10 @@ __global__ __launch_bounds__(kThreads, 1) void experts_split_kernel(ExpertsArgs 
             by[ni] = scale[ni] * __builtin_amdgcn_rcpf(next);
             scale[ni] = next;
         }
-        few_rescale<1>(tile, off, by);
-        few_product<1>(stage, w, dq, lane, tile, off);
+        if (p.Gs != 1) few_rescale<1>(tile, by);
+        few_product<1>(stage, w, dq, lane, tile);
     }
-    few_rescale<1>(tile, off, scale);
+    few_rescale<1>(tile, scale);
     wait_vector_loads<0>();
     wait_lds_reads();
     __syncthreads();
@@ -1067,17 +1111,17 @@ int64_t most_tiles(int rows, int experts, int block_rows) {
 // Which blocks a call takes, from what 128 of the contraction cost a block, us: `alone` on its compute unit, or `busy` where compute units have several (two side
 // by side take nearly twice as long: what they have to issue bounds them, not what they wait for); `rest` of a block to an expert for its last rows, `least` of
 // one to an expert of few.  us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
-//   forward    400 rows of 16 experts, 2560 -> 2048   23 /  32 /  34,   20 /  27,   28      800 of 32, 1280 -> 2048   19 /  20 /  22,  24 /  18,  34
-//              400 rows of  4 experts, 2560 -> 1024   21 /  30 /  39,   19 /  26,   11     4000 of 64, 2560 -> 1024   47 /  40 /  45,  54 /  45,  92
-//             3000 rows of 64 experts, 2560 -> 2048   67 /  53 /  56,   75 /  57,  143     8000 of  8, 1024 ->  512   16 /  19 /  24,  20 /  23,  47
-//             8000 rows of 64 experts, 2560 -> 2048  150 / 121 /  97,  162 / 128,  302    10000 of 16,  768 -> 1536   43 /  36 /  32,  62 /  44
-//            16384 rows of 64 experts, 2560 -> 2048  271 / 217 / 177,  308 / 246,  585
-//   gradient   400 rows of 16 experts, 2560 <- 2048   25 /  26 /  26,   23 /  24,   27      400 of 16,  768 <-  768   11 /  11 /  11,  10 /  11,   9
-//             2331 rows of 24 experts, 1280 <- 2048   34 /  26 /  38,   39 /  25,   48     6000 of 32, 2048 <-  768   46 /  33 /  32,  64 /  45,  98
-//             3000 rows of 64 experts, 2560 <- 2048   87 /  60 /  60,   99 /  70,  125     1500 of 64, 1024 <- 2560   41 /  43 /  30,  47 /  50,  44
-//            16384 rows of 64 experts, 2560 <- 2048  328 / 223 / 198,  415 / 265,  502
-// (The costs were fitted to 28 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory: what is
-// chosen is within 1 % of the best on average, 22 % off at the worst, 1000 rows of 8 experts, 512 -> 2048.)
+//   forward    400 rows of 16 experts, 2560 -> 2048   25 /  30 /  33,   22 /  27,   29      800 of 32, 1280 -> 2048   16 /  15 /  18,  16 /  16,  33
+//              400 rows of  4 experts, 2560 -> 1024   23 /  29 /  39,   20 /  26,   10     4000 of 64, 2560 -> 1024   54 /  46 /  59,  60 /  52,  89
+//             3000 rows of 64 experts, 2560 -> 2048   76 /  67 /  64,   84 /  73,  140     3000 of  8,  384 ->  256    7 /   8 /  12,   8 /   9,   9
+//             8000 rows of 64 experts, 2560 -> 2048  159 / 125 / 120,  178 / 137,  300    10000 of 16,  768 -> 1536   50 /  36 /  33,  69 /  47, 148
+//            16384 rows of 64 experts, 2560 -> 2048  273 / 222 / 197,  338 / 242,  568
+//   gradient   400 rows of 16 experts, 2560 <- 2048   24 /  26 /  26,   22 /  24,   27      400 of 16,  768 <-  768   11 /  12 /  11,  10 /  12,   9
+//             2331 rows of 24 experts, 1280 <- 2048   35 /  26 /  39,   40 /  26,   47     6000 of 32, 2048 <-  768   49 /  36 /  39,  67 /  46,  96
+//             3000 rows of 64 experts, 2560 <- 2048   88 /  67 /  77,  107 /  76,  121     5900 of 28,  256 <- 1536   20 /  21 /  31,  19 /  20,  23
+//            16384 rows of 64 experts, 2560 <- 2048  325 / 234 / 216,  408 / 271,  493
+// (The costs were fitted to 38 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory: what is
+// chosen is within 1 % of the best on average, 15 % off at the worst.)
 // Two sets and split blocks are one to a compute unit (LDS) and taken where one round of them does.
 enum class Blocks { kSplit, kOneTile, kTwoTiles, kFourTiles, kOneTileTwoSets, kTwoTilesTwoSets };
 struct BlockCost {
@@ -1107,14 +1151,14 @@ Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int con
 }
 // (of equals the larger: an expert with more rows than others then takes no second block)
 constexpr BlockCost kForwardCosts[5] = {{Blocks::kTwoTiles, 64, 1.37f, 0.84f, 1.f, 0.3f, 1.f, 0.f},
-                                        {Blocks::kOneTile, 32, 0.84f, 0.84f, 0.96f, 0.53f, 1.f, 0.f},
-                                        {Blocks::kFourTiles, 128, 1.9f, 0.84f, 1.59f, 0.26f, 0.41f, 3.5f},  // (its rows' sums are a launch)
+                                        {Blocks::kOneTile, 32, 0.84f, 0.84f, 1.f, 0.53f, 1.f, 0.f},
+                                        {Blocks::kFourTiles, 128, 1.9f, 0.84f, 1.59f, 0.26f, 0.51f, 3.5f},  // (its rows' sums are a launch)
                                         {Blocks::kTwoTilesTwoSets, 64, 1.25f, 0.71f, 0.f, 0.3f, 1.f, 1.f},
                                         {Blocks::kOneTileTwoSets, 32, 0.71f, 0.71f, 0.f, 0.53f, 1.f, 1.f}};
-constexpr BlockCost kGradientCosts[5] = {{Blocks::kTwoTiles, 64, 1.54f, 1.16f, 1.36f, 0.3f, 0.8f, 0.f},
-                                         {Blocks::kOneTile, 32, 1.16f, 1.16f, 1.27f, 0.5f, 1.f, 0.f},
+constexpr BlockCost kGradientCosts[5] = {{Blocks::kTwoTiles, 64, 1.54f, 1.16f, 1.36f, 0.3f, 0.97f, 0.f},
+                                         {Blocks::kOneTile, 32, 1.16f, 1.16f, 1.36f, 0.5f, 1.f, 0.f},
                                          {Blocks::kFourTiles, 128, 2.72f, 1.04f, 2.2f, 0.41f, 0.56f, 0.f},
-                                         {Blocks::kTwoTilesTwoSets, 64, 1.29f, 0.99f, 0.f, 0.3f, 0.8f, 1.f},
+                                         {Blocks::kTwoTilesTwoSets, 64, 1.3f, 0.98f, 0.f, 0.3f, 0.97f, 1.f},
                                          {Blocks::kOneTileTwoSets, 32, 0.99f, 0.99f, 0.f, 0.5f, 1.f, 1.f}};
 Blocks forward_blocks(int rows, int n, int k, int experts, int cus) { return choose_blocks(kForwardCosts, rows, experts, k, n / kColumns, n / 64, cus); }
 Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {

@@ -97,7 +97,7 @@ def test_every_kind_of_block_is_taken_by_some_size():
 
 SIZES = [(768, 2048, 512, 64), (1600, 512, 2048, 64), (3000, 2048, 512, 64), (3000, 512, 2048, 64), (6000, 1024, 1024, 32), (5000, 512, 512, 4),
          (360, 2560, 1024, 64), (400, 2048, 2560, 16), (800, 2048, 1280, 32), (1500, 2560, 1024, 64), (2331, 2048, 1280, 24),
-         (850, 2560, 1280, 4), (2350, 1024, 1280, 16), (1350, 1024, 512, 16)]
+         (850, 2560, 1280, 4), (2350, 1024, 1280, 16), (1350, 1024, 512, 16), (500, 512, 2560, 8), (1000, 512, 512, 8), (2000, 1024, 1024, 3)]
 
 
 @pytest.mark.parametrize("rows,n,k,experts", SIZES)
