@@ -199,7 +199,10 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs p) {
 
 // W wavefronts to a token, 4 / W tokens to a block: a lane goes over its units of dy and of every row; a row's product is summed in f32 in the lanes,
 // across them and across the wavefronts, in that order.
-template <int W>
+// LAST: the rows are read past the caches, for the last time.  Where they are too many to have stayed there it leaves room for what is written, which the next
+// product reads: 8 of 64, 2560 wide, 160 MB of rows 83.6 us, so 81.3 (with that product behind it 262 and 260), 58 MB 36.4 and 32.4, but 39 MB 18.4 and 20.4.
+// (Writes past the caches as well: 75.8, and 264 with the product.)
+template <int W, bool LAST>
 __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
     __shared__ float part[4][kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, of = wave % W, pairs = p.tokens * p.top, placed = min(p.first[p.experts], pairs);
@@ -222,7 +225,10 @@ __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
             u32x4 v[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                if (j0 + u < p.top && (unsigned)at[u] < (unsigned)placed) v[u] = reinterpret_cast<const u32x4 *>(p.rows)[(size_t)at[u] * p.units + unit];
+                if (j0 + u < p.top && (unsigned)at[u] < (unsigned)placed) {
+                    const u32x4 *from = reinterpret_cast<const u32x4 *>(p.rows) + (size_t)at[u] * p.units + unit;
+                    v[u] = LAST ? __builtin_nontemporal_load(from) : *from;
+                }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 if (j0 + u >= p.top || at[u] < 0) continue;
@@ -346,8 +352,11 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
         return KILN_W4A16_ERR_ARGUMENT;
     const RowsArgs a{(const uint16_t *)dy, (const uint16_t *)rows, weights, first, place, (uint16_t *)d_rows, d_weights, prob_m, top_k, experts, width / 8};
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
-    if (narrow) moe_combine_backward_kernel<1><<<(unsigned)blocks, 256, 0, hs>>>(a);
-    else moe_combine_backward_kernel<4><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    const bool last = pairs * width * 2 >= (size_t)48 << 20;
+    if (narrow && last) moe_combine_backward_kernel<1, true><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    else if (narrow) moe_combine_backward_kernel<1, false><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    else if (last) moe_combine_backward_kernel<4, true><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    else moe_combine_backward_kernel<4, false><<<(unsigned)blocks, 256, 0, hs>>>(a);
     return launched();
 }
 

@@ -41,7 +41,8 @@ def test_sort_is_the_same_every_time():
         assert all(torch.equal(a, b) for a, b in zip(once, mg.moe_sort(of, 64)))
 
 
-SHAPES = [(1, 8, 64, 0, 2560), (1, 1, 4, 0, 8), (5, 3, 4, 2, 24), (64, 8, 64, 0, 2560), (33, 16, 32, 8, 1032), (300, 2, 8, 2, 520), (100, 9, 10, 3, 512), (777, 4, 32, 32, 128)]
+SHAPES = [(1, 8, 64, 0, 2560), (1, 1, 4, 0, 8), (5, 3, 4, 2, 24), (64, 8, 64, 0, 2560), (33, 16, 32, 8, 1032), (300, 2, 8, 2, 520), (100, 9, 10, 3, 512), (777, 4, 32, 32, 128),
+          (1300, 8, 64, 8, 2560), (6200, 8, 64, 8, 512)]
 
 
 @pytest.mark.parametrize("m,top,experts,away,width", SHAPES)
