@@ -381,7 +381,7 @@ kiln_marlin_status_t kiln_w4a16_moe_sort(
  *                                                                           in the order of j, rounded once; y bf16 [m, width]
  *   combine_backward  d_rows[place[i, j]] = weights[i, j] * dy[i]           bf16 [m * top_k, width], rounded once
  *                     d_weights[i, j] = <rows[place[i, j]], dy[i]>          f32 [m, top_k], summed in f32; 0 without an expert
- * (Positions in `place` outside [0, m * top_k) are passed over.)  m * width <= 2^35 - 2048, and combine_backward m <= 2^24 - 1, with width <= 512 2^26 - 4.
+ * (Positions in `place` outside [0, m * top_k) are passed over.)  m * width <= 2^35 - 2048, and combine_backward m * top_k <= 2^26 - 4.
  */
 kiln_marlin_status_t kiln_w4a16_moe_gather(
     const void *x, const int *first, const int *place, void *rows,

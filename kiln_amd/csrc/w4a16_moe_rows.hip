@@ -197,68 +197,55 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(RowsArgs p) {
     reinterpret_cast<u32x4 *>(p.out)[i] = o;
 }
 
-// W wavefronts to a token, 4 / W tokens to a block: a lane goes over its units of dy and of every row; a row's product is summed in f32 in the lanes,
-// across them and across the wavefronts, in that order.
-// LAST: the rows are read past the caches, for the last time.  Where they are too many to have stayed there it leaves room for what is written, which the next
-// product reads: 8 of 64, 2560 wide, 160 MB of rows 83.6 us, so 81.3 (with that product behind it 262 and 260), 58 MB 36.4 and 32.4, but 39 MB 18.4 and 20.4.
-// (Writes past the caches as well: 75.8, and 264 with the product.)
-template <int W, bool LAST>
+constexpr int kAhead = 4;  // units of a lane in flight
+// A wavefront to a pair: its lanes go over the units of dy and of the pair's row together; the product is summed in f32 in the lanes and across them, in that
+// order.  dy is read once from memory and by the token's other pairs from the caches.  4096 tokens, 8 of 64, 2560 wide (357 MB) 73 us, 4.9 TB/s; a block to a
+// token, its wavefronts sharing out the units, 82 (five parts of 64 units do not go evenly to four), 64 tokens 3.9 and 7.9.
+// LAST: the rows are read past the caches, for the last time, which leaves room for what is written and the next product reads -- where they are too many to
+// have stayed there: 78 MB of rows 38 us without and 32, 58 MB 28 and 26, 39 MB level, but 27 MB 11.8 and 13.5; from 100 MB on level.
+template <bool LAST>
 __global__ __launch_bounds__(256) void moe_combine_backward_kernel(RowsArgs p) {
-    __shared__ float part[4][kMaxTop];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, of = wave % W, pairs = p.tokens * p.top, placed = min(p.first[p.experts], pairs);
-    const int token = blockIdx.x * (4 / W) + wave / W;
-    const bool live = token < p.tokens;
-    const int *place = p.place + (size_t)(live ? token : 0) * p.top;
-    const float *weights = p.weights + (size_t)(live ? token : 0) * p.top;
-    for (int j0 = 0; j0 < (live ? p.top : 0); j0 += 8) {
-        float dot[8] = {};
-        int at[8];
-        float w[8];
+    const int lane = threadIdx.x & 63, pairs = p.tokens * p.top, placed = min(p.first[p.experts], pairs);
+    const int pair = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (pair >= pairs) return;
+    const int at = p.place[pair], token = (int)((unsigned)pair / (unsigned)p.top);
+    const float w = p.weights[pair];
+    const bool here = at >= 0 && at < placed;
+    const u32x4 *dy = reinterpret_cast<const u32x4 *>(p.in) + (size_t)token * p.units;
+    float dot = 0.f;
+    if (here) {
+        const u32x4 *row = reinterpret_cast<const u32x4 *>(p.rows) + (size_t)at * p.units;
+        u32x4 *to = reinterpret_cast<u32x4 *>(p.out) + (size_t)at * p.units;
+        for (int unit0 = lane; unit0 < p.units; unit0 += 64 * kAhead) {
+            u32x4 d[kAhead], v[kAhead];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int j = min(j0 + u, p.top - 1);
-            at[u] = (unsigned)place[j] < (unsigned)pairs ? place[j] : -1;
-            w[u] = weights[j];
-        }
-        for (int unit = of * 64 + lane; unit < p.units; unit += W * 64) {
-            const u32x4 d = reinterpret_cast<const u32x4 *>(p.in)[(size_t)token * p.units + unit];
-            u32x4 v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (j0 + u < p.top && (unsigned)at[u] < (unsigned)placed) {
-                    const u32x4 *from = reinterpret_cast<const u32x4 *>(p.rows) + (size_t)at[u] * p.units + unit;
-                    v[u] = LAST ? __builtin_nontemporal_load(from) : *from;
+            for (int i = 0; i < kAhead; ++i) {
+                const int unit = unit0 + 64 * i;
+                if (unit < p.units) {
+                    v[i] = LAST ? __builtin_nontemporal_load(row + unit) : row[unit];
+                    d[i] = dy[unit];
                 }
+            }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                if (j0 + u >= p.top || at[u] < 0) continue;
-                u32x4 o = {0u, 0u, 0u, 0u};
-                if (at[u] < placed) {
+            for (int i = 0; i < kAhead; ++i) {
+                const int unit = unit0 + 64 * i;
+                if (unit >= p.units) break;
+                u32x4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[e] = bf16_pair(w[u] * bf16_low(d[e]), w[u] * bf16_high(d[e]));
-                        dot[u] = fmaf(bf16_low(d[e]), bf16_low(v[u][e]), dot[u]);
-                        dot[u] = fmaf(bf16_high(d[e]), bf16_high(v[u][e]), dot[u]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    o[e] = bf16_pair(w * bf16_low(d[i][e]), w * bf16_high(d[i][e]));
+                    dot = fmaf(bf16_low(d[i][e]), bf16_low(v[i][e]), dot);
+                    dot = fmaf(bf16_high(d[i][e]), bf16_high(v[i][e]), dot);
                 }
-                reinterpret_cast<u32x4 *>(p.out)[(size_t)at[u] * p.units + unit] = o;
+                to[unit] = o;
             }
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            float s = dot[u];
-#pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
-            if (lane == 0 && j0 + u < p.top) part[wave][j0 + u] = s;
-        }
+    } else if ((unsigned)at < (unsigned)pairs) {
+        for (int unit = lane; unit < p.units; unit += 64) reinterpret_cast<u32x4 *>(p.out)[(size_t)at * p.units + unit] = u32x4{0u, 0u, 0u, 0u};
     }
-    __syncthreads();
-    if (of == 0 && live && lane < p.top) {
-        float s = part[wave][lane];
 #pragma unroll
-        for (int i = 1; i < W; ++i) s += part[wave + i][lane];
-        p.d_weights[(size_t)token * p.top + lane] = s;
-    }
+    for (int d = 32; d >= 1; d >>= 1) dot += __shfl_xor(dot, d);
+    if (lane == 0) p.d_weights[pair] = dot;
 }
 
 // ---- the entry points' checks --------------------------------------------------------------------------------------
@@ -341,8 +328,7 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
                                                      void *d_rows, float *d_weights, int prob_m, int top_k, int experts, int width, int dev, void *stream) {
     (void)dev;
     if (const kiln_marlin_status_t st = rows_ok(prob_m, top_k, experts, width)) return st;
-    const bool narrow = width <= 512;
-    const int64_t blocks = narrow ? ((int64_t)prob_m + 3) / 4 : prob_m;
+    const int64_t blocks = ((int64_t)prob_m * top_k + 3) / 4;
     if (!launchable(blocks, 256)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (prob_m == 0) return KILN_W4A16_OK;
     if (!all_on(16, {dy, rows, d_rows}) || !all_on(4, {weights, first, place, d_weights})) return KILN_W4A16_ERR_ARGUMENT;
@@ -353,10 +339,8 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(const void *dy, const void 
     const RowsArgs a{(const uint16_t *)dy, (const uint16_t *)rows, weights, first, place, (uint16_t *)d_rows, d_weights, prob_m, top_k, experts, width / 8};
     hipStream_t hs = reinterpret_cast<hipStream_t>(stream);
     const bool last = pairs * width * 2 >= (size_t)48 << 20;
-    if (narrow && last) moe_combine_backward_kernel<1, true><<<(unsigned)blocks, 256, 0, hs>>>(a);
-    else if (narrow) moe_combine_backward_kernel<1, false><<<(unsigned)blocks, 256, 0, hs>>>(a);
-    else if (last) moe_combine_backward_kernel<4, true><<<(unsigned)blocks, 256, 0, hs>>>(a);
-    else moe_combine_backward_kernel<4, false><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    if (last) moe_combine_backward_kernel<true><<<(unsigned)blocks, 256, 0, hs>>>(a);
+    else moe_combine_backward_kernel<false><<<(unsigned)blocks, 256, 0, hs>>>(a);
     return launched();
 }
 

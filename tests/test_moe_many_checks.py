@@ -129,11 +129,11 @@ def test_calls_on_tensors_of_the_host_are_refused():
 def test_sizes_that_no_launch_has_work_items_for_are_refused():
     most = (1 << 24) - 1                        # blocks of 256
     assert gather(m=1 << 24, top=1, width=2048) == combine(m=1 << 24, top=1, width=2048) == _lib.ERR_KERN_SHAPE
-    assert combine_backward(m=1 << 24, top=1, width=1024) == combine_backward(m=1 << 26, top=1, width=64) == _lib.ERR_KERN_SHAPE
+    assert combine_backward(m=1 << 26, top=1, width=64) == combine_backward(m=1 << 23, top=8, width=64) == _lib.ERR_KERN_SHAPE
     assert keep(m=1 << 24, n=2048) == keep_backward(m=1 << 24, n=2048) == _lib.ERR_KERN_SHAPE
     assert experts(rows=1 << 24, x_rows=1 << 24, k=2048) == _lib.ERR_KERN_SHAPE                     # the rows' sums
     assert experts(rows=1 << 24, x_rows=1 << 24, k=128, n=1 << 17) == experts_backward(rows=1 << 24, k=1 << 17, n=256) == _lib.ERR_KERN_SHAPE
     # one less is asked for its pointers
     assert gather(m=most, top=1, width=2048, x=None) == combine(m=most, top=1, width=2048, y=None) == _lib.ERR_ARGUMENT
-    assert combine_backward(m=most, top=1, width=1024, dy=None) == combine_backward(m=4 * most, top=1, width=64, dy=None) == _lib.ERR_ARGUMENT
+    assert combine_backward(m=4 * most, top=1, width=64, dy=None) == combine_backward(m=most // 2, top=8, width=64, dy=None) == _lib.ERR_ARGUMENT
     assert keep(m=most, n=2048, h=None) == experts(rows=most, x_rows=most, k=2048, x=None) == _lib.ERR_ARGUMENT
