@@ -734,25 +734,28 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x2 turned_codes(unsigned lds_at, int offset) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2_ptr_t)(uintptr_t)lds_at + offset / 8));
 }
-// mask and magic number of the codes' expansion, one instruction with both in registers that the compiler cannot see through (as dequant_consts)
+// masks and magic numbers of the codes' expansion, one instruction with both in registers that the compiler cannot see through (as dequant_consts)
 struct TurnedConsts {
-    uint32_t mask, magic;
+    uint32_t mask[2], magic[2];
 };
 __device__ __forceinline__ TurnedConsts turned_consts() {
     TurnedConsts c;
-    asm volatile("s_mov_b32 %0, 0x000F000F" : "=s"(c.mask));
-    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(c.magic));
+    asm volatile("s_mov_b32 %0, 0x000F000F" : "=s"(c.mask[0]));
+    asm volatile("s_mov_b32 %0, 0x00F000F0" : "=s"(c.mask[1]));
+    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(c.magic[0]));
+    asm volatile("v_mov_b32 %0, 0x54005400" : "=v"(c.magic[1]));
     return c;
 }
 // Eight codes of one row of the pack in eight columns, and those columns' scales: half H of an operand's registers, codes 2 H, 2 H + 1 and four on.
-// 1024 + code in f16, less 1032, times the scale in f32: exact.
+// 1024 + code in f16, or 64 + code where the code lies four bits higher, less 1032 or 72, times the scale in f32: exact.
 template <int H>
 __device__ __forceinline__ void half_of_weights(uint32_t codes, const u32x4 &scales, const TurnedConsts &tc, u32x4 &operand) {
     const f16x2 low = __builtin_bit_cast(f16x2, (uint32_t)scales[H]), high = __builtin_bit_cast(f16x2, (uint32_t)scales[2 + H]);
     float v[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const f16x2 d = __builtin_bit_cast(f16x2, (codes >> (8 * H + 4 * i) & tc.mask) | tc.magic) - f16x2{(_Float16)1032.f, (_Float16)1032.f};
+        const _Float16 less = (_Float16)(i ? 72.f : 1032.f);
+        const f16x2 d = __builtin_bit_cast(f16x2, (codes >> 8 * H & tc.mask[i]) | tc.magic[i]) - f16x2{less, less};
         v[0][i] = fmaf((float)d.x, (float)low[i], 0.f);
         v[1][i] = fmaf((float)d.y, (float)high[i], 0.f);
     }
