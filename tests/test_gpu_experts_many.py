@@ -188,3 +188,33 @@ def test_the_same_bits_every_time():
     for _ in range(10):
         assert torch.equal(y, mg.marlin_w4a16_gemm_experts(x, first, b, s, 128, order=order, top_k=4))
         assert torch.equal(dx, mg.marlin_w4a16_gemm_experts_backward(dy, first, b, s, 128))
+
+
+@pytest.mark.parametrize("rows,k,n", [(5, 2560, 512), (90, 1152, 512), (300, 2560, 256), (600, 128, 256), (3000, 512, 1024)])
+def test_rows_of_one_sign(rows, k, n):
+    """The surplus of 136 times a row's sum is the largest there is: a partial sum is at most 144 * 128 times the largest value, each of k additions off by 2^-24
+    of it, at random, and the row's own sum, 64 additions of pairs off by three times as much, times 136; four times that."""
+    r = gen(rows)
+    first = first_of([rows // 2, 0, rows - rows // 2])
+    b, s = packs(r, 3, k, n, 128)
+    x = (3 + torch.rand((rows, k), device="cuda", generator=r)).bfloat16()
+    x[1::2] *= -1
+    y, bounds = mg.marlin_w4a16_gemm_experts(x, first, b, s, 128), first.tolist()
+    for e in (0, 2):
+        i, j = bounds[e], bounds[e + 1]
+        off = 4 * F32 * (math.sqrt(k) * 144 + 3 * math.sqrt(64) * 136) * 128 * 4 * float(s[e].double().max())
+        want = x[i:j].double() @ weight(b[e], s[e])
+        assert ((y[i:j].double() - want).abs() <= HALF * want.abs() + off).all(), e
+
+
+@pytest.mark.parametrize("experts", [62, 63, 64, 200, 1024])
+def test_more_experts_than_lanes(experts):
+    r = gen(experts)
+    counts = torch.randint(0, 5, (experts,), device="cuda", generator=r)
+    counts[experts // 2], counts[experts - 1] = 150, 40
+    first = first_of(counts.tolist())
+    rows = int(first[-1]) + 33
+    b, s = packs(r, experts, 128, 256, 128)
+    x, dy = bf16(r, rows, 128), bf16(r, rows, 256)
+    check_forward(x, first, b, s, 128)
+    check_backward(dy, first, b, s, 128)
