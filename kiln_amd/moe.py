@@ -65,7 +65,7 @@ def experts_many(x: torch.Tensor, expert_of: torch.Tensor, weights: torch.Tensor
 
 def moe_forward_many(x: torch.Tensor, router_t: torch.Tensor, experts: MoeExperts, top_k: int, renormalise: bool = True) -> torch.Tensor:
     """`moe_forward` for many tokens (`experts_many`): a prefill.  Worth it from 65 tokens on, where `marlin_w4a16_moe` reads packs a second time (64 experts, top 8,
-    2560 -> 1024 -> 2560: 64 tokens 69 us here and 60 there, 96 tokens 72 and 115, 256 tokens 105 and 243)."""
+    2560 -> 1024 -> 2560: 64 tokens 71 us here and 60 there, 96 tokens 71 and 113, 256 tokens 90 and 243)."""
     rows = x.reshape(-1, x.shape[-1])
     expert_of, weights = marlin_gemm.moe_route(rows @ router_t, top_k, renormalise)
     y = experts_many(rows, expert_of, weights, experts)
