@@ -1112,8 +1112,12 @@ int64_t most_tiles(int rows, int experts, int block_rows) {
     return (int64_t)rows / block_rows + std::min<int64_t>((int64_t)experts + 1, rows);
 }
 // Which blocks a call takes, from what 128 of the contraction cost a block, us: `alone` on its compute unit, or `busy` where compute units have several (two side
-// by side take nearly twice as long: what they have to issue bounds them, not what they wait for); `rest` of a block to an expert for its last rows, `least` of
-// one to an expert of few.  us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
+// by side take nearly twice as long: what they have to issue bounds them, not what they wait for; an eighth longer again where every one has two blocks of up to 64
+// rows, which load more to a product); `rest` of a block to an expert for its last rows, `least` of one to an expert of few; `launch` of the rows' sums, or of the
+// sets' exchange.  An expert with rows has a block to each column block, whatever it costs.  Experts of up to 32 rows, and of up to 64, run the same code in every
+// block that takes them, so what those cost agrees: `few`, and `busy` times `least`.  In the forward product the 128-row kernel has a launch in front beside, for
+// nothing where no expert has more than 64 rows (64 experts, 2560 -> 2048, 40 rows 24 us and 22; 8 experts, 4096 -> 28672, 200 rows 165 and 135).
+// us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
 //   forward    400 rows of 16 experts, 2560 -> 2048   25 /  30 /  33,   22 /  27,   29      800 of 32, 1280 -> 2048   16 /  15 /  18,  16 /  16,  33
 //              400 rows of  4 experts, 2560 -> 1024   23 /  29 /  39,   20 /  26,   10     4000 of 64, 2560 -> 1024   54 /  46 /  59,  60 /  52,  89
 //             3000 rows of 64 experts, 2560 -> 2048   76 /  67 /  64,   84 /  73,  140     3000 of  8,  384 ->  256    7 /   8 /  12,   8 /   9,   9
@@ -1123,8 +1127,9 @@ int64_t most_tiles(int rows, int experts, int block_rows) {
 //             2331 rows of 24 experts, 1280 <- 2048   35 /  26 /  39,   40 /  26,   47     6000 of 32, 2048 <-  768   49 /  36 /  39,  67 /  46,  96
 //             3000 rows of 64 experts, 2560 <- 2048   88 /  67 /  77,  107 /  76,  121     5900 of 28,  256 <- 1536   20 /  21 /  31,  19 /  20,  23
 //            16384 rows of 64 experts, 2560 <- 2048  325 / 234 / 216,  408 / 271,  493
-// (The costs were fitted to 38 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory: what is
-// chosen is within 1 % of the best on average, 15 % off at the worst.)
+// (The costs were fitted to 38 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory, where what is
+// chosen is within 1 % of the best on average, 15 % off at the worst; on 120 others, from 2 rows in all to 4000 of one expert, 2 %, and 49 % at the worst: the gradient of 16
+// rows of 16 experts, 2560 <- 9216, 68, in split blocks, which would take two rounds, 46.)
 // Two sets and split blocks are one to a compute unit (LDS) and taken where one round of them does.
 enum class Blocks { kSplit, kOneTile, kTwoTiles, kFourTiles, kOneTileTwoSets, kTwoTilesTwoSets };
 struct BlockCost {
@@ -1132,19 +1137,22 @@ struct BlockCost {
     int rows;
     float alone, few, busy, rest, least, launch;  // few: alone, and up to kFewEach rows to an expert;  busy 0: one to a compute unit at most
 };
-constexpr float kFewEach = 24.f;
+constexpr float kFewEach = 24.f;  // (128-row blocks: a third, as an expert in 32 may have four times the rows of another, and one of more than 64 takes twice as long there)
 Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int contraction, int column_blocks, int split_columns, int cus) {
     const float present = (float)std::min(rows, experts), each = rows / present, groups = contraction / 128.f;
     if (present * std::max(1.f, each / 32 + 0.5f) * split_columns <= 1.05f * cus) return Blocks::kSplit;
     const BlockCost *best = nullptr;
     float least = 0.f;
     for (const BlockCost &c : costs) {
-        float share = present * std::max(c.least, each / c.rows + c.rest) * column_blocks / cus;
-        if (c.busy == 0.f) {  // a block too many takes a second round: an expert in 32 may have four times the rows of another
-            if (each * 4 > c.rows) share += present / 32 * column_blocks / cus;
-            if (share > 1.f) continue;
-        }
-        const float time = groups * (share > 1.f ? c.busy * std::max(share, 2.f) : each <= kFewEach ? c.few : c.alone) + c.launch;
+        const bool tall = c.rows == 128;
+        if (tall && rows <= 64) continue;  // (what they are for needs an expert of more)
+        const float blocks = each / c.rows + c.rest, share = present * std::max(c.least, blocks) * column_blocks / cus;
+        float count = present * std::max(1.f, blocks) * column_blocks / cus;  // of blocks, to a compute unit
+        // where one round is taken for all there is, a block too many takes a second: an expert in 32 may have four times the rows of another
+        if ((tall || c.busy == 0.f) && each * 4 > c.rows) count += present / 32 * column_blocks / cus;
+        if (c.busy == 0.f && count > 1.f) continue;
+        const float side_by_side = tall ? 2.f : std::min(1.75f + share / 4, 2.25f);
+        const float time = groups * (count > 1.f ? c.busy * std::max(share, side_by_side) : each <= (tall ? kFewEach / 3 : kFewEach) ? c.few : c.alone) + c.launch;
         if (!best || time < least) {
             best = &c;
             least = time;
@@ -1153,15 +1161,15 @@ Blocks choose_blocks(const BlockCost (&costs)[5], int rows, int experts, int con
     return best->blocks;
 }
 // (of equals the larger: an expert with more rows than others then takes no second block)
-constexpr BlockCost kForwardCosts[5] = {{Blocks::kTwoTiles, 64, 1.37f, 0.84f, 1.f, 0.3f, 1.f, 0.f},
+constexpr BlockCost kForwardCosts[5] = {{Blocks::kFourTiles, 128, 1.9f, 0.84f, 1.59f, 0.26f, 0.63f, 3.5f},  // (its rows' sums are a launch)
+                                        {Blocks::kTwoTiles, 64, 1.37f, 0.84f, 1.f, 0.3f, 1.f, 0.f},
                                         {Blocks::kOneTile, 32, 0.84f, 0.84f, 1.f, 0.53f, 1.f, 0.f},
-                                        {Blocks::kFourTiles, 128, 1.9f, 0.84f, 1.59f, 0.26f, 0.51f, 3.5f},  // (its rows' sums are a launch)
                                         {Blocks::kTwoTilesTwoSets, 64, 1.25f, 0.71f, 0.f, 0.3f, 1.f, 1.f},
                                         {Blocks::kOneTileTwoSets, 32, 0.71f, 0.71f, 0.f, 0.53f, 1.f, 1.f}};
-constexpr BlockCost kGradientCosts[5] = {{Blocks::kTwoTiles, 64, 1.54f, 1.16f, 1.36f, 0.3f, 0.97f, 0.f},
+constexpr BlockCost kGradientCosts[5] = {{Blocks::kFourTiles, 128, 3.05f, 1.16f, 2.2f, 0.41f, 0.62f, 0.f},
+                                         {Blocks::kTwoTiles, 64, 1.54f, 1.16f, 1.36f, 0.3f, 1.f, 0.f},
                                          {Blocks::kOneTile, 32, 1.16f, 1.16f, 1.36f, 0.5f, 1.f, 0.f},
-                                         {Blocks::kFourTiles, 128, 2.72f, 1.04f, 2.2f, 0.41f, 0.56f, 0.f},
-                                         {Blocks::kTwoTilesTwoSets, 64, 1.3f, 0.98f, 0.f, 0.3f, 0.97f, 1.f},
+                                         {Blocks::kTwoTilesTwoSets, 64, 1.3f, 0.98f, 0.f, 0.3f, 1.f, 1.f},
                                          {Blocks::kOneTileTwoSets, 32, 0.99f, 0.99f, 0.f, 0.5f, 1.f, 1.f}};
 Blocks forward_blocks(int rows, int n, int k, int experts, int cus) { return choose_blocks(kForwardCosts, rows, experts, k, n / kColumns, n / 64, cus); }
 Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {
