@@ -407,6 +407,9 @@ kiln_marlin_status_t kiln_w4a16_moe_combine_backward(
  * The weights are exact, as in the plain GEMM; a row with an infinity is NaN.  n % 256 == 0, k % 128 == 0, experts 1 ... 1024, x_rows <= 2^29, x_rows * k <= 2^35 - 2048.
  * The gradient of the rows, the packs frozen: dx[p] = dy[p] * dequant(B_e, s_e)^T, bf16 [rows, k], rounded once; a weight enters the product
  * rounded to bf16, as in kiln_w4a16_gemm_bank_backward.
+ * One launch holds a call: with b = rows / 32 + min(experts + 1, rows), both take sizes up to b * (n / 256) <= 2^24 - 9, the gradient b * ((k + 255) / 256), as long as
+ * b * (max(n, k) / 64 + 1) <= 2^31 - 9.  Beyond the former it depends on the blocks that a call takes, of 32, 64 or 128 rows x 256 columns, at most 2^24 - 1 of them;
+ * what is too large is refused (KILN_W4A16_ERR_KERN_SHAPE).
  */
 size_t kiln_w4a16_gemm_experts_scratch_bytes(int x_rows, int prob_k);
 kiln_marlin_status_t kiln_w4a16_gemm_experts(

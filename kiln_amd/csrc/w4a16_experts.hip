@@ -1177,8 +1177,13 @@ Blocks gradient_blocks(int rows, int n, int k, int experts, int cus) {
 }
 int rows_of(Blocks blocks) { return blocks == Blocks::kFourTiles ? 128 : blocks == Blocks::kTwoTiles || blocks == Blocks::kTwoTilesTwoSets ? 64 : 32; }
 int threads_of(Blocks blocks) { return blocks == Blocks::kOneTileTwoSets || blocks == Blocks::kTwoTilesTwoSets ? 2 * kThreads : kThreads; }
+int forward_columns(Blocks blocks, int n) { return blocks == Blocks::kSplit ? n / 64 : n / kColumns; }
+int gradient_columns(Blocks blocks, int k) { return blocks == Blocks::kSplit ? k / kGroupK : (k + kColumns - 1) / kColumns; }
 // (Eight blocks more: a die's shares of both lists may be rounded up.)
 int64_t blocks_of(Blocks blocks, int rows, int experts, int column_blocks) { return most_tiles(rows, experts, rows_of(blocks)) * column_blocks + 8; }
+bool one_launch(Blocks blocks, int rows, int experts, int column_blocks) {
+    return launchable(blocks_of(blocks, rows, experts, column_blocks), threads_of(blocks));
+}
 template <auto Kernel>
 bool launch(const ExpertsArgs &a, Blocks blocks, int lds_bytes, hipStream_t stream) {
     if (allow_dynamic_lds<Kernel>(lds_bytes) != hipSuccess) return false;
@@ -1214,8 +1219,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts(const void *x, const int *first, co
     if (x_rows > kMaxRows || !launchable((items + 15) / 16, 256)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (rows == 0) return KILN_W4A16_OK;
     const Blocks blocks = forward_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
-    const int column_blocks = blocks == Blocks::kSplit ? prob_n / 64 : prob_n / kColumns;
-    if (!launchable(blocks_of(blocks, rows, experts, column_blocks), threads_of(blocks))) return KILN_W4A16_ERR_KERN_SHAPE;
+    const int column_blocks = forward_columns(blocks, prob_n);
+    if (!one_launch(blocks, rows, experts, column_blocks)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (!all_on(16, {x, b, s, y, scratch}) || !all_on(4, {first}) || reinterpret_cast<uintptr_t>(order) % 4 != 0) return KILN_W4A16_ERR_ARGUMENT;
     const size_t width = swiglu ? prob_n / 2 : prob_n;
     if (any_meet({{y, rows * width * 2}, {scratch, kiln_w4a16_gemm_experts_scratch_bytes(x_rows, prob_k)}},
@@ -1253,8 +1258,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(const void *dy, const int 
     if (const kiln_marlin_status_t st = experts_ok(rows, prob_n, prob_k, experts, groupsize)) return st;
     if (rows == 0) return KILN_W4A16_OK;
     const Blocks blocks = gradient_blocks(rows, prob_n, prob_k, experts, compute_units(dev));
-    const int column_blocks = blocks == Blocks::kSplit ? prob_k / kGroupK : (prob_k + kColumns - 1) / kColumns;
-    if (!launchable(blocks_of(blocks, rows, experts, column_blocks), threads_of(blocks))) return KILN_W4A16_ERR_KERN_SHAPE;
+    const int column_blocks = gradient_columns(blocks, prob_k);
+    if (!one_launch(blocks, rows, experts, column_blocks)) return KILN_W4A16_ERR_KERN_SHAPE;
     if (!all_on(16, {dy, b, s, dx}) || !all_on(4, {first})) return KILN_W4A16_ERR_ARGUMENT;
     if (any_meet({{dx, (size_t)rows * prob_k * 2}}, {{dy, (size_t)rows * prob_n * 2}, {first, ((size_t)experts + 1) * 4}, pack_of(b, prob_n, prob_k, experts),
                                                      scales_of(s, prob_n, prob_k, experts, groupsize)}))
@@ -1283,7 +1288,8 @@ kiln_marlin_status_t kiln_w4a16_gemm_experts_backward(const void *dy, const int 
 
 int kiln_w4a16_debug_experts_plan(int rows, int prob_n, int prob_k, int experts, int backward, int cus) {
     if (experts_ok(rows, prob_n, prob_k, experts, 128) != KILN_W4A16_OK || rows < 1 || cus < 1) return -1;
-    return (int)(backward ? gradient_blocks(rows, prob_n, prob_k, experts, cus) : forward_blocks(rows, prob_n, prob_k, experts, cus));
+    const Blocks blocks = backward ? gradient_blocks(rows, prob_n, prob_k, experts, cus) : forward_blocks(rows, prob_n, prob_k, experts, cus);
+    return one_launch(blocks, rows, experts, backward ? gradient_columns(blocks, prob_k) : forward_columns(blocks, prob_n)) ? (int)blocks : -1;
 }
 
 }  // extern "C"

@@ -45,3 +45,28 @@ def test_more_rows_never_take_smaller_blocks(n, k, experts, backward):
 def test_calls_of_few_rows_to_an_expert(rows, n, k, experts, backward):
     """They took blocks of 128 rows, which are up to 30 % slower there, and never faster."""
     assert plan(rows, n, k, experts, backward) in (1, 2, 4, 5)
+
+
+def forward(rows, n, k, experts):
+    """The call with pointers that are refused once the sizes have been taken."""
+    return _lib.load().kiln_w4a16_gemm_experts(None, None, None, None, None, None, rows, rows, 1, n, k, experts, 128, 0, 0, None, None)
+
+
+def gradient(rows, n, k, experts):
+    return _lib.load().kiln_w4a16_gemm_experts_backward(None, None, None, None, None, rows, n, k, experts, 128, 0, None)
+
+
+def test_sizes_that_a_call_refuses_have_no_plan():
+    for rows, n, k, experts in ((1 << 24, 1 << 17, 128, 4), (1 << 23, 1 << 17, 128, 4), (1 << 22, 1 << 17, 128, 4), (1 << 20, 1 << 17, 128, 4), (1 << 24, 1 << 14, 128, 1024)):
+        assert (plan(rows, n, k, experts, 0) == -1) == (forward(rows, n, k, experts) == _lib.ERR_KERN_SHAPE)
+        assert (plan(rows, 256, n, experts, 1) == -1) == (gradient(rows, 256, n, experts) == _lib.ERR_KERN_SHAPE)
+    assert plan(1 << 24, 1 << 17, 128, 4, 0) == plan(1 << 24, 256, 1 << 17, 4, 1) == -1
+
+
+def test_sizes_up_to_the_documented_bound_are_taken():
+    for experts, columns in itertools.product((1, 4, 63, 1024), (1, 2, 3, 10, 100, 512, 4096)):
+        blocks = ((1 << 24) - 9) // columns                                            # rows / 32 + experts + 1 of them
+        rows = (blocks - experts - 1) * 32 + 31
+        if rows * 128 <= (1 << 35) - 2048:
+            assert plan(rows, 256 * columns, 128, experts, 0) >= 0 and forward(rows, 256 * columns, 128, experts) == _lib.ERR_ARGUMENT
+        assert plan(rows, 256, 256 * columns, experts, 1) >= 0 and gradient(rows, 256, 256 * columns, experts) == _lib.ERR_ARGUMENT
