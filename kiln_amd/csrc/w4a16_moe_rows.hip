@@ -138,16 +138,15 @@ struct RowsArgs {
     int tokens, top, experts, units;
 };
 
-// a thread's token and unit (32 bits where they do: a division of 64 takes longer than a small call's loads)
+// a thread's token and unit (a launch has less than 2^32 of them, rows_ok sees to that)
 struct Place {
     int token, unit;
     size_t at;
     bool live;
 };
 __device__ __forceinline__ Place place_of(const RowsArgs &p) {
-    const size_t total = (size_t)p.tokens * p.units, i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int token = total >> 32 ? (int)(i / p.units) : (int)((unsigned)i / (unsigned)p.units);
-    return {token, (int)(i - (size_t)token * p.units), i, i < total};
+    const unsigned i = blockIdx.x * 256 + threadIdx.x, units = (unsigned)p.units, token = i / units;
+    return {(int)token, (int)(i - token * units), i, i < (unsigned)p.tokens * units};
 }
 
 __global__ __launch_bounds__(256) void moe_gather_kernel(RowsArgs p) {
