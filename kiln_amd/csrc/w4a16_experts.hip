@@ -15,10 +15,10 @@
 //   32 rows x 64 columns (the gradient: 128), the wavefronts sharing out the contraction, where the others would leave compute units idle.
 // In blocks of 128 and 64 rows what is left of an expert goes as in the smaller ones.
 //
-// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 177-185, the gradient 198-207: rounds of blocks that do not come out even (the same rows in
-// equal parts 167 and 185), and power: on values of this kind the matrix instructions alone reach 1.6 to 1.8 PFLOP/s, not the 2.2 that they do on zeros, and the vector
+// us a call and what bounds it: 16384 rows of 64 experts, 2560 -> 2048 (172 GFLOP): 177-195, the gradient 209-217: rounds of blocks that do not come out even (the same rows in
+// equal parts 167 and 187), and power: on values of this kind the matrix instructions alone reach 1.6 to 1.8 PFLOP/s, not the 2.2 that they do on zeros, and the vector
 // instructions that expand the codes, reads of LDS and loads come on top (each left out for a measurement took 2 to 8 % off); 768 rows of 64 experts, 2560 -> 2048:
-// 42, 4.1 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 25, a round and a half of blocks, each one's start (6 us with its stores), then 1.2 us to 128 of the
+// 42, 4.1 TB/s of packs; 2331 rows of 24 experts, 1280 -> 2048: 24-27, a round and a half of blocks, each one's start (6 us with its stores), then 1.2 us to 128 of the
 // contraction, 2.1 where two blocks share a compute unit: matrix products 0.5 of it, vector instructions, LDS and loads 0.1 to 0.2 each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -1118,15 +1118,16 @@ int64_t most_tiles(int rows, int experts, int block_rows) {
 // block that takes them, so what those cost agrees: `few`, and `busy` times `least`.  In the forward product the 128-row kernel has a launch in front beside, for
 // nothing where no expert has more than 64 rows (64 experts, 2560 -> 2048, 40 rows 24 us and 22; 8 experts, 4096 -> 28672, 200 rows 165 and 135).
 // us a call of blocks of 32 rows / 64 / 128, of 32 and 64 rows with two sets of wavefronts, and split:
-//   forward    400 rows of 16 experts, 2560 -> 2048   25 /  30 /  33,   22 /  27,   29      800 of 32, 1280 -> 2048   16 /  15 /  18,  16 /  16,  33
-//              400 rows of  4 experts, 2560 -> 1024   23 /  29 /  39,   20 /  26,   10     4000 of 64, 2560 -> 1024   54 /  46 /  59,  60 /  52,  89
-//             3000 rows of 64 experts, 2560 -> 2048   76 /  67 /  64,   84 /  73,  140     3000 of  8,  384 ->  256    7 /   8 /  12,   8 /   9,   9
-//             8000 rows of 64 experts, 2560 -> 2048  159 / 125 / 120,  178 / 137,  300    10000 of 16,  768 -> 1536   50 /  36 /  33,  69 /  47, 148
-//            16384 rows of 64 experts, 2560 -> 2048  273 / 222 / 197,  338 / 242,  568
-//   gradient   400 rows of 16 experts, 2560 <- 2048   24 /  26 /  26,   22 /  24,   27      400 of 16,  768 <-  768   11 /  12 /  11,  10 /  12,   9
-//             2331 rows of 24 experts, 1280 <- 2048   35 /  26 /  39,   40 /  26,   47     6000 of 32, 2048 <-  768   49 /  36 /  39,  67 /  46,  96
-//             3000 rows of 64 experts, 2560 <- 2048   88 /  67 /  77,  107 /  76,  121     5900 of 28,  256 <- 1536   20 /  21 /  31,  19 /  20,  23
-//            16384 rows of 64 experts, 2560 <- 2048  325 / 234 / 216,  408 / 271,  493
+//   forward    400 rows of 16 experts, 2560 -> 2048   24 /  29 /  36,   21 /  27,   28      800 of 32, 1280 -> 2048   20 /  21 /  23,  26 /  23,  36
+//              400 rows of  4 experts, 2560 -> 1024   22 /  28 /  39,   20 /  26,   10     4000 of 64, 2560 -> 1024   53 /  44 /  59,  60 /  50,  91
+//             3000 rows of 64 experts, 2560 -> 2048   74 /  75 /  76,   86 /  76,  137     3000 of  8,  384 ->  256    7 /   8 /  12,   7 /   8,   9
+//             8000 rows of 64 experts, 2560 -> 2048  154 / 123 / 116,  189 / 139,  300    10000 of 16,  768 -> 1536   46 /  34 /  38,  66 /  45, 146
+//            16384 rows of 64 experts, 2560 -> 2048  285 / 219 / 195,  348 / 251,  565     3000 of  2, 2560 -> 2048   52 /  48 /  44,  60 /  53, 108
+//   gradient   400 rows of 16 experts, 2560 <- 2048   22 /  24 /  30,   21 /  23,   24      400 of 16,  768 <-  768   10 /  11 /  13,  10 /  11,   8
+//             2331 rows of 24 experts, 1280 <- 2048   33 /  25 /  39,   38 /  25,   45     6000 of 32, 2048 <-  768   47 /  36 /  35,  66 /  45,  91
+//             3000 rows of 64 experts, 2560 <- 2048   85 /  77 /  81,  107 /  90,  120     5900 of 28,  256 <- 1536   18 /  19 /  30,  17 /  18,  20
+//            16384 rows of 64 experts, 2560 <- 2048  329 / 230 / 209,  412 / 270,  466
+// (rows spread over the experts by weights of exp(normal / 2); in equal parts the 16384 rows take 266 / 198 / 167 and 313 / 211 / 187.)
 // (The costs were fitted to 38 such sizes with their rows spread evenly and unevenly over the experts, packs in turn so that they come from memory, where what is
 // chosen is within 1 % of the best on average, 15 % off at the worst; on 120 others, from 2 rows in all to 4000 of one expert, 2 %, and 49 % at the worst: the gradient of 16
 // rows of 16 experts, 2560 <- 9216, 68, in split blocks, which would take two rounds, 46.)

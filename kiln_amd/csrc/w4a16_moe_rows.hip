@@ -126,7 +126,10 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(SortArgs p) {
 }
 
 // ---- rows ----------------------------------------------------------------------------------------------------------
-// Units of 16 bytes, a thread for each of a token's: it is read or written once, its rows at `top` places.  Eight of them are in flight together.
+// Units of 16 bytes, a thread for each of a token's: it is read or written once, its rows at `top` places.  The gather stores to one place after the other; the
+// combine asks for a place, waits for it, asks for its row and for the next place, so that a thread's rows come one after the other, and then for the weights.
+// Many tokens have enough wavefronts to cover that (8192 tokens of 8, 2048 wide 52 us, 6 TB/s; 1000 of 8, 2560 wide added up 8.4 us); one token's gather takes
+// 2.9 us, 64 tokens' combine 4.3.
 // (A place that no pair has is passed over: nothing is read or written out of bounds whatever `place` holds.)
 struct RowsArgs {
     const uint16_t *in;      // gather: x; combine: rows; combine backward: dy
